@@ -1,4 +1,4 @@
-"""ctypes binding of ``libkarpo_attn.so`` (``include/karpo_attn.h``, version 4). The library is the only compute path: if it is
+"""ctypes binding of ``libkarpo_attn.so`` (``include/karpo_attn.h``, version 4, and ``include/karpo_cache.h``). The library is the only compute path: if it is
 missing this module raises, it never falls back to another implementation."""
 
 from __future__ import annotations
@@ -15,6 +15,12 @@ EXPORTS = ("karpo_attn_fwd", "karpo_attn_plan", "karpo_attn_plan_capacity", "kar
            "karpo_attn_tile_shape", "karpo_attn_strerror", "karpo_attn_version", "karpo_attn_norm_rope",
            "karpo_attn_bwd_workspace_bytes", "karpo_attn_bwd_workspace_best_bytes", "karpo_attn_bwd",
            "karpo_attn_device_status", "karpo_attn_fwd_noalloc")
+
+#: Every symbol ``include/karpo_cache.h`` declares.
+CACHE_EXPORTS = ("karpo_cache_writes_capacity", "karpo_cache_reserve", "karpo_cache_append", "karpo_cache_read",
+                 "karpo_cache_attend_workspace_bytes", "karpo_cache_attend")
+#: karpo_cache_reserve's status word.
+CACHE_NO_BLOCKS, CACHE_BAD_LENGTHS = 10, 11
 
 OK = 0
 ERR_HEAD_DIM, ERR_HEADS, ERR_LAYOUT, ERR_WINDOW, ERR_SPANS, ERR_ARG, ERR_BOUNDS = 2, 3, 4, 6, 7, 9, 11
@@ -74,6 +80,56 @@ class KarpoAttnBwdArgs(ctypes.Structure):
     ]
 
 
+class KarpoCache(ctypes.Structure):
+    _fields_ = [
+        ("keys", ctypes.c_void_p), ("values", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+        ("blocks", ctypes.c_int64), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+    ]
+
+
+class KarpoCacheReserveArgs(ctypes.Structure):
+    _fields_ = [
+        ("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("width", ctypes.c_int32),
+        ("n_seq", ctypes.c_int32), ("lengths", ctypes.c_void_p), ("counts", ctypes.c_void_p),
+        ("free_blocks", ctypes.c_void_p), ("free_count", ctypes.c_void_p), ("free_capacity", ctypes.c_int32),
+        ("block_size", ctypes.c_int32), ("rows", ctypes.c_int64), ("q_cu", ctypes.c_void_p),
+        ("new_lengths", ctypes.c_void_p), ("slots", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+        ("writes", ctypes.c_void_p), ("writes_capacity", ctypes.c_int64), ("free_left", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class KarpoCacheAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", KarpoCache), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("k_stride_tok", ctypes.c_int64), ("k_stride_head", ctypes.c_int64),
+        ("v_stride_tok", ctypes.c_int64), ("v_stride_head", ctypes.c_int64), ("rows", ctypes.c_int64),
+        ("writes", ctypes.c_void_p), ("n_writes", ctypes.c_int64),
+    ]
+
+
+class KarpoCacheReadArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", KarpoCache), ("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("width", ctypes.c_int32),
+        ("n_seq", ctypes.c_int32), ("lengths", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("rows", ctypes.c_int64), ("k_cu", ctypes.c_void_p),
+    ]
+
+
+class KarpoCacheAttendArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", KarpoCache), ("q", ctypes.c_void_p), ("o", ctypes.c_void_p),
+        ("q_stride_tok", ctypes.c_int64), ("q_stride_head", ctypes.c_int64),
+        ("o_stride_tok", ctypes.c_int64), ("o_stride_head", ctypes.c_int64), ("q_cu", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p), ("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+        ("width", ctypes.c_int32), ("n_seq", ctypes.c_int32), ("heads", ctypes.c_int32), ("max_q", ctypes.c_int32),
+        ("total_q", ctypes.c_int64), ("total_keys", ctypes.c_int64), ("scale", ctypes.c_float),
+        ("window_left", ctypes.c_int32), ("window_right", ctypes.c_int32), ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 
@@ -118,6 +174,14 @@ def load() -> ctypes.CDLL:
         lib.karpo_attn_device_status.restype = ctypes.c_int
         lib.karpo_attn_fwd_noalloc.argtypes = [P(KarpoAttnArgs), ctypes.c_void_p]
         lib.karpo_attn_fwd_noalloc.restype = ctypes.c_int
+        lib.karpo_cache_writes_capacity.argtypes = [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32]
+        lib.karpo_cache_writes_capacity.restype = ctypes.c_int64
+        for name, args in (("reserve", KarpoCacheReserveArgs), ("append", KarpoCacheAppendArgs),
+                           ("read", KarpoCacheReadArgs), ("attend", KarpoCacheAttendArgs)):
+            fn = getattr(lib, "karpo_cache_" + name)
+            fn.argtypes, fn.restype = [P(args), ctypes.c_void_p], ctypes.c_int
+        lib.karpo_cache_attend_workspace_bytes.argtypes = [P(KarpoCacheAttendArgs), P(ctypes.c_size_t)]
+        lib.karpo_cache_attend_workspace_bytes.restype = ctypes.c_int
         _lib = lib
         return lib
 

@@ -1,0 +1,70 @@
+// The block cache's kernels' arguments (cache.hip, cache_attn.hip) and the layout of a block, shared with the C ABI
+// (cache_capi.cpp).
+#pragma once
+#include <hip/hip_runtime_api.h>
+#include <stdint.h>
+
+namespace karpo {
+
+constexpr int kCacheGroup = 32;  // tokens that a wave takes at once: two key tiles, one row of value tiles
+
+struct CacheRef {
+  uint8_t* keys;
+  uint8_t* values;
+  float* scales;
+  int64_t blocks;
+  int32_t kv_heads, head_dim, block_log2;
+};
+
+// A batch's cached tokens: request i's lie in the blocks table[i * table_stride + ..], lengths[i] of them, at most
+// `most` (the table row's).
+struct CacheRows {
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* lengths;
+  int32_t n_seq, most;
+};
+
+struct ReserveParams {
+  int32_t* table;
+  int64_t table_stride;
+  int64_t most;  // tokens a table row holds
+  const int32_t* lengths;
+  const int32_t* counts;
+  const int32_t* free_blocks;
+  const int32_t* free_count;
+  int32_t* q_cu;
+  int32_t* new_lengths;
+  int64_t* slots;
+  int32_t* positions;
+  int32_t* writes;
+  int32_t* free_left;
+  int32_t* status;
+  int32_t n_seq, free_capacity, block_log2;
+  int32_t rows, per, writes_capacity;  // per: rows of each workgroup (set by the launch)
+};
+hipError_t launch_cache_reserve(ReserveParams p, hipStream_t stream);
+
+struct AppendParams {
+  CacheRef c;
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t sk_t, sk_h, sv_t, sv_h;
+  const int32_t* writes;
+  int64_t rows;
+};
+hipError_t launch_cache_append(const AppendParams& p, int64_t n_writes, hipStream_t stream);
+
+struct ReadParams {
+  CacheRef c;
+  CacheRows r;
+  const int32_t* q_cu;  // with it: only the tokens that a request's queries can see (window_left before the first)
+  int32_t window_left;
+  uint16_t* k;
+  uint16_t* v;
+  int64_t rows;
+  int32_t* k_cu;
+};
+hipError_t launch_cache_read(const ReadParams& p, hipStream_t stream);
+
+}  // namespace karpo

@@ -1,0 +1,273 @@
+// The block cache's C ABI (karpo_cache.h): argument checks, workspace sizes and launches. Everything that the kernels
+// index with is checked here or in the kernel itself, before a launch or a load.
+#include <stdint.h>
+#include <string.h>
+
+#include "cache.h"
+#include "karpo_cache.h"
+
+using namespace karpo;
+
+namespace {
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+int block_log2(int32_t block_size) { return block_size == 32 ? 5 : block_size == 64 ? 6 : block_size == 128 ? 7 : -1; }
+
+bool overlaps(const void* a, int64_t na, const void* b, int64_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return na > 0 && nb > 0 && x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
+}
+
+// Tokens of a table's row: sums of 1,024 such counts in groups of 32 stay in 32 bits.
+constexpr int64_t kMostTokens = (int64_t)1 << 26;
+
+int check_cache(const KarpoCache& c, CacheRef* ref) {
+  const int b = block_log2(c.block_size);
+  if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256 && c.head_dim != 512) return KARPO_ATTN_ERR_HEAD_DIM;
+  if (c.kv_heads < 1 || c.kv_heads > 16384) return KARPO_ATTN_ERR_HEADS;
+  if (b < 0 || c.blocks < 1 || c.blocks > INT32_MAX) return KARPO_ATTN_ERR_ARG;
+  if (!c.keys || !c.values || !c.scales) return KARPO_ATTN_ERR_NULL;
+  if (!aligned(c.keys, 16) || !aligned(c.values, 16) || !aligned(c.scales, 8)) return KARPO_ATTN_ERR_LAYOUT;
+  ref->keys = static_cast<uint8_t*>(c.keys);
+  ref->values = static_cast<uint8_t*>(c.values);
+  ref->scales = c.scales;
+  ref->blocks = c.blocks;
+  ref->kv_heads = c.kv_heads;
+  ref->head_dim = c.head_dim;
+  ref->block_log2 = b;
+  return KARPO_ATTN_OK;
+}
+
+int check_rows(const int32_t* table, int64_t stride, int32_t width, const int32_t* lengths, int32_t n_seq,
+               int32_t block_size, CacheRows* rows) {
+  if (n_seq < 0 || width < 1 || stride < width || (int64_t)width * block_size > kMostTokens) return KARPO_ATTN_ERR_ARG;
+  if (n_seq > 0 && (!table || !lengths)) return KARPO_ATTN_ERR_NULL;
+  rows->table = table;
+  rows->table_stride = stride;
+  rows->lengths = lengths;
+  rows->n_seq = n_seq;
+  rows->most = (int32_t)(width * (int64_t)block_size);
+  return KARPO_ATTN_OK;
+}
+
+bool row_strides(const void* p, int64_t tok, int64_t head) {
+  return aligned(p, 16) && tok >= 0 && head >= 0 && tok % 8 == 0 && head % 8 == 0;
+}
+
+}  // namespace
+
+extern "C" int64_t karpo_cache_writes_capacity(int64_t rows, int32_t n_seq, int32_t block_size) {
+  const int b = block_log2(block_size);
+  if (rows < 0 || rows > INT32_MAX || n_seq < 0 || b < 0) return 0;
+  // a request's c > 0 tokens touch at most min(c, c / block_size + 2) blocks
+  const int64_t blocks = (rows >> b) + 2 * (int64_t)n_seq;
+  return rows < blocks ? rows : blocks;
+}
+
+extern "C" int karpo_cache_reserve(const KarpoCacheReserveArgs* a, void* stream) {
+  if (a == nullptr) return KARPO_ATTN_ERR_NULL;
+  const int b = block_log2(a->block_size);
+  if (b < 0 || a->rows < 0 || a->rows > INT32_MAX - 65536 || a->free_capacity < 0 ||
+      a->writes_capacity != karpo_cache_writes_capacity(a->rows, a->n_seq, a->block_size))
+    return KARPO_ATTN_ERR_ARG;
+  CacheRows rows;
+  const int st = check_rows(a->table, a->table_stride, a->width, a->lengths, a->n_seq, a->block_size, &rows);
+  if (st != KARPO_ATTN_OK) return st;
+  const int64_t n = a->n_seq;
+  if ((n > 0 && (!a->counts || !a->new_lengths)) || (a->free_capacity > 0 && !a->free_blocks) || !a->free_count ||
+      !a->q_cu || !a->free_left || !a->status ||
+      (a->rows > 0 && (!a->slots || !a->positions)) || (a->writes_capacity > 0 && !a->writes))
+    return KARPO_ATTN_ERR_NULL;
+  if (!aligned(a->slots, 8) || !aligned(a->writes, 16)) return KARPO_ATTN_ERR_LAYOUT;
+  // workgroups read the inputs while others write their outputs
+  const struct { const void* p; int64_t bytes; } in[] = {
+      {a->lengths, 4 * n}, {a->counts, 4 * n}, {a->free_blocks, 4 * (int64_t)a->free_capacity}, {a->free_count, 4}};
+  const struct { const void* p; int64_t bytes; } out[] = {
+      {a->table, n > 0 ? 4 * ((n - 1) * a->table_stride + a->width) : 0}, {a->q_cu, 4 * (n + 1)},
+      {a->new_lengths, 4 * n}, {a->slots, 8 * a->rows}, {a->positions, 4 * a->rows},
+      {a->writes, 16 * a->writes_capacity}, {a->free_left, 4}, {a->status, 4}};
+  for (size_t i = 0; i < sizeof(out) / sizeof(out[0]); ++i) {
+    for (const auto& x : in)
+      if (overlaps(x.p, x.bytes, out[i].p, out[i].bytes)) return KARPO_ATTN_ERR_ARG;
+    for (size_t j = 0; j < i; ++j)
+      if (overlaps(out[j].p, out[j].bytes, out[i].p, out[i].bytes)) return KARPO_ATTN_ERR_ARG;
+  }
+  ReserveParams p;
+  memset(&p, 0, sizeof(p));
+  p.table = a->table;
+  p.table_stride = a->table_stride;
+  p.most = rows.most;
+  p.lengths = a->lengths;
+  p.counts = a->counts;
+  p.free_blocks = a->free_blocks;
+  p.free_count = a->free_count;
+  p.q_cu = a->q_cu;
+  p.new_lengths = a->new_lengths;
+  p.slots = a->slots;
+  p.positions = a->positions;
+  p.writes = a->writes;
+  p.free_left = a->free_left;
+  p.status = a->status;
+  p.n_seq = a->n_seq;
+  p.free_capacity = a->free_capacity;
+  p.block_log2 = b;
+  p.rows = (int32_t)a->rows;
+  p.writes_capacity = (int32_t)a->writes_capacity;
+  if (launch_cache_reserve(p, static_cast<hipStream_t>(stream)) != hipSuccess) return KARPO_ATTN_ERR_LAUNCH;
+  return KARPO_ATTN_OK;
+}
+
+extern "C" int karpo_cache_append(const KarpoCacheAppendArgs* a, void* stream) {
+  if (a == nullptr) return KARPO_ATTN_ERR_NULL;
+  AppendParams p;
+  memset(&p, 0, sizeof(p));
+  const int st = check_cache(a->cache, &p.c);
+  if (st != KARPO_ATTN_OK) return st;
+  if (a->rows < 0 || a->rows > INT32_MAX || a->n_writes < 0 || a->n_writes > INT32_MAX / (2 * a->cache.kv_heads))
+    return KARPO_ATTN_ERR_ARG;
+  if (a->rows == 0 || a->n_writes == 0) return KARPO_ATTN_OK;
+  if (!a->k || !a->v || !a->writes) return KARPO_ATTN_ERR_NULL;
+  if (!row_strides(a->k, a->k_stride_tok, a->k_stride_head) || !row_strides(a->v, a->v_stride_tok, a->v_stride_head) ||
+      !aligned(a->writes, 16))
+    return KARPO_ATTN_ERR_LAYOUT;
+  p.k = static_cast<const uint16_t*>(a->k);
+  p.v = static_cast<const uint16_t*>(a->v);
+  p.sk_t = a->k_stride_tok;
+  p.sk_h = a->k_stride_head;
+  p.sv_t = a->v_stride_tok;
+  p.sv_h = a->v_stride_head;
+  p.writes = a->writes;
+  p.rows = a->rows;
+  if (launch_cache_append(p, a->n_writes, static_cast<hipStream_t>(stream)) != hipSuccess)
+    return KARPO_ATTN_ERR_LAUNCH;
+  return KARPO_ATTN_OK;
+}
+
+extern "C" int karpo_cache_read(const KarpoCacheReadArgs* a, void* stream) {
+  if (a == nullptr) return KARPO_ATTN_ERR_NULL;
+  ReadParams p;
+  memset(&p, 0, sizeof(p));
+  int st = check_cache(a->cache, &p.c);
+  if (st != KARPO_ATTN_OK) return st;
+  st = check_rows(a->table, a->table_stride, a->width, a->lengths, a->n_seq, a->cache.block_size, &p.r);
+  if (st != KARPO_ATTN_OK) return st;
+  if (a->rows < 0 || a->rows > INT32_MAX) return KARPO_ATTN_ERR_ARG;
+  if (!a->k_cu || (a->rows > 0 && (!a->k || !a->v))) return KARPO_ATTN_ERR_NULL;
+  if (!aligned(a->k, 16) || !aligned(a->v, 16)) return KARPO_ATTN_ERR_LAYOUT;
+  p.window_left = -1;
+  p.k = static_cast<uint16_t*>(a->k);
+  p.v = static_cast<uint16_t*>(a->v);
+  p.rows = a->rows;
+  p.k_cu = a->k_cu;
+  if (launch_cache_read(p, static_cast<hipStream_t>(stream)) != hipSuccess) return KARPO_ATTN_ERR_LAUNCH;
+  return KARPO_ATTN_OK;
+}
+
+namespace {
+
+int64_t round_up(int64_t x, int64_t n) { return (x + n - 1) / n * n; }
+
+// The rows that the queries can see, as packed bf16 keys and values, with the packed attention's own workspace behind them.
+struct Unpacked {
+  int64_t rows, k_offset, v_offset, ws_offset;
+  size_t bytes;
+  KarpoAttnArgs fwd;
+};
+
+int unpacked_of(const KarpoCacheAttendArgs* a, Unpacked* u) {
+  int64_t rows = a->total_keys;
+  if (a->window_left >= 0) {  // each request's queries and the window before the first, from a multiple of 32 on
+    const int64_t each = (int64_t)a->max_q + a->window_left + kCacheGroup - 1;
+    if (each < rows && each * a->n_seq < rows) rows = each * a->n_seq;
+  }
+  const int64_t row_bytes = 2 * (int64_t)a->cache.kv_heads * a->cache.head_dim;
+  u->rows = rows;
+  u->k_offset = round_up(4 * ((int64_t)a->n_seq + 1), 256);
+  u->v_offset = u->k_offset + round_up(rows * row_bytes, 256);
+  u->ws_offset = u->v_offset + round_up(rows * row_bytes, 256);
+  KarpoAttnArgs& f = u->fwd;
+  memset(&f, 0, sizeof(f));
+  f.q = a->q;
+  f.o = a->o;
+  f.q_stride_tok = a->q_stride_tok;
+  f.q_stride_head = a->q_stride_head;
+  f.o_stride_tok = a->o_stride_tok;
+  f.o_stride_head = a->o_stride_head;
+  f.k_stride_tok = f.v_stride_tok = (int64_t)a->cache.kv_heads * a->cache.head_dim;
+  f.k_stride_head = f.v_stride_head = a->cache.head_dim;
+  f.q_cu = a->q_cu;
+  f.n_seq = a->n_seq;
+  f.heads = a->heads;
+  f.kv_heads = a->cache.kv_heads;
+  f.head_dim = a->cache.head_dim;
+  f.total_q = a->total_q;
+  f.max_q = a->max_q;
+  f.scale = a->scale;
+  f.window_left = a->window_left;
+  f.window_right = a->window_right;
+  f.key_bound = rows;
+  size_t ws = 0;
+  const int st = karpo_attn_workspace_bytes(&f, &ws);
+  if (st != KARPO_ATTN_OK) return st;
+  u->bytes = (size_t)u->ws_offset + ws;
+  return KARPO_ATTN_OK;
+}
+
+// Sizes and head counts (everything the workspace's size depends on).
+int check_attend(const KarpoCacheAttendArgs* a, CacheRef* c, CacheRows* r) {
+  if (a == nullptr) return KARPO_ATTN_ERR_NULL;
+  int st = check_cache(a->cache, c);
+  if (st != KARPO_ATTN_OK) return st;
+  st = check_rows(a->table, a->table_stride, a->width, a->lengths, a->n_seq, a->cache.block_size, r);
+  if (st != KARPO_ATTN_OK) return st;
+  if (a->heads < 1 || a->heads % a->cache.kv_heads != 0) return KARPO_ATTN_ERR_HEADS;
+  if (a->window_left < -1 || a->window_right < -1) return KARPO_ATTN_ERR_WINDOW;
+  if (a->total_q < 0 || a->max_q < 0 || a->total_keys < 0 || a->total_keys > INT32_MAX) return KARPO_ATTN_ERR_ARG;
+  return KARPO_ATTN_OK;
+}
+
+}  // namespace
+
+extern "C" int karpo_cache_attend_workspace_bytes(const KarpoCacheAttendArgs* a, size_t* bytes) {
+  CacheRef c;
+  CacheRows r;
+  const int st = check_attend(a, &c, &r);
+  if (st != KARPO_ATTN_OK) return st;
+  if (bytes == nullptr) return KARPO_ATTN_ERR_NULL;
+  Unpacked u;
+  const int su = unpacked_of(a, &u);
+  if (su != KARPO_ATTN_OK) return su;
+  *bytes = u.bytes;
+  return KARPO_ATTN_OK;
+}
+
+extern "C" int karpo_cache_attend(const KarpoCacheAttendArgs* a, void* stream) {
+  ReadParams p;
+  memset(&p, 0, sizeof(p));
+  int st = check_attend(a, &p.c, &p.r);
+  if (st != KARPO_ATTN_OK) return st;
+  if (a->total_q == 0 || a->n_seq == 0) return KARPO_ATTN_OK;
+  if (!a->q || !a->o || !a->q_cu) return KARPO_ATTN_ERR_NULL;
+  if (!row_strides(a->q, a->q_stride_tok, a->q_stride_head) || !row_strides(a->o, a->o_stride_tok, a->o_stride_head))
+    return KARPO_ATTN_ERR_LAYOUT;
+  Unpacked u;
+  st = unpacked_of(a, &u);
+  if (st != KARPO_ATTN_OK) return st;
+  if (a->workspace == nullptr || a->workspace_bytes < u.bytes || !aligned(a->workspace, 16))
+    return KARPO_ATTN_ERR_WORKSPACE;
+  char* const ws = static_cast<char*>(a->workspace);
+  p.q_cu = a->q_cu;
+  p.window_left = a->window_left;
+  p.k = reinterpret_cast<uint16_t*>(ws + u.k_offset);
+  p.v = reinterpret_cast<uint16_t*>(ws + u.v_offset);
+  p.rows = u.rows;
+  p.k_cu = reinterpret_cast<int32_t*>(ws);
+  if (launch_cache_read(p, static_cast<hipStream_t>(stream)) != hipSuccess) return KARPO_ATTN_ERR_LAUNCH;
+  u.fwd.k = p.k;
+  u.fwd.v = p.v;
+  u.fwd.k_cu = p.k_cu;
+  u.fwd.workspace = ws + u.ws_offset;
+  u.fwd.workspace_bytes = a->workspace_bytes - (size_t)u.ws_offset;
+  return karpo_attn_fwd(&u.fwd, stream);
+}

@@ -1,0 +1,68 @@
+// Device helpers of the block cache's kernels.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "mfma_common.h"
+
+namespace karpo {
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+__host__ __device__ __forceinline__ int64_t ka_min64(int64_t a, int64_t b) { return a < b ? a : b; }
+
+// 2^e, -126 <= e <= 127.
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
+
+// Two e4m3 codes of `w` (its upper two with `up`) times `scale` (a power of two: exact) as packed bf16.
+__device__ __forceinline__ unsigned bf16_pair(unsigned w, float scale, bool up) {
+  return up ? __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true))
+            : __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false));
+}
+__device__ __forceinline__ u32x4 bf16_of_8(unsigned a, unsigned b, float scale) {
+  return u32x4{bf16_pair(a, scale, false), bf16_pair(a, scale, true), bf16_pair(b, scale, false),
+               bf16_pair(b, scale, true)};
+}
+
+// v: the sum over the workgroup's threads before this one, of N values; all: over all of them. `part` is free again after
+// the caller's next barrier.
+template <int THREADS, int N>
+__device__ __forceinline__ void block_scan(int (&v)[N], int (&all)[N], int (*part)[N]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int own[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    own[k] = v[k];
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int t = __shfl_up(v[k], o);
+      if (lane >= o) v[k] += t;
+    }
+    if (lane == 63) part[wave][k] = v[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    int before = 0, sum = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
+      const int t = part[w][k];
+      if (w < wave) before += t;
+      sum += t;
+    }
+    v[k] += before - own[k];
+    all[k] = sum;
+  }
+}
+
+// The last j < n with first[j] <= x (first[0] <= x, non-decreasing).
+__device__ __forceinline__ int last_at_most(const int* first, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first[mid] <= x) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+}  // namespace karpo
