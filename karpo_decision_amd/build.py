@@ -26,7 +26,7 @@ HIP_FLAGS = [
     "-munsafe-fp-atomics", f"-I{INCLUDE}", f"-I{CSRC}",
 ]
 SOURCES = ["attn_fwd.hip", "attn_fwd_128.hip", "attn_bwd.hip", "attn_bwd_pair.hip", "attn_bwd_wide.hip",
-           "cache.hip", "capi.cpp", "cache_capi.cpp", "plan.cpp", "scratch.hip"]
+           "cache.hip", "cache_attn.hip", "capi.cpp", "cache_capi.cpp", "plan.cpp", "scratch.hip"]
 # per-source flags: the head-size-128 wide / long forward tiles under the iterative-ILP machine scheduler; the backward's
 # live ranges split for few spills (otherwise the head-size-256 dK / dV kernel, at all 512 registers, spills inside its
 # loop; the other kernels of the file come out the same)

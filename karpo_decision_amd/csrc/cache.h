@@ -67,4 +67,29 @@ struct ReadParams {
 };
 hipError_t launch_cache_read(const ReadParams& p, hipStream_t stream);
 
+struct AttendParams {
+  CacheRef c;
+  CacheRows r;
+  const uint16_t* q;
+  uint16_t* o;
+  int64_t sq_t, sq_h, so_t, so_h;
+  const int32_t* q_cu;
+  int64_t total_q;
+  int32_t group;       // heads / kv_heads
+  int32_t left, right;
+  float scale;         // times log2(e)
+  int32_t parts;       // workgroups for each of the grid's y
+  float* partial;      // [y][parts][2] of (O [vectors][D], m [vectors], l [vectors])
+  int64_t* units;      // [n_seq + 1] groups of 32 tokens before each request
+};
+
+// The split path's launch for these sizes: `vectors` query vectors (position x head of the group) per workgroup, `tiles`
+// workgroups for a key/value head's max_q * group vectors, `parts` shares of the keys.
+struct AttendShape {
+  int vectors, tiles, parts;
+  int64_t units_bytes, bytes;  // of the workspace: the units, then the partials
+};
+AttendShape attend_shape(const CacheRef& c, int32_t n_seq, int32_t group, int32_t max_q);
+hipError_t launch_cache_attend(const AttendParams& p, const AttendShape& s, hipStream_t stream);
+
 }  // namespace karpo

@@ -1,0 +1,492 @@
+// Attention over the block cache for few queries per request (karpo_cache_attend): the keys of all requests are split evenly
+// over the GPU, 32 tokens at a time, and the shares of a request joined by a second launch.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "cache.h"
+#include "cache_common.h"
+
+namespace karpo {
+
+namespace {
+
+constexpr int kAttendWaves = 4;
+constexpr int kAttendThreads = 64 * kAttendWaves;
+// Waves per SIMD (and workgroups per CU).
+__host__ __device__ constexpr int attend_waves(int d, int nt) {
+  return d * nt <= 64 ? 4 : d * nt <= 128 ? 3 : d * nt <= 256 ? 2 : 1;
+}
+constexpr int kLeastUnits = kAttendWaves;  // groups of 32 tokens that a workgroup takes at least
+
+struct Seen {
+  int tokens, row, queries;  // cached tokens; first query row; query rows
+  int first, groups;         // first group of 32 tokens that a query sees, and how many up to the last token
+  int units;                 // groups, or 1 where there are queries and no tokens (their rows are zeros)
+};
+
+__device__ __forceinline__ Seen seen_of(const AttendParams& p, int i) {
+  Seen s;
+  s.tokens = min(max(p.r.lengths[i], 0), p.r.most);
+  const int a = p.q_cu[i], b = p.q_cu[i + 1];
+  s.row = a;
+  s.queries = a >= 0 && b > a && b <= p.total_q ? b - a : 0;
+  const int64_t before = (int64_t)s.tokens - s.queries - p.left;
+  s.first = p.left >= 0 && before > 0 ? (int)(before < s.tokens ? before : s.tokens) / kCacheGroup : 0;
+  s.groups = (s.tokens + kCacheGroup - 1) / kCacheGroup - s.first;
+  s.units = s.queries > 0 ? max(s.groups, 1) : 0;
+  return s;
+}
+
+// Workgroup p of `parts` takes the units [total * p / parts, total * (p + 1) / parts); parts <= total, so none is empty.
+__device__ __forceinline__ int64_t parts_of(int64_t total, int parts) {
+  const int64_t most = total / kLeastUnits;
+  return most < 1 ? 1 : most < parts ? most : parts;
+}
+// The workgroup that takes unit u.
+__device__ __forceinline__ int64_t part_of(int64_t u, int64_t total, int64_t parts) { return ((u + 1) * parts - 1) / total; }
+
+// x's maximum / sum over the four lanes of a column (16 apart).
+__device__ __forceinline__ float column_max(float x) {
+  x = half_swap_max(x);
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __builtin_elementwise_maximum(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float column_sum(float x) {
+  x = half_swap_sum(x);
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ bf16x8 operand(unsigned a, unsigned b, float scale) {
+  return __builtin_bit_cast(bf16x8, bf16_of_8(a, b, scale));
+}
+
+// Which of a word's four codes are NaN, as 0x80 in their bytes.
+__device__ __forceinline__ unsigned nan_codes(unsigned w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+// One lane's view of a group of 32 tokens with 16x16x32 matrix instructions: S^T = K Q^T has the keys as rows (two tiles),
+// the query vectors as columns: column lane % 16, keys 16 t + 4 (lane / 16) + i. Those are this lane's eight weights, and as
+// they stand the second operand of O^T = V^T P^T, whose first operand, 8 of these keys of one element, is 8 bytes of the cache.
+// The products are of bf16 operands (a cached element is one exactly); the weights enter as two bf16 terms, 2^-17 off, which
+// costs matrix work that this kernel, bound by the codes' way from HBM, has to spare.
+template <int D, int NT>
+__global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_kernel(
+    const AttendParams p) {
+  constexpr int kLoads = D / 32;       // KiB of keys, and of values, in a group
+  constexpr int kChunks = D / 64;      // 64-element chunks of a key tile
+  constexpr int kSlab = 128 / NT < D ? 128 / NT : D;  // elements that the waves join at once
+  constexpr int kVectors = 16 * NT;
+  __shared__ int s_unit[kAttendThreads + 1];
+  __shared__ int s_part[kAttendWaves][1];
+  __shared__ int64_t s_sum[kAttendWaves];
+  __shared__ float s_m[kAttendWaves][kVectors], s_l[kAttendWaves][kVectors], s_top[kVectors], s_total[kVectors];
+  // the query vectors' operands while the groups are walked, then the waves' sums
+  constexpr int kSums = kAttendWaves * kVectors * (kSlab + 4) * 4, kQueries = kVectors * D * 2;
+  __shared__ __align__(16) char s_data[kSums > kQueries ? kSums : kQueries];
+  u32x4* const s_q = reinterpret_cast<u32x4*>(s_data);
+  float(*const s_o)[kVectors][kSlab + 4] = reinterpret_cast<float(*)[kVectors][kSlab + 4]>(s_data);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, quad = lane >> 4;
+  const int heads = p.c.kv_heads, b = p.c.block_log2;
+  const int h = blockIdx.y % heads, vector0 = (blockIdx.y / heads) * kVectors;
+
+  int64_t total = 0;
+  for (int i = tid; i < p.r.n_seq; i += kAttendThreads) total += seen_of(p, i).units;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
+  if (lane == 0) s_sum[wave] = total;
+  __syncthreads();
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kAttendWaves; ++w) total += s_sum[w];
+  const bool writes_units = blockIdx.x == 0 && blockIdx.y == 0;
+  const int64_t parts = parts_of(total, p.parts);
+  if (total == 0 || (int64_t)blockIdx.x >= parts) {
+    if (writes_units && tid == 0) p.units[p.r.n_seq] = 0;  // (total is 0: nothing to join)
+    return;
+  }
+  const int64_t u0 = total * blockIdx.x / parts, u1 = total * (blockIdx.x + 1) / parts;
+
+  int64_t carry = 0;
+  for (int c0 = 0; c0 < p.r.n_seq && (writes_units || carry < u1); c0 += kAttendThreads) {
+    const int m = min(kAttendThreads, p.r.n_seq - c0);
+    int v[1] = {tid < m ? seen_of(p, c0 + tid).units : 0}, all[1];
+    block_scan<kAttendThreads, 1>(v, all, s_part);
+    if (tid < m) {
+      s_unit[tid] = v[0];
+      if (writes_units) p.units[c0 + tid] = carry + v[0];
+    }
+    if (tid == 0) s_unit[m] = all[0];
+    __syncthreads();
+    const int64_t from = u0 > carry ? u0 : carry, to = u1 < carry + all[0] ? u1 : carry + all[0];
+    for (int64_t at = from; at < to;) {
+      const int j = __builtin_amdgcn_readfirstlane(last_at_most(s_unit, m, (int)(at - carry)));
+      const int i = c0 + j;
+      const int64_t begin = carry + s_unit[j], end = carry + s_unit[j + 1];
+      const int64_t stop = to < end ? to : end;
+      const Seen s = seen_of(p, i);
+      const int g0 = s.first + (int)(at - begin);
+      const int g1 = s.groups > 0 ? s.first + (int)(stop - begin) : g0;
+      at = stop;
+      const int vectors = (int)min<int64_t>((int64_t)s.queries * p.group - vector0, kVectors);
+      if (vectors <= 0) continue;
+
+      // the query vectors' operands (entry (2 c + k) * NT + n, one lane's 16 bytes after the other), and the keys that each
+      // vector sees: lo .. hi
+      int lo[NT], hi[NT];
+      const int shift = s.tokens - s.queries;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int vec = vector0 + 16 * n + col;
+        const bool valid = 16 * n + col < vectors;
+        const int pos = valid ? vec / p.group : 0;
+        const uint16_t* const src =
+            p.q + (s.row + (int64_t)pos) * p.sq_t + (int64_t)(h * p.group + (valid ? vec - pos * p.group : 0)) * p.sq_h;
+        for (int c = wave; c < 2 * kChunks; c += kAttendWaves)
+          s_q[(c * NT + n) * 64 + lane] = *reinterpret_cast<const u32x4*>(src + (c >> 1) * 64 + quad * 16 + (c & 1) * 8);
+        lo[n] = p.left < 0 ? 0 : pos + shift - p.left;
+        hi[n] = p.right < 0 ? s.tokens - 1 : (int)min<int64_t>((int64_t)pos + shift + p.right, s.tokens - 1);
+      }
+      // groups that every vector sees whole
+      const int pos_first = vector0 / p.group, pos_last = (vector0 + vectors - 1) / p.group;
+      const int full_lo = p.left < 0 ? 0 : pos_last + shift - p.left;
+      const int full_hi =
+          p.right < 0 ? s.tokens - 1 : (int)min<int64_t>((int64_t)pos_first + shift + p.right, s.tokens - 1);
+
+      f32x4 o[NT][D / 16];
+      float top[NT], sum[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        top[n] = -INFINITY;
+        sum[n] = 0.f;
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) o[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+
+      u32x4 kr[kLoads], vr[kLoads];
+      const int32_t* const table = p.r.table + (int64_t)i * p.r.table_stride;
+      const int lane_offset = col * 64 + quad * 16;
+      int ids = 0;
+      float k_scales = 1.f, v_scales = 1.f;
+      // lane k looks up the wave's groups g + 4 k
+      auto look_up = [&](int g) {
+        const int mine = min(g + lane * kAttendWaves, g1 - 1);
+        ids = table[mine >> (b - 5)];
+        if (ids < 0 || ids >= p.c.blocks) ids = -1;
+        const float2 sc = *reinterpret_cast<const float2*>(p.c.scales + 2 * ((int64_t)max(ids, 0) * heads + h));
+        k_scales = sc.x;
+        v_scales = sc.y;
+      };
+      auto offset = [&](int g, int k) {
+        const int id = max(__builtin_amdgcn_readlane(ids, k), 0);
+        return ((((int64_t)id * heads + h) << b) + (int64_t)(g & ((1 << (b - 5)) - 1)) * kCacheGroup) * D;
+      };
+      auto load_keys = [&](int g, int k) {
+        const uint8_t* const src = p.c.keys + offset(g, k);
+#pragma unroll
+        for (int t = 0; t < kLoads; ++t) kr[t] = *reinterpret_cast<const u32x4*>(src + t * 1024 + lane_offset);
+      };
+      auto load_values = [&](int g, int k) {
+        const uint8_t* const src = p.c.values + offset(g, k);
+#pragma unroll
+        for (int t = 0; t < kLoads; ++t) vr[t] = *reinterpret_cast<const u32x4*>(src + t * 1024 + lane_offset);
+      };
+
+      int k = 0;
+      if (g0 + wave < g1) {
+        look_up(g0 + wave);
+        load_keys(g0 + wave, 0);
+        load_values(g0 + wave, 0);
+      }
+      __syncthreads();
+      for (int g = g0 + wave; g < g1; g += kAttendWaves) {
+        const bool known = __builtin_amdgcn_readlane(ids, k) >= 0;
+        const float k_scale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(k_scales), k));
+        const float v_scale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v_scales), k));
+        const int next = g + kAttendWaves;
+        if (!known) {
+#pragma unroll
+          for (int t = 0; t < kLoads; ++t) kr[t] = vr[t] = u32x4{0, 0, 0, 0};
+        }
+        f32x4 st[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) st[n][0] = st[n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 2 * kChunks; ++c) {
+          bf16x8 q[NT];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) q[n] = __builtin_bit_cast(bf16x8, s_q[(c * NT + n) * 64 + lane]);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const u32x4& w = kr[t * kChunks + (c >> 1)];
+            const bf16x8 a = operand(w[2 * (c & 1)], w[2 * (c & 1) + 1], k_scale);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) st[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q[n], st[n][t], 0, 0, 0);
+          }
+        }
+        if (++k == 64 && next < g1) {
+          look_up(next);
+          k = 0;
+        }
+        if (next < g1) load_keys(next, k);
+
+        const int key0 = g * kCacheGroup;
+        const bool masked = key0 < full_lo || key0 + kCacheGroup - 1 > full_hi;
+        bf16x8 weight[NT][2], is_seen[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = st[n][e >> 2][e & 3] * p.scale;
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int key = key0 + (e >> 2) * 16 + quad * 4 + (e & 3);
+              const bool sees = key >= lo[n] && key <= hi[n];
+              x[e] = sees ? x[e] : -INFINITY;
+              is_seen[n][e] = sees ? (__bf16)1.f : (__bf16)0.f;
+            }
+          }
+          float best = x[0];
+#pragma unroll
+          for (int e = 1; e < 8; ++e) best = __builtin_elementwise_maximum(best, x[e]);
+          best = column_max(best);
+          // the running maximum is raised (and O rescaled) only where it grows by more than 2^8: weights are then at most 2^8
+          if (__any(!(best <= top[n] + 8.f) && best != -INFINITY)) {
+            const float up = __builtin_elementwise_maximum(top[n], best);
+            const float f = top[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top[n] - up);
+            top[n] = up;
+            sum[n] *= f;
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) o[n][t] *= f;
+          }
+          const float base = top[n] == -INFINITY ? 0.f : top[n];
+          float add = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float w = __builtin_amdgcn_exp2f(x[e] - base);
+            add += w;
+            const __bf16 high = (__bf16)w;
+            weight[n][0][e] = high;
+            weight[n][1][e] = (__bf16)(w - (float)high);
+          }
+          sum[n] += add;
+        }
+
+        bool nan = false;
+        if (masked) {
+          unsigned any = 0;
+#pragma unroll
+          for (int t = 0; t < kLoads; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) any |= nan_codes(vr[t][e]);
+          nan = __any(any != 0);
+        }
+        if (nan) {  // a NaN reaches the vectors that see its token, and no others (zero times NaN would be NaN)
+#pragma unroll
+          for (int t = 0; t < kLoads; ++t)
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+              const unsigned f0 = nan_codes(vr[t][2 * d]), f1 = nan_codes(vr[t][2 * d + 1]);
+              const bf16x8 marks = operand(f0 >> 1, f1 >> 1, 1.f);  // 2.0 where NaN
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                const f32x4 count =
+                    __builtin_amdgcn_mfma_f32_16x16x32_bf16(marks, is_seen[n], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[n][2 * t + d][e] += count[e] > 0.f ? NAN : 0.f;
+              }
+              vr[t][2 * d] &= ~((f0 >> 7) * 255u);
+              vr[t][2 * d + 1] &= ~((f1 >> 7) * 255u);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < kLoads; ++t)
+#pragma unroll
+          for (int d = 0; d < 2; ++d) {
+            const bf16x8 a = operand(vr[t][2 * d], vr[t][2 * d + 1], v_scale);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              o[n][2 * t + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, weight[n][0], o[n][2 * t + d], 0, 0, 0);
+              o[n][2 * t + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, weight[n][1], o[n][2 * t + d], 0, 0, 0);
+            }
+          }
+        if (next < g1) load_values(next, k);
+      }
+
+      // join the waves
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float l = column_sum(sum[n]);
+        if (quad == 0) {
+          s_m[wave][16 * n + col] = top[n];
+          s_l[wave][16 * n + col] = l;
+        }
+      }
+      __syncthreads();
+      if (tid < kVectors) {
+        float up = s_m[0][tid], l = 0.f;
+#pragma unroll
+        for (int w = 1; w < kAttendWaves; ++w) up = __builtin_elementwise_maximum(up, s_m[w][tid]);
+#pragma unroll
+        for (int w = 0; w < kAttendWaves; ++w)
+          l += s_m[w][tid] == -INFINITY ? 0.f : s_l[w][tid] * __builtin_amdgcn_exp2f(s_m[w][tid] - up);
+        s_top[tid] = up;
+        s_total[tid] = l;
+      }
+      __syncthreads();
+      const bool whole = begin >= u0 && end <= u1;
+      float* const part =
+          p.partial + (((int64_t)blockIdx.y * p.parts + blockIdx.x) * 2 + (begin <= u0 ? 0 : 1)) * (kVectors * (D + 2));
+      if (!whole && tid < vectors) {
+        part[kVectors * D + tid] = s_top[tid];
+        part[kVectors * D + kVectors + tid] = s_total[tid];
+      }
+      for (int d0 = 0; d0 < D; d0 += kSlab) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const float f = top[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top[n] - s_top[16 * n + col]);
+#pragma unroll
+          for (int t = 0; t < D / 16; ++t)
+            if (t * 16 >= d0 && t * 16 < d0 + kSlab)
+              *reinterpret_cast<f32x4*>(&s_o[wave][16 * n + col][t * 16 - d0 + quad * 4]) = o[n][t] * f;
+        }
+        __syncthreads();
+        for (int e = tid; e < vectors * (kSlab / 4); e += kAttendThreads) {
+          const int c = e / (kSlab / 4), d = (e % (kSlab / 4)) * 4;
+          f32x4 x = *reinterpret_cast<const f32x4*>(&s_o[0][c][d]);
+#pragma unroll
+          for (int w = 1; w < kAttendWaves; ++w) x += *reinterpret_cast<const f32x4*>(&s_o[w][c][d]);
+          if (whole) {
+            const float l = s_total[c];
+            const int vec = vector0 + c, pos = vec / p.group, head = h * p.group + vec - pos * p.group;
+            if (l == 0.f) x = f32x4{0.f, 0.f, 0.f, 0.f}; else x = x * (1.f / l);
+            *reinterpret_cast<u32x2*>(p.o + (s.row + (int64_t)pos) * p.so_t + head * p.so_h + d0 + d) =
+                u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+          } else {
+            *reinterpret_cast<f32x4*>(part + c * D + d0 + d) = x;
+          }
+        }
+        __syncthreads();
+      }
+    }
+    carry += all[0];
+    __syncthreads();  // the next chunk's requests take s_unit
+  }
+  if (writes_units && tid == 0) p.units[p.r.n_seq] = total;
+}
+
+// Joins a request's shares: O = sum of 2^(m_w - M) O_w over sum of 2^(m_w - M) l_w, in the shares' order. Requests that one
+// workgroup took whole are done already. The shares' factors first, 64 at a time by the lanes of a wave, so that the sums'
+// loads wait on nothing but the memory.
+template <int D>
+__global__ __launch_bounds__(256) void join_kernel(const AttendParams p, int vectors_per) {
+  constexpr int kRow = D / 4, kAtOnce = 256 / kRow < 4 ? 256 / kRow : 4;  // vectors of a workgroup
+  __shared__ float s_f[kAtOnce][64];
+  __shared__ float s_l[kAtOnce], s_back[kAtOnce];
+  const int i = blockIdx.x, heads = p.c.kv_heads;
+  const int64_t total = p.units[p.r.n_seq], begin = p.units[i], end = p.units[i + 1];
+  if (total == 0 || begin == end) return;
+  const int64_t parts = parts_of(total, p.parts);
+  const int first = (int)part_of(begin, total, parts), last = (int)part_of(end - 1, total, parts);
+  if (first == last) return;
+  const Seen s = seen_of(p, i);
+  const int h = blockIdx.y % heads, vector0 = (blockIdx.y / heads) * vectors_per;
+  const int c0 = blockIdx.z * kAtOnce;
+  const int vectors = (int)min<int64_t>((int64_t)s.queries * p.group - vector0, vectors_per);
+  if (c0 >= vectors) return;
+  const int64_t size = (int64_t)vectors_per * (D + 2);
+  const float* const base = p.partial + (int64_t)blockIdx.y * p.parts * 2 * size;
+  auto share = [&](int w) { return base + (2 * (int64_t)w + (begin <= total * w / parts ? 0 : 1)) * size; };
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int mine = tid / kRow, c = c0 + mine, d = (tid % kRow) * 4;
+  const bool active = mine < kAtOnce && c < vectors;
+  float up = -INFINITY, l = 0.f;  // of vector c0 + wave, in every lane of its wave
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+  for (int w0 = first; w0 <= last; w0 += 64) {
+    if (wave < kAtOnce && c0 + wave < vectors) {
+      const int w = w0 + lane;
+      float m = -INFINITY, lw = 0.f;
+      if (w <= last) {
+        const float* const part = share(w) + vectors_per * D + c0 + wave;
+        m = part[0];
+        lw = part[vectors_per];
+      }
+      float next = __builtin_elementwise_maximum(up, m);
+      next = column_max(next);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) next = __builtin_elementwise_maximum(next, __shfl_xor(next, o));
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - next);
+      const float back = up == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(up - next);
+      float add = column_sum(lw * f);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) add += __shfl_xor(add, o);
+      l = l * back + add;
+      up = next;
+      s_f[wave][lane] = f;
+      if (lane == 0) {
+        s_l[wave] = l;
+        s_back[wave] = back;
+      }
+    }
+    __syncthreads();
+    if (active) {
+      x *= s_back[mine];
+      const int n = min(64, last - w0 + 1);
+#pragma unroll 8
+      for (int w = 0; w < n; ++w) x += *reinterpret_cast<const f32x4*>(share(w0 + w) + c * D + d) * s_f[mine][w];
+    }
+    __syncthreads();
+  }
+  if (!active) return;
+  l = s_l[mine];
+  const int vec = vector0 + c, pos = vec / p.group, head = h * p.group + vec - pos * p.group;
+  if (l == 0.f) x = f32x4{0.f, 0.f, 0.f, 0.f}; else x = x * (1.f / l);
+  *reinterpret_cast<u32x2*>(p.o + (s.row + (int64_t)pos) * p.so_t + head * p.so_h + d) =
+      u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+}
+
+template <int D, int NT>
+void launch(const AttendParams& p, const AttendShape& s, hipStream_t stream) {
+  const unsigned y = (unsigned)(p.c.kv_heads * s.tiles);
+  attend_kernel<D, NT><<<dim3((unsigned)s.parts, y), dim3(kAttendThreads), 0, stream>>>(p);
+  const unsigned z = (unsigned)(16 * NT / (D == 512 ? 2 : 4));
+  join_kernel<D><<<dim3((unsigned)p.r.n_seq, y, z), dim3(256), 0, stream>>>(p, 16 * NT);
+}
+
+}  // namespace
+
+AttendShape attend_shape(const CacheRef& c, int32_t n_seq, int32_t group, int32_t max_q) {
+  AttendShape s;
+  const int64_t vectors = (int64_t)max_q * group;
+  const int most = c.head_dim <= 128 ? 4 : c.head_dim == 256 ? 2 : 1;  // tiles of 16 vectors that the registers hold
+  const int tiles = vectors <= 16 || most == 1 ? 1 : vectors <= 32 || most == 2 ? 2 : 4;
+  s.vectors = 16 * tiles;
+  s.tiles = (int)((vectors + s.vectors - 1) / s.vectors);
+  if (s.tiles < 1) s.tiles = 1;
+  const int at_once = attend_waves(c.head_dim, tiles);
+  const int64_t y = (int64_t)c.kv_heads * s.tiles;
+  const int64_t parts = 256 * at_once / y;
+  s.parts = parts < 1 ? 1 : (int)parts;
+  s.units_bytes = (8 * ((int64_t)n_seq + 1) + 255) / 256 * 256;
+  s.bytes = s.units_bytes + y * s.parts * 2 * s.vectors * (c.head_dim + 2) * 4;
+  return s;
+}
+
+hipError_t launch_cache_attend(const AttendParams& p, const AttendShape& s, hipStream_t stream) {
+  switch (p.c.head_dim * 8 + s.vectors / 16) {
+    case 64 * 8 + 1: launch<64, 1>(p, s, stream); break;
+    case 64 * 8 + 2: launch<64, 2>(p, s, stream); break;
+    case 64 * 8 + 4: launch<64, 4>(p, s, stream); break;
+    case 128 * 8 + 1: launch<128, 1>(p, s, stream); break;
+    case 128 * 8 + 2: launch<128, 2>(p, s, stream); break;
+    case 128 * 8 + 4: launch<128, 4>(p, s, stream); break;
+    case 256 * 8 + 1: launch<256, 1>(p, s, stream); break;
+    case 256 * 8 + 2: launch<256, 2>(p, s, stream); break;
+    case 512 * 8 + 1: launch<512, 1>(p, s, stream); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace karpo

@@ -227,6 +227,11 @@ int check_attend(const KarpoCacheAttendArgs* a, CacheRef* c, CacheRows* r) {
   return KARPO_ATTN_OK;
 }
 
+// Whether the call's queries are few enough for the split path.
+bool split(const KarpoCacheAttendArgs* a) {
+  return (int64_t)a->max_q * (a->heads / a->cache.kv_heads) <= 64;
+}
+
 }  // namespace
 
 extern "C" int karpo_cache_attend_workspace_bytes(const KarpoCacheAttendArgs* a, size_t* bytes) {
@@ -235,6 +240,10 @@ extern "C" int karpo_cache_attend_workspace_bytes(const KarpoCacheAttendArgs* a,
   const int st = check_attend(a, &c, &r);
   if (st != KARPO_ATTN_OK) return st;
   if (bytes == nullptr) return KARPO_ATTN_ERR_NULL;
+  if (split(a)) {
+    *bytes = (size_t)attend_shape(c, a->n_seq, a->heads / a->cache.kv_heads, a->max_q).bytes;
+    return KARPO_ATTN_OK;
+  }
   Unpacked u;
   const int su = unpacked_of(a, &u);
   if (su != KARPO_ATTN_OK) return su;
@@ -251,6 +260,32 @@ extern "C" int karpo_cache_attend(const KarpoCacheAttendArgs* a, void* stream) {
   if (!a->q || !a->o || !a->q_cu) return KARPO_ATTN_ERR_NULL;
   if (!row_strides(a->q, a->q_stride_tok, a->q_stride_head) || !row_strides(a->o, a->o_stride_tok, a->o_stride_head))
     return KARPO_ATTN_ERR_LAYOUT;
+  if (split(a)) {
+    const AttendShape shape = attend_shape(p.c, a->n_seq, a->heads / a->cache.kv_heads, a->max_q);
+    if (a->workspace == nullptr || a->workspace_bytes < (size_t)shape.bytes || !aligned(a->workspace, 16))
+      return KARPO_ATTN_ERR_WORKSPACE;
+    AttendParams t;
+    memset(&t, 0, sizeof(t));
+    t.c = p.c;
+    t.r = p.r;
+    t.q = static_cast<const uint16_t*>(a->q);
+    t.o = static_cast<uint16_t*>(a->o);
+    t.sq_t = a->q_stride_tok;
+    t.sq_h = a->q_stride_head;
+    t.so_t = a->o_stride_tok;
+    t.so_h = a->o_stride_head;
+    t.q_cu = a->q_cu;
+    t.total_q = a->total_q;
+    t.group = a->heads / a->cache.kv_heads;
+    t.left = a->window_left >= kMostTokens ? -1 : a->window_left;  // (sees everything, and stays within 32 bits)
+    t.right = a->window_right;
+    t.scale = a->scale * 1.4426950408889634f;
+    t.parts = shape.parts;
+    t.units = static_cast<int64_t*>(a->workspace);
+    t.partial = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + shape.units_bytes);
+    if (launch_cache_attend(t, shape, static_cast<hipStream_t>(stream)) != hipSuccess) return KARPO_ATTN_ERR_LAUNCH;
+    return KARPO_ATTN_OK;
+  }
   Unpacked u;
   st = unpacked_of(a, &u);
   if (st != KARPO_ATTN_OK) return st;
