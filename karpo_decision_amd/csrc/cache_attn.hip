@@ -14,7 +14,17 @@ constexpr int kAttendWaves = 4;
 constexpr int kAttendThreads = 64 * kAttendWaves;
 // Waves per SIMD (and workgroups per CU).
 __host__ __device__ constexpr int attend_waves(int d, int nt) {
-  return d * nt <= 64 ? 4 : d * nt <= 128 ? 3 : d * nt <= 256 ? 2 : 1;
+  return nt == 1 && d <= 128 ? 4 : d == 64 && nt == 2 ? 3 : d <= 128 || (d == 256 && nt == 1) ? 2 : 1;
+}
+// Bytes of LDS for the waves' copies of a group's keys and values, and behind them the query vectors; the waves' sums take
+// the same bytes when the groups are done.
+constexpr int ring_bytes(int d) { return kAttendWaves * 2 * kCacheGroup * d; }
+constexpr int data_bytes(int d, int nt) { return ring_bytes(d) + 16 * nt * d * 2; }
+// Elements of the output that the waves join at once.
+constexpr int slab_of(int d, int nt) {
+  int slab = d;
+  while (kAttendWaves * 16 * nt * (slab + 4) * 4 > data_bytes(d, nt)) slab /= 2;
+  return slab;
 }
 constexpr int kLeastUnits = kAttendWaves;  // groups of 32 tokens that a workgroup takes at least
 
@@ -74,19 +84,20 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
     const AttendParams p) {
   constexpr int kLoads = D / 32;       // KiB of keys, and of values, in a group
   constexpr int kChunks = D / 64;      // 64-element chunks of a key tile
-  constexpr int kSlab = 128 / NT < D ? 128 / NT : D;  // elements that the waves join at once
+  constexpr int kSlab = slab_of(D, NT);
   constexpr int kVectors = 16 * NT;
   __shared__ int s_unit[kAttendThreads + 1];
   __shared__ int s_part[kAttendWaves][1];
   __shared__ int64_t s_sum[kAttendWaves];
   __shared__ float s_m[kAttendWaves][kVectors], s_l[kAttendWaves][kVectors], s_top[kVectors], s_total[kVectors];
-  // the query vectors' operands while the groups are walked, then the waves' sums
-  constexpr int kSums = kAttendWaves * kVectors * (kSlab + 4) * 4, kQueries = kVectors * D * 2;
-  __shared__ __align__(16) char s_data[kSums > kQueries ? kSums : kQueries];
-  u32x4* const s_q = reinterpret_cast<u32x4*>(s_data);
+  __shared__ __align__(16) char s_data[data_bytes(D, NT)];
+  static_assert(kSlab % 16 == 0);
+  u32x4* const s_q = reinterpret_cast<u32x4*>(s_data + ring_bytes(D));
   float(*const s_o)[kVectors][kSlab + 4] = reinterpret_cast<float(*)[kVectors][kSlab + 4]>(s_data);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
+  KA_LDS char* const key_ring = (KA_LDS char*)s_data + wave * (2 * kCacheGroup * D);
+  KA_LDS char* const value_ring = key_ring + kCacheGroup * D;
   const int heads = p.c.kv_heads, b = p.c.block_log2;
   const int h = blockIdx.y % heads, vector0 = (blockIdx.y / heads) * kVectors;
 
@@ -163,7 +174,6 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
         for (int t = 0; t < D / 16; ++t) o[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
 
-      u32x4 kr[kLoads], vr[kLoads];
       const int32_t* const table = p.r.table + (int64_t)i * p.r.table_stride;
       const int lane_offset = col * 64 + quad * 16;
       int ids = 0;
@@ -177,37 +187,39 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
         k_scales = sc.x;
         v_scales = sc.y;
       };
-      auto offset = [&](int g, int k) {
-        const int id = max(__builtin_amdgcn_readlane(ids, k), 0);
-        return ((((int64_t)id * heads + h) << b) + (int64_t)(g & ((1 << (b - 5)) - 1)) * kCacheGroup) * D;
-      };
-      auto load_keys = [&](int g, int k) {
-        const uint8_t* const src = p.c.keys + offset(g, k);
+      // one group's codes into the wave's ring, 16 bytes a lane and KiB; zeros for a block that is not of the pool
+      auto copy = [&](const uint8_t* from, KA_LDS char* to, int g, int k) {
+        const int id = __builtin_amdgcn_readlane(ids, k);
+        const int64_t head = (int64_t)max(id, 0) * heads + h;
+        const uint8_t* const src = from + ((head << b) + (int64_t)(g & ((1 << (b - 5)) - 1)) * kCacheGroup) * D;
+        const __amdgpu_buffer_rsrc_t r =
+            __builtin_amdgcn_make_buffer_rsrc((void*)src, (short)0, id >= 0 ? kCacheGroup * D : 0, kBufferFlags);
 #pragma unroll
-        for (int t = 0; t < kLoads; ++t) kr[t] = *reinterpret_cast<const u32x4*>(src + t * 1024 + lane_offset);
+        for (int t = 0; t < kLoads; ++t)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (KA_LDS void*)(to + t * 1024), 16, lane_offset, t * 1024, 0, 0);
       };
-      auto load_values = [&](int g, int k) {
-        const uint8_t* const src = p.c.values + offset(g, k);
-#pragma unroll
-        for (int t = 0; t < kLoads; ++t) vr[t] = *reinterpret_cast<const u32x4*>(src + t * 1024 + lane_offset);
+      auto tile = [&](const KA_LDS char* ring, int t) {
+        return *reinterpret_cast<const KA_LDS u32x4*>(ring + t * 1024 + lane * 16);
       };
+      // the copies of all but the last `later` KiB have arrived / the reads of the ring are done
+      auto arrived = [&](bool later) {
+        if (later) wait_vmcnt<kLoads>(); else wait_vmcnt<0>();
+        asm volatile("" ::: "memory");
+      };
+      auto read_out = [&]() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
 
       int k = 0;
       if (g0 + wave < g1) {
         look_up(g0 + wave);
-        load_keys(g0 + wave, 0);
-        load_values(g0 + wave, 0);
+        copy(p.c.keys, key_ring, g0 + wave, 0);
+        copy(p.c.values, value_ring, g0 + wave, 0);
       }
       __syncthreads();
       for (int g = g0 + wave; g < g1; g += kAttendWaves) {
-        const bool known = __builtin_amdgcn_readlane(ids, k) >= 0;
         const float k_scale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(k_scales), k));
         const float v_scale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v_scales), k));
         const int next = g + kAttendWaves;
-        if (!known) {
-#pragma unroll
-          for (int t = 0; t < kLoads; ++t) kr[t] = vr[t] = u32x4{0, 0, 0, 0};
-        }
+        arrived(true);
         f32x4 st[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) st[n][0] = st[n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -218,33 +230,36 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
           for (int n = 0; n < NT; ++n) q[n] = __builtin_bit_cast(bf16x8, s_q[(c * NT + n) * 64 + lane]);
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            const u32x4& w = kr[t * kChunks + (c >> 1)];
+            const u32x4 w = tile(key_ring, t * kChunks + (c >> 1));
             const bf16x8 a = operand(w[2 * (c & 1)], w[2 * (c & 1) + 1], k_scale);
 #pragma unroll
             for (int n = 0; n < NT; ++n) st[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q[n], st[n][t], 0, 0, 0);
           }
         }
+        read_out();
         if (++k == 64 && next < g1) {
           look_up(next);
           k = 0;
         }
-        if (next < g1) load_keys(next, k);
+        if (next < g1) copy(p.c.keys, key_ring, next, k);
 
         const int key0 = g * kCacheGroup;
         const bool masked = key0 < full_lo || key0 + kCacheGroup - 1 > full_hi;
-        bf16x8 weight[NT][2], is_seen[NT];
+        bf16x8 weight[NT][2];
+        unsigned is_seen[NT];  // one bit of each of the lane's eight keys
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float x[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = st[n][e >> 2][e & 3] * p.scale;
+          is_seen[n] = 0;
           if (masked) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const int key = key0 + (e >> 2) * 16 + quad * 4 + (e & 3);
               const bool sees = key >= lo[n] && key <= hi[n];
               x[e] = sees ? x[e] : -INFINITY;
-              is_seen[n][e] = sees ? (__bf16)1.f : (__bf16)0.f;
+              is_seen[n] |= sees ? 1u << e : 0u;
             }
           }
           float best = x[0];
@@ -273,45 +288,60 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
           sum[n] += add;
         }
 
+        arrived(next < g1);
         bool nan = false;
         if (masked) {
           unsigned any = 0;
 #pragma unroll
-          for (int t = 0; t < kLoads; ++t)
+          for (int t = 0; t < kLoads; ++t) {
+            const u32x4 w = tile(value_ring, t);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) any |= nan_codes(vr[t][e]);
+            for (int e = 0; e < 4; ++e) any |= nan_codes(w[e]);
+          }
           nan = __any(any != 0);
         }
         if (nan) {  // a NaN reaches the vectors that see its token, and no others (zero times NaN would be NaN)
 #pragma unroll
-          for (int t = 0; t < kLoads; ++t)
+          for (int t = 0; t < kLoads; ++t) {
+            u32x4 w = tile(value_ring, t);
+            u32x4 f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              f[e] = nan_codes(w[e]);
+              w[e] &= ~((f[e] >> 7) * 255u);
+            }
 #pragma unroll
             for (int d = 0; d < 2; ++d) {
-              const unsigned f0 = nan_codes(vr[t][2 * d]), f1 = nan_codes(vr[t][2 * d + 1]);
-              const bf16x8 marks = operand(f0 >> 1, f1 >> 1, 1.f);  // 2.0 where NaN
+              const bf16x8 marks = operand(f[2 * d] >> 1, f[2 * d + 1] >> 1, 1.f);  // 2.0 where NaN
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
+                bf16x8 sees;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sees[e] = is_seen[n] >> e & 1 ? (__bf16)1.f : (__bf16)0.f;
                 const f32x4 count =
-                    __builtin_amdgcn_mfma_f32_16x16x32_bf16(marks, is_seen[n], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                    __builtin_amdgcn_mfma_f32_16x16x32_bf16(marks, sees, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[n][2 * t + d][e] += count[e] > 0.f ? NAN : 0.f;
               }
-              vr[t][2 * d] &= ~((f0 >> 7) * 255u);
-              vr[t][2 * d + 1] &= ~((f1 >> 7) * 255u);
             }
+            *reinterpret_cast<KA_LDS u32x4*>(value_ring + t * 1024 + lane * 16) = w;
+          }
         }
 #pragma unroll
-        for (int t = 0; t < kLoads; ++t)
+        for (int t = 0; t < kLoads; ++t) {
+          const u32x4 w = tile(value_ring, t);
 #pragma unroll
           for (int d = 0; d < 2; ++d) {
-            const bf16x8 a = operand(vr[t][2 * d], vr[t][2 * d + 1], v_scale);
+            const bf16x8 a = operand(w[2 * d], w[2 * d + 1], v_scale);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               o[n][2 * t + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, weight[n][0], o[n][2 * t + d], 0, 0, 0);
               o[n][2 * t + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, weight[n][1], o[n][2 * t + d], 0, 0, 0);
             }
           }
-        if (next < g1) load_values(next, k);
+        }
+        read_out();
+        if (next < g1) copy(p.c.values, value_ring, next, k);
       }
 
       // join the waves
