@@ -86,7 +86,7 @@ struct AttendParams {
 // The split path's launch for these sizes: `vectors` query vectors (position x head of the group) per workgroup, `tiles`
 // workgroups for a key/value head's max_q * group vectors, `parts` shares of the keys.
 struct AttendShape {
-  int vectors, tiles, parts;
+  int vectors, used, tiles, parts;  // used: the most of them that any workgroup has
   int64_t units_bytes, bytes;  // of the workspace: the units, then the partials
 };
 AttendShape attend_shape(const CacheRef& c, int32_t n_seq, int32_t group, int32_t max_q);

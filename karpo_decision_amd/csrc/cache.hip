@@ -18,18 +18,6 @@ struct Request {
   int tokens, count, held, need, touched;  // held, need: blocks; touched: blocks that get tokens
 };
 
-__device__ __forceinline__ Request request_of(const ReserveParams& p, int i) {
-  Request r;
-  r.tokens = p.lengths[i];
-  r.count = p.counts[i];
-  const int64_t after = (int64_t)r.tokens + r.count;
-  const int b = p.block_log2, round = (1 << b) - 1;
-  r.held = (int)(((int64_t)r.tokens + round) >> b);
-  r.need = (int)((after + round) >> b) - r.held;
-  r.touched = r.count > 0 ? (int)((after - 1) >> b) - (r.tokens >> b) + 1 : 0;
-  return r;
-}
-
 // One launch: every workgroup adds up all requests by itself (a few hundred loads that L2 holds) and then writes the rows
 // of its own range, so nothing waits on another workgroup. A new block's first token, and a request's first new token, write
 // the block's entries; which block a token's is follows from the sums alone. Bound by the launch and one round of dependent
@@ -37,41 +25,49 @@ __device__ __forceinline__ Request request_of(const ReserveParams& p, int i) {
 __global__ __launch_bounds__(kReserveThreads) void reserve_kernel(const ReserveParams p) {
   __shared__ int s_first[kReserveThreads + 1], s_need[kReserveThreads], s_write[kReserveThreads],
       s_tokens[kReserveThreads];
-  __shared__ int s_part[kReserveThreads / 64][3];
-  __shared__ int64_t s_sum[kReserveThreads / 64][2];
+  __shared__ int s_part[kReserveThreads / 64][4];
   const int tid = threadIdx.x;
   const int b = p.block_log2, block = 1 << b;
 
-  // all requests: are they in range, how many rows and blocks do they take
-  int64_t sums[2] = {0, 0};
   const int free_count = *p.free_count;
-  bool bad = free_count < 0 || free_count > p.free_capacity;
-  for (int i = tid; i < p.n_seq; i += kReserveThreads) {
-    const int tokens = p.lengths[i], count = p.counts[i];
-    if (tokens < 0 || count < 0 || (int64_t)tokens + count > p.most) {
-      bad = true;
-    } else {
-      const Request r = request_of(p, i);
-      sums[0] += count;
-      sums[1] += r.need;
+  const bool bad_list = free_count < 0 || free_count > p.free_capacity;
+  // request i and whether it is out of range (then it counts as none)
+  auto take = [&](int i, bool* bad) {
+    Request r = {0, 0, 0, 0, 0};
+    if (i >= p.n_seq) return r;
+    r.tokens = p.lengths[i];
+    r.count = p.counts[i];
+    if (r.tokens < 0 || r.count < 0 || (int64_t)r.tokens + r.count > p.most || r.count > p.rows) {
+      *bad = true;
+      r.tokens = r.count = 0;
     }
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    sums[0] += __shfl_xor(sums[0], o);
-    sums[1] += __shfl_xor(sums[1], o);
-  }
-  if ((tid & 63) == 0) {
-    s_sum[tid >> 6][0] = sums[0];
-    s_sum[tid >> 6][1] = sums[1];
+    const int after = r.tokens + r.count, round = block - 1;
+    r.held = (r.tokens + round) >> b;
+    r.need = ((after + round) >> b) - r.held;
+    r.touched = r.count > 0 ? ((after - 1) >> b) - (r.tokens >> b) + 1 : 0;
+    return r;
+  };
+  // Of a chunk of requests: the sums before each (rows, blocks taken, blocks written) and over all of them. The fourth, of
+  // counts / 2,048, tells a sum of rows that 32 bits do not hold: where it is within `rows` / 2,048, they do.
+  Request r;
+  bool bad = bad_list;
+  int v[4], all[4];
+  auto scan = [&](int c0) {
+    r = take(c0 + tid, &bad);
+    v[0] = r.count;
+    v[1] = r.need;
+    v[2] = r.touched;
+    v[3] = r.count >> 11;
+    block_scan<kReserveThreads, 4>(v, all, s_part);
+  };
+  int64_t total = 0, need = 0;
+  for (int c0 = 0; c0 < p.n_seq; c0 += kReserveThreads) {
+    if (c0 > 0) __syncthreads();
+    scan(c0);
+    total += all[3] > p.rows >> 11 ? (int64_t)p.rows + 1 : (int64_t)(unsigned)all[0];
+    need += all[1];
   }
   bad = __syncthreads_or(bad);
-  int64_t total = 0, need = 0;
-#pragma unroll
-  for (int w = 0; w < kReserveThreads / 64; ++w) {
-    total += s_sum[w][0];
-    need += s_sum[w][1];
-  }
   const int status = bad || total > p.rows ? KARPO_CACHE_BAD_LENGTHS : need > free_count ? KARPO_CACHE_NO_BLOCKS : 0;
 
   const int r0 = (int)ka_min64((int64_t)blockIdx.x * p.per, p.rows);
@@ -79,10 +75,8 @@ __global__ __launch_bounds__(kReserveThreads) void reserve_kernel(const ReserveP
   int carry[3] = {0, 0, 0};  // rows, blocks taken, writes before the chunk's requests
   for (int c0 = 0; c0 < p.n_seq; c0 += kReserveThreads) {
     const int i = c0 + tid, m = min(kReserveThreads, p.n_seq - c0);
-    Request r = {0, 0, 0, 0, 0};
-    if (i < p.n_seq && status == 0) r = request_of(p, i);
-    int v[3] = {r.count, r.need, r.touched}, all[3];
-    block_scan<kReserveThreads, 3>(v, all, s_part);
+    if (p.n_seq > kReserveThreads) scan(c0);  // (one chunk's sums are there)
+    if (status != 0) r.count = v[0] = v[1] = v[2] = all[0] = all[1] = all[2] = 0;
     if (tid < m) {
       s_first[tid] = carry[0] + v[0];
       s_need[tid] = carry[1] + v[1];
@@ -309,7 +303,6 @@ __global__ __launch_bounds__(64 * kReadWaves) void read_kernel(const ReadParams 
   constexpr int kThreads = 64 * kReadWaves;
   __shared__ int s_group[kThreads + 1], s_row[kThreads], s_start[kThreads], s_tokens[kThreads];
   __shared__ int s_part[kReadWaves][2];
-  __shared__ int64_t s_sum[kReadWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int h = blockIdx.y >> 1, heads = p.c.kv_heads, d = p.c.head_dim, b = p.c.block_log2;
   const bool value = blockIdx.y & 1;
@@ -328,31 +321,30 @@ __global__ __launch_bounds__(64 * kReadWaves) void read_kernel(const ReadParams 
       }
     }
   };
+  // Of a chunk of requests: groups of 32 rows, and the last group's missing rows, before each and over all.
+  int start = 0, tokens = 0, v[2], all[2];
+  auto scan = [&](int c0) {
+    start = tokens = 0;
+    if (c0 + tid < p.r.n_seq) range(c0 + tid, &start, &tokens);
+    v[0] = (tokens - start + kCacheGroup - 1) / kCacheGroup;
+    v[1] = tokens - start - v[0] * kCacheGroup;
+    block_scan<kThreads, 2>(v, all, s_part);
+  };
   int64_t groups = 0;
-  for (int i = tid; i < p.r.n_seq; i += kThreads) {
-    int start, tokens;
-    range(i, &start, &tokens);
-    groups += (tokens - start + kCacheGroup - 1) / kCacheGroup;
+  for (int c0 = 0; c0 < p.r.n_seq; c0 += kThreads) {
+    if (c0 > 0) __syncthreads();
+    scan(c0);
+    groups += all[0];
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) groups += __shfl_xor(groups, o);
-  if (lane == 0) s_sum[wave] = groups;
-  __syncthreads();
-  groups = 0;
-#pragma unroll
-  for (int w = 0; w < kReadWaves; ++w) groups += s_sum[w];
   const int64_t g0 = groups * blockIdx.x / gridDim.x, g1 = groups * (blockIdx.x + 1) / gridDim.x;
 
   int64_t carry_groups = 0, carry_rows = 0;
   for (int c0 = 0; c0 < p.r.n_seq; c0 += kThreads) {
     const int i = c0 + tid, m = min(kThreads, p.r.n_seq - c0);
-    int start = 0, tokens = 0;
-    if (i < p.r.n_seq) range(i, &start, &tokens);
-    int v[2] = {(tokens - start + kCacheGroup - 1) / kCacheGroup, 0}, all[2];
-    // (rows as groups of 32 and the last group's tokens: sums of up to 256 requests stay in 32 bits)
-    const int rest = tokens - start - v[0] * kCacheGroup;  // 0 or negative
-    v[1] = rest;
-    block_scan<kThreads, 2>(v, all, s_part);
+    if (p.r.n_seq > kThreads) {
+      __syncthreads();
+      scan(c0);  // (one chunk's sums are there)
+    }
     const int64_t row = carry_rows + (int64_t)v[0] * kCacheGroup + v[1];
     if (tid < m) {
       s_group[tid] = v[0];

@@ -71,6 +71,8 @@ __device__ __forceinline__ bf16x8 operand(unsigned a, unsigned b, float scale) {
   return __builtin_bit_cast(bf16x8, bf16_of_8(a, b, scale));
 }
 
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // Which of a word's four codes are NaN, as 0x80 in their bytes.
 __device__ __forceinline__ unsigned nan_codes(unsigned w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
@@ -88,7 +90,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
   constexpr int kVectors = 16 * NT;
   __shared__ int s_unit[kAttendThreads + 1];
   __shared__ int s_part[kAttendWaves][1];
-  __shared__ int64_t s_sum[kAttendWaves];
+  __shared__ Seen s_seen;
   __shared__ float s_m[kAttendWaves][kVectors], s_l[kAttendWaves][kVectors], s_top[kVectors], s_total[kVectors];
   __shared__ __align__(16) char s_data[data_bytes(D, NT)];
   static_assert(kSlab % 16 == 0);
@@ -101,15 +103,21 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
   const int heads = p.c.kv_heads, b = p.c.block_log2;
   const int h = blockIdx.y % heads, vector0 = (blockIdx.y / heads) * kVectors;
 
+  // a chunk of requests, one a thread: their units, summed up to each and over all of them
+  Seen own;
+  int v[1], all[1];
+  auto scan = [&](int c0) {
+    own = Seen{0, 0, 0, 0, 0, 0};
+    if (c0 + tid < p.r.n_seq) own = seen_of(p, c0 + tid);
+    v[0] = own.units;
+    block_scan<kAttendThreads, 1>(v, all, s_part);
+  };
   int64_t total = 0;
-  for (int i = tid; i < p.r.n_seq; i += kAttendThreads) total += seen_of(p, i).units;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
-  if (lane == 0) s_sum[wave] = total;
-  __syncthreads();
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kAttendWaves; ++w) total += s_sum[w];
+  for (int c0 = 0; c0 < p.r.n_seq; c0 += kAttendThreads) {
+    if (c0 > 0) __syncthreads();
+    scan(c0);
+    total += all[0];
+  }
   const bool writes_units = blockIdx.x == 0 && blockIdx.y == 0;
   const int64_t parts = parts_of(total, p.parts);
   if (total == 0 || (int64_t)blockIdx.x >= parts) {
@@ -121,8 +129,10 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
   int64_t carry = 0;
   for (int c0 = 0; c0 < p.r.n_seq && (writes_units || carry < u1); c0 += kAttendThreads) {
     const int m = min(kAttendThreads, p.r.n_seq - c0);
-    int v[1] = {tid < m ? seen_of(p, c0 + tid).units : 0}, all[1];
-    block_scan<kAttendThreads, 1>(v, all, s_part);
+    if (p.r.n_seq > kAttendThreads) {
+      __syncthreads();
+      scan(c0);  // (one chunk's sums are there)
+    }
     if (tid < m) {
       s_unit[tid] = v[0];
       if (writes_units) p.units[c0 + tid] = carry + v[0];
@@ -130,17 +140,24 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
     if (tid == 0) s_unit[m] = all[0];
     __syncthreads();
     const int64_t from = u0 > carry ? u0 : carry, to = u1 < carry + all[0] ? u1 : carry + all[0];
+    int j = from < to ? last_at_most(s_unit, m, (int)(from - carry)) : 0;
     for (int64_t at = from; at < to;) {
-      const int j = __builtin_amdgcn_readfirstlane(last_at_most(s_unit, m, (int)(at - carry)));
-      const int i = c0 + j;
-      const int64_t begin = carry + s_unit[j], end = carry + s_unit[j + 1];
+      while (carry + s_unit[j + 1] <= at) ++j;
+      if (tid == j) s_seen = own;
+      __syncthreads();
+      const Seen s = {uniform(s_seen.tokens), uniform(s_seen.row),   uniform(s_seen.queries),
+                      uniform(s_seen.first),  uniform(s_seen.groups), uniform(s_seen.units)};
+      const int i = c0 + uniform(j);
+      const int64_t begin = carry + uniform(s_unit[j]), end = begin + s.units;
       const int64_t stop = to < end ? to : end;
-      const Seen s = seen_of(p, i);
       const int g0 = s.first + (int)(at - begin);
       const int g1 = s.groups > 0 ? s.first + (int)(stop - begin) : g0;
       at = stop;
       const int vectors = (int)min<int64_t>((int64_t)s.queries * p.group - vector0, kVectors);
-      if (vectors <= 0) continue;
+      if (vectors <= 0) {
+        __syncthreads();  // s_seen is read
+        continue;
+      }
 
       // the query vectors' operands (entry (2 c + k) * NT + n, one lane's 16 bytes after the other), and the keys that each
       // vector sees: lo .. hi
@@ -406,71 +423,61 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
   if (writes_units && tid == 0) p.units[p.r.n_seq] = total;
 }
 
-// Joins a request's shares: O = sum of 2^(m_w - M) O_w over sum of 2^(m_w - M) l_w, in the shares' order. Requests that one
-// workgroup took whole are done already. The shares' factors first, 64 at a time by the lanes of a wave, so that the sums'
-// loads wait on nothing but the memory.
+// Joins a request's shares: O = sum of 2^(m_w - M) O_w over sum of 2^(m_w - M) l_w. Requests that one workgroup took whole
+// are done already. A workgroup takes 64 elements of one vector: 16 threads of four elements each, and 16 such rows that
+// walk every sixteenth share with a running maximum, so that up to 16 shares cost one round of loads; the rows are joined
+// through LDS, all in an order that the sizes alone set.
 template <int D>
 __global__ __launch_bounds__(256) void join_kernel(const AttendParams p, int vectors_per) {
-  constexpr int kRow = D / 4, kAtOnce = 256 / kRow < 4 ? 256 / kRow : 4;  // vectors of a workgroup
-  __shared__ float s_f[kAtOnce][64];
-  __shared__ float s_l[kAtOnce], s_back[kAtOnce];
+  constexpr int kSlabs = D / 64;
+  __shared__ float s_m[16], s_l[16];
+  __shared__ f32x4 s_x[16][16];
   const int i = blockIdx.x, heads = p.c.kv_heads;
   const int64_t total = p.units[p.r.n_seq], begin = p.units[i], end = p.units[i + 1];
+  const Seen s = seen_of(p, i);
   if (total == 0 || begin == end) return;
   const int64_t parts = parts_of(total, p.parts);
   const int first = (int)part_of(begin, total, parts), last = (int)part_of(end - 1, total, parts);
   if (first == last) return;
-  const Seen s = seen_of(p, i);
   const int h = blockIdx.y % heads, vector0 = (blockIdx.y / heads) * vectors_per;
-  const int c0 = blockIdx.z * kAtOnce;
-  const int vectors = (int)min<int64_t>((int64_t)s.queries * p.group - vector0, vectors_per);
-  if (c0 >= vectors) return;
+  const int c = blockIdx.z / kSlabs, vec = vector0 + c;
+  if (vec >= (int64_t)s.queries * p.group) return;
   const int64_t size = (int64_t)vectors_per * (D + 2);
   const float* const base = p.partial + (int64_t)blockIdx.y * p.parts * 2 * size;
-  auto share = [&](int w) { return base + (2 * (int64_t)w + (begin <= total * w / parts ? 0 : 1)) * size; };
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int mine = tid / kRow, c = c0 + mine, d = (tid % kRow) * 4;
-  const bool active = mine < kAtOnce && c < vectors;
-  float up = -INFINITY, l = 0.f;  // of vector c0 + wave, in every lane of its wave
+  const int tid = threadIdx.x, row = tid >> 4, lane = tid & 15, d = (blockIdx.z % kSlabs) * 64 + lane * 4;
+  float up = -INFINITY, l = 0.f;
   f32x4 x = {0.f, 0.f, 0.f, 0.f};
-  for (int w0 = first; w0 <= last; w0 += 64) {
-    if (wave < kAtOnce && c0 + wave < vectors) {
-      const int w = w0 + lane;
-      float m = -INFINITY, lw = 0.f;
-      if (w <= last) {
-        const float* const part = share(w) + vectors_per * D + c0 + wave;
-        m = part[0];
-        lw = part[vectors_per];
-      }
-      float next = __builtin_elementwise_maximum(up, m);
-      next = column_max(next);
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) next = __builtin_elementwise_maximum(next, __shfl_xor(next, o));
-      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - next);
-      const float back = up == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(up - next);
-      float add = column_sum(lw * f);
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) add += __shfl_xor(add, o);
-      l = l * back + add;
-      up = next;
-      s_f[wave][lane] = f;
-      if (lane == 0) {
-        s_l[wave] = l;
-        s_back[wave] = back;
-      }
-    }
-    __syncthreads();
-    if (active) {
-      x *= s_back[mine];
-      const int n = min(64, last - w0 + 1);
-#pragma unroll 8
-      for (int w = 0; w < n; ++w) x += *reinterpret_cast<const f32x4*>(share(w0 + w) + c * D + d) * s_f[mine][w];
-    }
-    __syncthreads();
+#pragma unroll 2
+  for (int w = first + row; w <= last; w += 16) {
+    const float* const part = base + (2 * (int64_t)w + (begin <= total * w / parts ? 0 : 1)) * size;
+    const float m = part[vectors_per * D + c], lw = part[vectors_per * D + vectors_per + c];
+    const f32x4 xw = *reinterpret_cast<const f32x4*>(part + c * D + d);
+    const float next = __builtin_elementwise_maximum(up, m);
+    const float fo = up == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(up - next);
+    const float fw = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - next);
+    x = x * fo + xw * fw;
+    l = l * fo + lw * fw;
+    up = next;
   }
-  if (!active) return;
-  l = s_l[mine];
-  const int vec = vector0 + c, pos = vec / p.group, head = h * p.group + vec - pos * p.group;
+  s_x[row][lane] = x;
+  if (lane == 0) {
+    s_m[row] = up;
+    s_l[row] = l;
+  }
+  __syncthreads();
+  if (row > 0) return;
+  up = s_m[0];
+#pragma unroll
+  for (int w = 1; w < 16; ++w) up = __builtin_elementwise_maximum(up, s_m[w]);
+  x = f32x4{0.f, 0.f, 0.f, 0.f};
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    const float f = s_m[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[w] - up);
+    x += s_x[w][lane] * f;
+    l += s_l[w] * f;
+  }
+  const int pos = vec / p.group, head = h * p.group + vec - pos * p.group;
   if (l == 0.f) x = f32x4{0.f, 0.f, 0.f, 0.f}; else x = x * (1.f / l);
   *reinterpret_cast<u32x2*>(p.o + (s.row + (int64_t)pos) * p.so_t + head * p.so_h + d) =
       u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
@@ -480,7 +487,7 @@ template <int D, int NT>
 void launch(const AttendParams& p, const AttendShape& s, hipStream_t stream) {
   const unsigned y = (unsigned)(p.c.kv_heads * s.tiles);
   attend_kernel<D, NT><<<dim3((unsigned)s.parts, y), dim3(kAttendThreads), 0, stream>>>(p);
-  const unsigned z = (unsigned)(16 * NT / (D == 512 ? 2 : 4));
+  const unsigned z = (unsigned)(s.used * (D / 64));
   join_kernel<D><<<dim3((unsigned)p.r.n_seq, y, z), dim3(256), 0, stream>>>(p, 16 * NT);
 }
 
@@ -498,6 +505,7 @@ AttendShape attend_shape(const CacheRef& c, int32_t n_seq, int32_t group, int32_
   const int64_t y = (int64_t)c.kv_heads * s.tiles;
   const int64_t parts = 256 * at_once / y;
   s.parts = parts < 1 ? 1 : (int)parts;
+  s.used = (int)(vectors < s.vectors ? vectors : s.vectors);
   s.units_bytes = (8 * ((int64_t)n_seq + 1) + 255) / 256 * 256;
   s.bytes = s.units_bytes + y * s.parts * 2 * s.vectors * (c.head_dim + 2) * 4;
   return s;

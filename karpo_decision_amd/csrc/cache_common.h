@@ -24,6 +24,17 @@ __device__ __forceinline__ u32x4 bf16_of_8(unsigned a, unsigned b, float scale) 
                bf16_pair(b, scale, true)};
 }
 
+// The sum over the wave's lanes up to this one, in registers (six additions across lanes, no LDS).
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // from the lane 1, 2, 4, 8 before, within 16
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lane 15 of the row of 16 before, into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31, into rows 2 and 3
+  return x;
+}
+
 // v: the sum over the workgroup's threads before this one, of N values; all: over all of them. `part` is free again after
 // the caller's next barrier.
 template <int THREADS, int N>
@@ -33,11 +44,7 @@ __device__ __forceinline__ void block_scan(int (&v)[N], int (&all)[N], int (*par
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     own[k] = v[k];
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int t = __shfl_up(v[k], o);
-      if (lane >= o) v[k] += t;
-    }
+    v[k] = wave_scan(v[k]);
     if (lane == 63) part[wave][k] = v[k];
   }
   __syncthreads();

@@ -95,35 +95,43 @@ def create(blocks: int, kv_heads: int, head_dim: int, block_size: int = 64,
 def _cache_args(cache: Cache, device: torch.device) -> _lib.KarpoCache:
     keys, values, scales, block = cache
     shape, fp8 = keys.shape, torch.float8_e4m3fn
-    if (block not in BLOCK_SIZES or len(shape) != 3 or shape[2] % block or shape[2] // block not in HEAD_DIMS
-            or values.shape != shape or tuple(scales.shape) != (shape[0], shape[1], 2) or shape[0] < 1 or shape[1] < 1):
-        raise ValueError(f"a cache has keys and values (blocks, kv heads, block_size * head_dim) and scales (blocks, kv "
-                         f"heads, 2), block_size 32, 64 or 128 and head_dim 64, 128, 256 or 512, not {tuple(shape)}, "
-                         f"{tuple(values.shape)}, {tuple(scales.shape)} and {block}")
+    if len(shape) == 3 and block in BLOCK_SIZES:  # all is well: one pass
+        blocks, heads, size = shape
+        head_dim = size // block
+        if (head_dim in HEAD_DIMS and size == head_dim * block and values.shape == shape and blocks > 0 and heads > 0
+                and scales.shape == (blocks, heads, 2) and keys.dtype is fp8 and values.dtype is fp8
+                and scales.dtype is torch.float32 and keys.is_contiguous() and values.is_contiguous()
+                and scales.is_contiguous() and keys.device == device and values.device == device
+                and scales.device == device):
+            return _lib.KarpoCache(keys.data_ptr(), values.data_ptr(), scales.data_ptr(), blocks, heads, head_dim, block)
+    # the refusal's message
     if keys.dtype != fp8 or values.dtype != fp8 or scales.dtype != torch.float32:
         raise ValueError(f"a cache has float8_e4m3fn keys and values and float32 scales, not {keys.dtype}, "
                          f"{values.dtype} and {scales.dtype}")
-    if not (keys.is_contiguous() and values.is_contiguous() and scales.is_contiguous()):
-        raise ValueError("a cache's tensors must be contiguous")
     if keys.device != device or values.device != device or scales.device != device:
-        raise ValueError(f"the cache is on {keys.device}, the other tensors on {device}")
-    return _lib.KarpoCache(keys.data_ptr(), values.data_ptr(), scales.data_ptr(), shape[0], shape[1],
-                           shape[2] // block, block)
+        raise ValueError(f"the cache is on {keys.device}, {values.device} and {scales.device}, the other tensors on {device}")
+    raise ValueError(f"a cache has contiguous keys and values (blocks, kv heads, block_size * head_dim) and scales (blocks, "
+                     f"kv heads, 2), block_size 32, 64 or 128 and head_dim 64, 128, 256 or 512, not {tuple(shape)}, "
+                     f"{tuple(values.shape)}, {tuple(scales.shape)} and {block}")
 
 
-def _check_ints(device: torch.device, **tensors: Tensor) -> None:
+def _check_ints(device: torch.device, tensors: dict[str, Tensor]) -> None:
     for name, t in tensors.items():
-        if t.dtype != torch.int32 or t.device != device or t.dim() != 1 or not t.is_contiguous():
+        if t.dtype is not torch.int32 or t.dim() != 1 or t.device != device or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous 1-D int32 tensor on {device}")
 
 
-def _check_table(table: Tensor, lengths: Tensor, device: torch.device) -> None:
-    if (table.dim() != 2 or table.dtype != torch.int32 or table.device != device or table.shape[1] < 1
-            or table.stride(1) != 1 or (table.stride(0) < table.shape[1] and table.shape[0] > 1)):
-        raise ValueError(f"table must be a (requests, blocks) int32 tensor with contiguous rows on {device}")
-    _check_ints(device, lengths=lengths)
-    if lengths.numel() != table.shape[0]:
-        raise ValueError(f"the table has {table.shape[0]} requests, lengths {lengths.numel()}")
+def _check_table(table: Tensor, lengths: Tensor, device: torch.device) -> tuple[int, int, int]:
+    """(requests, blocks of a row, row stride) of a block table that fits ``lengths``."""
+    if table.dim() != 2 or table.dtype is not torch.int32 or table.device != device:
+        raise ValueError(f"table must be a (requests, blocks) int32 tensor on {device}")
+    (n, width), (stride, inner) = table.shape, table.stride()
+    if width < 1 or inner != 1 or (stride < width and n > 1):
+        raise ValueError(f"table must have contiguous rows of at least one block, not {(n, width)} with strides "
+                         f"{(stride, inner)}")
+    if lengths.numel() != n:
+        raise ValueError(f"the table has {n} requests, lengths {lengths.numel()}")
+    return n, width, stride if stride >= width else width
 
 
 def _on_gpu(what: str, t: Tensor) -> None:
@@ -144,9 +152,9 @@ def reserve(table: Tensor, lengths: Tensor, counts: Tensor, free: Tensor, free_c
     the counts' sum and is the packed new tokens' row count. The inputs but the table are left as they are: the free
     list goes on with ``free_left``, the requests with ``Step.lengths``."""
     device = table.device
-    _check_table(table, lengths, device)
-    _check_ints(device, counts=counts, free=free, free_count=free_count)
-    n, rows = table.shape[0], int(rows)
+    n, width, stride = _check_table(table, lengths, device)
+    _check_ints(device, {"lengths": lengths, "counts": counts, "free": free, "free_count": free_count})
+    rows, capacity = int(rows), free.numel()
     if counts.numel() != n or free_count.numel() != 1:
         raise ValueError(f"counts must hold {n} requests and free_count one number, not {counts.numel()} and "
                          f"{free_count.numel()}")
@@ -154,23 +162,25 @@ def reserve(table: Tensor, lengths: Tensor, counts: Tensor, free: Tensor, free_c
         raise ValueError(f"rows must be non-negative and block_size 32, 64 or 128, not {rows} and {block_size}")
     _on_gpu("reserve", table)
     lib = _lib.load()
-    capacity = lib.karpo_cache_writes_capacity(rows, n, block_size)
-    # one allocation for the step, 16-byte aligned writes first
-    buffer = torch.empty(4 * capacity + 3 * rows + 2 * n + 3, dtype=torch.int32, device=device)
-    writes, slots, positions, q_cu, new, left, status = buffer.split((4 * capacity, 2 * rows, rows, n + 1, n, 1, 1))
+    jobs = lib.karpo_cache_writes_capacity(rows, n, block_size)
+    # one allocation for the step: writes (16-byte aligned) and slots first
+    buffer = torch.empty(4 * jobs + 3 * rows + 2 * n + 3, dtype=torch.int32, device=device)
+    writes, slots, positions, q_cu, new, left, status = torch.split_with_sizes(
+        buffer, (4 * jobs, 2 * rows, rows, n + 1, n, 1, 1))
     at = buffer.data_ptr()
-    at_slots = at + 16 * capacity
-    at_positions = at_slots + 8 * rows
-    at_q = at_positions + 4 * rows
-    at_new = at_q + 4 * n + 4
-    at_left = at_new + 4 * n
+    slots_at = at + 16 * jobs
+    positions_at = slots_at + 8 * rows
+    q_at = positions_at + 4 * rows
+    new_at = q_at + 4 * n + 4
+    left_at = new_at + 4 * n
     args = _lib.KarpoCacheReserveArgs(
-        table.data_ptr(), max(table.stride(0), table.shape[1]), table.shape[1], n, lengths.data_ptr(),
-        counts.data_ptr(), free.data_ptr(), free_count.data_ptr(), free.numel(), block_size, rows, at_q, at_new,
-        at_slots, at_positions, at, capacity, at_left, at_left + 4)
-    with _on_device(device.index):
-        _lib.check(lib.karpo_cache_reserve(ctypes.byref(args), _current_stream(device.index)), "reserve")
-    return Step(q_cu, new, slots.view(torch.int64), positions, writes.view(capacity, 4), left, status)
+        table.data_ptr(), stride, width, n, lengths.data_ptr(), counts.data_ptr(), free.data_ptr(),
+        free_count.data_ptr(), capacity, block_size, rows, q_at, new_at, slots_at, positions_at, at, jobs, left_at,
+        left_at + 4)
+    index = device.index
+    with _on_device(index):
+        _lib.check(lib.karpo_cache_reserve(ctypes.byref(args), _current_stream(index)), "reserve")
+    return Step(q_cu, new, slots.view(torch.int64), positions, writes.view(jobs, 4), left, status)
 
 
 def append(cache: Cache, key: Tensor, value: Tensor, writes: Tensor) -> None:
@@ -181,11 +191,11 @@ def append(cache: Cache, key: Tensor, value: Tensor, writes: Tensor) -> None:
     _no_grad("append", key, value)
     device, bf16 = key.device, torch.bfloat16
     c = _cache_args(cache, device)
-    sk, sv = key.stride(), value.stride()
-    if (key.dim() != 3 or key.shape != value.shape or key.shape[1] != c.kv_heads or key.shape[2] != c.head_dim
-            or key.dtype != bf16 or value.dtype != bf16 or value.device != device):
+    shape, sk, sv = key.shape, key.stride(), value.stride()
+    if (len(shape) != 3 or value.shape != shape or shape[1] != c.kv_heads or shape[2] != c.head_dim
+            or key.dtype is not bf16 or value.dtype is not bf16 or value.device != device):
         raise ValueError(f"append takes bf16 keys and values (rows, {c.kv_heads}, {c.head_dim}) on {device}, not "
-                         f"{tuple(key.shape)} {key.dtype} and {tuple(value.shape)} {value.dtype} on {value.device}")
+                         f"{tuple(shape)} {key.dtype} and {tuple(value.shape)} {value.dtype} on {value.device}")
     if sk[2] != 1 or sv[2] != 1 or (sk[0] | sk[1] | sv[0] | sv[1]) & 7:
         raise ValueError(f"keys and values need a contiguous head_dim and row/head strides that are multiples of 8 "
                          f"(strides {sk}, {sv})")
@@ -193,7 +203,7 @@ def append(cache: Cache, key: Tensor, value: Tensor, writes: Tensor) -> None:
             or not writes.is_contiguous()):
         raise ValueError(f"writes must be a contiguous (n, 4) int32 tensor on {device}")
     _on_gpu("append", key)
-    args = _lib.KarpoCacheAppendArgs(c, key.data_ptr(), value.data_ptr(), sk[0], sk[1], sv[0], sv[1], key.shape[0],
+    args = _lib.KarpoCacheAppendArgs(c, key.data_ptr(), value.data_ptr(), sk[0], sk[1], sv[0], sv[1], shape[0],
                                      writes.data_ptr(), writes.shape[0])
     with _on_device(device.index):
         _lib.check(_lib.load().karpo_cache_append(ctypes.byref(args), _current_stream(device.index)), "append")
@@ -205,15 +215,16 @@ def read(cache: Cache, table: Tensor, lengths: Tensor, rows: int) -> tuple[Tenso
     takes. ``rows`` bounds the lengths' sum; rows behind the last request are not written."""
     device = table.device
     c = _cache_args(cache, device)
-    _check_table(table, lengths, device)
-    n, rows = table.shape[0], int(rows)
+    n, width, stride = _check_table(table, lengths, device)
+    _check_ints(device, {"lengths": lengths})
+    rows = int(rows)
     if rows < 0:
         raise ValueError(f"rows must be non-negative, not {rows}")
     _on_gpu("read", table)
     key, value = (torch.empty((rows, c.kv_heads, c.head_dim), dtype=torch.bfloat16, device=device) for _ in range(2))
     k_cu = torch.empty(n + 1, dtype=torch.int32, device=device)
-    args = _lib.KarpoCacheReadArgs(c, table.data_ptr(), max(table.stride(0), table.shape[1]), table.shape[1], n,
-                                   lengths.data_ptr(), key.data_ptr(), value.data_ptr(), rows, k_cu.data_ptr())
+    args = _lib.KarpoCacheReadArgs(c, table.data_ptr(), stride, width, n, lengths.data_ptr(), key.data_ptr(),
+                                   value.data_ptr(), rows, k_cu.data_ptr())
     with _on_device(device.index):
         _lib.check(_lib.load().karpo_cache_read(ctypes.byref(args), _current_stream(device.index)), "read")
     return key, value, k_cu
@@ -231,38 +242,40 @@ def attend(query: Tensor, cache: Cache, table: Tensor, q_cu: Tensor, lengths: Te
     _no_grad("attend", query)
     device = query.device
     c = _cache_args(cache, device)
-    if (query.dim() != 3 or query.dtype != torch.bfloat16 or query.shape[2] != c.head_dim
-            or query.shape[1] % c.kv_heads or query.shape[1] < 1):
+    shape = query.shape
+    if (len(shape) != 3 or query.dtype is not torch.bfloat16 or shape[2] != c.head_dim or shape[1] < 1
+            or shape[1] % c.kv_heads):
         raise ValueError(f"attend takes a (rows, heads, {c.head_dim}) bf16 query, its heads a multiple of {c.kv_heads}, "
-                         f"not {tuple(query.shape)} {query.dtype}")
+                         f"not {tuple(shape)} {query.dtype}")
     sq = query.stride()
     if sq[2] != 1 or (sq[0] | sq[1]) & 7:
         raise ValueError(f"query needs a contiguous head_dim and row/head strides that are multiples of 8 (strides {sq})")
-    _check_table(table, lengths, device)
-    _check_ints(device, q_cu=q_cu)
-    n = table.shape[0]
+    n, width, stride = _check_table(table, lengths, device)
+    _check_ints(device, {"lengths": lengths, "q_cu": q_cu})
     if q_cu.numel() != n + 1:
         raise ValueError(f"the table has {n} requests, q_cu {q_cu.numel()} bounds")
     if max_q < 0 or window < -1:
         raise ValueError(f"max_q must be non-negative and window at least -1, not {max_q} and {window}")
     if total_keys is None:
-        total_keys = min(n * table.shape[1] * cache.block_size, _MOST)
+        total_keys = min(n * width * c.block_size, _MOST)
     elif not 0 <= total_keys <= _MOST:
         raise ValueError(f"total_keys must lie in 0 .. {_MOST}, not {total_keys}")
     _on_gpu("attend", query)
     lib = _lib.load()
-    out = torch.empty(query.shape, dtype=query.dtype, device=device)
-    if query.shape[0] == 0:
+    out = torch.empty(shape, dtype=torch.bfloat16, device=device)
+    if shape[0] == 0:
         return out
     so = out.stride()
     args = _lib.KarpoCacheAttendArgs(
         c, query.data_ptr(), out.data_ptr(), sq[0], sq[1], so[0], so[1], q_cu.data_ptr(), lengths.data_ptr(),
-        table.data_ptr(), max(table.stride(0), table.shape[1]), table.shape[1], n, query.shape[1], int(max_q),
-        query.shape[0], int(total_keys), float(scale), int(window), 0 if causal else -1)
-    need = ctypes.c_size_t()
-    _lib.check(lib.karpo_cache_attend_workspace_bytes(ctypes.byref(args), ctypes.byref(need)), "attend")
-    with _on_device(device.index):
+        table.data_ptr(), stride, width, n, shape[1], int(max_q), shape[0], int(total_keys), float(scale), int(window),
+        0 if causal else -1)
+    pointer, need = ctypes.byref(args), ctypes.c_size_t()
+    _lib.check(lib.karpo_cache_attend_workspace_bytes(pointer, ctypes.byref(need)), "attend")
+    index = device.index
+    with _on_device(index):
+        # from the caching allocator (stream-ordered reuse)
         workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
         args.workspace, args.workspace_bytes = workspace.data_ptr(), need.value
-        _lib.check(lib.karpo_cache_attend(ctypes.byref(args), _current_stream(device.index)), "attend")
+        _lib.check(lib.karpo_cache_attend(pointer, _current_stream(index)), "attend")
     return out

@@ -512,3 +512,30 @@ def test_a_captured_step_replays(gpu, counts):
                 s["lengths"].copy_(r.lengths)
                 s["left"].copy_(r.free_left)
             assert torch.equal(bits(captured.values), bits(eager.values))
+
+
+@pytest.mark.parametrize("head_dim,heads,kv_heads,counts", [(64, 4, 2, [6, 1]), (128, 8, 2, [9, 2]), (512, 8, 1, [2, 1]),
+                                                            (256, 16, 8, [16, 3])])
+def test_nan_reaches_the_queries_that_see_it_and_no_others(gpu, head_dim, heads, kv_heads, counts):
+    """NaN in one element of a new token's value, and in another's key: earlier queries of the same call do not see them."""
+    lengths, block = [70, 33], 32
+    cache, want, table, query, q_cu, scale = _attend_case(gpu, head_dim, heads, kv_heads, block, lengths, counts)
+    raw_k, raw_v = cache.keys.view(torch.uint8), cache.values.view(torch.uint8)
+    at = lengths[0] - 1  # the first request's last token: its value's element 5, head 0
+    raw_v[table[0][at // block], 0, oracle.value_offset(at % block, 5, head_dim)] = 0x7f
+    at = lengths[1] - 1  # the second's: its key, head 0
+    raw_k[table[1][at // block], 0, oracle.key_offset(at % block, 7, head_dim)] = 0xff
+    with torch.inference_mode():
+        out = kv_cache.attend(query.to(gpu), cache, ints(table, gpu), ints(q_cu, gpu), ints(lengths, gpu), max(counts),
+                              scale, total_keys=sum(lengths))
+    group = heads // kv_heads
+    nan = torch.isnan(out.cpu())
+    expected = torch.zeros_like(nan)
+    expected[q_cu[1] - 1, :group, 5] = True
+    expected[q_cu[2] - 1, :group] = True
+    assert torch.equal(nan, expected)
+    for i, n in enumerate(lengths):
+        key, value = (x.nan_to_num(0.0) for x in want.rows(table[i], 0, n))
+        rows = slice(q_cu[i], q_cu[i + 1] - 1)  # the queries before the last, which see neither
+        if rows.start < rows.stop:
+            _close(out[rows], query[rows], key[:n - 1], value[:n - 1], scale)
