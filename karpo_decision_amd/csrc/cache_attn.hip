@@ -88,10 +88,10 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
   constexpr int kChunks = D / 64;      // 64-element chunks of a key tile
   constexpr int kSlab = slab_of(D, NT);
   constexpr int kVectors = 16 * NT;
-  __shared__ int s_unit[kAttendThreads + 1];
   __shared__ int s_part[kAttendWaves][1];
   __shared__ Seen s_seen;
-  __shared__ float s_m[kAttendWaves][kVectors], s_l[kAttendWaves][kVectors], s_top[kVectors], s_total[kVectors];
+  __shared__ int s_at[2];
+  __shared__ float s_m[kAttendWaves][kVectors], s_l[kAttendWaves][kVectors];
   __shared__ __align__(16) char s_data[data_bytes(D, NT)];
   static_assert(kSlab % 16 == 0);
   u32x4* const s_q = reinterpret_cast<u32x4*>(s_data + ring_bytes(D));
@@ -128,27 +128,24 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
 
   int64_t carry = 0;
   for (int c0 = 0; c0 < p.r.n_seq && (writes_units || carry < u1); c0 += kAttendThreads) {
-    const int m = min(kAttendThreads, p.r.n_seq - c0);
     if (p.r.n_seq > kAttendThreads) {
       __syncthreads();
       scan(c0);  // (one chunk's sums are there)
     }
-    if (tid < m) {
-      s_unit[tid] = v[0];
-      if (writes_units) p.units[c0 + tid] = carry + v[0];
-    }
-    if (tid == 0) s_unit[m] = all[0];
-    __syncthreads();
+    if (writes_units && c0 + tid < p.r.n_seq) p.units[c0 + tid] = carry + v[0];
     const int64_t from = u0 > carry ? u0 : carry, to = u1 < carry + all[0] ? u1 : carry + all[0];
-    int j = from < to ? last_at_most(s_unit, m, (int)(from - carry)) : 0;
     for (int64_t at = from; at < to;) {
-      while (carry + s_unit[j + 1] <= at) ++j;
-      if (tid == j) s_seen = own;
+      const int unit = (int)(at - carry);
+      if (unit >= v[0] && unit - v[0] < own.units) {  // this thread's request
+        s_seen = own;
+        s_at[0] = tid;
+        s_at[1] = v[0];
+      }
       __syncthreads();
       const Seen s = {uniform(s_seen.tokens), uniform(s_seen.row),   uniform(s_seen.queries),
                       uniform(s_seen.first),  uniform(s_seen.groups), uniform(s_seen.units)};
-      const int i = c0 + uniform(j);
-      const int64_t begin = carry + uniform(s_unit[j]), end = begin + s.units;
+      const int i = c0 + uniform(s_at[0]);
+      const int64_t begin = carry + uniform(s_at[1]), end = begin + s.units;
       const int64_t stop = to < end ? to : end;
       const int g0 = s.first + (int)(at - begin);
       const int g1 = s.groups > 0 ? s.first + (int)(stop - begin) : g0;
@@ -161,6 +158,8 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
 
       // the query vectors' operands (entry (2 c + k) * NT + n, one lane's 16 bytes after the other), and the keys that each
       // vector sees: lo .. hi
+      constexpr int kMine = (2 * kChunks + kAttendWaves - 1) / kAttendWaves;  // of the entries of a tile, this wave's
+      u32x4 q_mine[NT][kMine];
       int lo[NT], hi[NT];
       const int shift = s.tokens - s.queries;
 #pragma unroll
@@ -170,8 +169,12 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
         const int pos = valid ? vec / p.group : 0;
         const uint16_t* const src =
             p.q + (s.row + (int64_t)pos) * p.sq_t + (int64_t)(h * p.group + (valid ? vec - pos * p.group : 0)) * p.sq_h;
-        for (int c = wave; c < 2 * kChunks; c += kAttendWaves)
-          s_q[(c * NT + n) * 64 + lane] = *reinterpret_cast<const u32x4*>(src + (c >> 1) * 64 + quad * 16 + (c & 1) * 8);
+#pragma unroll
+        for (int c = 0; c < kMine; ++c) {
+          const int e = wave + c * kAttendWaves;
+          if (2 * kChunks >= kAttendWaves || e < 2 * kChunks)
+            q_mine[n][c] = *reinterpret_cast<const u32x4*>(src + (e >> 1) * 64 + quad * 16 + (e & 1) * 8);
+        }
         lo[n] = p.left < 0 ? 0 : pos + shift - p.left;
         hi[n] = p.right < 0 ? s.tokens - 1 : (int)min<int64_t>((int64_t)pos + shift + p.right, s.tokens - 1);
       }
@@ -231,7 +234,15 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
         copy(p.c.keys, key_ring, g0 + wave, 0);
         copy(p.c.values, value_ring, g0 + wave, 0);
       }
-      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < kMine; ++c) {
+          const int e = wave + c * kAttendWaves;
+          if (2 * kChunks >= kAttendWaves || e < 2 * kChunks) s_q[(e * NT + n) * 64 + lane] = q_mine[n][c];
+        }
+      // (a barrier that leaves the copies in flight)
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
       for (int g = g0 + wave; g < g1; g += kAttendWaves) {
         const float k_scale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(k_scales), k));
         const float v_scale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v_scales), k));
@@ -371,28 +382,32 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
         }
       }
       __syncthreads();
-      if (tid < kVectors) {
-        float up = s_m[0][tid], l = 0.f;
+      // vector c's maximum and sum over the waves
+      auto top_of = [&](int c) {
+        float up = s_m[0][c];
 #pragma unroll
-        for (int w = 1; w < kAttendWaves; ++w) up = __builtin_elementwise_maximum(up, s_m[w][tid]);
+        for (int w = 1; w < kAttendWaves; ++w) up = __builtin_elementwise_maximum(up, s_m[w][c]);
+        return up;
+      };
+      auto total_of = [&](int c, float up) {
+        float l = 0.f;
 #pragma unroll
         for (int w = 0; w < kAttendWaves; ++w)
-          l += s_m[w][tid] == -INFINITY ? 0.f : s_l[w][tid] * __builtin_amdgcn_exp2f(s_m[w][tid] - up);
-        s_top[tid] = up;
-        s_total[tid] = l;
-      }
-      __syncthreads();
+          l += s_m[w][c] == -INFINITY ? 0.f : s_l[w][c] * __builtin_amdgcn_exp2f(s_m[w][c] - up);
+        return l;
+      };
       const bool whole = begin >= u0 && end <= u1;
       float* const part =
           p.partial + (((int64_t)blockIdx.y * p.parts + blockIdx.x) * 2 + (begin <= u0 ? 0 : 1)) * (kVectors * (D + 2));
       if (!whole && tid < vectors) {
-        part[kVectors * D + tid] = s_top[tid];
-        part[kVectors * D + kVectors + tid] = s_total[tid];
+        const float up = top_of(tid);
+        part[kVectors * D + tid] = up;
+        part[kVectors * D + kVectors + tid] = total_of(tid, up);
       }
       for (int d0 = 0; d0 < D; d0 += kSlab) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const float f = top[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top[n] - s_top[16 * n + col]);
+          const float f = top[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top[n] - top_of(16 * n + col));
 #pragma unroll
           for (int t = 0; t < D / 16; ++t)
             if (t * 16 >= d0 && t * 16 < d0 + kSlab)
@@ -405,7 +420,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
 #pragma unroll
           for (int w = 1; w < kAttendWaves; ++w) x += *reinterpret_cast<const f32x4*>(&s_o[w][c][d]);
           if (whole) {
-            const float l = s_total[c];
+            const float l = total_of(c, top_of(c));
             const int vec = vector0 + c, pos = vec / p.group, head = h * p.group + vec - pos * p.group;
             if (l == 0.f) x = f32x4{0.f, 0.f, 0.f, 0.f}; else x = x * (1.f / l);
             *reinterpret_cast<u32x2*>(p.o + (s.row + (int64_t)pos) * p.so_t + head * p.so_h + d0 + d) =
@@ -418,18 +433,17 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
       }
     }
     carry += all[0];
-    __syncthreads();  // the next chunk's requests take s_unit
   }
   if (writes_units && tid == 0) p.units[p.r.n_seq] = total;
 }
 
-// Joins a request's shares: O = sum of 2^(m_w - M) O_w over sum of 2^(m_w - M) l_w. Requests that one workgroup took whole
-// are done already. A workgroup takes 64 elements of one vector: 16 threads of four elements each, and 16 such rows that
-// walk every sixteenth share with a running maximum, so that up to 16 shares cost one round of loads; the rows are joined
-// through LDS, all in an order that the sizes alone set.
+// Joins a request's shares: O = sum of 2^(m_w - M) O_w over sum of 2^(m_w - M) l_w, in an order that the sizes alone set.
+// Requests that one workgroup took whole are done already. Up to kFew shares: a thread walks them for four elements of a
+// vector. More: 64 elements of a vector by 16 threads of four and 16 rows, each row with every sixteenth share (so that
+// up to 16 cost one round of loads), and the rows joined through LDS.
 template <int D>
 __global__ __launch_bounds__(256) void join_kernel(const AttendParams p, int vectors_per) {
-  constexpr int kSlabs = D / 64;
+  constexpr int kSlabs = D / 64, kFew = 4;
   __shared__ float s_m[16], s_l[16];
   __shared__ f32x4 s_x[16][16];
   const int i = blockIdx.x, heads = p.c.kv_heads;
@@ -440,54 +454,80 @@ __global__ __launch_bounds__(256) void join_kernel(const AttendParams p, int vec
   const int first = (int)part_of(begin, total, parts), last = (int)part_of(end - 1, total, parts);
   if (first == last) return;
   const int h = blockIdx.y % heads, vector0 = (blockIdx.y / heads) * vectors_per;
-  const int c = blockIdx.z / kSlabs, vec = vector0 + c;
-  if (vec >= (int64_t)s.queries * p.group) return;
+  const int vectors = (int)min<int64_t>((int64_t)s.queries * p.group - vector0, vectors_per);
   const int64_t size = (int64_t)vectors_per * (D + 2);
   const float* const base = p.partial + (int64_t)blockIdx.y * p.parts * 2 * size;
-  const int tid = threadIdx.x, row = tid >> 4, lane = tid & 15, d = (blockIdx.z % kSlabs) * 64 + lane * 4;
-  float up = -INFINITY, l = 0.f;
-  f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-  for (int w = first + row; w <= last; w += 16) {
-    const float* const part = base + (2 * (int64_t)w + (begin <= total * w / parts ? 0 : 1)) * size;
+  const int tid = threadIdx.x;
+
+  struct Sum {
+    float up, l;
+    f32x4 x;
+  };
+  auto add = [&](Sum& a, int w, int c, int d) {
+    // (only the first share can have begun before the request: then the request is its workgroup's second)
+    const float* const part = base + (2 * (int64_t)w + (w == first && begin > total * w / parts ? 1 : 0)) * size;
     const float m = part[vectors_per * D + c], lw = part[vectors_per * D + vectors_per + c];
     const f32x4 xw = *reinterpret_cast<const f32x4*>(part + c * D + d);
-    const float next = __builtin_elementwise_maximum(up, m);
-    const float fo = up == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(up - next);
+    const float next = __builtin_elementwise_maximum(a.up, m);
+    const float fo = a.up == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(a.up - next);
     const float fw = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - next);
-    x = x * fo + xw * fw;
-    l = l * fo + lw * fw;
-    up = next;
-  }
-  s_x[row][lane] = x;
-  if (lane == 0) {
-    s_m[row] = up;
-    s_l[row] = l;
-  }
-  __syncthreads();
-  if (row > 0) return;
-  up = s_m[0];
+    a.x = a.x * fo + xw * fw;
+    a.l = a.l * fo + lw * fw;
+    a.up = next;
+  };
+  auto store = [&](const Sum& a, int c, int d) {
+    const int vec = vector0 + c, pos = vec / p.group, head = h * p.group + vec - pos * p.group;
+    const f32x4 x = a.l == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : a.x * (1.f / a.l);
+    *reinterpret_cast<u32x2*>(p.o + (s.row + (int64_t)pos) * p.so_t + head * p.so_h + d) =
+        u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+  };
+  const Sum none = {-INFINITY, 0.f, f32x4{0.f, 0.f, 0.f, 0.f}};
+  if (last - first < kFew) {
+    for (int e = blockIdx.z * 256 + tid; e < vectors * (D / 4); e += gridDim.z * 256) {
+      const int c = e / (D / 4), d = (e % (D / 4)) * 4;
+      Sum a = none;
 #pragma unroll
-  for (int w = 1; w < 16; ++w) up = __builtin_elementwise_maximum(up, s_m[w]);
-  x = f32x4{0.f, 0.f, 0.f, 0.f};
-  l = 0.f;
-#pragma unroll
-  for (int w = 0; w < 16; ++w) {
-    const float f = s_m[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[w] - up);
-    x += s_x[w][lane] * f;
-    l += s_l[w] * f;
+      for (int w = 0; w < kFew; ++w)
+        if (first + w <= last) add(a, first + w, c, d);
+      store(a, c, d);
+    }
+    return;
   }
-  const int pos = vec / p.group, head = h * p.group + vec - pos * p.group;
-  if (l == 0.f) x = f32x4{0.f, 0.f, 0.f, 0.f}; else x = x * (1.f / l);
-  *reinterpret_cast<u32x2*>(p.o + (s.row + (int64_t)pos) * p.so_t + head * p.so_h + d) =
-      u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+  const int row = tid >> 4, lane = tid & 15;
+  for (int e = blockIdx.z; e < vectors * kSlabs; e += gridDim.z) {
+    const int c = e / kSlabs, d = (e % kSlabs) * 64 + lane * 4;
+    Sum a = none;
+#pragma unroll 2
+    for (int w = first + row; w <= last; w += 16) add(a, w, c, d);
+    __syncthreads();  // the last round's sums are read
+    s_x[row][lane] = a.x;
+    if (lane == 0) {
+      s_m[row] = a.up;
+      s_l[row] = a.l;
+    }
+    __syncthreads();
+    if (row == 0) {
+      a = none;
+#pragma unroll
+      for (int w = 0; w < 16; ++w) a.up = __builtin_elementwise_maximum(a.up, s_m[w]);
+#pragma unroll
+      for (int w = 0; w < 16; ++w) {
+        const float f = s_m[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[w] - a.up);
+        a.x += s_x[w][lane] * f;
+        a.l += s_l[w] * f;
+      }
+      store(a, c, d);
+    }
+  }
 }
 
 template <int D, int NT>
 void launch(const AttendParams& p, const AttendShape& s, hipStream_t stream) {
   const unsigned y = (unsigned)(p.c.kv_heads * s.tiles);
   attend_kernel<D, NT><<<dim3((unsigned)s.parts, y), dim3(kAttendThreads), 0, stream>>>(p);
-  const unsigned z = (unsigned)(s.used * (D / 64));
+  // a workgroup for 64 elements of each vector, or as many as fill the GPU several times over
+  const int64_t pairs = (int64_t)p.r.n_seq * y, most = (2048 + pairs - 1) / pairs, items = (int64_t)s.used * (D / 64);
+  const unsigned z = (unsigned)(items < most ? items : most);
   join_kernel<D><<<dim3((unsigned)p.r.n_seq, y, z), dim3(256), 0, stream>>>(p, 16 * NT);
 }
 
