@@ -127,29 +127,51 @@ __global__ __launch_bounds__(kReserveThreads) void reserve_kernel(const ReserveP
 
 // ---- append
 
-// Four fp32 as e4m3 (nearest, ties to even), past the range at its end, NaN as NaN.
-__device__ __forceinline__ float in_range(float x) {
-  return x != x ? x : __builtin_amdgcn_fmed3f(x, -448.f, 448.f);
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+
+// Two packed bf16 over `scale` (a power of two) as e4m3 codes (nearest, ties to even; NaN as NaN; no more than 448 in
+// magnitude), into the lower or the upper half of `into`. Equal to torch's conversion for every bf16 value.
+template <bool UP>
+__device__ __forceinline__ unsigned codes2(unsigned into, unsigned x, float scale) {
+  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(
+                                          __builtin_bit_cast(s16x2, into), __builtin_bit_cast(bf16x2, x), scale, UP));
 }
-__device__ __forceinline__ unsigned codes4(float a, float b, float c, float d) {
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(in_range(a), in_range(b), 0, false);
-  return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(in_range(c), in_range(d), w, true);
+__device__ __forceinline__ unsigned codes4(unsigned x, unsigned y, float scale) {
+  return codes2<true>(codes2<false>(0, x, scale), y, scale);
 }
-// Four codes times `f` (a power of two, at most 1), rounded again.
-__device__ __forceinline__ unsigned codes_again(unsigned w, float f) {
-  const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
-  return codes4(lo[0] * f, lo[1] * f, hi[0] * f, hi[1] * f);
+// Four codes under the scale `old` as codes under `scale`: rounded again (the elements are bf16 values).
+__device__ __forceinline__ unsigned codes_again(unsigned w, float old, float scale) {
+  return codes4(bf16_pair(w, old, false), bf16_pair(w, old, true), scale);
 }
 
-// Largest finite magnitude of packed bf16 pairs, as bits.
-__device__ __forceinline__ unsigned largest_of(unsigned best, const u32x4& x) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const unsigned lo = x[i] & 0x7fffu, hi = (x[i] >> 16) & 0x7fffu;
-    best = max(best, lo < 0x7f80u ? lo : 0u);
-    best = max(best, hi < 0x7f80u ? hi : 0u);
-  }
-  return best;
+// The larger magnitudes, as bits, of packed bf16 pairs.
+__device__ __forceinline__ unsigned larger(unsigned best, unsigned x) {
+  return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, best),
+                                                                __builtin_bit_cast(u16x2, x & 0x7fff7fffu)));
+}
+// A pair with its infinities and NaN as zeros / with what is past `most` (a magnitude's bits) at `most`, NaN as it is.
+__device__ __forceinline__ unsigned finite(unsigned x) {
+  return ((x & 0x7fff) < 0x7f80 ? x & 0xffffu : 0u) | ((x >> 16 & 0x7fff) < 0x7f80 ? x & 0xffff0000u : 0u);
+}
+__device__ __forceinline__ unsigned at_most(unsigned x, unsigned most) {
+  auto one = [&](unsigned v) {
+    const unsigned m = v & 0x7fff;
+    return m > most && m <= 0x7f80 ? (v & 0x8000) | most : v;
+  };
+  return one(x & 0xffff) | one(x >> 16) << 16;
+}
+// The maximum over the wave's lanes, in every lane.
+__device__ __forceinline__ unsigned wave_largest(unsigned x) {
+  // (as wave_scan: each lane's maximum with the lanes before it; lane 63 has all)
+  auto step = [&](unsigned y) { x = max(x, y); };
+  step(__builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));
+  step(__builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+  step(__builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+  step(__builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+  step(__builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+  step(__builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(x, 63);
 }
 
 // The least e with m <= 448 * 2^e for the bf16 magnitude with these bits (448 = 1.75 * 2^8).
@@ -179,6 +201,8 @@ __global__ __launch_bounds__(64 * WAVES) void append_kernel(const AppendParams p
   uint8_t* const out = (value ? p.c.values : p.c.keys) + (head << p.c.block_log2) * d;
   const int64_t stride = value ? p.sv_t : p.sk_t;
   const uint16_t* const in = (value ? p.v + h * p.sv_h : p.k + h * p.sk_h) + ((int64_t)row - first) * stride;
+  float* const scale_of = p.c.scales + 2 * head + (value ? 1 : 0);
+  const unsigned old_bits = first > 0 ? __float_as_uint(*scale_of) : 0;
 
   // keys: tile i of the wave, token lane / 4 of its 16, elements (lane % 4) * 16 of its 64: x[2 i], x[2 i + 1]
   const int k_chunks = d >> 6;
@@ -187,72 +211,88 @@ __global__ __launch_bounds__(64 * WAVES) void append_kernel(const AppendParams p
   const int v_tile = wave * TILES + (lane >> 3), v_chunks = d >> 5;
   const int v_token = (v_tile / v_chunks) * 32 + (lane & 3) * 4, v_elem = (v_tile % v_chunks) * 32 + ((lane >> 2) & 1) * 8;
   const bool v_lane = (lane >> 3) < TILES;
-  const u32x4 zero = {0, 0, 0, 0};
+  constexpr int kKeys = TILES * 2;
   u32x4 x[16];
-  unsigned best = 0;
+  auto load = [&](int i, const uint16_t* src, bool mine) {
+    x[i] = mine ? *reinterpret_cast<const u32x4*>(src) : u32x4{0, 0, 0, 0};
+  };
+  unsigned pair = 0;
   if (!value) {
 #pragma unroll
     for (int i = 0; i < TILES; ++i) {
       const int tile = wave * TILES + i, token = (tile / k_chunks) * 16 + (lane >> 2);
       const uint16_t* const src = in + token * stride + (tile % k_chunks) * 64 + (lane & 3) * 16;
       const bool mine = token >= first && token < first + count;
-      x[2 * i] = mine ? *reinterpret_cast<const u32x4*>(src) : zero;
-      x[2 * i + 1] = mine ? *reinterpret_cast<const u32x4*>(src + 8) : zero;
+      load(2 * i, src, mine);
+      load(2 * i + 1, src + 8, mine);
     }
 #pragma unroll
-    for (int i = 0; i < TILES * 2; ++i) best = largest_of(best, x[i]);
+    for (int i = kKeys; i < 16; ++i) x[i] = u32x4{0, 0, 0, 0};
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int token = v_token + (j >> 2) * 16 + (j & 3);
       const uint16_t* const src = in + token * stride + v_elem;
       const bool mine = v_lane && token >= first && token < first + count;
-      x[2 * j] = mine ? *reinterpret_cast<const u32x4*>(src) : zero;
-      x[2 * j + 1] = mine ? *reinterpret_cast<const u32x4*>(src + 16) : zero;
+      load(2 * j, src, mine);
+      load(2 * j + 1, src + 16, mine);
     }
-#pragma unroll
-    for (int j = 0; j < 16; ++j) best = largest_of(best, x[j]);
   }
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) best = max(best, (unsigned)__shfl_xor((int)best, o));
-  if constexpr (WAVES > 1) {
-    __shared__ unsigned s_best[WAVES];
-    if (lane == 0) s_best[wave] = best;
-    __syncthreads();
+  for (int i = 0; i < 16; ++i)
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) best = max(best, s_best[w]);
+    for (int j = 0; j < 4; ++j) pair = larger(pair, x[i][j]);
+  auto joined = [&](unsigned both) {  // over the workgroup
+    unsigned best = wave_largest(max(both & 0xffffu, both >> 16));
+    if constexpr (WAVES > 1) {
+      __shared__ unsigned s_best[WAVES];
+      __syncthreads();
+      if (lane == 0) s_best[wave] = best;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) best = max(best, s_best[w]);
+    }
+    return best;
+  };
+  unsigned best = joined(pair);
+  const bool odd = best >= 0x7f80;  // infinities or NaN: the largest of the others
+  if (__builtin_expect(odd, 0)) {
+    pair = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) pair = larger(pair, finite(x[i][j]));
+    best = joined(pair);
   }
-  int e = exponent_of(best);
-  float again = 1.f;  // what the earlier tokens' codes are multiplied by
-  float* const scale = p.c.scales + 2 * head + (value ? 1 : 0);
+  int e = exponent_of(best), old = e;
   if (first > 0) {
-    const int old = min(max((int)((__float_as_uint(*scale) >> 23) & 0xff) - 127, KARPO_CACHE_MIN_EXP), KARPO_CACHE_MAX_EXP);
+    old = min(max((int)((old_bits >> 23) & 0xff) - 127, KARPO_CACHE_MIN_EXP), KARPO_CACHE_MAX_EXP);
     e = max(e, old);
-    again = power_of_two(max(old - e, -126));  // (448 * 2^-126 rounds to zero too)
   }
-  const bool grown = again != 1.f;
-  const float inv = power_of_two(-e);
-  if constexpr (WAVES > 1) __syncthreads();  // every wave has read the old scale
-  if (threadIdx.x == 0) *scale = power_of_two(e);
+  const bool grown = old < e;  // the earlier tokens' codes are rounded again
+  const float scale = power_of_two(e), old_scale = power_of_two(old);
+  if (threadIdx.x == 0) *scale_of = scale;
+  if (__builtin_expect(odd || e == KARPO_CACHE_MAX_EXP, 0)) {
+    const unsigned most = (unsigned)(e + 8 + 127) << 7 | 0x60;  // 448 * 2^e
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[i][j] = at_most(x[i][j], most);
+  }
 
   if (!value) {
 #pragma unroll
     for (int i = 0; i < TILES; ++i) {
       const int tile = wave * TILES + i, token = (tile / k_chunks) * 16 + (lane >> 2);
       u32x4* const dst = reinterpret_cast<u32x4*>(out + tile * 1024 + lane * 16);
-      u32x4 w;
       if (token >= first && token < first + count) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const u32x4& s = x[2 * i + (j >> 1)];
-          const int o = (j & 1) * 4;
-          w[j] = codes4(bf16_at(s, o) * inv, bf16_at(s, o + 1) * inv, bf16_at(s, o + 2) * inv, bf16_at(s, o + 3) * inv);
-        }
-        *dst = w;
+        const u32x4 a = x[2 * i], b = x[2 * i + 1];
+        *dst = u32x4{codes4(a[0], a[1], scale), codes4(a[2], a[3], scale), codes4(b[0], b[1], scale),
+                     codes4(b[2], b[3], scale)};
       } else if (grown && token < first) {
-        w = *dst;
+        u32x4 w = *dst;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = codes_again(w[j], again);
+        for (int j = 0; j < 4; ++j) w[j] = codes_again(w[j], old_scale, scale);
         *dst = w;
       }
     }
@@ -270,22 +310,30 @@ __global__ __launch_bounds__(64 * WAVES) void append_kernel(const AppendParams p
   if (!v_lane || (is_new[0] | is_new[1] | is_old[0] | is_old[1]) == 0) return;
   const bool whole = (is_new[0] & is_new[1]) == 0xffffffffu;
   u32x4* const dst = reinterpret_cast<u32x4*>(out + v_tile * 1024 + ((lane >> 2) & 1) * 512 + (lane & 3) * 16);
+  u32x4 was[8];
+  if (!whole) {
+#pragma unroll
+    for (int s = 0; s < 8; ++s) was[s] = dst[4 * s];
+  }
 #pragma unroll
   for (int s = 0; s < 8; ++s) {
     u32x4 w;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {  // dh = j / 2, t = j % 2
+    for (int j = 0; j < 4; ++j) {  // dh = j / 2, t = j % 2: element s of four tokens
       const int t = j & 1, dh = j >> 1;
-      w[j] = codes4(bf16_at(x[2 * (4 * t) + dh], s) * inv, bf16_at(x[2 * (4 * t + 1) + dh], s) * inv,
-                    bf16_at(x[2 * (4 * t + 2) + dh], s) * inv, bf16_at(x[2 * (4 * t + 3) + dh], s) * inv);
+      auto tokens = [&](int i) {
+        return __builtin_amdgcn_perm(x[2 * (4 * t + i + 1) + dh][s >> 1], x[2 * (4 * t + i) + dh][s >> 1],
+                                     s & 1 ? 0x07060302u : 0x05040100u);
+      };
+      w[j] = codes4(tokens(0), tokens(2), scale);
     }
     if (!whole) {
-      const u32x4 was = dst[4 * s];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const unsigned n = is_new[j & 1], o = is_old[j & 1];
-        const unsigned old = o != 0 ? (codes_again(was[j], again) & o) | (was[j] & ~o) : was[j];
-        w[j] = (w[j] & n) | (old & ~n);
+        unsigned kept = was[s][j];
+        if (grown) kept = (codes_again(kept, old_scale, scale) & o) | (kept & ~o);
+        w[j] = (w[j] & n) | (kept & ~n);
       }
     }
     dst[4 * s] = w;
@@ -296,16 +344,21 @@ __global__ __launch_bounds__(64 * WAVES) void append_kernel(const AppendParams p
 
 constexpr int kReadWaves = 4;
 
-// 32 tokens of one head, keys or values, per wave and turn. A key tile's lane turns 16 codes into 32 bytes of one row; a
-// value tile's holds 8 tokens x 8 elements (four 16-byte loads), which it turns into four elements of each token's row
-// twice. Each workgroup adds up all lengths by itself and takes an equal share of all groups of 32 tokens.
+// A wave takes 32 tokens of one head's keys or values at a time, the heads of a group one after the other, so that the rows
+// that a workgroup writes lie side by side. Keys: 8 codes a lane make 16 bytes of a row, 8 lanes the 128 of a tile's row.
+// Values: the tokens lie innermost, so the codes go through LDS (one tile after the other, 64 bytes between their halves
+// against bank conflicts), out of which a lane takes 4 tokens x 8 elements: 16 bytes of four rows. Each workgroup adds up all
+// lengths by itself and takes an equal share of all groups.
+template <int D>
 __global__ __launch_bounds__(64 * kReadWaves) void read_kernel(const ReadParams p) {
-  constexpr int kThreads = 64 * kReadWaves;
-  __shared__ int s_group[kThreads + 1], s_row[kThreads], s_start[kThreads], s_tokens[kThreads];
+  constexpr int kThreads = 64 * kReadWaves, kTiles = D / 32;
+  constexpr int kAtOnce = kTiles < 4 ? kTiles : 4;  // KiB of codes that a lane's loads have in flight
+  constexpr int kTileBytes = 2 * (512 + 64);
   __shared__ int s_part[kReadWaves][2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int h = blockIdx.y >> 1, heads = p.c.kv_heads, d = p.c.head_dim, b = p.c.block_log2;
-  const bool value = blockIdx.y & 1;
+  __shared__ int s_group[kThreads + 1], s_row[kThreads], s_start[kThreads], s_tokens[kThreads];
+  __shared__ __align__(16) char s_codes[kReadWaves][kAtOnce * kTileBytes];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int heads = p.c.kv_heads, b = p.c.block_log2;
 
   // first and last token of request i that are read
   auto range = [&](int i, int* start, int* tokens) {
@@ -317,7 +370,7 @@ __global__ __launch_bounds__(64 * kReadWaves) void read_kernel(const ReadParams 
         *tokens = 0;
       } else if (p.window_left >= 0) {
         const int64_t s = (int64_t)*tokens - queries - p.window_left;
-        *start = s > 0 ? (int)min<int64_t>(s, *tokens) & ~(kCacheGroup - 1) : 0;
+        *start = s > 0 ? (int)ka_min64(s, *tokens) & ~(kCacheGroup - 1) : 0;
       }
     }
   };
@@ -336,7 +389,10 @@ __global__ __launch_bounds__(64 * kReadWaves) void read_kernel(const ReadParams 
     scan(c0);
     groups += all[0];
   }
-  const int64_t g0 = groups * blockIdx.x / gridDim.x, g1 = groups * (blockIdx.x + 1) / gridDim.x;
+  // units: (group, head, keys or values, kAtOnce tiles of them)
+  constexpr int kPieces = kTiles / kAtOnce;
+  const int sides = 2 * heads * kPieces;
+  const int64_t u0 = groups * sides * blockIdx.x / gridDim.x, u1 = groups * sides * (blockIdx.x + 1) / gridDim.x;
 
   int64_t carry_groups = 0, carry_rows = 0;
   for (int c0 = 0; c0 < p.r.n_seq; c0 += kThreads) {
@@ -353,61 +409,79 @@ __global__ __launch_bounds__(64 * kReadWaves) void read_kernel(const ReadParams 
       s_tokens[tid] = tokens;
     }
     if (tid == 0) s_group[m] = all[0];
-    if (blockIdx.x == 0 && blockIdx.y == 0 && i < p.r.n_seq) p.k_cu[i] = (int)ka_min64(row, INT32_MAX);
+    if (blockIdx.x == 0 && i < p.r.n_seq) p.k_cu[i] = (int)ka_min64(row, INT32_MAX);
     __syncthreads();
-    const int64_t hi = ka_min64(g1, carry_groups + all[0]);
-    for (int64_t g = (g0 > carry_groups ? g0 : carry_groups) + wave; g < hi; g += kReadWaves) {
-      const int u = (int)(g - carry_groups);
-      const int j = last_at_most(s_group, m, u);
-      const int token0 = s_start[j] + (u - s_group[j]) * kCacheGroup;
-      const int64_t out_row = (int64_t)s_row[j] + token0 - s_start[j];
-      const int tokens_left = (int)ka_min64(ka_min64(s_tokens[j] - token0, p.rows - out_row), kCacheGroup);
+    const int64_t from = u0 > carry_groups * sides ? u0 : carry_groups * sides;
+    const int64_t to = ka_min64(u1, (carry_groups + all[0]) * sides);
+    int j = -1, token0 = 0, tokens_left = 0, id = 0;
+    int64_t out_row = 0, group = -1;
+    for (int64_t unit = from + wave; unit < to; unit += kReadWaves) {
+      const int64_t g = unit / sides;
+      const int side = (int)(unit - g * sides), h = side / (2 * kPieces), t0 = (side % kPieces) * kAtOnce;
+      const bool value = (side / kPieces) & 1;
+      if (g != group) {
+        group = g;
+        const int u = (int)(g - carry_groups);
+        j = last_at_most(s_group, m, u);
+        token0 = s_start[j] + (u - s_group[j]) * kCacheGroup;
+        out_row = (int64_t)s_row[j] + token0 - s_start[j];
+        tokens_left = (int)ka_min64(ka_min64(s_tokens[j] - token0, p.rows - out_row), kCacheGroup);
+        id = p.r.table[(int64_t)(c0 + j) * p.r.table_stride + (token0 >> b)];
+      }
       if (tokens_left <= 0) continue;
-      const int id = p.r.table[(int64_t)(c0 + j) * p.r.table_stride + (token0 >> b)];
       const bool known = id >= 0 && id < p.c.blocks;
       const int64_t head = (int64_t)(known ? id : 0) * heads + h;
       const int inside = token0 & ((1 << b) - 1);
-      const uint8_t* const src = (value ? p.c.values : p.c.keys) + (head << b) * d + inside * d;
+      const uint8_t* const src = (value ? p.c.values : p.c.keys) + (head << b) * D + inside * D;
       const float scale = p.c.scales[2 * head + (value ? 1 : 0)];
-      uint16_t* const dst = (value ? p.v : p.k) + (out_row * heads + h) * d;
-      const int64_t step = (int64_t)heads * d;
+      uint16_t* const dst = (value ? p.v : p.k) + (out_row * heads + h) * D;
+      const int64_t step = (int64_t)heads * D;
       if (!value) {
-        const int chunks = d >> 6;
-        for (int t = 0; t < 2 * chunks; ++t) {  // tiles of 16 tokens x 64 elements
-          const int token = (t / chunks) * 16 + (lane >> 2);
-          u32x4 w = *reinterpret_cast<const u32x4*>(src + t * 1024 + lane * 16);
-          if (!known) w = u32x4{0, 0, 0, 0};
-          if (token >= tokens_left) continue;
-          u32x4* const to = reinterpret_cast<u32x4*>(dst + token * step + (t % chunks) * 64 + (lane & 3) * 16);
-          to[0] = bf16_of_8(w[0], w[1], scale);
-          to[1] = bf16_of_8(w[2], w[3], scale);
+        constexpr int kChunks = D / 64;  // tiles of 16 tokens x 64 elements, each in two halves of 8 tokens
+        u32x2 w[2 * kAtOnce];
+#pragma unroll
+        for (int t = 0; t < 2 * kAtOnce; ++t)
+          w[t] = known ? *reinterpret_cast<const u32x2*>(src + (2 * t0 + t) * 512 + lane * 8) : u32x2{0, 0};
+#pragma unroll
+        for (int t = 0; t < 2 * kAtOnce; ++t) {
+          const int tile = t0 + (t >> 1), token = (tile / kChunks) * 16 + (t & 1) * 8 + (lane >> 3);
+          if (token < tokens_left)
+            *reinterpret_cast<u32x4*>(dst + token * step + (tile % kChunks) * 64 + (lane & 7) * 8) =
+                bf16_of_8(w[t][0], w[t][1], scale);
         }
       } else {
-        const int q = lane & 3, part = (lane >> 2) & 3;
-        for (int t = lane >> 4; t < d >> 5; t += 4) {  // tiles of 32 tokens x 32 elements: 16 lanes each
-          u32x4 w[4];
+        // of each two tiles: lane = (dlow half, dh, tile of the two, t, q): elements 16 dh + 8 (dlow half) + 0 .. 7 of the tile
+        const int half = lane & 1, dh = (lane >> 1) & 1, which = (lane >> 2) & 1, t16 = (lane >> 3) & 1, q = lane >> 4;
+        char* const codes = s_codes[wave];
+        u32x4 w[kAtOnce];
 #pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            w[s] = *reinterpret_cast<const u32x4*>(src + t * 1024 + (4 * part + s) * 64 + q * 16);
-            if (!known) w[s] = u32x4{0, 0, 0, 0};
+        for (int t = 0; t < kAtOnce; ++t)
+          w[t] = known ? *reinterpret_cast<const u32x4*>(src + (t0 + t) * 1024 + lane * 16) : u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < kAtOnce; ++t)
+          *reinterpret_cast<u32x4*>(codes + t * kTileBytes + (lane >> 5) * (512 + 64) + (lane & 31) * 16) = w[t];
+#pragma unroll
+        for (int t = 0; t < kAtOnce; t += 2) {
+          const char* const from_codes =
+              codes + (t + which) * kTileBytes + half * (512 + 64) + q * 16 + dh * 8 + t16 * 4;
+          unsigned pair[2][8];  // tokens 0, 1 and 2, 3 of the four, of each element
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const unsigned c = *reinterpret_cast<const unsigned*>(from_codes + e * 64);
+            pair[0][e] = bf16_pair(c, scale, false);
+            pair[1][e] = bf16_pair(c, scale, true);
           }
+          const int token = 16 * t16 + 4 * q;
+          uint16_t* const to_row = dst + token * step + (t0 + t + which) * 32 + dh * 16 + half * 8;
 #pragma unroll
-          for (int dh = 0; dh < 2; ++dh)
-#pragma unroll
-            for (int j2 = 0; j2 < 4; ++j2) {  // two tokens: 16 (j2 / 2) + 4 q + 2 (j2 % 2) + 0, 1
-              const int t2 = j2 >> 1, up = j2 & 1;
-              unsigned pair[4];
-#pragma unroll
-              for (int s = 0; s < 4; ++s) pair[s] = bf16_pair(w[s][2 * dh + t2], scale, up);
-              const int token = 16 * t2 + 4 * q + 2 * up;
-              uint16_t* const to = dst + token * step + t * 32 + dh * 16 + part * 4;
-              if (token < tokens_left)
-                *reinterpret_cast<u32x2*>(to) = u32x2{__builtin_amdgcn_perm(pair[1], pair[0], 0x05040100u),
-                                                      __builtin_amdgcn_perm(pair[3], pair[2], 0x05040100u)};
-              if (token + 1 < tokens_left)
-                *reinterpret_cast<u32x2*>(to + step) = u32x2{__builtin_amdgcn_perm(pair[1], pair[0], 0x07060302u),
-                                                             __builtin_amdgcn_perm(pair[3], pair[2], 0x07060302u)};
-            }
+          for (int e = 0; e < 4; ++e) {
+            const unsigned(&x)[8] = pair[e >> 1];
+            const unsigned pick = e & 1 ? 0x07060302u : 0x05040100u;
+            if (token + e < tokens_left)
+              *reinterpret_cast<u32x4*>(to_row + e * step) =
+                  u32x4{__builtin_amdgcn_perm(x[1], x[0], pick), __builtin_amdgcn_perm(x[3], x[2], pick),
+                        __builtin_amdgcn_perm(x[5], x[4], pick), __builtin_amdgcn_perm(x[7], x[6], pick)};
+          }
         }
       }
     }
@@ -415,7 +489,7 @@ __global__ __launch_bounds__(64 * kReadWaves) void read_kernel(const ReadParams 
     carry_rows += (int64_t)all[0] * kCacheGroup + all[1];
     __syncthreads();
   }
-  if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) p.k_cu[p.r.n_seq] = (int)ka_min64(carry_rows, INT32_MAX);
+  if (blockIdx.x == 0 && tid == 0) p.k_cu[p.r.n_seq] = (int)ka_min64(carry_rows, INT32_MAX);
 }
 
 }  // namespace
@@ -445,12 +519,16 @@ hipError_t launch_cache_append(const AppendParams& p, int64_t n_writes, hipStrea
 }
 
 hipError_t launch_cache_read(const ReadParams& p, hipStream_t stream) {
-  // enough workgroups to fill the GPU several times over, no more than the groups of 32 rows ask for
-  const int64_t sides = 2 * (int64_t)p.c.kv_heads;
+  // enough workgroups to fill the GPU, no more than the groups of 32 rows
   const int64_t groups = p.rows / kCacheGroup + p.r.n_seq;
-  const int64_t wanted = (groups + kReadWaves - 1) / kReadWaves, fill = (256 * 16 + sides - 1) / sides;
-  const int64_t x = ka_min64(wanted < 1 ? 1 : wanted, fill);
-  read_kernel<<<dim3((unsigned)x, (unsigned)sides), dim3(64 * kReadWaves), 0, stream>>>(p);
+  const dim3 grid((unsigned)ka_min64(groups < 1 ? 1 : groups, 256 * 8)), threads(64 * kReadWaves);
+  switch (p.c.head_dim) {
+    case 64: read_kernel<64><<<grid, threads, 0, stream>>>(p); break;
+    case 128: read_kernel<128><<<grid, threads, 0, stream>>>(p); break;
+    case 256: read_kernel<256><<<grid, threads, 0, stream>>>(p); break;
+    case 512: read_kernel<512><<<grid, threads, 0, stream>>>(p); break;
+    default: return hipErrorInvalidValue;
+  }
   return hipGetLastError();
 }
 
