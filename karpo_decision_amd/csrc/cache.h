@@ -64,6 +64,7 @@ struct ReadParams {
   uint16_t* v;
   int64_t rows;
   int32_t* k_cu;
+  int32_t stream;  // the rows are more than the L2 caches hold: stored through them
 };
 hipError_t launch_cache_read(const ReadParams& p, hipStream_t stream);
 
@@ -76,20 +77,27 @@ struct AttendParams {
   const int32_t* q_cu;
   int64_t total_q;
   int32_t group;       // heads / kv_heads
+  float per_group;     // 1 / group
+  int32_t whole;       // a workgroup takes a request whole (nothing to join)
+  // one workgroup's walk reads a request's codes, once: streamed through the caches (48 requests at head size 128 58.8 ->
+  // 52.8 us, 131,072 tokens at 512 105.0 -> 93.6; where several read them, 128 vectors over 32,768 tokens, 80 -> 88)
+  int32_t once;
   int32_t left, right;
   float scale;         // times log2(e)
   int32_t parts;       // workgroups for each of the grid's y
   float* partial;      // [y][parts][2] of (O [vectors][D], m [vectors], l [vectors])
-  int64_t* units;      // [n_seq + 1] groups of 32 tokens before each request
+  int32_t* units;      // [n_seq + 1] groups of 32 tokens before each request
 };
 
 // The split path's launch for these sizes: `vectors` query vectors (position x head of the group) per workgroup, `tiles`
 // workgroups for a key/value head's max_q * group vectors, `parts` shares of the keys.
 struct AttendShape {
   int vectors, used, tiles, parts;  // used: the most of them that any workgroup has
+  bool whole;
   int64_t units_bytes, bytes;  // of the workspace: the units, then the partials
 };
-AttendShape attend_shape(const CacheRef& c, int32_t n_seq, int32_t group, int32_t max_q);
+// `longest`: a bound of a request's tokens.
+AttendShape attend_shape(const CacheRef& c, int32_t n_seq, int32_t group, int32_t max_q, int64_t longest);
 hipError_t launch_cache_attend(const AttendParams& p, const AttendShape& s, hipStream_t stream);
 
 }  // namespace karpo

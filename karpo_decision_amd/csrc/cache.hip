@@ -2,6 +2,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "cache.h"
 #include "cache_common.h"
 #include "karpo_cache.h"
@@ -349,7 +351,7 @@ constexpr int kReadWaves = 4;
 // Values: the tokens lie innermost, so the codes go through LDS (one tile after the other, 64 bytes between their halves
 // against bank conflicts), out of which a lane takes 4 tokens x 8 elements: 16 bytes of four rows. Each workgroup adds up all
 // lengths by itself and takes an equal share of all groups.
-template <int D>
+template <int D, bool STREAM>
 __global__ __launch_bounds__(64 * kReadWaves) void read_kernel(const ReadParams p) {
   constexpr int kThreads = 64 * kReadWaves, kTiles = D / 32;
   constexpr int kAtOnce = kTiles < 4 ? kTiles : 4;  // KiB of codes that a lane's loads have in flight
@@ -383,18 +385,23 @@ __global__ __launch_bounds__(64 * kReadWaves) void read_kernel(const ReadParams 
     v[1] = tokens - start - v[0] * kCacheGroup;
     block_scan<kThreads, 2>(v, all, s_part);
   };
-  int64_t groups = 0;
+  int groups = 0;
   for (int c0 = 0; c0 < p.r.n_seq; c0 += kThreads) {
     if (c0 > 0) __syncthreads();
     scan(c0);
     groups += all[0];
   }
+  auto store = [&](uint16_t* to, const u32x4& x) {
+    if constexpr (STREAM) __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(to)); else *reinterpret_cast<u32x4*>(to) = x;
+  };
   // units: (group, head, keys or values, kAtOnce tiles of them)
   constexpr int kPieces = kTiles / kAtOnce;
   const int sides = 2 * heads * kPieces;
-  const int64_t u0 = groups * sides * blockIdx.x / gridDim.x, u1 = groups * sides * (blockIdx.x + 1) / gridDim.x;
+  const int64_t units = (int64_t)groups * sides;
+  const int64_t u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
 
-  int64_t carry_groups = 0, carry_rows = 0;
+  int carry_groups = 0;
+  int64_t carry_rows = 0;
   for (int c0 = 0; c0 < p.r.n_seq; c0 += kThreads) {
     const int i = c0 + tid, m = min(kThreads, p.r.n_seq - c0);
     if (p.r.n_seq > kThreads) {
@@ -411,18 +418,19 @@ __global__ __launch_bounds__(64 * kReadWaves) void read_kernel(const ReadParams 
     if (tid == 0) s_group[m] = all[0];
     if (blockIdx.x == 0 && i < p.r.n_seq) p.k_cu[i] = (int)ka_min64(row, INT32_MAX);
     __syncthreads();
-    const int64_t from = u0 > carry_groups * sides ? u0 : carry_groups * sides;
-    const int64_t to = ka_min64(u1, (carry_groups + all[0]) * sides);
-    int j = -1, token0 = 0, tokens_left = 0, id = 0;
-    int64_t out_row = 0, group = -1;
-    for (int64_t unit = from + wave; unit < to; unit += kReadWaves) {
-      const int64_t g = unit / sides;
-      const int side = (int)(unit - g * sides), h = side / (2 * kPieces), t0 = (side % kPieces) * kAtOnce;
+    const int64_t chunk0 = (int64_t)carry_groups * sides, from = u0 > chunk0 ? u0 : chunk0;
+    const int64_t to = ka_min64(u1, chunk0 + (int64_t)all[0] * sides);
+    int token0 = 0, tokens_left = 0, id = 0, group = -1;
+    int64_t out_row = 0;
+    int g = (int)(from / sides), side = (int)(from - (int64_t)g * sides) + wave;
+    for (int64_t unit = from + wave; unit < to; unit += kReadWaves, side += kReadWaves) {
+      for (; side >= sides; side -= sides) ++g;
+      const int h = side / (2 * kPieces), t0 = (side % kPieces) * kAtOnce;
       const bool value = (side / kPieces) & 1;
       if (g != group) {
         group = g;
-        const int u = (int)(g - carry_groups);
-        j = last_at_most(s_group, m, u);
+        const int u = g - carry_groups;
+        const int j = last_at_most(s_group, m, u);
         token0 = s_start[j] + (u - s_group[j]) * kCacheGroup;
         out_row = (int64_t)s_row[j] + token0 - s_start[j];
         tokens_left = (int)ka_min64(ka_min64(s_tokens[j] - token0, p.rows - out_row), kCacheGroup);
@@ -446,8 +454,7 @@ __global__ __launch_bounds__(64 * kReadWaves) void read_kernel(const ReadParams 
         for (int t = 0; t < 2 * kAtOnce; ++t) {
           const int tile = t0 + (t >> 1), token = (tile / kChunks) * 16 + (t & 1) * 8 + (lane >> 3);
           if (token < tokens_left)
-            *reinterpret_cast<u32x4*>(dst + token * step + (tile % kChunks) * 64 + (lane & 7) * 8) =
-                bf16_of_8(w[t][0], w[t][1], scale);
+            store(dst + token * step + (tile % kChunks) * 64 + (lane & 7) * 8, bf16_of_8(w[t][0], w[t][1], scale));
         }
       } else {
         // of each two tiles: lane = (dlow half, dh, tile of the two, t, q): elements 16 dh + 8 (dlow half) + 0 .. 7 of the tile
@@ -478,9 +485,9 @@ __global__ __launch_bounds__(64 * kReadWaves) void read_kernel(const ReadParams 
             const unsigned(&x)[8] = pair[e >> 1];
             const unsigned pick = e & 1 ? 0x07060302u : 0x05040100u;
             if (token + e < tokens_left)
-              *reinterpret_cast<u32x4*>(to_row + e * step) =
-                  u32x4{__builtin_amdgcn_perm(x[1], x[0], pick), __builtin_amdgcn_perm(x[3], x[2], pick),
-                        __builtin_amdgcn_perm(x[5], x[4], pick), __builtin_amdgcn_perm(x[7], x[6], pick)};
+              store(to_row + e * step,
+                    u32x4{__builtin_amdgcn_perm(x[1], x[0], pick), __builtin_amdgcn_perm(x[3], x[2], pick),
+                        __builtin_amdgcn_perm(x[5], x[4], pick), __builtin_amdgcn_perm(x[7], x[6], pick)});
           }
         }
       }
@@ -519,14 +526,19 @@ hipError_t launch_cache_append(const AppendParams& p, int64_t n_writes, hipStrea
 }
 
 hipError_t launch_cache_read(const ReadParams& p, hipStream_t stream) {
-  // enough workgroups to fill the GPU, no more than the groups of 32 rows
-  const int64_t groups = p.rows / kCacheGroup + p.r.n_seq;
-  const dim3 grid((unsigned)ka_min64(groups < 1 ? 1 : groups, 256 * 8)), threads(64 * kReadWaves);
+  // A unit each wave, at most 32 workgroups per CU: 32,768 rows of 16 heads at 128 96.9 us with 1,024 workgroups, 85.5 with
+  // 2,048, 82.0 with 4,096, 77.6 with 8,192 (5.2 TB/s: how evenly the rows being written lie over the memory's channels).
+  const int64_t units = (p.rows / kCacheGroup + p.r.n_seq) * 2 * p.c.kv_heads * (p.c.head_dim == 64 ? 1 : p.c.head_dim / 128);
+  const dim3 grid((unsigned)ka_min64((units + kReadWaves - 1) / kReadWaves + 1, 8192)), threads(64 * kReadWaves);
+  auto launch = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    if (p.stream) read_kernel<D, true><<<grid, threads, 0, stream>>>(p); else read_kernel<D, false><<<grid, threads, 0, stream>>>(p);
+  };
   switch (p.c.head_dim) {
-    case 64: read_kernel<64><<<grid, threads, 0, stream>>>(p); break;
-    case 128: read_kernel<128><<<grid, threads, 0, stream>>>(p); break;
-    case 256: read_kernel<256><<<grid, threads, 0, stream>>>(p); break;
-    case 512: read_kernel<512><<<grid, threads, 0, stream>>>(p); break;
+    case 64: launch(std::integral_constant<int, 64>()); break;
+    case 128: launch(std::integral_constant<int, 128>()); break;
+    case 256: launch(std::integral_constant<int, 256>()); break;
+    case 512: launch(std::integral_constant<int, 512>()); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();

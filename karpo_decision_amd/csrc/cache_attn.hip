@@ -26,6 +26,11 @@ constexpr int slab_of(int d, int nt) {
   while (kAttendWaves * 16 * nt * (slab + 4) * 4 > data_bytes(d, nt)) slab /= 2;
   return slab;
 }
+// Requests whose tokens times the head size cannot pass this are not split: a workgroup walks at most 32 of their groups (16 at
+// head size 256, 8 at 512), and there is nothing to join. Split against whole, 4 requests: head size 128, 1,024 tokens 18.4,
+// 15.3 us (both the host's), 2,048 tokens 18.8, 22.1; 256, 512 tokens 18.7, 15.4, 2,048 tokens 18.6, 31.3; 512, 256 tokens
+// 18.5, 16.0, 512 tokens 18.6, 22.7; 256 requests of 512 tokens at head size 128 105.9, 96.9.
+constexpr int64_t kWhole = 1 << 17;
 constexpr int kLeastUnits = kAttendWaves;  // groups of 32 tokens that a workgroup takes at least
 
 struct Seen {
@@ -47,13 +52,25 @@ __device__ __forceinline__ Seen seen_of(const AttendParams& p, int i) {
   return s;
 }
 
-// Workgroup p of `parts` takes the units [total * p / parts, total * (p + 1) / parts); parts <= total, so none is empty.
-__device__ __forceinline__ int64_t parts_of(int64_t total, int parts) {
-  const int64_t most = total / kLeastUnits;
-  return most < 1 ? 1 : most < parts ? most : parts;
-}
-// The workgroup that takes unit u.
-__device__ __forceinline__ int64_t part_of(int64_t u, int64_t total, int64_t parts) { return ((u + 1) * parts - 1) / total; }
+// A vector's position among its request's queries: vec / group, exactly (vec + 1/2 is no multiple of the group, and below
+// 2^16 further from one than the product's rounding).
+__device__ __forceinline__ int position_of(int vec, const AttendParams& p) { return (int)((vec + 0.5f) * p.per_group); }
+
+// The workgroups' shares of `total` units: of `parts` workgroups (fewer where each would get less than kLeastUnits) the first
+// `more` take `each` + 1, the others `each`.
+struct Shares {
+  int each, more;
+  __device__ __forceinline__ Shares(int total, int parts) {
+    const unsigned n = max(min(parts, total / kLeastUnits), 1);
+    each = (int)((unsigned)total / n);
+    more = total - each * (int)n;
+  }
+  __device__ __forceinline__ int begin(int part) const { return part * each + min(part, more); }
+  __device__ __forceinline__ int part_of(int unit) const {
+    const int longer = more * (each + 1);
+    return unit < longer ? (int)((unsigned)unit / (unsigned)(each + 1)) : more + (int)((unsigned)(unit - longer) / (unsigned)each);
+  }
+};
 
 // x's maximum / sum over the four lanes of a column (16 apart).
 __device__ __forceinline__ float column_max(float x) {
@@ -112,30 +129,40 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
     v[0] = own.units;
     block_scan<kAttendThreads, 1>(v, all, s_part);
   };
-  int64_t total = 0;
-  for (int c0 = 0; c0 < p.r.n_seq; c0 += kAttendThreads) {
-    if (c0 > 0) __syncthreads();
-    scan(c0);
-    total += all[0];
+  int total = 0, c0 = 0, c_end = p.r.n_seq, u0, u1;
+  if (p.whole) {  // workgroup i takes request i
+    c0 = blockIdx.x;
+    c_end = c0 + 1;
+    own = seen_of(p, c0);
+    all[0] = total = own.units;
+    v[0] = 0;
+    if (tid != 0) own.units = 0;  // (thread 0's)
+    u0 = 0;
+    u1 = total;
+  } else {
+    for (int c = 0; c < p.r.n_seq; c += kAttendThreads) {
+      if (c > 0) __syncthreads();
+      scan(c);
+      total += all[0];
+    }
+    const Shares shares(total, p.parts);
+    u0 = min(shares.begin(blockIdx.x), total);  // (workgroups past the shares: none)
+    u1 = min(shares.begin(blockIdx.x + 1), total);
   }
-  const bool writes_units = blockIdx.x == 0 && blockIdx.y == 0;
-  const int64_t parts = parts_of(total, p.parts);
-  if (total == 0 || (int64_t)blockIdx.x >= parts) {
-    if (writes_units && tid == 0) p.units[p.r.n_seq] = 0;  // (total is 0: nothing to join)
-    return;
-  }
-  const int64_t u0 = total * blockIdx.x / parts, u1 = total * (blockIdx.x + 1) / parts;
+  const bool writes_units = !p.whole && blockIdx.x == 0 && blockIdx.y == 0;
+  if (writes_units && tid == 0) p.units[p.r.n_seq] = total;
+  if (u0 >= u1) return;
 
-  int64_t carry = 0;
-  for (int c0 = 0; c0 < p.r.n_seq && (writes_units || carry < u1); c0 += kAttendThreads) {
-    if (p.r.n_seq > kAttendThreads) {
+  int carry = 0;
+  for (; c0 < c_end && (writes_units || carry < u1); c0 += kAttendThreads) {
+    if (!p.whole && p.r.n_seq > kAttendThreads) {
       __syncthreads();
       scan(c0);  // (one chunk's sums are there)
     }
     if (writes_units && c0 + tid < p.r.n_seq) p.units[c0 + tid] = carry + v[0];
-    const int64_t from = u0 > carry ? u0 : carry, to = u1 < carry + all[0] ? u1 : carry + all[0];
-    for (int64_t at = from; at < to;) {
-      const int unit = (int)(at - carry);
+    const int to = min(u1, carry + all[0]);
+    for (int at = max(u0, carry); at < to;) {
+      const int unit = at - carry;
       if (unit >= v[0] && unit - v[0] < own.units) {  // this thread's request
         s_seen = own;
         s_at[0] = tid;
@@ -145,10 +172,10 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
       const Seen s = {uniform(s_seen.tokens), uniform(s_seen.row),   uniform(s_seen.queries),
                       uniform(s_seen.first),  uniform(s_seen.groups), uniform(s_seen.units)};
       const int i = c0 + uniform(s_at[0]);
-      const int64_t begin = carry + uniform(s_at[1]), end = begin + s.units;
-      const int64_t stop = to < end ? to : end;
-      const int g0 = s.first + (int)(at - begin);
-      const int g1 = s.groups > 0 ? s.first + (int)(stop - begin) : g0;
+      const int begin = carry + uniform(s_at[1]), end = begin + s.units;
+      const int stop = min(to, end);
+      const int g0 = s.first + at - begin;
+      const int g1 = s.groups > 0 ? s.first + stop - begin : g0;
       at = stop;
       const int vectors = (int)min<int64_t>((int64_t)s.queries * p.group - vector0, kVectors);
       if (vectors <= 0) {
@@ -166,7 +193,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
       for (int n = 0; n < NT; ++n) {
         const int vec = vector0 + 16 * n + col;
         const bool valid = 16 * n + col < vectors;
-        const int pos = valid ? vec / p.group : 0;
+        const int pos = valid ? position_of(vec, p) : 0;
         const uint16_t* const src =
             p.q + (s.row + (int64_t)pos) * p.sq_t + (int64_t)(h * p.group + (valid ? vec - pos * p.group : 0)) * p.sq_h;
 #pragma unroll
@@ -179,7 +206,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
         hi[n] = p.right < 0 ? s.tokens - 1 : (int)min<int64_t>((int64_t)pos + shift + p.right, s.tokens - 1);
       }
       // groups that every vector sees whole
-      const int pos_first = vector0 / p.group, pos_last = (vector0 + vectors - 1) / p.group;
+      const int pos_first = position_of(vector0, p), pos_last = position_of(vector0 + vectors - 1, p);
       const int full_lo = p.left < 0 ? 0 : pos_last + shift - p.left;
       const int full_hi =
           p.right < 0 ? s.tokens - 1 : (int)min<int64_t>((int64_t)pos_first + shift + p.right, s.tokens - 1);
@@ -214,9 +241,16 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
         const uint8_t* const src = from + ((head << b) + (int64_t)(g & ((1 << (b - 5)) - 1)) * kCacheGroup) * D;
         const __amdgpu_buffer_rsrc_t r =
             __builtin_amdgcn_make_buffer_rsrc((void*)src, (short)0, id >= 0 ? kCacheGroup * D : 0, kBufferFlags);
+        if (p.once) {
 #pragma unroll
-        for (int t = 0; t < kLoads; ++t)
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (KA_LDS void*)(to + t * 1024), 16, lane_offset, t * 1024, 0, 0);
+          for (int t = 0; t < kLoads; ++t)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (KA_LDS void*)(to + t * 1024), 16, lane_offset, t * 1024, 0,
+                                                     kCopyStream);
+        } else {
+#pragma unroll
+          for (int t = 0; t < kLoads; ++t)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (KA_LDS void*)(to + t * 1024), 16, lane_offset, t * 1024, 0, 0);
+        }
       };
       auto tile = [&](const KA_LDS char* ring, int t) {
         return *reinterpret_cast<const KA_LDS u32x4*>(ring + t * 1024 + lane * 16);
@@ -421,7 +455,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
           for (int w = 1; w < kAttendWaves; ++w) x += *reinterpret_cast<const f32x4*>(&s_o[w][c][d]);
           if (whole) {
             const float l = total_of(c, top_of(c));
-            const int vec = vector0 + c, pos = vec / p.group, head = h * p.group + vec - pos * p.group;
+            const int vec = vector0 + c, pos = position_of(vec, p), head = h * p.group + vec - pos * p.group;
             if (l == 0.f) x = f32x4{0.f, 0.f, 0.f, 0.f}; else x = x * (1.f / l);
             *reinterpret_cast<u32x2*>(p.o + (s.row + (int64_t)pos) * p.so_t + head * p.so_h + d0 + d) =
                 u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
@@ -434,7 +468,6 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
     }
     carry += all[0];
   }
-  if (writes_units && tid == 0) p.units[p.r.n_seq] = total;
 }
 
 // Joins a request's shares: O = sum of 2^(m_w - M) O_w over sum of 2^(m_w - M) l_w, in an order that the sizes alone set.
@@ -447,11 +480,11 @@ __global__ __launch_bounds__(256) void join_kernel(const AttendParams p, int vec
   __shared__ float s_m[16], s_l[16];
   __shared__ f32x4 s_x[16][16];
   const int i = blockIdx.x, heads = p.c.kv_heads;
-  const int64_t total = p.units[p.r.n_seq], begin = p.units[i], end = p.units[i + 1];
+  const int total = p.units[p.r.n_seq], begin = p.units[i], end = p.units[i + 1];
   const Seen s = seen_of(p, i);
   if (total == 0 || begin == end) return;
-  const int64_t parts = parts_of(total, p.parts);
-  const int first = (int)part_of(begin, total, parts), last = (int)part_of(end - 1, total, parts);
+  const Shares shares(total, p.parts);
+  const int first = shares.part_of(begin), last = shares.part_of(end - 1);
   if (first == last) return;
   const int h = blockIdx.y % heads, vector0 = (blockIdx.y / heads) * vectors_per;
   const int vectors = (int)min<int64_t>((int64_t)s.queries * p.group - vector0, vectors_per);
@@ -465,7 +498,7 @@ __global__ __launch_bounds__(256) void join_kernel(const AttendParams p, int vec
   };
   auto add = [&](Sum& a, int w, int c, int d) {
     // (only the first share can have begun before the request: then the request is its workgroup's second)
-    const float* const part = base + (2 * (int64_t)w + (w == first && begin > total * w / parts ? 1 : 0)) * size;
+    const float* const part = base + (2 * (int64_t)w + (w == first && begin > shares.begin(w) ? 1 : 0)) * size;
     const float m = part[vectors_per * D + c], lw = part[vectors_per * D + vectors_per + c];
     const f32x4 xw = *reinterpret_cast<const f32x4*>(part + c * D + d);
     const float next = __builtin_elementwise_maximum(a.up, m);
@@ -476,7 +509,7 @@ __global__ __launch_bounds__(256) void join_kernel(const AttendParams p, int vec
     a.up = next;
   };
   auto store = [&](const Sum& a, int c, int d) {
-    const int vec = vector0 + c, pos = vec / p.group, head = h * p.group + vec - pos * p.group;
+    const int vec = vector0 + c, pos = position_of(vec, p), head = h * p.group + vec - pos * p.group;
     const f32x4 x = a.l == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : a.x * (1.f / a.l);
     *reinterpret_cast<u32x2*>(p.o + (s.row + (int64_t)pos) * p.so_t + head * p.so_h + d) =
         u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
@@ -523,8 +556,9 @@ __global__ __launch_bounds__(256) void join_kernel(const AttendParams p, int vec
 
 template <int D, int NT>
 void launch(const AttendParams& p, const AttendShape& s, hipStream_t stream) {
-  const unsigned y = (unsigned)(p.c.kv_heads * s.tiles);
-  attend_kernel<D, NT><<<dim3((unsigned)s.parts, y), dim3(kAttendThreads), 0, stream>>>(p);
+  const unsigned y = (unsigned)(p.c.kv_heads * s.tiles), x = (unsigned)(p.whole ? p.r.n_seq : s.parts);
+  attend_kernel<D, NT><<<dim3(x, y), dim3(kAttendThreads), 0, stream>>>(p);
+  if (p.whole) return;
   // a workgroup for 64 elements of each vector, or as many as fill the GPU several times over
   const int64_t pairs = (int64_t)p.r.n_seq * y, most = (2048 + pairs - 1) / pairs, items = (int64_t)s.used * (D / 64);
   const unsigned z = (unsigned)(items < most ? items : most);
@@ -533,7 +567,7 @@ void launch(const AttendParams& p, const AttendShape& s, hipStream_t stream) {
 
 }  // namespace
 
-AttendShape attend_shape(const CacheRef& c, int32_t n_seq, int32_t group, int32_t max_q) {
+AttendShape attend_shape(const CacheRef& c, int32_t n_seq, int32_t group, int32_t max_q, int64_t longest) {
   AttendShape s;
   const int64_t vectors = (int64_t)max_q * group;
   const int most = c.head_dim <= 128 ? 4 : c.head_dim == 256 ? 2 : 1;  // tiles of 16 vectors that the registers hold
@@ -546,8 +580,9 @@ AttendShape attend_shape(const CacheRef& c, int32_t n_seq, int32_t group, int32_
   const int64_t parts = 256 * at_once / y;
   s.parts = parts < 1 ? 1 : (int)parts;
   s.used = (int)(vectors < s.vectors ? vectors : s.vectors);
-  s.units_bytes = (8 * ((int64_t)n_seq + 1) + 255) / 256 * 256;
-  s.bytes = s.units_bytes + y * s.parts * 2 * s.vectors * (c.head_dim + 2) * 4;
+  s.whole = longest * c.head_dim <= kWhole;
+  s.units_bytes = (4 * ((int64_t)n_seq + 1) + 255) / 256 * 256;
+  s.bytes = s.whole ? 0 : s.units_bytes + y * s.parts * 2 * s.vectors * (c.head_dim + 2) * 4;
   return s;
 }
 

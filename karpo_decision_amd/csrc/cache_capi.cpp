@@ -19,7 +19,7 @@ bool overlaps(const void* a, int64_t na, const void* b, int64_t nb) {
   return na > 0 && nb > 0 && x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
 }
 
-// Tokens of a table's row: sums of 1,024 such counts in groups of 32 stay in 32 bits.
+// Tokens of a table's row; and all rows of a table in groups of 32 tokens stay in 32 bits.
 constexpr int64_t kMostTokens = (int64_t)1 << 26;
 
 int check_cache(const KarpoCache& c, CacheRef* ref) {
@@ -42,6 +42,7 @@ int check_cache(const KarpoCache& c, CacheRef* ref) {
 int check_rows(const int32_t* table, int64_t stride, int32_t width, const int32_t* lengths, int32_t n_seq,
                int32_t block_size, CacheRows* rows) {
   if (n_seq < 0 || width < 1 || stride < width || (int64_t)width * block_size > kMostTokens) return KARPO_ATTN_ERR_ARG;
+  if ((int64_t)n_seq * ((int64_t)width * block_size / kCacheGroup) > INT32_MAX) return KARPO_ATTN_ERR_ARG;
   if (n_seq > 0 && (!table || !lengths)) return KARPO_ATTN_ERR_NULL;
   rows->table = table;
   rows->table_stride = stride;
@@ -50,6 +51,10 @@ int check_rows(const int32_t* table, int64_t stride, int32_t width, const int32_
   rows->most = (int32_t)(width * (int64_t)block_size);
   return KARPO_ATTN_OK;
 }
+
+// The eight L2 caches. Rows past them are stored through: 32,768 of 16 heads at 128 77.9 -> 71.4 us, six requests at head size
+// 512 (75 MB) 22.5 -> 20.0; the attention's own unpacked rows are read next and are not (chunks over 30,000 tokens: equal).
+constexpr int64_t kL2Bytes = (int64_t)32 << 20;
 
 bool row_strides(const void* p, int64_t tok, int64_t head) {
   return aligned(p, 16) && tok >= 0 && head >= 0 && tok % 8 == 0 && head % 8 == 0;
@@ -160,6 +165,7 @@ extern "C" int karpo_cache_read(const KarpoCacheReadArgs* a, void* stream) {
   p.v = static_cast<uint16_t*>(a->v);
   p.rows = a->rows;
   p.k_cu = a->k_cu;
+  p.stream = 4 * a->rows * a->cache.kv_heads * a->cache.head_dim > kL2Bytes;
   if (launch_cache_read(p, static_cast<hipStream_t>(stream)) != hipSuccess) return KARPO_ATTN_ERR_LAUNCH;
   return KARPO_ATTN_OK;
 }
@@ -227,9 +233,17 @@ int check_attend(const KarpoCacheAttendArgs* a, CacheRef* c, CacheRows* r) {
   return KARPO_ATTN_OK;
 }
 
-// Whether the call's queries are few enough for the split path.
+// Whether the call's queries are few enough for the split path, which walks the keys once for each 64 vectors (head size 256:
+// 32, 512: 16); the other path unpacks them first. Unpacked against split, one request of 32,768 tokens: 128 vectors at head
+// size 128 181 us, 79 us; 256 vectors 230, 134; 1,024 vectors 471, 430; 16 requests of 2,048: 115, 87; 129, 141; 16 requests,
+// 256 vectors, two key/value heads 46, 58. Head size 256, 128 vectors: 190, 110; 128, 111; 256 vectors 218, 193; 149, 195.
+// Head size 512, 128 vectors: 214, 126; 157, 120; 256 vectors 227, 218; 195, 209.
 bool split(const KarpoCacheAttendArgs* a) {
-  return (int64_t)a->max_q * (a->heads / a->cache.kv_heads) <= 64;
+  return (int64_t)a->max_q * (a->heads / a->cache.kv_heads) <= (a->cache.head_dim <= 128 ? 256 : 128);
+}
+
+AttendShape shape_of(const KarpoCacheAttendArgs* a, const CacheRef& c, const CacheRows& r) {
+  return attend_shape(c, a->n_seq, a->heads / a->cache.kv_heads, a->max_q, a->total_keys < r.most ? a->total_keys : r.most);
 }
 
 }  // namespace
@@ -241,7 +255,7 @@ extern "C" int karpo_cache_attend_workspace_bytes(const KarpoCacheAttendArgs* a,
   if (st != KARPO_ATTN_OK) return st;
   if (bytes == nullptr) return KARPO_ATTN_ERR_NULL;
   if (split(a)) {
-    *bytes = (size_t)attend_shape(c, a->n_seq, a->heads / a->cache.kv_heads, a->max_q).bytes;
+    *bytes = (size_t)shape_of(a, c, r).bytes;
     return KARPO_ATTN_OK;
   }
   Unpacked u;
@@ -261,8 +275,9 @@ extern "C" int karpo_cache_attend(const KarpoCacheAttendArgs* a, void* stream) {
   if (!row_strides(a->q, a->q_stride_tok, a->q_stride_head) || !row_strides(a->o, a->o_stride_tok, a->o_stride_head))
     return KARPO_ATTN_ERR_LAYOUT;
   if (split(a)) {
-    const AttendShape shape = attend_shape(p.c, a->n_seq, a->heads / a->cache.kv_heads, a->max_q);
-    if (a->workspace == nullptr || a->workspace_bytes < (size_t)shape.bytes || !aligned(a->workspace, 16))
+    const AttendShape shape = shape_of(a, p.c, p.r);
+    if (shape.bytes > 0 &&
+        (a->workspace == nullptr || a->workspace_bytes < (size_t)shape.bytes || !aligned(a->workspace, 16)))
       return KARPO_ATTN_ERR_WORKSPACE;
     AttendParams t;
     memset(&t, 0, sizeof(t));
@@ -280,9 +295,14 @@ extern "C" int karpo_cache_attend(const KarpoCacheAttendArgs* a, void* stream) {
     t.left = a->window_left >= kMostTokens ? -1 : a->window_left;  // (sees everything, and stays within 32 bits)
     t.right = a->window_right;
     t.scale = a->scale * 1.4426950408889634f;
+    t.per_group = 1.f / t.group;
+    t.whole = shape.whole;
+    t.once = shape.tiles == 1;
     t.parts = shape.parts;
-    t.units = static_cast<int64_t*>(a->workspace);
-    t.partial = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + shape.units_bytes);
+    if (!shape.whole) {
+      t.units = static_cast<int32_t*>(a->workspace);
+      t.partial = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + shape.units_bytes);
+    }
     if (launch_cache_attend(t, shape, static_cast<hipStream_t>(stream)) != hipSuccess) return KARPO_ATTN_ERR_LAUNCH;
     return KARPO_ATTN_OK;
   }

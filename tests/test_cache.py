@@ -221,12 +221,13 @@ def test_writes_capacity(rows, n, block, want):
     ({"heads": 3}, _lib.ERR_HEADS), ({"heads": 0}, _lib.ERR_HEADS), ({"window_left": -2}, _lib.ERR_WINDOW),
     ({"window_right": -2}, _lib.ERR_WINDOW), ({"max_q": -1}, _lib.ERR_ARG), ({"total_q": -1}, _lib.ERR_ARG),
     ({"total_keys": -1}, _lib.ERR_ARG), ({"total_keys": 1 << 31}, _lib.ERR_ARG), ({"n_seq": -1}, _lib.ERR_ARG),
+    ({"n_seq": 1 << 23}, _lib.ERR_ARG), ({"table_stride": 255}, _lib.ERR_ARG),
     ({"table": None}, 1), ({"lengths": None}, 1), ({"q": None}, 1), ({"o": None}, 1), ({"q_cu": None}, 1),
     ({"q": 4104}, _lib.ERR_LAYOUT), ({"q_stride_tok": 4}, _lib.ERR_LAYOUT), ({"o_stride_head": 60}, _lib.ERR_LAYOUT),
     ({"workspace": None}, 5), ({"workspace_bytes": 16}, 5), ({"workspace": 4104}, 5)], ids=str)
 def test_c_abi_attend_refuses(change, status):
-    a = _lib.KarpoCacheAttendArgs(_c_cache(), 4096, 4096, 128, 64, 128, 64, 4096, 4096, 4096, 2, 2, 1, 4, 3, 3, 3, 0.1, -1, 0,
-                                  4096, 1 << 40)
+    a = _lib.KarpoCacheAttendArgs(_c_cache(), 4096, 4096, 128, 64, 128, 64, 4096, 4096, 4096, 256, 256, 1, 4, 3, 3, 8000, 0.1,
+                                  -1, 0, 4096, 1 << 40)
     for name, value in change.items():
         setattr(a, name, value)
     assert _lib.load().karpo_cache_attend(ctypes.byref(a), None) == status
