@@ -176,11 +176,10 @@ def load() -> ctypes.CDLL:
         lib.karpo_attn_fwd_noalloc.restype = ctypes.c_int
         lib.karpo_cache_writes_capacity.argtypes = [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32]
         lib.karpo_cache_writes_capacity.restype = ctypes.c_int64
-        for name, args in (("reserve", KarpoCacheReserveArgs), ("append", KarpoCacheAppendArgs),
-                           ("read", KarpoCacheReadArgs), ("attend", KarpoCacheAttendArgs)):
+        for name in ("reserve", "append", "read", "attend"):  # by the structures, or by their bytes (kv_cache)
             fn = getattr(lib, "karpo_cache_" + name)
-            fn.argtypes, fn.restype = [P(args), ctypes.c_void_p], ctypes.c_int
-        lib.karpo_cache_attend_workspace_bytes.argtypes = [P(KarpoCacheAttendArgs), P(ctypes.c_size_t)]
+            fn.argtypes, fn.restype = [ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int
+        lib.karpo_cache_attend_workspace_bytes.argtypes = [ctypes.c_void_p, P(ctypes.c_size_t)]
         lib.karpo_cache_attend_workspace_bytes.restype = ctypes.c_int
         _lib = lib
         return lib

@@ -17,6 +17,7 @@ current stream of the tensors' device and capture into graphs. All of it is forw
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import NamedTuple
 
 import torch
@@ -28,6 +29,14 @@ from .ops import _current_stream, _on_device
 BLOCK_SIZES = (32, 64, 128)
 HEAD_DIMS = (64, 128, 256, 512)
 _MOST = (1 << 31) - 1
+
+# The argument structures of karpo_cache.h, field by field (_lib has them by name): packing them costs a third of what
+# building them by name does, and a small call's time is its host path.
+_CACHE = "PPPqiii4x"
+_RESERVE = struct.Struct("@PqiiPPPPiiqPPPPPqPP")
+_APPEND = struct.Struct("@" + _CACHE + "PPqqqqqPq")
+_READ = struct.Struct("@" + _CACHE + "PqiiPPPqP")
+_ATTEND = struct.Struct("@" + _CACHE + "PPqqqqPPPqiiiiqqfii4xPN")
 
 
 class Cache(NamedTuple):
@@ -92,7 +101,8 @@ def create(blocks: int, kv_heads: int, head_dim: int, block_size: int = 64,
     return Cache(keys, values, torch.zeros((blocks, kv_heads, 2), dtype=torch.float32, device=device), block_size)
 
 
-def _cache_args(cache: Cache, device: torch.device) -> _lib.KarpoCache:
+def _cache_fields(cache: Cache, index: int) -> tuple[int, ...]:
+    """The cache's fields of an argument structure; ``index``: the other tensors' device."""
     keys, values, scales, block = cache
     shape, fp8 = keys.shape, torch.float8_e4m3fn
     if len(shape) == 3 and block in BLOCK_SIZES:  # all is well: one pass
@@ -101,42 +111,49 @@ def _cache_args(cache: Cache, device: torch.device) -> _lib.KarpoCache:
         if (head_dim in HEAD_DIMS and size == head_dim * block and values.shape == shape and blocks > 0 and heads > 0
                 and scales.shape == (blocks, heads, 2) and keys.dtype is fp8 and values.dtype is fp8
                 and scales.dtype is torch.float32 and keys.is_contiguous() and values.is_contiguous()
-                and scales.is_contiguous() and keys.device == device and values.device == device
-                and scales.device == device):
-            return _lib.KarpoCache(keys.data_ptr(), values.data_ptr(), scales.data_ptr(), blocks, heads, head_dim, block)
+                and scales.is_contiguous() and keys.get_device() == values.get_device() == scales.get_device() == index):
+            return keys.data_ptr(), values.data_ptr(), scales.data_ptr(), blocks, heads, head_dim, block
     # the refusal's message
     if keys.dtype != fp8 or values.dtype != fp8 or scales.dtype != torch.float32:
         raise ValueError(f"a cache has float8_e4m3fn keys and values and float32 scales, not {keys.dtype}, "
                          f"{values.dtype} and {scales.dtype}")
-    if keys.device != device or values.device != device or scales.device != device:
-        raise ValueError(f"the cache is on {keys.device}, {values.device} and {scales.device}, the other tensors on {device}")
+    if not keys.get_device() == values.get_device() == scales.get_device() == index:
+        raise ValueError(f"the cache is on {keys.device}, {values.device} and {scales.device}, the other tensors elsewhere")
     raise ValueError(f"a cache has contiguous keys and values (blocks, kv heads, block_size * head_dim) and scales (blocks, "
                      f"kv heads, 2), block_size 32, 64 or 128 and head_dim 64, 128, 256 or 512, not {tuple(shape)}, "
                      f"{tuple(values.shape)}, {tuple(scales.shape)} and {block}")
 
 
-def _check_ints(device: torch.device, tensors: dict[str, Tensor]) -> None:
+def _check_ints(index: int, **tensors: Tensor) -> None:
+    """The refusal of device numbers (``_ints`` finds that there is one)."""
     for name, t in tensors.items():
-        if t.dtype is not torch.int32 or t.dim() != 1 or t.device != device or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous 1-D int32 tensor on {device}")
+        if t.dtype != torch.int32 or t.dim() != 1 or t.get_device() != index or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous 1-D int32 tensor on the other tensors' device")
 
 
-def _check_table(table: Tensor, lengths: Tensor, device: torch.device) -> tuple[int, int, int]:
-    """(requests, blocks of a row, row stride) of a block table that fits ``lengths``."""
-    if table.dim() != 2 or table.dtype is not torch.int32 or table.device != device:
-        raise ValueError(f"table must be a (requests, blocks) int32 tensor on {device}")
-    (n, width), (stride, inner) = table.shape, table.stride()
+def _ints(t: Tensor, index: int) -> bool:
+    return t.dtype is torch.int32 and t.dim() == 1 and t.get_device() == index and t.is_contiguous()
+
+
+def _table_fields(table: Tensor, lengths: Tensor, index: int) -> tuple[int, int, int, int]:
+    """(pointer, row stride, blocks of a row, requests) of a block table that fits ``lengths``."""
+    shape, strides = table.shape, table.stride()
+    if len(shape) != 2 or table.dtype is not torch.int32 or table.get_device() != index:
+        raise ValueError("table must be a (requests, blocks) int32 tensor on the other tensors' device")
+    (n, width), (stride, inner) = shape, strides
     if width < 1 or inner != 1 or (stride < width and n > 1):
         raise ValueError(f"table must have contiguous rows of at least one block, not {(n, width)} with strides "
                          f"{(stride, inner)}")
+    if not _ints(lengths, index):
+        _check_ints(index, lengths=lengths)
     if lengths.numel() != n:
         raise ValueError(f"the table has {n} requests, lengths {lengths.numel()}")
-    return n, width, stride if stride >= width else width
+    return table.data_ptr(), stride if stride >= width else width, width, n
 
 
-def _on_gpu(what: str, t: Tensor) -> None:
-    if t.device.type != "cuda":
-        raise ValueError(f"{what} runs on an MI355X GPU, not on {t.device}")
+def _on_gpu(what: str, index: int) -> None:
+    if index < 0:
+        raise ValueError(f"{what} runs on an MI355X GPU, not on the CPU")
 
 
 def _no_grad(what: str, *tensors: Tensor) -> None:
@@ -151,20 +168,21 @@ def reserve(table: Tensor, lengths: Tensor, counts: Tensor, free: Tensor, free_c
     end of the first ``free_count[0]`` entries of ``free``, and what the step's layers need (``Step``). ``rows`` bounds
     the counts' sum and is the packed new tokens' row count. The inputs but the table are left as they are: the free
     list goes on with ``free_left``, the requests with ``Step.lengths``."""
-    device = table.device
-    n, width, stride = _check_table(table, lengths, device)
-    _check_ints(device, {"lengths": lengths, "counts": counts, "free": free, "free_count": free_count})
-    rows, capacity = int(rows), free.numel()
+    index = table.get_device()
+    fields = _table_fields(table, lengths, index)
+    n, rows = fields[3], int(rows)
+    if not (_ints(counts, index) and _ints(free, index) and _ints(free_count, index)):
+        _check_ints(index, counts=counts, free=free, free_count=free_count)
     if counts.numel() != n or free_count.numel() != 1:
         raise ValueError(f"counts must hold {n} requests and free_count one number, not {counts.numel()} and "
                          f"{free_count.numel()}")
     if rows < 0 or block_size not in BLOCK_SIZES:
         raise ValueError(f"rows must be non-negative and block_size 32, 64 or 128, not {rows} and {block_size}")
-    _on_gpu("reserve", table)
+    _on_gpu("reserve", index)
     lib = _lib.load()
     jobs = lib.karpo_cache_writes_capacity(rows, n, block_size)
     # one allocation for the step: writes (16-byte aligned) and slots first
-    buffer = torch.empty(4 * jobs + 3 * rows + 2 * n + 3, dtype=torch.int32, device=device)
+    buffer = table.new_empty(4 * jobs + 3 * rows + 2 * n + 3)
     writes, slots, positions, q_cu, new, left, status = torch.split_with_sizes(
         buffer, (4 * jobs, 2 * rows, rows, n + 1, n, 1, 1))
     at = buffer.data_ptr()
@@ -173,13 +191,11 @@ def reserve(table: Tensor, lengths: Tensor, counts: Tensor, free: Tensor, free_c
     q_at = positions_at + 4 * rows
     new_at = q_at + 4 * n + 4
     left_at = new_at + 4 * n
-    args = _lib.KarpoCacheReserveArgs(
-        table.data_ptr(), stride, width, n, lengths.data_ptr(), counts.data_ptr(), free.data_ptr(),
-        free_count.data_ptr(), capacity, block_size, rows, q_at, new_at, slots_at, positions_at, at, jobs, left_at,
-        left_at + 4)
-    index = device.index
+    args = _RESERVE.pack(*fields, lengths.data_ptr(), counts.data_ptr(), free.data_ptr(), free_count.data_ptr(),
+                         free.numel(), block_size, rows, q_at, new_at, slots_at, positions_at, at, jobs, left_at,
+                         left_at + 4)
     with _on_device(index):
-        _lib.check(lib.karpo_cache_reserve(ctypes.byref(args), _current_stream(index)), "reserve")
+        _lib.check(lib.karpo_cache_reserve(args, _current_stream(index)), "reserve")
     return Step(q_cu, new, slots.view(torch.int64), positions, writes.view(jobs, 4), left, status)
 
 
@@ -189,44 +205,44 @@ def append(cache: Cache, key: Tensor, value: Tensor, writes: Tensor) -> None:
     block's earlier tokens are rounded again to it. What lies past e4m3's range at the largest scale, infinities too, is
     stored at the range's end, NaN as NaN. Rows and slots that no write names are left as they were."""
     _no_grad("append", key, value)
-    device, bf16 = key.device, torch.bfloat16
-    c = _cache_args(cache, device)
+    index, bf16 = key.get_device(), torch.bfloat16
+    fields = _cache_fields(cache, index)
+    heads, head_dim = fields[4], fields[5]
     shape, sk, sv = key.shape, key.stride(), value.stride()
-    if (len(shape) != 3 or value.shape != shape or shape[1] != c.kv_heads or shape[2] != c.head_dim
-            or key.dtype is not bf16 or value.dtype is not bf16 or value.device != device):
-        raise ValueError(f"append takes bf16 keys and values (rows, {c.kv_heads}, {c.head_dim}) on {device}, not "
-                         f"{tuple(shape)} {key.dtype} and {tuple(value.shape)} {value.dtype} on {value.device}")
+    if (len(shape) != 3 or value.shape != shape or shape[1] != heads or shape[2] != head_dim or key.dtype is not bf16
+            or value.dtype is not bf16 or value.get_device() != index):
+        raise ValueError(f"append takes bf16 keys and values (rows, {heads}, {head_dim}) on one device, not {tuple(shape)} "
+                         f"{key.dtype} on {key.device} and {tuple(value.shape)} {value.dtype} on {value.device}")
     if sk[2] != 1 or sv[2] != 1 or (sk[0] | sk[1] | sv[0] | sv[1]) & 7:
         raise ValueError(f"keys and values need a contiguous head_dim and row/head strides that are multiples of 8 "
                          f"(strides {sk}, {sv})")
-    if (writes.dim() != 2 or writes.shape[1] != 4 or writes.dtype != torch.int32 or writes.device != device
+    if (writes.dim() != 2 or writes.shape[1] != 4 or writes.dtype is not torch.int32 or writes.get_device() != index
             or not writes.is_contiguous()):
-        raise ValueError(f"writes must be a contiguous (n, 4) int32 tensor on {device}")
-    _on_gpu("append", key)
-    args = _lib.KarpoCacheAppendArgs(c, key.data_ptr(), value.data_ptr(), sk[0], sk[1], sv[0], sv[1], shape[0],
-                                     writes.data_ptr(), writes.shape[0])
-    with _on_device(device.index):
-        _lib.check(_lib.load().karpo_cache_append(ctypes.byref(args), _current_stream(device.index)), "append")
+        raise ValueError("writes must be a contiguous (n, 4) int32 tensor on the other tensors' device")
+    _on_gpu("append", index)
+    args = _APPEND.pack(*fields, key.data_ptr(), value.data_ptr(), sk[0], sk[1], sv[0], sv[1], shape[0],
+                        writes.data_ptr(), writes.shape[0])
+    with _on_device(index):
+        _lib.check(_lib.load().karpo_cache_append(args, _current_stream(index)), "append")
 
 
 def read(cache: Cache, table: Tensor, lengths: Tensor, rows: int) -> tuple[Tensor, Tensor, Tensor]:
     """(key, value, k_cu): the first ``lengths[i]`` cached tokens of each request as packed bf16 keys and values
     (``rows``, kv heads, D), request i's at k_cu[i]:k_cu[i + 1] (int32 on the device), what ``hip_attention.attend``
     takes. ``rows`` bounds the lengths' sum; rows behind the last request are not written."""
-    device = table.device
-    c = _cache_args(cache, device)
-    n, width, stride = _check_table(table, lengths, device)
-    _check_ints(device, {"lengths": lengths})
+    index = table.get_device()
+    fields = _cache_fields(cache, index)
+    rows_fields = _table_fields(table, lengths, index)
     rows = int(rows)
     if rows < 0:
         raise ValueError(f"rows must be non-negative, not {rows}")
-    _on_gpu("read", table)
-    key, value = (torch.empty((rows, c.kv_heads, c.head_dim), dtype=torch.bfloat16, device=device) for _ in range(2))
-    k_cu = torch.empty(n + 1, dtype=torch.int32, device=device)
-    args = _lib.KarpoCacheReadArgs(c, table.data_ptr(), stride, width, n, lengths.data_ptr(), key.data_ptr(),
-                                   value.data_ptr(), rows, k_cu.data_ptr())
-    with _on_device(device.index):
-        _lib.check(_lib.load().karpo_cache_read(ctypes.byref(args), _current_stream(device.index)), "read")
+    _on_gpu("read", index)
+    shape = (rows, fields[4], fields[5])
+    key, value = table.new_empty(shape, dtype=torch.bfloat16), table.new_empty(shape, dtype=torch.bfloat16)
+    k_cu = table.new_empty(rows_fields[3] + 1)
+    args = _READ.pack(*fields, *rows_fields, lengths.data_ptr(), key.data_ptr(), value.data_ptr(), rows, k_cu.data_ptr())
+    with _on_device(index):
+        _lib.check(_lib.load().karpo_cache_read(args, _current_stream(index)), "read")
     return key, value, k_cu
 
 
@@ -240,42 +256,42 @@ def attend(query: Tensor, cache: Cache, table: Tensor, q_cu: Tensor, lengths: Te
     sum (default: all that the table can hold; it sizes the workspace of long query runs). Rows behind the last request
     are not written."""
     _no_grad("attend", query)
-    device = query.device
-    c = _cache_args(cache, device)
-    shape = query.shape
-    if (len(shape) != 3 or query.dtype is not torch.bfloat16 or shape[2] != c.head_dim or shape[1] < 1
-            or shape[1] % c.kv_heads):
-        raise ValueError(f"attend takes a (rows, heads, {c.head_dim}) bf16 query, its heads a multiple of {c.kv_heads}, "
-                         f"not {tuple(shape)} {query.dtype}")
-    sq = query.stride()
+    index = query.get_device()
+    fields = _cache_fields(cache, index)
+    heads, head_dim = fields[4], fields[5]
+    shape, sq = query.shape, query.stride()
+    if (len(shape) != 3 or query.dtype is not torch.bfloat16 or shape[2] != head_dim or shape[1] < 1
+            or shape[1] % heads):
+        raise ValueError(f"attend takes a (rows, heads, {head_dim}) bf16 query, its heads a multiple of {heads}, not "
+                         f"{tuple(shape)} {query.dtype}")
     if sq[2] != 1 or (sq[0] | sq[1]) & 7:
         raise ValueError(f"query needs a contiguous head_dim and row/head strides that are multiples of 8 (strides {sq})")
-    n, width, stride = _check_table(table, lengths, device)
-    _check_ints(device, {"lengths": lengths, "q_cu": q_cu})
+    rows_fields = _table_fields(table, lengths, index)
+    n = rows_fields[3]
+    if not _ints(q_cu, index):
+        _check_ints(index, q_cu=q_cu)
     if q_cu.numel() != n + 1:
         raise ValueError(f"the table has {n} requests, q_cu {q_cu.numel()} bounds")
     if max_q < 0 or window < -1:
         raise ValueError(f"max_q must be non-negative and window at least -1, not {max_q} and {window}")
     if total_keys is None:
-        total_keys = min(n * width * c.block_size, _MOST)
+        total_keys = min(n * rows_fields[2] * cache.block_size, _MOST)
     elif not 0 <= total_keys <= _MOST:
         raise ValueError(f"total_keys must lie in 0 .. {_MOST}, not {total_keys}")
-    _on_gpu("attend", query)
+    _on_gpu("attend", index)
     lib = _lib.load()
-    out = torch.empty(shape, dtype=torch.bfloat16, device=device)
+    out = query.new_empty(shape)
     if shape[0] == 0:
         return out
-    so = out.stride()
-    args = _lib.KarpoCacheAttendArgs(
-        c, query.data_ptr(), out.data_ptr(), sq[0], sq[1], so[0], so[1], q_cu.data_ptr(), lengths.data_ptr(),
-        table.data_ptr(), stride, width, n, shape[1], int(max_q), shape[0], int(total_keys), float(scale), int(window),
-        0 if causal else -1)
-    pointer, need = ctypes.byref(args), ctypes.c_size_t()
-    _lib.check(lib.karpo_cache_attend_workspace_bytes(pointer, ctypes.byref(need)), "attend")
-    index = device.index
+    call = (*fields, query.data_ptr(), out.data_ptr(), sq[0], sq[1], shape[1] * head_dim, head_dim, q_cu.data_ptr(),
+            lengths.data_ptr(), *rows_fields, shape[1], int(max_q), shape[0], int(total_keys), float(scale),
+            int(window), 0 if causal else -1)
+    need = ctypes.c_size_t()
+    _lib.check(lib.karpo_cache_attend_workspace_bytes(_ATTEND.pack(*call, 0, 0), need), "attend")
+    size, at = need.value, 0
     with _on_device(index):
-        # from the caching allocator (stream-ordered reuse)
-        workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
-        args.workspace, args.workspace_bytes = workspace.data_ptr(), need.value
-        _lib.check(lib.karpo_cache_attend(pointer, _current_stream(index)), "attend")
+        if size:  # from the caching allocator (stream-ordered reuse)
+            workspace = table.new_empty(size, dtype=torch.uint8)
+            at = workspace.data_ptr()
+        _lib.check(lib.karpo_cache_attend(_ATTEND.pack(*call, at, size), _current_stream(index)), "attend")
     return out

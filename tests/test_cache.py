@@ -23,6 +23,23 @@ def test_library_exports_every_declared_function():
         assert hasattr(_lib.load(), name), name
 
 
+@pytest.mark.parametrize("packed,named", [
+    (kv_cache._RESERVE, _lib.KarpoCacheReserveArgs), (kv_cache._APPEND, _lib.KarpoCacheAppendArgs),
+    (kv_cache._READ, _lib.KarpoCacheReadArgs), (kv_cache._ATTEND, _lib.KarpoCacheAttendArgs)], ids=lambda x: "")
+def test_packed_arguments_are_the_structures(packed, named):
+    def leaves(s):
+        for name, kind in s._fields_:
+            if issubclass(kind, ctypes.Structure):
+                yield from leaves(getattr(s, name))
+            else:
+                yield getattr(s, name)
+
+    assert packed.size == ctypes.sizeof(named)
+    count = len(list(leaves(named())))
+    values = list(range(1, count + 1))
+    assert list(leaves(named.from_buffer_copy(packed.pack(*values)))) == values
+
+
 # ---- the oracle
 
 def test_oracle_codes_are_torchs():

@@ -276,8 +276,9 @@ def test_read_writes_no_row_past_its_bound(gpu):
 
     from karpo_decision_amd import _lib, ops
     lengths, k_cu = ints([-5, 1000, 40], gpu), torch.empty(4, dtype=torch.int32, device=gpu)
-    args = _lib.KarpoCacheReadArgs(kv_cache._cache_args(cache, table.device), table.data_ptr(), 2, 2, 3, lengths.data_ptr(),
-                                   backing[0].data_ptr(), backing[1].data_ptr(), 90, k_cu.data_ptr())
+    c = _lib.KarpoCache(*(t.data_ptr() for t in cache[:3]), 4, 1, 64, 32)
+    args = _lib.KarpoCacheReadArgs(c, table.data_ptr(), 2, 2, 3, lengths.data_ptr(), backing[0].data_ptr(),
+                                   backing[1].data_ptr(), 90, k_cu.data_ptr())
     _lib.check(_lib.load().karpo_cache_read(ctypes.byref(args), ops._current_stream(0)), "read")
     assert k_cu.tolist() == [0, 0, 64, 104]
     assert (backing[:, 90:] == 3).all() and not (backing[:, :90] == 3).all(-1).all()
