@@ -56,6 +56,12 @@ __device__ __forceinline__ Seen seen_of(const AttendParams& p, int i) {
 // 2^16 further from one than the product's rounding).
 __device__ __forceinline__ int position_of(int vec, const AttendParams& p) { return (int)((vec + 0.5f) * p.per_group); }
 
+// What a request takes of the sums: a workgroup that goes on to a next request spends about as long on the change (joining its
+// waves, the new queries and tables, the first copies) as on kStart groups. Shares by groups alone left the last workgroups of
+// 48 ragged requests 15 us behind the middle one.
+constexpr int kStart = 4;
+__device__ __forceinline__ int weight_of(int units) { return units > 0 ? units + kStart : 0; }
+
 // The workgroups' shares of `total` units: of `parts` workgroups (fewer where each would get less than kLeastUnits) the first
 // `more` take `each` + 1, the others `each`.
 struct Shares {
@@ -126,7 +132,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
   auto scan = [&](int c0) {
     own = Seen{0, 0, 0, 0, 0, 0};
     if (c0 + tid < p.r.n_seq) own = seen_of(p, c0 + tid);
-    v[0] = own.units;
+    v[0] = weight_of(own.units);
     block_scan<kAttendThreads, 1>(v, all, s_part);
   };
   int total = 0, c0 = 0, c_end = p.r.n_seq, u0, u1;
@@ -145,6 +151,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
       scan(c);
       total += all[0];
     }
+    total = max(total - kStart, 0);  // (none comes after the last)
     const Shares shares(total, p.parts);
     u0 = min(shares.begin(blockIdx.x), total);  // (workgroups past the shares: none)
     u1 = min(shares.begin(blockIdx.x + 1), total);
@@ -162,17 +169,21 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
     if (writes_units && c0 + tid < p.r.n_seq) p.units[c0 + tid] = carry + v[0];
     const int to = min(u1, carry + all[0]);
     for (int at = max(u0, carry); at < to;) {
-      const int unit = at - carry;
-      if (unit >= v[0] && unit - v[0] < own.units) {  // this thread's request
+      // the request that `at` lies in, or the one behind the gap that it lies in: one thread's, or none's
+      const int unit = at - carry - v[0];
+      const bool mine = own.units > 0 && unit < own.units && unit >= (v[0] > 0 ? -kStart : 0);
+      if (mine) {
         s_seen = own;
         s_at[0] = tid;
         s_at[1] = v[0];
       }
-      __syncthreads();
+      if (!__syncthreads_or(mine)) break;
       const Seen s = {uniform(s_seen.tokens), uniform(s_seen.row),   uniform(s_seen.queries),
                       uniform(s_seen.first),  uniform(s_seen.groups), uniform(s_seen.units)};
       const int i = c0 + uniform(s_at[0]);
       const int begin = carry + uniform(s_at[1]), end = begin + s.units;
+      at = max(at, begin);
+      if (at >= to) break;
       const int stop = min(to, end);
       const int g0 = s.first + at - begin;
       const int g1 = s.groups > 0 ? s.first + stop - begin : g0;
@@ -480,11 +491,11 @@ __global__ __launch_bounds__(256) void join_kernel(const AttendParams p, int vec
   __shared__ float s_m[16], s_l[16];
   __shared__ f32x4 s_x[16][16];
   const int i = blockIdx.x, heads = p.c.kv_heads;
-  const int total = p.units[p.r.n_seq], begin = p.units[i], end = p.units[i + 1];
+  const int total = p.units[p.r.n_seq], begin = p.units[i];
   const Seen s = seen_of(p, i);
-  if (total == 0 || begin == end) return;
+  if (s.units == 0) return;
   const Shares shares(total, p.parts);
-  const int first = shares.part_of(begin), last = shares.part_of(end - 1);
+  const int first = shares.part_of(begin), last = shares.part_of(begin + s.units - 1);
   if (first == last) return;
   const int h = blockIdx.y % heads, vector0 = (blockIdx.y / heads) * vectors_per;
   const int vectors = (int)min<int64_t>((int64_t)s.queries * p.group - vector0, vectors_per);

@@ -19,7 +19,7 @@ bool overlaps(const void* a, int64_t na, const void* b, int64_t nb) {
   return na > 0 && nb > 0 && x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
 }
 
-// Tokens of a table's row; and all rows of a table in groups of 32 tokens stay in 32 bits.
+// Tokens of a table's row; all rows of a table in groups of 32 tokens (and 64 more each, which the shares add) fit 32 bits.
 constexpr int64_t kMostTokens = (int64_t)1 << 26;
 
 int check_cache(const KarpoCache& c, CacheRef* ref) {
@@ -42,7 +42,7 @@ int check_cache(const KarpoCache& c, CacheRef* ref) {
 int check_rows(const int32_t* table, int64_t stride, int32_t width, const int32_t* lengths, int32_t n_seq,
                int32_t block_size, CacheRows* rows) {
   if (n_seq < 0 || width < 1 || stride < width || (int64_t)width * block_size > kMostTokens) return KARPO_ATTN_ERR_ARG;
-  if ((int64_t)n_seq * ((int64_t)width * block_size / kCacheGroup) > INT32_MAX) return KARPO_ATTN_ERR_ARG;
+  if ((int64_t)n_seq * ((int64_t)width * block_size / kCacheGroup + 64) > INT32_MAX) return KARPO_ATTN_ERR_ARG;
   if (n_seq > 0 && (!table || !lengths)) return KARPO_ATTN_ERR_NULL;
   rows->table = table;
   rows->table_stride = stride;
