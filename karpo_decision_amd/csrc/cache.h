@@ -96,8 +96,8 @@ struct AttendShape {
   bool whole;
   int64_t units_bytes, bytes;  // of the workspace: the units, then the partials
 };
-// `longest`: a bound of a request's tokens.
-AttendShape attend_shape(const CacheRef& c, int32_t n_seq, int32_t group, int32_t max_q, int64_t longest);
+// `seen`: a bound of the tokens that a request's queries see.
+AttendShape attend_shape(const CacheRef& c, int32_t n_seq, int32_t group, int32_t max_q, int64_t seen);
 hipError_t launch_cache_attend(const AttendParams& p, const AttendShape& s, hipStream_t stream);
 
 }  // namespace karpo

@@ -26,11 +26,12 @@ constexpr int slab_of(int d, int nt) {
   while (kAttendWaves * 16 * nt * (slab + 4) * 4 > data_bytes(d, nt)) slab /= 2;
   return slab;
 }
-// Requests whose tokens times the head size cannot pass this are not split: a workgroup walks at most 32 of their groups (16 at
-// head size 256, 8 at 512), and there is nothing to join. Split against whole, 4 requests: head size 128, 1,024 tokens 18.4,
-// 15.3 us (both the host's), 2,048 tokens 18.8, 22.1; 256, 512 tokens 18.7, 15.4, 2,048 tokens 18.6, 31.3; 512, 256 tokens
-// 18.5, 16.0, 512 tokens 18.6, 22.7; 256 requests of 512 tokens at head size 128 105.9, 96.9.
-constexpr int64_t kWhole = 1 << 17;
+// Requests of which at most this many tokens are seen are not split (a quarter of it at head size 512): one workgroup walks
+// their groups, five a wave, and there is nothing to join. Split against whole, 8 requests: head size 64, 512 tokens 16.9,
+// 12.8 us, 2,048 tokens 16.7, 21.6; 128, 768 tokens 16.7, 13.9, 1,024 tokens 16.6, 16.7; 256, 512 tokens 16.7, 14.5, 768
+// tokens 16.6, 18.3; 512, 128 tokens 17.0, 13.3, 256 tokens 16.8, 18.0. 128 requests of 512 tokens at head size 128 49.6,
+// 44.0; at 512 61.4, 60.7.
+constexpr int64_t kWholeTokens = 640;
 constexpr int kLeastUnits = kAttendWaves;  // groups of 32 tokens that a workgroup takes at least
 
 struct Seen {
@@ -578,7 +579,7 @@ void launch(const AttendParams& p, const AttendShape& s, hipStream_t stream) {
 
 }  // namespace
 
-AttendShape attend_shape(const CacheRef& c, int32_t n_seq, int32_t group, int32_t max_q, int64_t longest) {
+AttendShape attend_shape(const CacheRef& c, int32_t n_seq, int32_t group, int32_t max_q, int64_t seen) {
   AttendShape s;
   const int64_t vectors = (int64_t)max_q * group;
   const int most = c.head_dim <= 128 ? 4 : c.head_dim == 256 ? 2 : 1;  // tiles of 16 vectors that the registers hold
@@ -591,7 +592,7 @@ AttendShape attend_shape(const CacheRef& c, int32_t n_seq, int32_t group, int32_
   const int64_t parts = 256 * at_once / y;
   s.parts = parts < 1 ? 1 : (int)parts;
   s.used = (int)(vectors < s.vectors ? vectors : s.vectors);
-  s.whole = longest * c.head_dim <= kWhole;
+  s.whole = seen <= (c.head_dim == 512 ? kWholeTokens / 4 : kWholeTokens);
   s.units_bytes = (4 * ((int64_t)n_seq + 1) + 255) / 256 * 256;
   s.bytes = s.whole ? 0 : s.units_bytes + y * s.parts * 2 * s.vectors * (c.head_dim + 2) * 4;
   return s;

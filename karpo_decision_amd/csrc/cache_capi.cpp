@@ -1,5 +1,6 @@
 // The block cache's C ABI (karpo_cache.h): argument checks, workspace sizes and launches. Everything that the kernels
 // index with is checked here or in the kernel itself, before a launch or a load.
+#include <math.h>
 #include <stdint.h>
 #include <string.h>
 
@@ -25,7 +26,7 @@ constexpr int64_t kMostTokens = (int64_t)1 << 26;
 int check_cache(const KarpoCache& c, CacheRef* ref) {
   const int b = block_log2(c.block_size);
   if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256 && c.head_dim != 512) return KARPO_ATTN_ERR_HEAD_DIM;
-  if (c.kv_heads < 1 || c.kv_heads > 16384) return KARPO_ATTN_ERR_HEADS;
+  if (c.kv_heads < 1 || c.kv_heads > 8192) return KARPO_ATTN_ERR_HEADS;
   if (b < 0 || c.blocks < 1 || c.blocks > INT32_MAX) return KARPO_ATTN_ERR_ARG;
   if (!c.keys || !c.values || !c.scales) return KARPO_ATTN_ERR_NULL;
   if (!aligned(c.keys, 16) || !aligned(c.values, 16) || !aligned(c.scales, 8)) return KARPO_ATTN_ERR_LAYOUT;
@@ -174,6 +175,12 @@ namespace {
 
 int64_t round_up(int64_t x, int64_t n) { return (x + n - 1) / n * n; }
 
+// A bound of the tokens that the queries of all requests see.
+int64_t seen_keys(const KarpoCacheAttendArgs* a) {
+  const int64_t each = (int64_t)a->max_q + a->window_left;
+  return a->window_left >= 0 && each < a->total_keys && each * a->n_seq < a->total_keys ? each * a->n_seq : a->total_keys;
+}
+
 // The rows that the queries can see, as packed bf16 keys and values, with the packed attention's own workspace behind them.
 struct Unpacked {
   int64_t rows, k_offset, v_offset, ws_offset;
@@ -182,10 +189,11 @@ struct Unpacked {
 };
 
 int unpacked_of(const KarpoCacheAttendArgs* a, Unpacked* u) {
-  int64_t rows = a->total_keys;
-  if (a->window_left >= 0) {  // each request's queries and the window before the first, from a multiple of 32 on
-    const int64_t each = (int64_t)a->max_q + a->window_left + kCacheGroup - 1;
-    if (each < rows && each * a->n_seq < rows) rows = each * a->n_seq;
+  // (with a window, each request's rows begin at a multiple of 32)
+  int64_t rows = seen_keys(a);
+  if (rows < a->total_keys) {
+    rows += (int64_t)(kCacheGroup - 1) * a->n_seq;
+    if (rows > a->total_keys) rows = a->total_keys;
   }
   const int64_t row_bytes = 2 * (int64_t)a->cache.kv_heads * a->cache.head_dim;
   u->rows = rows;
@@ -233,17 +241,34 @@ int check_attend(const KarpoCacheAttendArgs* a, CacheRef* c, CacheRows* r) {
   return KARPO_ATTN_OK;
 }
 
-// Whether the call's queries are few enough for the split path, which walks the keys once for each 64 vectors (head size 256:
-// 32, 512: 16); the other path unpacks them first. Unpacked against split, one request of 32,768 tokens: 128 vectors at head
-// size 128 181 us, 79 us; 256 vectors 230, 134; 1,024 vectors 471, 430; 16 requests of 2,048: 115, 87; 129, 141; 16 requests,
-// 256 vectors, two key/value heads 46, 58. Head size 256, 128 vectors: 190, 110; 128, 111; 256 vectors 218, 193; 149, 195.
-// Head size 512, 128 vectors: 214, 126; 157, 120; 256 vectors 227, 218; 195, 209.
+// Whether the split path, which walks the keys once for each tile of query vectors, is the faster one; the other unpacks the
+// keys and values first and has four launches. Both estimated in microseconds from the sizes, as measured: the split path's
+// walks (a tile holds 64 vectors, 32 at head size 256, 16 at 512), and the unpacking at the memory's rate and the packed
+// attention at the rate that it reaches with many query tiles, or with few of one request. Unpacked against split:
+//   one request of 32,768 tokens, 16 key/value heads of 128: 128 vectors 181, 79 us; 512 vectors 323, 232; 1,024 471, 430
+//   16 requests of 2,048: 128 vectors 115, 87; 256 vectors 129, 141; 512 vectors 174, 241
+//   8 heads of 256: one request, 256 vectors 218, 193; 512 vectors 291, 367; 16 requests, 128 vectors 128, 111; 256 149, 195
+//   4 heads of 512: one request, 128 vectors 214, 126; 512 vectors 294, 414; 16 requests, 128 vectors 157, 120
+//   one request of 2,000 tokens: 16 heads of 128, 1,024 vectors 67, 54; 8 of 256, 1,024 vectors 82, 72
 bool split(const KarpoCacheAttendArgs* a) {
-  return (int64_t)a->max_q * (a->heads / a->cache.kv_heads) <= (a->cache.head_dim <= 128 ? 256 : 128);
+  const int d = a->cache.head_dim;
+  const double vectors = (double)a->max_q * (a->heads / a->cache.kv_heads);
+  if (vectors <= 64) return true;
+  if (vectors >= 1 << 15) return false;  // (position_of holds below 2^16)
+  const double keys = (double)seen_keys(a) * a->cache.kv_heads, tile = d <= 128 ? 64 : d == 256 ? 32 : 16;
+  if (ceil(vectors / tile) * a->cache.kv_heads > 65535) return false;  // (a launch's second dimension)
+  const double walk = d == 64 ? 3.6e-5 : d == 128 ? 4.8e-5 : d == 256 ? 8e-5 : 9.3e-5;
+  const double query_tiles = a->n_seq * ceil(vectors / 128) * a->cache.kv_heads;
+  const double rate = a->n_seq == 1 && query_tiles < 256 ? 0.55e9 : d == 512 ? 0.8e9 : 1.3e9;  // operations a microsecond
+  const double by_split = 17 + keys * (walk * ceil(vectors / tile) + (a->n_seq > 1 ? 3e-5 : 0));
+  const double unpacked = 33 + keys * d * 0.9e-6 + 4 * vectors * keys * d / rate;
+  return by_split <= unpacked;
 }
 
 AttendShape shape_of(const KarpoCacheAttendArgs* a, const CacheRef& c, const CacheRows& r) {
-  return attend_shape(c, a->n_seq, a->heads / a->cache.kv_heads, a->max_q, a->total_keys < r.most ? a->total_keys : r.most);
+  int64_t seen = a->total_keys < r.most ? a->total_keys : r.most;
+  if (a->window_left >= 0 && (int64_t)a->max_q + a->window_left < seen) seen = (int64_t)a->max_q + a->window_left;
+  return attend_shape(c, a->n_seq, a->heads / a->cache.kv_heads, a->max_q, seen);
 }
 
 }  // namespace

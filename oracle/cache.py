@@ -147,3 +147,22 @@ def attention(query, key, value, scale, causal, window):
         s = torch.einsum("hgd,khd->hgk", q, k) * scale
         out[i] = torch.einsum("hgk,khd->hgd", torch.softmax(s, -1), v).reshape(query.shape[1:])
     return out
+
+
+def attention_whole(query, key, value, scale, causal, window):
+    """``attention`` of long runs at once, by a mask (no NaN among the keys and values)."""
+    lq, heads, d = query.shape
+    lk, kv_heads = key.shape[:2]
+    if lk == 0:
+        return torch.zeros_like(query)
+    q = query.view(lq, kv_heads, -1, d).permute(1, 2, 0, 3).reshape(kv_heads, -1, d)
+    s = torch.matmul(q, key.permute(1, 2, 0).contiguous()) * scale
+    at = torch.arange(lq, device=query.device)[:, None] + lk - lq
+    j = torch.arange(lk, device=query.device)[None, :]
+    seen = (j <= at) if causal else torch.ones((lq, lk), dtype=torch.bool, device=query.device)
+    if window >= 0:
+        seen = seen & (j >= at - window)
+    s.view(kv_heads, -1, lq, lk).masked_fill_(~seen, -math.inf)
+    p = torch.softmax(s, -1).nan_to_num(0.0)  # (a row that sees nothing)
+    o = torch.matmul(p, value.transpose(0, 1).contiguous())
+    return o.view(kv_heads, -1, lq, d).permute(2, 0, 1, 3).reshape(lq, heads, d)

@@ -81,6 +81,16 @@ def test_oracle_reserve_by_hand():
     assert out["free_left"] == 0 and out["lengths"] == [33, 65, 33]
 
 
+@pytest.mark.parametrize("causal,window", [(True, -1), (False, -1), (True, 3), (False, 0)])
+def test_oracle_attention_row_by_row_and_whole(causal, window):
+    gen = torch.Generator().manual_seed(0)
+    query, key, value = (torch.randn(n, h, 8, generator=gen, dtype=torch.float64) for n, h in ((9, 4), (7, 2), (7, 2)))
+    a = oracle.attention(query, key, value, 0.5, causal, window)
+    b = oracle.attention_whole(query, key, value, 0.5, causal, window)
+    assert torch.allclose(a, b, atol=1e-12)
+    assert not causal or (a[:2] == 0).all()
+
+
 # ---- refusals of the Python entry points (nothing here has a GPU: a call that passes the checks ends at the device's)
 
 def _cache(blocks=4, kv_heads=2, head_dim=64, block=32):
@@ -195,7 +205,7 @@ def _c_cache(**change):
 
 
 @pytest.mark.parametrize("change,status", [
-    ({"head_dim": 96}, _lib.ERR_HEAD_DIM), ({"kv_heads": 0}, _lib.ERR_HEADS), ({"block_size": 16}, _lib.ERR_ARG),
+    ({"head_dim": 96}, _lib.ERR_HEAD_DIM), ({"kv_heads": 0}, _lib.ERR_HEADS), ({"kv_heads": 8193}, _lib.ERR_HEADS), ({"block_size": 16}, _lib.ERR_ARG),
     ({"blocks": 0}, _lib.ERR_ARG), ({"blocks": 1 << 31}, _lib.ERR_ARG), ({"keys": None}, 1), ({"values": None}, 1),
     ({"scales": None}, 1), ({"keys": 4100}, _lib.ERR_LAYOUT), ({"scales": 4100}, _lib.ERR_LAYOUT)], ids=str)
 def test_c_abi_refuses_caches(change, status):

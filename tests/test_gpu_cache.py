@@ -287,7 +287,7 @@ def test_read_writes_no_row_past_its_bound(gpu):
 # ---- attend
 
 def _attend_case(device, head_dim, heads, kv_heads, block, lengths, counts, window=-1, causal=True, scale=None, seed=0,
-                 trailing=0, wide=1):
+                 trailing=0, wide=1, oracle_too=True):
     scale = 1 / math.sqrt(head_dim) if scale is None else scale
     width = max(1, -(-max(lengths) // block)) + wide
     gen = torch.Generator().manual_seed(seed)
@@ -295,7 +295,6 @@ def _attend_case(device, head_dim, heads, kv_heads, block, lengths, counts, wind
     blocks = len(pool)
     cache = _random_cache(device, blocks, kv_heads, head_dim, block, seed)
     cache.scales.copy_(torch.exp2(torch.randint(-9, -6, cache.scales.shape, generator=gen).float()))
-    want = oracle.Cache(cache.keys, cache.values, cache.scales, block)
     table = [[pool.pop() for _ in range(-(-x // block))] for x in lengths]
     table = [r + [-1] * (width - len(r)) for r in table]
     # the tokens in use hold no NaN (leftovers behind them do)
@@ -307,7 +306,7 @@ def _attend_case(device, head_dim, heads, kv_heads, block, lengths, counts, wind
                 n = min(block, x - j * block)
                 part = raw[table[i][j]][:, at[:n].reshape(-1)]
                 raw[table[i][j]][:, at[:n].reshape(-1)] = torch.where((part & 127) == 127, part - 1, part)
-    want = oracle.Cache(cache.keys, cache.values, cache.scales, block)
+    want = oracle.Cache(cache.keys, cache.values, cache.scales, block) if oracle_too else None
     rows = sum(counts) + trailing
     query = torch.randn((rows, heads, head_dim), generator=gen).bfloat16()
     q_cu = [0]
@@ -355,6 +354,54 @@ def test_windows(gpu, window, causal):
     (512, 4, 1, [260, 33], [120, 33], -1)])
 def test_chunks_of_prompts(gpu, head_dim, heads, kv_heads, lengths, counts, window):
     _attend_and_compare(gpu, head_dim, heads, kv_heads, 64, lengths, counts, window=window)
+
+
+def _workspace(cache, heads, max_q, total_q, total_keys, n, width, window):
+    """Bytes that the call's path asks for: the unpacked keys and values are in them, or they are not."""
+    import ctypes
+
+    from karpo_decision_amd import _lib
+    c = _lib.KarpoCache(*(t.data_ptr() for t in cache[:3]), cache.blocks, cache.kv_heads, cache.head_dim, cache.block_size)
+    a = _lib.KarpoCacheAttendArgs(c, 4096, 4096, 8, 8, 8, 8, 4096, 4096, 4096, width, width, n, heads, max_q, total_q,
+                                  total_keys, 0.1, window, 0)
+    need = ctypes.c_size_t()
+    _lib.check(_lib.load().karpo_cache_attend_workspace_bytes(ctypes.byref(a), ctypes.byref(need)), "bytes")
+    return need.value
+
+
+@pytest.mark.parametrize("head_dim,heads,kv_heads,lengths,counts,window,causal", [
+    (64, 32, 2, [5100, 3000], [1500, 900], -1, True), (128, 32, 4, [3000, 1777], [1500, 1777], -1, True),
+    (128, 32, 4, [3000, 2100, 0, 40], [1500, 1000, 3, 41], 600, True), (256, 16, 2, [2500, 1900], [800, 700], -1, False),
+    (256, 16, 2, [2500, 2900], [900, 800], 333, True), (512, 8, 1, [2000, 900], [700, 900], -1, True)])
+def test_long_chunks(gpu, head_dim, heads, kv_heads, lengths, counts, window, causal):
+    """Chunks long enough that the keys are unpacked first, against 64-bit products on the GPU."""
+    block = 64
+    cache, _, table, query, q_cu, scale = _attend_case(gpu, head_dim, heads, kv_heads, block, lengths, counts, oracle_too=False)
+    rows = sum(lengths)
+    need = _workspace(cache, heads, max(counts), sum(counts), rows, len(lengths), len(table[0]), window)
+    seen = rows if window < 0 else min(rows, len(lengths) * (max(counts) + window))
+    assert need > 4 * seen * kv_heads * head_dim  # the path that unpacks
+    query = query.to(gpu)
+    with torch.inference_mode():
+        out = kv_cache.attend(query, cache, ints(table, gpu), ints(q_cu, gpu), ints(lengths, gpu), max(counts), scale,
+                              causal=causal, window=window, total_keys=rows)
+        key, value, k_cu = kv_cache.read(cache, ints(table, gpu), ints(lengths, gpu), rows)  # (test_read: exact)
+    k_cu = k_cu.tolist()
+    for i in range(len(lengths)):
+        q, k, v = query[q_cu[i]:q_cu[i + 1]].double(), key[k_cu[i]:k_cu[i + 1]].double(), value[k_cu[i]:k_cu[i + 1]].double()
+        want = oracle.attention_whole(q, k, v, scale, causal, window)
+        size = oracle.attention_whole(q, k, v.abs(), scale, causal, window)
+        off = (out[q_cu[i]:q_cu[i + 1]].double() - want).abs()
+        assert (off <= want.abs() * 2.0 ** -8 + size * (2.0 ** -8 + 2.0 ** -14)).all(), (i, off.max())
+
+
+@pytest.mark.parametrize("head_dim,heads,kv_heads,lengths,counts", [
+    (64, 16, 1, [700, 41], [70, 41]), (128, 24, 2, [1100, 300], [100, 7]), (256, 12, 1, [900], [60]),
+    (512, 16, 1, [500, 64], [30, 64])])
+def test_many_tiles_of_queries(gpu, head_dim, heads, kv_heads, lengths, counts):
+    """The split path with several workgroups for a request's query vectors, the last of them not full."""
+    _attend_and_compare(gpu, head_dim, heads, kv_heads, 32, lengths, counts)
+    assert max(counts) * heads // kv_heads > 64
 
 
 def test_more_queries_than_tokens(gpu):
