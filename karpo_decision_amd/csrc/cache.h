@@ -83,7 +83,8 @@ struct AttendParams {
   // 52.8 us, 131,072 tokens at 512 105.0 -> 93.6; where several read them, 128 vectors over 32,768 tokens, 80 -> 88)
   int32_t once;
   int32_t left, right;
-  float scale;         // times log2(e)
+  float scale;         // its magnitude times log2(e), at least 1e-30 (hidden scores, -infinity, stay that)
+  uint32_t sign;       // 0x80008000 where the scale is negative: the queries are
   int32_t parts;       // workgroups for each of the grid's y
   float* partial;      // [y][parts][2] of (O [vectors][D], m [vectors], l [vectors])
   int32_t* units;      // [n_seq + 1] groups of 32 tokens before each request

@@ -95,6 +95,15 @@ __device__ __forceinline__ bf16x8 operand(unsigned a, unsigned b, float scale) {
   return __builtin_bit_cast(bf16x8, bf16_of_8(a, b, scale));
 }
 
+// Two fp32 as packed bf16, in one instruction.
+__device__ __forceinline__ unsigned pair_of(float a, float b) {
+  return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{a, b}), bf16x2));
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
+}
+
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // Which of a word's four codes are NaN, as 0x80 in their bytes.
@@ -212,7 +221,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
         for (int c = 0; c < kMine; ++c) {
           const int e = wave + c * kAttendWaves;
           if (2 * kChunks >= kAttendWaves || e < 2 * kChunks)
-            q_mine[n][c] = *reinterpret_cast<const u32x4*>(src + (e >> 1) * 64 + quad * 16 + (e & 1) * 8);
+            q_mine[n][c] = *reinterpret_cast<const u32x4*>(src + (e >> 1) * 64 + quad * 16 + (e & 1) * 8) ^ p.sign;
         }
         lo[n] = p.left < 0 ? 0 : pos + shift - p.left;
         hi[n] = p.right < 0 ? s.tokens - 1 : (int)min<int64_t>((int64_t)pos + shift + p.right, s.tokens - 1);
@@ -325,7 +334,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
         for (int n = 0; n < NT; ++n) {
           float x[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = st[n][e >> 2][e & 3] * p.scale;
+          for (int e = 0; e < 8; ++e) x[e] = st[n][e >> 2][e & 3];
           is_seen[n] = 0;
           if (masked) {
 #pragma unroll
@@ -336,10 +345,8 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
               is_seen[n] |= sees ? 1u << e : 0u;
             }
           }
-          float best = x[0];
-#pragma unroll
-          for (int e = 1; e < 8; ++e) best = __builtin_elementwise_maximum(best, x[e]);
-          best = column_max(best);
+          float best = max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max3(x[6], x[7], x[7]));
+          best = column_max(best) * p.scale;
           // the running maximum is raised (and O rescaled) only where it grows by more than 2^8: weights are then at most 2^8
           if (__any(!(best <= top[n] + 8.f) && best != -INFINITY)) {
             const float up = __builtin_elementwise_maximum(top[n], best);
@@ -350,15 +357,19 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
             for (int t = 0; t < D / 16; ++t) o[n][t] *= f;
           }
           const float base = top[n] == -INFINITY ? 0.f : top[n];
-          float add = 0.f;
+          float w[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float w = __builtin_amdgcn_exp2f(x[e] - base);
-            add += w;
-            const __bf16 high = (__bf16)w;
-            weight[n][0][e] = high;
-            weight[n][1][e] = (__bf16)(w - (float)high);
+          for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], p.scale, -base));
+          u32x4 high, low;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            high[e] = pair_of(w[2 * e], w[2 * e + 1]);
+            low[e] = pair_of(w[2 * e] - __uint_as_float(high[e] << 16),
+                             w[2 * e + 1] - __uint_as_float(high[e] & 0xffff0000u));
           }
+          weight[n][0] = __builtin_bit_cast(bf16x8, high);
+          weight[n][1] = __builtin_bit_cast(bf16x8, low);
+          const float add = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
           sum[n] += add;
         }
 

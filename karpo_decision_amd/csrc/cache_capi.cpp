@@ -319,7 +319,9 @@ extern "C" int karpo_cache_attend(const KarpoCacheAttendArgs* a, void* stream) {
     t.group = a->heads / a->cache.kv_heads;
     t.left = a->window_left >= kMostTokens ? -1 : a->window_left;  // (sees everything, and stays within 32 bits)
     t.right = a->window_right;
-    t.scale = a->scale * 1.4426950408889634f;
+    t.scale = fabsf(a->scale) * 1.4426950408889634f;
+    if (!(t.scale > 1e-30f)) t.scale = 1e-30f;
+    t.sign = a->scale < 0.f ? 0x80008000u : 0u;
     t.per_group = 1.f / t.group;
     t.whole = shape.whole;
     t.once = shape.tiles == 1;
