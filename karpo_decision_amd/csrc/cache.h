@@ -79,9 +79,6 @@ struct AttendParams {
   int32_t group;       // heads / kv_heads
   float per_group;     // 1 / group
   int32_t whole;       // a workgroup takes a request whole (nothing to join)
-  // one workgroup's walk reads a request's codes, once: streamed through the caches (48 requests at head size 128 58.8 ->
-  // 52.8 us, 131,072 tokens at 512 105.0 -> 93.6; where several read them, 128 vectors over 32,768 tokens, 80 -> 88)
-  int32_t once;
   int32_t left, right;
   float scale;         // its magnitude times log2(e), at least 1e-30 (hidden scores, -infinity, stay that)
   uint32_t sign;       // 0x80008000 where the scale is negative: the queries are

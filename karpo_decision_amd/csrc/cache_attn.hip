@@ -16,16 +16,12 @@ constexpr int kAttendThreads = 64 * kAttendWaves;
 __host__ __device__ constexpr int attend_waves(int d, int nt) {
   return nt == 1 && d <= 128 ? 4 : d == 64 && nt == 2 ? 3 : d <= 128 || (d == 256 && nt == 1) ? 2 : 1;
 }
-// Bytes of LDS for the waves' copies of a group's keys and values, and behind them the query vectors; the waves' sums take
-// the same bytes when the groups are done.
-constexpr int ring_bytes(int d) { return kAttendWaves * 2 * kCacheGroup * d; }
-constexpr int data_bytes(int d, int nt) { return ring_bytes(d) + 16 * nt * d * 2; }
-// Elements of the output that the waves join at once.
-constexpr int slab_of(int d, int nt) {
-  int slab = d;
-  while (kAttendWaves * 16 * nt * (slab + 4) * 4 > data_bytes(d, nt)) slab /= 2;
-  return slab;
-}
+// Bytes of LDS for the waves' copies of a group's keys (as many for the values).
+constexpr int ring_bytes(int d) { return kAttendWaves * kCacheGroup * d; }
+// Elements of the output that the waves join at once, and their sums' bytes (in the keys' array, when the groups are done).
+constexpr int slab_of(int d, int nt) { return nt == 1 && d > 64 ? d / 2 : d / 4 > 32 ? d / 4 : 32; }
+constexpr int sums_bytes(int d, int nt) { return kAttendWaves * 16 * nt * (slab_of(d, nt) + 4) * 4; }
+
 // Requests of which at most this many tokens are seen are not split (a quarter of it at head size 512): one workgroup walks
 // their groups, five a wave, and there is nothing to join. Split against whole, 8 requests: head size 64, 512 tokens 16.9,
 // 12.8 us, 2,048 tokens 16.7, 21.6; 128, 768 tokens 16.7, 13.9, 1,024 tokens 16.6, 16.7; 256, 512 tokens 16.7, 14.5, 768
@@ -109,12 +105,15 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 // Which of a word's four codes are NaN, as 0x80 in their bytes.
 __device__ __forceinline__ unsigned nan_codes(unsigned w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
+// ONCE: one workgroup reads a request's codes of a head, once; they are streamed through the caches (48 requests at head size
+// 128 58.8 -> 52.8 us, 131,072 tokens at 512 105.0 -> 93.6; where several workgroups read them, 128 vectors over 32,768
+// tokens, 80 -> 88).
 // One lane's view of a group of 32 tokens with 16x16x32 matrix instructions: S^T = K Q^T has the keys as rows (two tiles),
 // the query vectors as columns: column lane % 16, keys 16 t + 4 (lane / 16) + i. Those are this lane's eight weights, and as
 // they stand the second operand of O^T = V^T P^T, whose first operand, 8 of these keys of one element, is 8 bytes of the cache.
 // The products are of bf16 operands (a cached element is one exactly); the weights enter as two bf16 terms, 2^-17 off, which
 // costs matrix work that this kernel, bound by the codes' way from HBM, has to spare.
-template <int D, int NT>
+template <int D, int NT, bool ONCE>
 __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_kernel(
     const AttendParams p) {
   constexpr int kLoads = D / 32;       // KiB of keys, and of values, in a group
@@ -125,14 +124,15 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
   __shared__ Seen s_seen;
   __shared__ int s_at[2];
   __shared__ float s_m[kAttendWaves][kVectors], s_l[kAttendWaves][kVectors];
-  __shared__ __align__(16) char s_data[data_bytes(D, NT)];
-  static_assert(kSlab % 16 == 0);
-  u32x4* const s_q = reinterpret_cast<u32x4*>(s_data + ring_bytes(D));
-  float(*const s_o)[kVectors][kSlab + 4] = reinterpret_cast<float(*)[kVectors][kSlab + 4]>(s_data);
+  // (arrays of their own: a read then waits for the copies into its own array and no others)
+  __shared__ __align__(16) char s_keys[ring_bytes(D) > sums_bytes(D, NT) ? ring_bytes(D) : sums_bytes(D, NT)];
+  __shared__ __align__(16) char s_values[ring_bytes(D)];
+  __shared__ u32x4 s_q[kVectors * D / 8];
+  float(*const s_o)[kVectors][kSlab + 4] = reinterpret_cast<float(*)[kVectors][kSlab + 4]>(s_keys);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
-  KA_LDS char* const key_ring = (KA_LDS char*)s_data + wave * (2 * kCacheGroup * D);
-  KA_LDS char* const value_ring = key_ring + kCacheGroup * D;
+  KA_LDS char* const key_ring = (KA_LDS char*)s_keys + wave * (kCacheGroup * D);
+  KA_LDS char* const value_ring = (KA_LDS char*)s_values + wave * (kCacheGroup * D);
   const int heads = p.c.kv_heads, b = p.c.block_log2;
   const int h = blockIdx.y % heads, vector0 = (blockIdx.y / heads) * kVectors;
 
@@ -255,40 +255,32 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
         k_scales = sc.x;
         v_scales = sc.y;
       };
-      // one group's codes into the wave's ring, 16 bytes a lane and KiB; zeros for a block that is not of the pool
-      auto copy = [&](const uint8_t* from, KA_LDS char* to, int g, int k) {
-        const int id = __builtin_amdgcn_readlane(ids, k);
+      // One group's codes into the wave's ring, 16 bytes a lane and KiB; zeros for a block that is not of the pool, and where
+      // there is no group (so that every turn of the loop issues the same copies, and a wait can count them).
+      auto copy = [&](const uint8_t* from, KA_LDS char* to, int g, int k, bool any) {
+        const int id = __builtin_amdgcn_readlane(ids, k & 63);
         const int64_t head = (int64_t)max(id, 0) * heads + h;
         const uint8_t* const src = from + ((head << b) + (int64_t)(g & ((1 << (b - 5)) - 1)) * kCacheGroup) * D;
         const __amdgpu_buffer_rsrc_t r =
-            __builtin_amdgcn_make_buffer_rsrc((void*)src, (short)0, id >= 0 ? kCacheGroup * D : 0, kBufferFlags);
-        if (p.once) {
+            __builtin_amdgcn_make_buffer_rsrc((void*)src, (short)0, any && id >= 0 ? kCacheGroup * D : 0, kBufferFlags);
 #pragma unroll
-          for (int t = 0; t < kLoads; ++t)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (KA_LDS void*)(to + t * 1024), 16, lane_offset, t * 1024, 0,
-                                                     kCopyStream);
-        } else {
-#pragma unroll
-          for (int t = 0; t < kLoads; ++t)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (KA_LDS void*)(to + t * 1024), 16, lane_offset, t * 1024, 0, 0);
-        }
+        for (int t = 0; t < kLoads; ++t)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (KA_LDS void*)(to + t * 1024), 16, lane_offset, t * 1024, 0,
+                                                   ONCE ? kCopyStream : 0);
       };
       auto tile = [&](const KA_LDS char* ring, int t) {
         return *reinterpret_cast<const KA_LDS u32x4*>(ring + t * 1024 + lane * 16);
       };
-      // the copies of all but the last `later` KiB have arrived / the reads of the ring are done
-      auto arrived = [&](bool later) {
-        if (later) wait_vmcnt<kLoads>(); else wait_vmcnt<0>();
+      // all but the last issued group's keys, or values, have arrived / the reads of the ring are done
+      auto arrived = [&]() {
+        wait_vmcnt<kLoads>();
         asm volatile("" ::: "memory");
       };
       auto read_out = [&]() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
 
       int k = 0;
-      if (g0 + wave < g1) {
-        look_up(g0 + wave);
-        copy(p.c.keys, key_ring, g0 + wave, 0);
-        copy(p.c.values, value_ring, g0 + wave, 0);
-      }
+      const bool some = g0 + wave < g1;
+      if (some) look_up(g0 + wave);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -296,13 +288,17 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
           const int e = wave + c * kAttendWaves;
           if (2 * kChunks >= kAttendWaves || e < 2 * kChunks) s_q[(e * NT + n) * 64 + lane] = q_mine[n][c];
         }
+      if (some) {
+        copy(p.c.keys, key_ring, g0 + wave, 0, true);
+        copy(p.c.values, value_ring, g0 + wave, 0, true);
+      }
       // (a barrier that leaves the copies in flight)
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
       for (int g = g0 + wave; g < g1; g += kAttendWaves) {
         const float k_scale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(k_scales), k));
         const float v_scale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v_scales), k));
         const int next = g + kAttendWaves;
-        arrived(true);
+        arrived();
         f32x4 st[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) st[n][0] = st[n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -324,7 +320,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
           look_up(next);
           k = 0;
         }
-        if (next < g1) copy(p.c.keys, key_ring, next, k);
+        copy(p.c.keys, key_ring, next, k, next < g1);
 
         const int key0 = g * kCacheGroup;
         const bool masked = key0 < full_lo || key0 + kCacheGroup - 1 > full_hi;
@@ -373,7 +369,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
           sum[n] += add;
         }
 
-        arrived(next < g1);
+        arrived();
         bool nan = false;
         if (masked) {
           unsigned any = 0;
@@ -426,8 +422,10 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
           }
         }
         read_out();
-        if (next < g1) copy(p.c.values, value_ring, next, k);
+        copy(p.c.values, value_ring, next, k, next < g1);
       }
+
+      wait_vmcnt<0>();  // (the copies of no group, into what the sums take)
 
       // join the waves
 #pragma unroll
@@ -580,7 +578,10 @@ __global__ __launch_bounds__(256) void join_kernel(const AttendParams p, int vec
 template <int D, int NT>
 void launch(const AttendParams& p, const AttendShape& s, hipStream_t stream) {
   const unsigned y = (unsigned)(p.c.kv_heads * s.tiles), x = (unsigned)(p.whole ? p.r.n_seq : s.parts);
-  attend_kernel<D, NT><<<dim3(x, y), dim3(kAttendThreads), 0, stream>>>(p);
+  if (s.tiles == 1)
+    attend_kernel<D, NT, true><<<dim3(x, y), dim3(kAttendThreads), 0, stream>>>(p);
+  else
+    attend_kernel<D, NT, false><<<dim3(x, y), dim3(kAttendThreads), 0, stream>>>(p);
   if (p.whole) return;
   // a workgroup for 64 elements of each vector, or as many as fill the GPU several times over
   const int64_t pairs = (int64_t)p.r.n_seq * y, most = (2048 + pairs - 1) / pairs, items = (int64_t)s.used * (D / 64);

@@ -244,12 +244,14 @@ int check_attend(const KarpoCacheAttendArgs* a, CacheRef* c, CacheRows* r) {
 // Whether the split path, which walks the keys once for each tile of query vectors, is the faster one; the other unpacks the
 // keys and values first and has four launches. Both estimated in microseconds from the sizes, as measured: the split path's
 // walks (a tile holds 64 vectors, 32 at head size 256, 16 at 512), and the unpacking at the memory's rate and the packed
-// attention at the rate that it reaches with many query tiles, or with few of one request. Unpacked against split:
-//   one request of 32,768 tokens, 16 key/value heads of 128: 128 vectors 181, 79 us; 512 vectors 323, 232; 1,024 471, 430
-//   16 requests of 2,048: 128 vectors 115, 87; 256 vectors 129, 141; 512 vectors 174, 241
-//   8 heads of 256: one request, 256 vectors 218, 193; 512 vectors 291, 367; 16 requests, 128 vectors 128, 111; 256 149, 195
-//   4 heads of 512: one request, 128 vectors 214, 126; 512 vectors 294, 414; 16 requests, 128 vectors 157, 120
-//   one request of 2,000 tokens: 16 heads of 128, 1,024 vectors 67, 54; 8 of 256, 1,024 vectors 82, 72
+// attention at the rate that it reaches with many query tiles, or with few of one or two requests. Of 198 shapes (head sizes
+// 64 to 512, 1 to 16 requests of 700 to 32,768 tokens, 16 to 4,096 vectors) the rule's choice is over 15% slower than the
+// other for four. Unpacked against split:
+//   one request of 32,768 tokens, 16 key/value heads of 128: 128 vectors 166, 76 us; 512 vectors 307, 213; 1,024 460, 402
+//   16 requests of 2,048: 128 vectors 103, 82; 256 vectors 119, 126; 512 vectors 168, 213
+//   8 heads of 256: one request, 256 vectors 210, 158; 1,024 vectors 445, 584; 16 requests, 128 vectors 118, 101; 256 144, 175
+//   4 heads of 512: one request, 512 vectors 284, 306; 1,024 vectors 436, 589; 16 requests, 512 vectors 251, 305
+//   one request of 2,000 tokens: 16 heads of 128, 1,024 vectors 62, 53; 8 of 256, 71, 64; 4 of 512, 77, 60
 bool split(const KarpoCacheAttendArgs* a) {
   const int d = a->cache.head_dim;
   const double vectors = (double)a->max_q * (a->heads / a->cache.kv_heads);
@@ -257,9 +259,10 @@ bool split(const KarpoCacheAttendArgs* a) {
   if (vectors >= 1 << 15) return false;  // (position_of holds below 2^16)
   const double keys = (double)seen_keys(a) * a->cache.kv_heads, tile = d <= 128 ? 64 : d == 256 ? 32 : 16;
   if (ceil(vectors / tile) * a->cache.kv_heads > 65535) return false;  // (a launch's second dimension)
-  const double walk = d == 64 ? 3.6e-5 : d == 128 ? 4.8e-5 : d == 256 ? 8e-5 : 9.3e-5;
+  const double walk = d == 64 ? 3.5e-5 : d == 128 ? 4.6e-5 : 6.5e-5;
   const double query_tiles = a->n_seq * ceil(vectors / 128) * a->cache.kv_heads;
-  const double rate = a->n_seq == 1 && query_tiles < 256 ? 0.55e9 : d == 512 ? 0.8e9 : 1.3e9;  // operations a microsecond
+  const double most = d == 512 ? 0.8e9 : 1.3e9, few = 0.35e9 + 0.5e6 * vectors;  // operations a microsecond
+  const double rate = a->n_seq <= 2 && query_tiles < 256 && few < most ? few : most;
   const double by_split = 17 + keys * (walk * ceil(vectors / tile) + (a->n_seq > 1 ? 3e-5 : 0));
   const double unpacked = 33 + keys * d * 0.9e-6 + 4 * vectors * keys * d / rate;
   return by_split <= unpacked;
@@ -324,7 +327,6 @@ extern "C" int karpo_cache_attend(const KarpoCacheAttendArgs* a, void* stream) {
     t.sign = a->scale < 0.f ? 0x80008000u : 0u;
     t.per_group = 1.f / t.group;
     t.whole = shape.whole;
-    t.once = shape.tiles == 1;
     t.parts = shape.parts;
     if (!shape.whole) {
       t.units = static_cast<int32_t*>(a->workspace);
