@@ -105,14 +105,26 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 // Which of a word's four codes are NaN, as 0x80 in their bytes.
 __device__ __forceinline__ unsigned nan_codes(unsigned w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
-// ONCE: one workgroup reads a request's codes of a head, once; they are streamed through the caches (48 requests at head size
-// 128 58.8 -> 52.8 us, 131,072 tokens at 512 105.0 -> 93.6; where several workgroups read them, 128 vectors over 32,768
-// tokens, 80 -> 88).
 // One lane's view of a group of 32 tokens with 16x16x32 matrix instructions: S^T = K Q^T has the keys as rows (two tiles),
 // the query vectors as columns: column lane % 16, keys 16 t + 4 (lane / 16) + i. Those are this lane's eight weights, and as
 // they stand the second operand of O^T = V^T P^T, whose first operand, 8 of these keys of one element, is 8 bytes of the cache.
 // The products are of bf16 operands (a cached element is one exactly); the weights enter as two bf16 terms, 2^-17 off, which
-// costs matrix work that this kernel, bound by the codes' way from HBM, has to spare.
+// costs matrix work that this kernel, bound by the codes' way from HBM, has to spare (one term: 1.4 times the plain form's
+// error against 64 bits; two: the plain form's).
+//
+// A wave takes every fourth group of its workgroup's share by itself, its running maximum and sums in registers, the next
+// group's keys on their way to LDS while this one's weights are made, the next values while the next keys are read: a group in
+// flight a wave (8 KiB at head size 128, four waves a SIMD; 32 KiB at 512, one). Registers for them instead of LDS spilled at
+// head size 512: 240 us for one token over 131,072, 119 with LDS. Nothing but a request's end joins the waves.
+//
+// Measured (codes read / time of this kernel): 48 requests, 60,000 tokens in all, 16 heads of 128: 43.6 us, 5.6 TB/s; one of
+// 131,072 tokens, 4 heads of 512: 87.6 us, 6.1 TB/s; 32 requests, 4 tokens each, 1,024 seen, 8 heads of 256: 28.9 us, 3.9 TB/s
+// (8 us of it start and end: 2.3 us to the first table entry, then every wave's first group at once, 33 MB). A large copy
+// moves 4.9 TB/s.
+//
+// ONCE: one workgroup reads a request's codes of a head, once; they are streamed through the caches (48 requests at head size
+// 128 58.8 -> 52.8 us, 131,072 tokens at 512 105.0 -> 93.6; where several workgroups read them, 128 vectors over 32,768
+// tokens, 80 -> 88).
 template <int D, int NT, bool ONCE>
 __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_kernel(
     const AttendParams p) {
@@ -494,7 +506,8 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
 // Joins a request's shares: O = sum of 2^(m_w - M) O_w over sum of 2^(m_w - M) l_w, in an order that the sizes alone set.
 // Requests that one workgroup took whole are done already. Up to kFew shares: a thread walks them for four elements of a
 // vector. More: 64 elements of a vector by 16 threads of four and 16 rows, each row with every sixteenth share (so that
-// up to 16 cost one round of loads), and the rows joined through LDS.
+// up to 16 cost one round of loads), and the rows joined through LDS. 4.2 to 5.9 us, launch and four rounds of loads; 33 us with
+// one walk over 64 shares of one request.
 template <int D>
 __global__ __launch_bounds__(256) void join_kernel(const AttendParams p, int vectors_per) {
   constexpr int kSlabs = D / 64, kFew = 4;
