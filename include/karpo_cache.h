@@ -48,7 +48,7 @@ extern "C" {
                                       free_count outside the list */
 
 typedef struct KarpoCache {
-  void* keys;        /* device, [blocks][kv_heads][block_size * head_dim] e4m3, 16-byte aligned */
+  void* keys;        /* device, apart from values, [blocks][kv_heads][block_size * head_dim] e4m3, 16-byte aligned */
   void* values;      /* the same */
   float* scales;     /* device, [blocks][kv_heads][2] fp32: 2^e of the keys, of the values; 8-byte aligned */
   int64_t blocks;
@@ -106,7 +106,7 @@ typedef struct KarpoCacheReadArgs {
 typedef struct KarpoCacheAttendArgs {
   KarpoCache cache;
   const void* q; /* device, [total_q][heads][head_dim] bf16, head_dim contiguous, strides multiples of 8, 16-byte aligned */
-  void* o;       /* the same */
+  void* o;       /* the same; must not overlap q */
   int64_t q_stride_tok, q_stride_head, o_stride_tok, o_stride_head;
   const int32_t* q_cu;    /* device, [n_seq + 1]: query rows of each request */
   const int32_t* lengths; /* device, [n_seq]: cached tokens of each request, its queries' own tokens among them: query
@@ -118,7 +118,7 @@ typedef struct KarpoCacheAttendArgs {
   int32_t heads; /* a multiple of cache.kv_heads */
   int32_t max_q; /* a bound of every request's query rows */
   int64_t total_q;
-  int64_t total_keys; /* a bound of the lengths' sum */
+  int64_t total_keys; /* a bound of the lengths' sum: the keys of long query runs are unpacked into the workspace */
   float scale;
   int32_t window_left, window_right; /* -1: unbounded; causal is window_right 0 */
   void* workspace;

@@ -132,6 +132,8 @@ extern "C" int karpo_cache_append(const KarpoCacheAppendArgs* a, void* stream) {
   if (st != KARPO_ATTN_OK) return st;
   if (a->rows < 0 || a->rows > INT32_MAX || a->n_writes < 0 || a->n_writes > INT32_MAX / (2 * a->cache.kv_heads))
     return KARPO_ATTN_ERR_ARG;
+  const int64_t bytes = p.c.blocks * ((int64_t)p.c.kv_heads * p.c.head_dim << p.c.block_log2);
+  if (overlaps(p.c.keys, bytes, p.c.values, bytes)) return KARPO_ATTN_ERR_ARG;  // (either's writes would be the other's)
   if (a->rows == 0 || a->n_writes == 0) return KARPO_ATTN_OK;
   if (!a->k || !a->v || !a->writes) return KARPO_ATTN_ERR_NULL;
   if (!row_strides(a->k, a->k_stride_tok, a->k_stride_head) || !row_strides(a->v, a->v_stride_tok, a->v_stride_head) ||
@@ -195,6 +197,7 @@ int unpacked_of(const KarpoCacheAttendArgs* a, Unpacked* u) {
     rows += (int64_t)(kCacheGroup - 1) * a->n_seq;
     if (rows > a->total_keys) rows = a->total_keys;
   }
+  if (rows < 1) rows = 1;  // (a key bound of 0 would not be checked)
   const int64_t row_bytes = 2 * (int64_t)a->cache.kv_heads * a->cache.head_dim;
   u->rows = rows;
   u->k_offset = round_up(4 * ((int64_t)a->n_seq + 1), 256);
@@ -298,7 +301,7 @@ extern "C" int karpo_cache_attend(const KarpoCacheAttendArgs* a, void* stream) {
   memset(&p, 0, sizeof(p));
   int st = check_attend(a, &p.c, &p.r);
   if (st != KARPO_ATTN_OK) return st;
-  if (a->total_q == 0 || a->n_seq == 0) return KARPO_ATTN_OK;
+  if (a->total_q == 0 || a->n_seq == 0 || a->max_q == 0) return KARPO_ATTN_OK;
   if (!a->q || !a->o || !a->q_cu) return KARPO_ATTN_ERR_NULL;
   if (!row_strides(a->q, a->q_stride_tok, a->q_stride_head) || !row_strides(a->o, a->o_stride_tok, a->o_stride_head))
     return KARPO_ATTN_ERR_LAYOUT;
@@ -323,7 +326,7 @@ extern "C" int karpo_cache_attend(const KarpoCacheAttendArgs* a, void* stream) {
     t.left = a->window_left >= kMostTokens ? -1 : a->window_left;  // (sees everything, and stays within 32 bits)
     t.right = a->window_right;
     t.scale = fabsf(a->scale) * 1.4426950408889634f;
-    if (!(t.scale > 1e-30f)) t.scale = 1e-30f;
+    if (t.scale < 1e-30f) t.scale = 1e-30f;  // (NaN stays)
     t.sign = a->scale < 0.f ? 0x80008000u : 0u;
     t.per_group = 1.f / t.group;
     t.whole = shape.whole;

@@ -9,6 +9,7 @@ A serving step over requests that hold cached tokens (a prompt that more rounds 
 ``hip_attention.attend`` reads keys that live for one call; here they live in a pool of blocks of 32, 64 or 128 tokens
 (``Cache``), found through a block table. An element is stored as an e4m3 code times a power of two that its block and
 head share, so a cached element is a bf16 value exactly, and ``read`` and ``attend`` work on the same numbers.
+Blocks that several requests' tables share are read only: a request appends to blocks of its own.
 
 Lengths, bounds, tables and free lists are read on the device when the kernels run: nothing syncs, calls go on the
 current stream of the tensors' device and capture into graphs. All of it is forward only.
@@ -29,6 +30,7 @@ from .ops import _current_stream, _on_device
 BLOCK_SIZES = (32, 64, 128)
 HEAD_DIMS = (64, 128, 256, 512)
 _MOST = (1 << 31) - 1
+_MOST_ROWS = _MOST - (1 << 16)
 
 # The argument structures of karpo_cache.h, field by field (_lib has them by name): packing them costs a third of what
 # building them by name does, and a small call's time is its host path.
@@ -176,8 +178,8 @@ def reserve(table: Tensor, lengths: Tensor, counts: Tensor, free: Tensor, free_c
     if counts.numel() != n or free_count.numel() != 1:
         raise ValueError(f"counts must hold {n} requests and free_count one number, not {counts.numel()} and "
                          f"{free_count.numel()}")
-    if rows < 0 or block_size not in BLOCK_SIZES:
-        raise ValueError(f"rows must be non-negative and block_size 32, 64 or 128, not {rows} and {block_size}")
+    if not 0 <= rows <= _MOST_ROWS or block_size not in BLOCK_SIZES:
+        raise ValueError(f"rows must lie in 0 .. {_MOST_ROWS} and block_size be 32, 64 or 128, not {rows} and {block_size}")
     _on_gpu("reserve", index)
     lib = _lib.load()
     jobs = lib.karpo_cache_writes_capacity(rows, n, block_size)
@@ -234,8 +236,8 @@ def read(cache: Cache, table: Tensor, lengths: Tensor, rows: int) -> tuple[Tenso
     fields = _cache_fields(cache, index)
     rows_fields = _table_fields(table, lengths, index)
     rows = int(rows)
-    if rows < 0:
-        raise ValueError(f"rows must be non-negative, not {rows}")
+    if not 0 <= rows <= _MOST_ROWS:
+        raise ValueError(f"rows must lie in 0 .. {_MOST_ROWS}, not {rows}")
     _on_gpu("read", index)
     shape = (rows, fields[4], fields[5])
     key, value = table.new_empty(shape, dtype=torch.bfloat16), table.new_empty(shape, dtype=torch.bfloat16)
@@ -252,7 +254,8 @@ def attend(query: Tensor, cache: Cache, table: Tensor, q_cu: Tensor, lengths: Te
     ``query`` ((Lq, heads, D) bf16) and ``lengths[i]`` cached tokens, its queries' own among them: the last query sits
     at the last token. Query head h reads key/value head h // (heads / kv heads). Visible tokens: all of the request's,
     or with ``causal`` those up to the query's own, narrowed by ``window`` (how many earlier tokens stay visible; -1 for
-    all); a query that sees none gets zeros. ``max_q`` bounds every request's query count, ``total_keys`` the lengths'
+    all); a query that sees none gets zeros. A NaN reaches the queries that see its token, and in long chunks (whose keys are
+    unpacked for the packed attention first) it can reach others of its tile, as there. ``max_q`` bounds every request's query count, ``total_keys`` the lengths'
     sum (default: all that the table can hold; it sizes the workspace of long query runs). Rows behind the last request
     are not written."""
     _no_grad("attend", query)
@@ -272,8 +275,8 @@ def attend(query: Tensor, cache: Cache, table: Tensor, q_cu: Tensor, lengths: Te
         _check_ints(index, q_cu=q_cu)
     if q_cu.numel() != n + 1:
         raise ValueError(f"the table has {n} requests, q_cu {q_cu.numel()} bounds")
-    if max_q < 0 or window < -1:
-        raise ValueError(f"max_q must be non-negative and window at least -1, not {max_q} and {window}")
+    if not 0 <= max_q <= _MOST or not -1 <= window <= _MOST:
+        raise ValueError(f"max_q must lie in 0 .. {_MOST} and window in -1 .. {_MOST}, not {max_q} and {window}")
     if total_keys is None:
         total_keys = min(n * rows_fields[2] * cache.block_size, _MOST)
     elif not 0 <= total_keys <= _MOST:

@@ -126,7 +126,7 @@ def test_calls_on_the_cpu_are_refused():
     {"table": torch.zeros((1, 4), dtype=torch.int32).expand(2, 4)},
     {"lengths": _ints(0)}, {"lengths": torch.zeros(2, dtype=torch.int64)}, {"counts": _ints(1, 2, 3)},
     {"counts": _ints(1, 0, 2, 0)[::2]}, {"free": torch.zeros((1, 3), dtype=torch.int32)}, {"free_count": _ints(1, 2)},
-    {"rows": -1}, {"block_size": 16}, {"block_size": 48}], ids=str)
+    {"rows": -1}, {"rows": 1 << 31}, {"block_size": 16}, {"block_size": 48}], ids=str)
 def test_reserve_refuses(change):
     with pytest.raises(ValueError) as e:
         _reserve(**change)
@@ -183,7 +183,8 @@ def test_append_and_attend_refuse_an_autograd_call():
     {"query": torch.zeros((3, 4, 64))}, {"query": torch.zeros((3, 3, 64), dtype=torch.bfloat16)},
     {"query": torch.zeros((3, 4, 128), dtype=torch.bfloat16)},
     {"query": torch.zeros((3, 4, 128), dtype=torch.bfloat16)[..., ::2]}, {"q_cu": _ints(0, 1, 3)},
-    {"q_cu": torch.zeros(2, dtype=torch.int64)}, {"lengths": _ints(3, 3)}, {"max_q": -1}, {"window": -2},
+    {"q_cu": torch.zeros(2, dtype=torch.int64)}, {"lengths": _ints(3, 3)}, {"max_q": -1}, {"max_q": 1 << 31},
+    {"window": -2}, {"window": 1 << 31},
     {"total_keys": -1}, {"total_keys": 1 << 31},
     {"table": torch.zeros((1, 2), dtype=torch.int64)}], ids=str)
 def test_attend_refuses(change):
@@ -198,7 +199,7 @@ def test_attend_refuses(change):
 # ---- refusals of the C ABI (the pointers are never followed)
 
 def _c_cache(**change):
-    c = _lib.KarpoCache(4096, 8192, 12288, 4, 2, 64, 32)
+    c = _lib.KarpoCache(0x100000, 0x200000, 0x300000, 4, 2, 64, 32)
     for name, value in change.items():
         setattr(c, name, value)
     return c
@@ -260,9 +261,16 @@ def test_c_abi_attend_refuses(change, status):
     assert _lib.load().karpo_cache_attend(ctypes.byref(a), None) == status
 
 
+def test_c_abi_append_refuses_keys_and_values_of_one_memory():
+    a = _lib.KarpoCacheAppendArgs(_c_cache(values=0x100000 + 16), 4096, 4096, 128, 64, 128, 64, 3, 4096, 1)
+    assert _lib.load().karpo_cache_append(ctypes.byref(a), None) == _lib.ERR_ARG
+
+
 def test_c_abi_calls_without_rows_launch_nothing():
     lib = _lib.load()
     a = _lib.KarpoCacheAppendArgs(_c_cache(), 4096, 4096, 128, 64, 128, 64, 0, 4096, 1)
     assert lib.karpo_cache_append(ctypes.byref(a), None) == 0
     b = _lib.KarpoCacheAttendArgs(_c_cache(), 4096, 4096, 128, 64, 128, 64, 4096, 4096, 4096, 2, 2, 1, 4, 3, 0, 3, 0.1, -1, 0)
+    assert lib.karpo_cache_attend(ctypes.byref(b), None) == 0
+    b.total_q, b.max_q = 3, 0
     assert lib.karpo_cache_attend(ctypes.byref(b), None) == 0

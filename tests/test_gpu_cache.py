@@ -416,6 +416,41 @@ def test_scales(gpu, scale):
     _attend_and_compare(gpu, 64, 4, 2, 32, [130, 20], [1, 2], scale=scale)
 
 
+def test_a_scale_that_is_no_number(gpu):
+    cache, _, table, query, q_cu, _ = _attend_case(gpu, 64, 4, 2, 32, [130, 20], [1, 1], oracle_too=False)
+    with torch.inference_mode():
+        out = kv_cache.attend(query.to(gpu), cache, ints(table, gpu), ints(q_cu, gpu), ints([130, 20], gpu), 1, math.nan)
+    assert torch.isnan(out).all()
+
+
+def test_bounds_out_of_range_write_nothing(gpu):
+    """Query bounds past the query, decreasing or negative: their requests have no queries, the others theirs."""
+    cache, want, table, query, q_cu, scale = _attend_case(gpu, 64, 4, 2, 32, [130, 20, 50, 60], [2, 2, 2, 2])
+    import ctypes
+
+    from karpo_decision_amd import _lib, ops
+    for bounds, good in (([0, 2, 4, 6, 9], (0, 1, 2)), ([0, 2, 1, 3, 5], (0,)), ([-3, 2, 4, 6, 8], (1, 2, 3))):
+        q, cu = query.to(gpu), ints(bounds, gpu)
+        out = torch.full_like(q, 7.0)
+        lengths, dev_table = ints([130, 20, 50, 60], gpu), ints(table, gpu)
+        c = _lib.KarpoCache(*(t.data_ptr() for t in cache[:3]), cache.blocks, 2, 64, 32)
+        a = _lib.KarpoCacheAttendArgs(c, q.data_ptr(), out.data_ptr(), 256, 64, 256, 64, cu.data_ptr(), lengths.data_ptr(),
+                                      dev_table.data_ptr(), len(table[0]), len(table[0]), 4, 4, 2, 8, 260, scale, -1, 0)
+        need = ctypes.c_size_t()
+        _lib.check(_lib.load().karpo_cache_attend_workspace_bytes(ctypes.byref(a), ctypes.byref(need)), "bytes")
+        workspace = torch.empty(need.value + 16, dtype=torch.uint8, device=gpu)
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), need.value
+        _lib.check(_lib.load().karpo_cache_attend(ctypes.byref(a), ops._current_stream(0)), "attend")
+        written = torch.zeros(8, dtype=torch.bool)
+        for i, n in enumerate((130, 20, 50, 60)):
+            if i in good or (bounds == [0, 2, 1, 3, 5] and i in (2, 3)):
+                written[bounds[i]:bounds[i + 1]] = True
+            if i in good and bounds != [0, 2, 1, 3, 5]:
+                rows = slice(bounds[i], bounds[i + 1])
+                _close(out[rows], query[rows], *want.rows(table[i], 0, n), scale)
+        assert (out[~written.to(gpu)] == 7).all()
+
+
 def test_many_requests(gpu):
     lengths = [(37 * i) % 200 for i in range(600)]
     _attend_and_compare(gpu, 64, 4, 2, 32, lengths, [1 + (i % 3 == 0) for i in range(600)])
@@ -510,6 +545,35 @@ def test_a_step_on_another_stream(gpu):
     for a, b in zip(want, got):
         assert torch.equal(a[4], b[4])
     assert torch.equal(bits(caches[0].keys), bits(caches[1].keys))
+
+
+def test_a_captured_long_chunk_replays(gpu):
+    """The path that unpacks, captured: each replay reads the lengths and the cache as they are then."""
+    block, heads, kv_heads, head_dim, counts = 64, 32, 2, 64, [1500, 900]
+    cache, _, table, query, q_cu, scale = _attend_case(gpu, head_dim, heads, kv_heads, block, [5100, 3000], counts,
+                                                       oracle_too=False)
+    query, table, q_cu, lengths = query.to(gpu), ints(table, gpu), ints(q_cu, gpu), ints([5100, 3000], gpu)
+
+    def call():
+        return kv_cache.attend(query, cache, table, q_cu, lengths, 1500, scale, total_keys=8200)
+
+    with torch.inference_mode():
+        call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        seen = []
+        for change in ([5100, 3000], [4000, 3001], [1500, 899]):
+            lengths.copy_(ints(change, gpu))
+            query.mul_(-0.75)
+            graph.replay()
+            want = call()
+            torch.cuda.synchronize()
+            # bit for bit (a request's 3,001st token is a leftover, NaN among its codes)
+            assert torch.equal(out.view(torch.int16), want.view(torch.int16))
+            seen.append(out.clone())
+    assert not torch.equal(seen[0], seen[1]) and not torch.equal(seen[1], seen[2])
 
 
 @pytest.mark.parametrize("counts", [[1, 1, 1], [70, 1, 33]])
