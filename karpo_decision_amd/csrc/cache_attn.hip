@@ -100,6 +100,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 
+// A barrier for what goes through LDS: copies and stores stay in flight.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // Which of a word's four codes are NaN, as 0x80 in their bytes.
@@ -189,17 +192,16 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
       scan(c0);  // (one chunk's sums are there)
     }
     if (writes_units && c0 + tid < p.r.n_seq) p.units[c0 + tid] = carry + v[0];
-    const int to = min(u1, carry + all[0]);
+    const int to = min(u1, carry + all[0] - (p.whole ? 0 : kStart));  // (what the last request counts more has none behind it)
     for (int at = max(u0, carry); at < to;) {
-      // the request that `at` lies in, or the one behind the gap that it lies in: one thread's, or none's
+      // the request that `at` lies in, or the one behind the gap that it lies in: one thread's
       const int unit = at - carry - v[0];
-      const bool mine = own.units > 0 && unit < own.units && unit >= (v[0] > 0 ? -kStart : 0);
-      if (mine) {
+      if (own.units > 0 && unit < own.units && unit >= (v[0] > 0 ? -kStart : 0)) {
         s_seen = own;
         s_at[0] = tid;
         s_at[1] = v[0];
       }
-      if (!__syncthreads_or(mine)) break;
+      lds_barrier();
       const Seen s = {uniform(s_seen.tokens), uniform(s_seen.row),   uniform(s_seen.queries),
                       uniform(s_seen.first),  uniform(s_seen.groups), uniform(s_seen.units)};
       const int i = c0 + uniform(s_at[0]);
@@ -212,7 +214,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
       at = stop;
       const int vectors = (int)min<int64_t>((int64_t)s.queries * p.group - vector0, kVectors);
       if (vectors <= 0) {
-        __syncthreads();  // s_seen is read
+        lds_barrier();  // s_seen is read
         continue;
       }
 
@@ -304,8 +306,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
         copy(p.c.keys, key_ring, g0 + wave, 0, true);
         copy(p.c.values, value_ring, g0 + wave, 0, true);
       }
-      // (a barrier that leaves the copies in flight)
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      lds_barrier();
       for (int g = g0 + wave; g < g1; g += kAttendWaves) {
         const float k_scale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(k_scales), k));
         const float v_scale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v_scales), k));
@@ -448,7 +449,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
           s_l[wave][16 * n + col] = l;
         }
       }
-      __syncthreads();
+      lds_barrier();
       // vector c's maximum and sum over the waves
       auto top_of = [&](int c) {
         float up = s_m[0][c];
@@ -480,7 +481,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
             if (t * 16 >= d0 && t * 16 < d0 + kSlab)
               *reinterpret_cast<f32x4*>(&s_o[wave][16 * n + col][t * 16 - d0 + quad * 4]) = o[n][t] * f;
         }
-        __syncthreads();
+        lds_barrier();
         for (int e = tid; e < vectors * (kSlab / 4); e += kAttendThreads) {
           const int c = e / (kSlab / 4), d = (e % (kSlab / 4)) * 4;
           f32x4 x = *reinterpret_cast<const f32x4*>(&s_o[0][c][d]);
@@ -496,7 +497,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
             *reinterpret_cast<f32x4*>(part + c * D + d0 + d) = x;
           }
         }
-        __syncthreads();
+        lds_barrier();
       }
     }
     carry += all[0];
