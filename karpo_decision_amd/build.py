@@ -29,9 +29,11 @@ SOURCES = ["attn_fwd.hip", "attn_fwd_128.hip", "attn_bwd.hip", "attn_bwd_pair.hi
            "cache.hip", "cache_attn.hip", "capi.cpp", "cache_capi.cpp", "plan.cpp", "scratch.hip"]
 # per-source flags: the head-size-128 wide / long forward tiles under the iterative-ILP machine scheduler; the backward's
 # live ranges split for few spills (otherwise the head-size-256 dK / dV kernel, at all 512 registers, spills inside its
-# loop; the other kernels of the file come out the same)
+# loop; the other kernels of the file come out the same); the block cache's attention with its accumulators in VGPRs (at one
+# wave per SIMD they are kept in AGPRs otherwise, and copied 128 to 200 registers a step across the rescale's branch)
 SOURCE_FLAGS = {"attn_fwd_128.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
-                "attn_bwd.hip": ["-mllvm", "-split-spill-mode=size"]}
+                "attn_bwd.hip": ["-mllvm", "-split-spill-mode=size"],
+                "cache_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def hipcc() -> str:

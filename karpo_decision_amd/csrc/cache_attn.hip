@@ -235,7 +235,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
         for (int c = 0; c < kMine; ++c) {
           const int e = wave + c * kAttendWaves;
           if (2 * kChunks >= kAttendWaves || e < 2 * kChunks)
-            q_mine[n][c] = *reinterpret_cast<const u32x4*>(src + (e >> 1) * 64 + quad * 16 + (e & 1) * 8) ^ p.sign;
+            q_mine[n][c] = *reinterpret_cast<const u32x4*>(src + (e >> 1) * 64 + quad * 16 + (e & 1) * 8);
         }
         lo[n] = p.left < 0 ? 0 : pos + shift - p.left;
         hi[n] = p.right < 0 ? s.tokens - 1 : (int)min<int64_t>((int64_t)pos + shift + p.right, s.tokens - 1);
@@ -300,7 +300,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
 #pragma unroll
         for (int c = 0; c < kMine; ++c) {
           const int e = wave + c * kAttendWaves;
-          if (2 * kChunks >= kAttendWaves || e < 2 * kChunks) s_q[(e * NT + n) * 64 + lane] = q_mine[n][c];
+          if (2 * kChunks >= kAttendWaves || e < 2 * kChunks) s_q[(e * NT + n) * 64 + lane] = q_mine[n][c] ^ p.sign;
         }
       if (some) {
         copy(p.c.keys, key_ring, g0 + wave, 0, true);
