@@ -249,12 +249,12 @@ int check_attend(const KarpoCacheAttendArgs* a, CacheRef* c, CacheRows* r) {
 // walks (a tile holds 64 vectors, 32 at head size 256, 16 at 512), and the unpacking at the memory's rate and the packed
 // attention at the rate that it reaches with many query tiles, or with few of one or two requests. Of 198 shapes (head sizes
 // 64 to 512, 1 to 16 requests of 700 to 32,768 tokens, 16 to 4,096 vectors) the rule's choice is over 15% slower than the
-// other for four. Unpacked against split:
-//   one request of 32,768 tokens, 16 key/value heads of 128: 128 vectors 166, 76 us; 512 vectors 307, 213; 1,024 460, 402
-//   16 requests of 2,048: 128 vectors 103, 82; 256 vectors 119, 126; 512 vectors 168, 213
-//   8 heads of 256: one request, 256 vectors 210, 158; 1,024 vectors 445, 584; 16 requests, 128 vectors 118, 101; 256 144, 175
-//   4 heads of 512: one request, 512 vectors 284, 306; 1,024 vectors 436, 589; 16 requests, 512 vectors 251, 305
-//   one request of 2,000 tokens: 16 heads of 128, 1,024 vectors 62, 53; 8 of 256, 71, 64; 4 of 512, 77, 60
+// other for two. Unpacked against split:
+//   one request of 32,768 tokens, 16 key/value heads of 128: 128 vectors 166, 71 us; 512 vectors 307, 210; 1,024 458, 392
+//   16 requests of 2,048: 128 vectors 102, 80; 256 vectors 117, 123; 512 vectors 165, 209
+//   8 heads of 256: one request, 256 vectors 210, 134; 1,024 vectors 443, 474; 16 requests, 128 vectors 119, 88; 256 143, 149
+//   4 heads of 512: one request, 512 vectors 284, 282; 1,024 vectors 436, 542; 16 requests, 512 vectors 251, 280
+//   one request of 2,000 tokens: 16 heads of 128, 1,024 vectors 62, 52; 8 of 256, 71, 54; 4 of 512, 78, 56
 bool split(const KarpoCacheAttendArgs* a) {
   const int d = a->cache.head_dim;
   const double vectors = (double)a->max_q * (a->heads / a->cache.kv_heads);
@@ -262,7 +262,7 @@ bool split(const KarpoCacheAttendArgs* a) {
   if (vectors >= 1 << 15) return false;  // (position_of holds below 2^16)
   const double keys = (double)seen_keys(a) * a->cache.kv_heads, tile = d <= 128 ? 64 : d == 256 ? 32 : 16;
   if (ceil(vectors / tile) * a->cache.kv_heads > 65535) return false;  // (a launch's second dimension)
-  const double walk = d == 64 ? 3.5e-5 : d == 128 ? 4.6e-5 : 6.5e-5;
+  const double walk = d == 64 ? 3.5e-5 : d == 128 ? 4.6e-5 : d == 256 ? 5.3e-5 : 6.1e-5;
   const double query_tiles = a->n_seq * ceil(vectors / 128) * a->cache.kv_heads;
   const double most = d == 512 ? 0.8e9 : 1.3e9, few = 0.35e9 + 0.5e6 * vectors;  // operations a microsecond
   const double rate = a->n_seq <= 2 && query_tiles < 256 && few < most ? few : most;
