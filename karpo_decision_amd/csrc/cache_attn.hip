@@ -112,8 +112,9 @@ __device__ __forceinline__ unsigned nan_codes(unsigned w) { return ((w & 0x7f7f7
 // the query vectors as columns: column lane % 16, keys 16 t + 4 (lane / 16) + i. Those are this lane's eight weights, and as
 // they stand the second operand of O^T = V^T P^T, whose first operand, 8 of these keys of one element, is 8 bytes of the cache.
 // The products are of bf16 operands (a cached element is one exactly); the weights enter as two bf16 terms, 2^-17 off, which
-// costs matrix work that this kernel, bound by the codes' way from HBM, has to spare (one term: 1.4 times the plain form's
-// error against 64 bits; two: the plain form's).
+// costs matrix work that this kernel, bound by the codes' way from HBM, has to spare (2-norm error against 64 bits with
+// one term and with two, the latter the output's own rounding: 2.31e-3, 1.67e-3 for one query over 131,073 tokens at head size
+// 512; 1.04e-3, 0.81e-3 for 48 requests at 128; in time 91.2, 91.3 us and 48.8, 50.8 us).
 //
 // A wave takes every fourth group of its workgroup's share by itself, its running maximum and sums in registers, the next
 // group's keys on their way to LDS while this one's weights are made, the next values while the next keys are read: a group in

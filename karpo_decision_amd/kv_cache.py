@@ -254,10 +254,10 @@ def attend(query: Tensor, cache: Cache, table: Tensor, q_cu: Tensor, lengths: Te
     ``query`` ((Lq, heads, D) bf16) and ``lengths[i]`` cached tokens, its queries' own among them: the last query sits
     at the last token. Query head h reads key/value head h // (heads / kv heads). Visible tokens: all of the request's,
     or with ``causal`` those up to the query's own, narrowed by ``window`` (how many earlier tokens stay visible; -1 for
-    all); a query that sees none gets zeros. A NaN reaches the queries that see its token, and in long chunks (whose keys are
-    unpacked for the packed attention first) it can reach others of its tile, as there. ``max_q`` bounds every request's query count, ``total_keys`` the lengths'
-    sum (default: all that the table can hold; it sizes the workspace of long query runs). Rows behind the last request
-    are not written."""
+    all); a query that sees none gets zeros. A NaN reaches the queries that see its token, and in long chunks (whose keys
+    are unpacked for the packed attention first) it can reach others of its tile, as there. ``max_q`` bounds every
+    request's query count, ``total_keys`` the lengths' sum (default: all that the table can hold; it sizes the workspace
+    of long query runs). Rows behind the last request are not written."""
     _no_grad("attend", query)
     index = query.get_device()
     fields = _cache_fields(cache, index)
