@@ -444,7 +444,7 @@ __global__ __launch_bounds__(64 * kReadWaves) void read_kernel(const ReadParams 
       const int64_t head = (int64_t)(known ? id : 0) * heads + h;
       const int inside = token0 & ((1 << b) - 1);
       const uint8_t* const src = (value ? p.c.values : p.c.keys) + (head << b) * D + inside * D;
-      const float scale = p.c.scales[2 * head + (value ? 1 : 0)];
+      const float scale = known ? p.c.scales[2 * head + (value ? 1 : 0)] : 1.f;  // (zeros under any other block's could be NaN)
       uint16_t* const dst = (value ? p.v : p.k) + (out_row * heads + h) * D;
       const int64_t step = (int64_t)heads * D;
       if (!value) {

@@ -267,8 +267,8 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
         ids = table[mine >> (b - 5)];
         if (ids < 0 || ids >= p.c.blocks) ids = -1;
         const float2 sc = *reinterpret_cast<const float2*>(p.c.scales + 2 * ((int64_t)max(ids, 0) * heads + h));
-        k_scales = sc.x;
-        v_scales = sc.y;
+        k_scales = ids < 0 ? 1.f : sc.x;  // (zeros under another block's scale, NaN where it was never written, could be NaN)
+        v_scales = ids < 0 ? 1.f : sc.y;
       };
       // One group's codes into the wave's ring, 16 bytes a lane and KiB; zeros for a block that is not of the pool, and where
       // there is no group (so that every turn of the loop issues the same copies, and a wait can count them).
