@@ -119,6 +119,10 @@ typedef struct KarpoCacheAttendArgs {
   int32_t max_q; /* a bound of every request's query rows */
   int64_t total_q;
   int64_t total_keys; /* a bound of the lengths' sum: the keys of long query runs are unpacked into the workspace */
+                      /* Where a bound does not hold, the rows that are not computed become NaN: a request's rows past its
+                         first max_q or, where the keys are unpacked, the rows of all requests (for more tokens than
+                         total_keys too). A request whose q_cu are not within 0 .. total_q in order has no rows; with
+                         max_q 0 nothing is written at all. */
   float scale;
   int32_t window_left, window_right; /* -1: unbounded; causal is window_right 0 */
   void* workspace;

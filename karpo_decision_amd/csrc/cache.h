@@ -60,6 +60,13 @@ struct ReadParams {
   CacheRows r;
   const int32_t* q_cu;  // with it: only the tokens that a request's queries can see (window_left before the first)
   int32_t window_left;
+  // with q_cu, where bounds do not hold (query rows past total_q or out of order, more than max_q of them, more tokens than
+  // `rows`): the packed attention behind this computes nothing then, and all requests' rows of o become NaN
+  int32_t max_q;
+  int64_t total_q;
+  uint16_t* o;
+  int64_t so_t, so_h;
+  int32_t heads;
   uint16_t* k;
   uint16_t* v;
   int64_t rows;
@@ -76,6 +83,7 @@ struct AttendParams {
   int64_t sq_t, sq_h, so_t, so_h;
   const int32_t* q_cu;
   int64_t total_q;
+  int32_t max_q;       // rows of a request's queries behind this many become NaN
   int32_t group;       // heads / kv_heads
   float per_group;     // 1 / group
   int32_t whole;       // a workgroup takes a request whole (nothing to join)

@@ -366,11 +366,14 @@ __global__ __launch_bounds__(64 * kReadWaves) void read_kernel(const ReadParams 
   const int heads = p.c.kv_heads, b = p.c.block_log2;
 
   // first and last token of request i that are read
+  bool bad = false;  // (with q_cu) bounds that the attention's planner refuses
   auto range = [&](int i, int* start, int* tokens) {
     *tokens = min(max(p.r.lengths[i], 0), p.r.most);
     *start = 0;
     if (p.q_cu != nullptr) {
-      const int queries = p.q_cu[i + 1] - p.q_cu[i];
+      const int q0 = p.q_cu[i], q1 = p.q_cu[i + 1];
+      const int64_t queries = (int64_t)q1 - q0;
+      bad |= q0 < 0 || queries < 0 || queries > p.max_q || q1 > p.total_q;
       if (queries <= 0) {
         *tokens = 0;
       } else if (p.window_left >= 0) {
@@ -389,10 +392,20 @@ __global__ __launch_bounds__(64 * kReadWaves) void read_kernel(const ReadParams 
     block_scan<kThreads, 2>(v, all, s_part);
   };
   int groups = 0;
+  int64_t rows = 0;
   for (int c0 = 0; c0 < p.r.n_seq; c0 += kThreads) {
     if (c0 > 0) __syncthreads();
     scan(c0);
     groups += all[0];
+    rows += (int64_t)all[0] * kCacheGroup + all[1];
+  }
+  if (p.q_cu != nullptr && __syncthreads_or(bad || rows > p.rows)) {
+    for (int i = 0; i < p.r.n_seq; ++i) {
+      const int q0 = p.q_cu[i], q1 = p.q_cu[i + 1];
+      if (q0 >= 0 && q1 > q0 && q1 <= p.total_q)
+        fill_nan<D>(p.o + q0 * p.so_t, p.so_t, p.so_h, q1 - q0, p.heads, (int64_t)blockIdx.x * kThreads + tid,
+                    (int64_t)gridDim.x * kThreads);
+    }
   }
   auto store = [&](uint16_t* to, const u32x4& x) {
     if constexpr (STREAM) __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(to)); else *reinterpret_cast<u32x4*>(to) = x;

@@ -49,6 +49,15 @@ __device__ __forceinline__ Seen seen_of(const AttendParams& p, int i) {
   return s;
 }
 
+// NaN into a request's rows past max_q, which nothing computes, of the key/value head's query heads (by the workgroups of its
+// first vectors; here, at the attention kernel's end or in the join, it costs that kernel's loop no registers).
+template <int D>
+__device__ __forceinline__ void fill_past(const AttendParams& p, const Seen& s, int y, int first, int step) {
+  if (s.queries > p.max_q && y < p.c.kv_heads)
+    fill_nan<D>(p.o + (s.row + (int64_t)p.max_q) * p.so_t + (int64_t)y * p.group * p.so_h, p.so_t, p.so_h,
+                s.queries - p.max_q, p.group, first, step);
+}
+
 // A vector's position among its request's queries: vec / group, exactly (vec + 1/2 is no multiple of the group, and below
 // 2^16 further from one than the product's rounding).
 __device__ __forceinline__ int position_of(int vec, const AttendParams& p) { return (int)((vec + 0.5f) * p.per_group); }
@@ -213,7 +222,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
       const int g0 = s.first + at - begin;
       const int g1 = s.groups > 0 ? s.first + stop - begin : g0;
       at = stop;
-      const int vectors = (int)min<int64_t>((int64_t)s.queries * p.group - vector0, kVectors);
+      const int vectors = (int)min<int64_t>((int64_t)min(s.queries, p.max_q) * p.group - vector0, kVectors);
       if (vectors <= 0) {
         lds_barrier();  // s_seen is read
         continue;
@@ -503,6 +512,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
     }
     carry += all[0];
   }
+  if (p.whole) fill_past<D>(p, seen_of(p, blockIdx.x), blockIdx.y, tid, kAttendThreads);
 }
 
 // Joins a request's shares: O = sum of 2^(m_w - M) O_w over sum of 2^(m_w - M) l_w, in an order that the sizes alone set.
@@ -519,11 +529,12 @@ __global__ __launch_bounds__(256) void join_kernel(const AttendParams p, int vec
   const int total = p.units[p.r.n_seq], begin = p.units[i];
   const Seen s = seen_of(p, i);
   if (s.units == 0) return;
+  fill_past<D>(p, s, blockIdx.y, blockIdx.z * 256 + threadIdx.x, gridDim.z * 256);
   const Shares shares(total, p.parts);
   const int first = shares.part_of(begin), last = shares.part_of(begin + s.units - 1);
   if (first == last) return;
   const int h = blockIdx.y % heads, vector0 = (blockIdx.y / heads) * vectors_per;
-  const int vectors = (int)min<int64_t>((int64_t)s.queries * p.group - vector0, vectors_per);
+  const int vectors = (int)min<int64_t>((int64_t)min(s.queries, p.max_q) * p.group - vector0, vectors_per);
   const int64_t size = (int64_t)vectors_per * (D + 2);
   const float* const base = p.partial + (int64_t)blockIdx.y * p.parts * 2 * size;
   const int tid = threadIdx.x;

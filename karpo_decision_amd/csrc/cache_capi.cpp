@@ -322,6 +322,7 @@ extern "C" int karpo_cache_attend(const KarpoCacheAttendArgs* a, void* stream) {
     t.so_h = a->o_stride_head;
     t.q_cu = a->q_cu;
     t.total_q = a->total_q;
+    t.max_q = a->max_q;
     t.group = a->heads / a->cache.kv_heads;
     t.left = a->window_left >= kMostTokens ? -1 : a->window_left;  // (sees everything, and stays within 32 bits)
     t.right = a->window_right;
@@ -346,6 +347,12 @@ extern "C" int karpo_cache_attend(const KarpoCacheAttendArgs* a, void* stream) {
   char* const ws = static_cast<char*>(a->workspace);
   p.q_cu = a->q_cu;
   p.window_left = a->window_left;
+  p.max_q = a->max_q;
+  p.total_q = a->total_q;
+  p.o = static_cast<uint16_t*>(a->o);
+  p.so_t = a->o_stride_tok;
+  p.so_h = a->o_stride_head;
+  p.heads = a->heads;
   p.k = reinterpret_cast<uint16_t*>(ws + u.k_offset);
   p.v = reinterpret_cast<uint16_t*>(ws + u.v_offset);
   p.rows = u.rows;

@@ -24,6 +24,17 @@ __device__ __forceinline__ u32x4 bf16_of_8(unsigned a, unsigned b, float scale) 
                bf16_pair(b, scale, true)};
 }
 
+// NaN into `count` rows of `heads` heads from o on, by threads `first`, `first` + `step`, ...
+template <int D>
+__device__ __forceinline__ void fill_nan(uint16_t* o, int64_t s_row, int64_t s_head, int64_t count, int heads, int64_t first,
+                                         int64_t step) {
+  for (int64_t e = first; e < count * heads * (D / 8); e += step) {
+    const int64_t vec = e / (D / 8), row = vec / heads;
+    *reinterpret_cast<u32x4*>(o + row * s_row + (vec - row * heads) * s_head + e % (D / 8) * 8) =
+        u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+  }
+}
+
 // The sum over the wave's lanes up to this one, in registers (six additions across lanes, no LDS).
 __device__ __forceinline__ int wave_scan(int x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // from the lane 1, 2, 4, 8 before, within 16

@@ -18,6 +18,7 @@ current stream of the tensors' device and capture into graphs. All of it is forw
 from __future__ import annotations
 
 import ctypes
+import math
 import struct
 from typing import NamedTuple
 
@@ -257,7 +258,8 @@ def attend(query: Tensor, cache: Cache, table: Tensor, q_cu: Tensor, lengths: Te
     all); a query that sees none gets zeros. A NaN reaches the queries that see its token, and in long chunks (whose keys
     are unpacked for the packed attention first) it can reach others of its tile, as there. ``max_q`` bounds every
     request's query count, ``total_keys`` the lengths' sum (default: all that the table can hold; it sizes the workspace
-    of long query runs). Rows behind the last request are not written."""
+    of long query runs). Where one of them does not hold, rows that were not computed are NaN: those of a request past
+    its first ``max_q``, or, in long chunks, those of all requests. Rows behind the last request are not written."""
     _no_grad("attend", query)
     index = query.get_device()
     fields = _cache_fields(cache, index)
@@ -286,6 +288,8 @@ def attend(query: Tensor, cache: Cache, table: Tensor, q_cu: Tensor, lengths: Te
     out = query.new_empty(shape)
     if shape[0] == 0:
         return out
+    if max_q == 0:  # (the C call writes nothing)
+        return out.fill_(math.nan)
     call = (*fields, query.data_ptr(), out.data_ptr(), sq[0], sq[1], shape[1] * head_dim, head_dim, q_cu.data_ptr(),
             lengths.data_ptr(), *rows_fields, shape[1], int(max_q), shape[0], int(total_keys), float(scale),
             int(window), 0 if causal else -1)

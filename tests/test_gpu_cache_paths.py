@@ -27,9 +27,9 @@ def ints(values, device):
     return torch.tensor(values, dtype=torch.int32, device=device)
 
 
-def path_of(cache, heads, counts, rows, n, width, window=-1, total_keys=None):
+def path_of(cache, heads, counts, rows, n, width, window=-1, total_keys=None, max_q=None):
     """The path that a call of these sizes takes, by the workspace it asks for."""
-    max_q = max(counts)
+    max_q = max(counts) if max_q is None else max_q
     total = n * width * cache.block_size if total_keys is None else total_keys
     c = _lib.KarpoCache(*(t.data_ptr() for t in cache[:3]), cache.blocks, cache.kv_heads, cache.head_dim, cache.block_size)
     a = _lib.KarpoCacheAttendArgs(c, 4096, 4096, 8, 8, 8, 8, 4096, 4096, 4096, width, width, n, heads, max_q, rows, total,
@@ -118,3 +118,104 @@ def test_attend_of_unknown_blocks_beside_a_block_without_scales(gpu, head_dim, h
     for i, n in enumerate(lengths):
         close(out[q_cu[i]:q_cu[i + 1]], query[q_cu[i]:q_cu[i + 1]], *want.rows(table[i], 0, n), 0.1,
               weights=2.0 ** -8 if path == UNPACKED else 0.0)
+
+
+# ---- bounds that do not hold
+
+def attend_into(device, out, cache, table, query, q_cu, lengths, max_q, scale, total_keys):
+    """``attend`` by the C ABI, into ``out`` (contiguous)."""
+    from karpo_decision_amd import ops
+    q, cu, n, dev_table = query.to(device), ints(q_cu, device), ints(lengths, device), ints(table, device)
+    rows, heads, d = q.shape
+    c = _lib.KarpoCache(*(t.data_ptr() for t in cache[:3]), cache.blocks, cache.kv_heads, d, cache.block_size)
+    a = _lib.KarpoCacheAttendArgs(c, q.data_ptr(), out.data_ptr(), heads * d, d, heads * d, d, cu.data_ptr(), n.data_ptr(),
+                                  dev_table.data_ptr(), len(table[0]), len(table[0]), len(table), heads, max_q, rows,
+                                  total_keys, scale, -1, 0)
+    need = ctypes.c_size_t()
+    _lib.check(_lib.load().karpo_cache_attend_workspace_bytes(ctypes.byref(a), ctypes.byref(need)), "bytes")
+    workspace = torch.empty(need.value + 16, dtype=torch.uint8, device=device)
+    a.workspace, a.workspace_bytes = workspace.data_ptr(), need.value
+    _lib.check(_lib.load().karpo_cache_attend(ctypes.byref(a), ops._current_stream(0)), "attend")
+    return out
+
+
+CHUNKS = (64, 16, 2, 64, [3000, 2900], [2000, 1900])  # the path that unpacks
+
+
+@pytest.mark.parametrize("change", ["total_keys", "max_q", "past the query", "out of order", "negative"])
+def test_a_long_chunk_with_bounds_that_do_not_hold_is_nan(gpu, change):
+    """Nothing is computed then: the requests' rows are NaN, and no others are written."""
+    lengths, counts = CHUNKS[4:]
+    cache, table, query, q_cu = make(gpu, *CHUNKS)
+    query = torch.cat((query, query[:7]))  # rows behind the last request
+    total, max_q, known = sum(lengths), max(counts), torch.ones(query.shape[0], dtype=torch.bool)
+    known[sum(counts):] = False
+    if change == "total_keys":
+        total -= 1
+    elif change == "max_q":
+        max_q -= 1
+    elif change == "past the query":
+        q_cu[2] = query.shape[0] + 1
+        known[q_cu[1]:] = False
+    elif change == "out of order":
+        q_cu[1], q_cu[2] = q_cu[1] - 1, 1
+        known[q_cu[1]:] = False
+    else:
+        q_cu[0] = -1
+        known[:q_cu[1]] = False
+    assert path_of(cache, 16, counts, query.shape[0], 2, len(table[0]), total_keys=total, max_q=max_q) == UNPACKED
+    out = attend_into(gpu, torch.full(query.shape, 7.0, dtype=torch.bfloat16, device=gpu), cache, table, query, q_cu, lengths,
+                      max_q, 0.1, total)
+    assert torch.isnan(out[known.to(gpu)]).all() and (out[~known.to(gpu)] == 7).all()
+    if change in ("total_keys", "max_q"):
+        assert torch.isnan(attend(gpu, cache, table, query, q_cu, lengths, max_q, 0.1, total_keys=total)[:sum(counts)]).all()
+
+
+def test_a_long_chunk_with_bounds_that_hold_again(gpu):
+    """Strided output, requests without queries among more than a workgroup's 256: the bounds' check finds nothing."""
+    lengths, counts = [40] * 300 + [3000], [0, 3] * 150 + [2000]
+    cache, table, query, q_cu = make(gpu, 64, 16, 2, 64, lengths, counts)
+    assert path_of(cache, 16, counts, sum(counts), 301, len(table[0]), total_keys=sum(lengths)) == UNPACKED
+    out = attend(gpu, cache, table, query, q_cu, lengths, 2000, 0.1, total_keys=sum(lengths))
+    want = oracle.Cache(cache.keys, cache.values, cache.scales, 64)
+    for i in (1, 3, 149, 255, 257, 299, 300):
+        close(out[q_cu[i]:q_cu[i + 1]], query[q_cu[i]:q_cu[i + 1]], *want.rows(table[i], 0, lengths[i]), 0.1, weights=2.0 ** -8)
+    q_cu[150] = q_cu[151] + 1  # one request out of order: all NaN, those of the other 255 too
+    out = attend(gpu, cache, table, query, q_cu, lengths, 2000, 0.1, total_keys=sum(lengths))
+    assert torch.isnan(out[:q_cu[149]]).all() and torch.isnan(out[q_cu[200]:]).all()
+
+
+@pytest.mark.parametrize("head_dim,heads,kv_heads,lengths,counts,max_q,path", [
+    (64, 4, 2, [130, 100], [5, 2], 2, WHOLE), (64, 80, 2, [130, 100], [1, 7], 2, WHOLE), (512, 4, 2, [100, 60], [9, 1], 1, WHOLE),
+    (64, 4, 2, [900, 100, 0], [5, 3, 3], 2, SPLIT), (64, 80, 2, [900, 700], [7, 2], 2, SPLIT),
+    (256, 4, 2, [900, 100], [1, 40], 33, SPLIT), (512, 4, 2, [300, 100], [9, 9], 1, SPLIT)])
+def test_queries_past_max_q_are_nan(gpu, head_dim, heads, kv_heads, lengths, counts, max_q, path):
+    """A request's first ``max_q`` rows are right, the others NaN (and nothing else is written)."""
+    n = len(lengths)
+    cache, table, query, q_cu = make(gpu, head_dim, heads, kv_heads, 32, lengths, counts)
+    query = torch.cat((query, query[:3]))
+    assert path_of(cache, heads, counts, query.shape[0], n, len(table[0]), max_q=max_q) == path
+    out = attend_into(gpu, torch.full(query.shape, 7.0, dtype=torch.bfloat16, device=gpu), cache, table, query, q_cu, lengths,
+                      max_q, 0.1, n * len(table[0]) * 32)
+    want = oracle.Cache(cache.keys, cache.values, cache.scales, 32)
+    for i, tokens in enumerate(lengths):
+        a, b, served = q_cu[i], q_cu[i + 1], min(counts[i], max_q)
+        assert torch.isnan(out[a + served:b]).all()
+        key, value = (x[:tokens - counts[i] + served] if tokens else x for x in want.rows(table[i], 0, tokens))
+        close(out[a:a + served], query[a:a + served], key, value, 0.1)
+    assert (out[q_cu[-1]:] == 7).all()
+
+
+def test_more_tokens_than_total_keys_are_no_matter_where_nothing_is_unpacked(gpu):
+    lengths, counts = [900, 100], [2, 2]
+    cache, table, query, q_cu = make(gpu, 64, 4, 2, 32, lengths, counts)
+    want = oracle.Cache(cache.keys, cache.values, cache.scales, 32)
+    for total in (0, 999):
+        out = attend(gpu, cache, table, query, q_cu, lengths, 2, 0.1, total_keys=total)
+        for i, n in enumerate(lengths):
+            close(out[q_cu[i]:q_cu[i + 1]], query[q_cu[i]:q_cu[i + 1]], *want.rows(table[i], 0, n), 0.1)
+
+
+def test_queries_without_a_bound_are_nan(gpu):
+    cache, table, query, q_cu = make(gpu, 64, 4, 2, 32, [40], [2])
+    assert torch.isnan(attend(gpu, cache, table, query, q_cu, [40], 0, 0.1)).all()
