@@ -123,7 +123,7 @@ typedef struct KarpoCacheAttendArgs {
                          first max_q or, where the keys are unpacked, the rows of all requests (for more tokens than
                          total_keys too). A request whose q_cu are not within 0 .. total_q in order has no rows; with
                          max_q 0 nothing is written at all. */
-  float scale;
+  float scale; /* NaN makes the rows of every request with tokens NaN */
   int32_t window_left, window_right; /* -1: unbounded; causal is window_right 0 */
   void* workspace;
   size_t workspace_bytes;

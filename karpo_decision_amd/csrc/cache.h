@@ -67,6 +67,7 @@ struct ReadParams {
   uint16_t* o;
   int64_t so_t, so_h;
   int32_t heads;
+  int32_t no_scale;  // the scale is NaN, and nothing runs behind this: NaN as well, zeros for requests without tokens
   uint16_t* k;
   uint16_t* v;
   int64_t rows;

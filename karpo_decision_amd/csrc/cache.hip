@@ -399,12 +399,12 @@ __global__ __launch_bounds__(64 * kReadWaves) void read_kernel(const ReadParams 
     groups += all[0];
     rows += (int64_t)all[0] * kCacheGroup + all[1];
   }
-  if (p.q_cu != nullptr && __syncthreads_or(bad || rows > p.rows)) {
+  if (p.q_cu != nullptr && __syncthreads_or(bad || rows > p.rows || p.no_scale)) {
     for (int i = 0; i < p.r.n_seq; ++i) {
       const int q0 = p.q_cu[i], q1 = p.q_cu[i + 1];
       if (q0 >= 0 && q1 > q0 && q1 <= p.total_q)
-        fill_nan<D>(p.o + q0 * p.so_t, p.so_t, p.so_h, q1 - q0, p.heads, (int64_t)blockIdx.x * kThreads + tid,
-                    (int64_t)gridDim.x * kThreads);
+        fill_rows<D>(p.no_scale && p.r.lengths[i] <= 0 ? 0u : kNanPair, p.o + q0 * p.so_t, p.so_t, p.so_h, q1 - q0, p.heads,
+                     (int64_t)blockIdx.x * kThreads + tid, (int64_t)gridDim.x * kThreads);
     }
   }
   auto store = [&](uint16_t* to, const u32x4& x) {

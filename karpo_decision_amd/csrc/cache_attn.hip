@@ -54,8 +54,8 @@ __device__ __forceinline__ Seen seen_of(const AttendParams& p, int i) {
 template <int D>
 __device__ __forceinline__ void fill_past(const AttendParams& p, const Seen& s, int y, int first, int step) {
   if (s.queries > p.max_q && y < p.c.kv_heads)
-    fill_nan<D>(p.o + (s.row + (int64_t)p.max_q) * p.so_t + (int64_t)y * p.group * p.so_h, p.so_t, p.so_h,
-                s.queries - p.max_q, p.group, first, step);
+    fill_rows<D>(kNanPair, p.o + (s.row + (int64_t)p.max_q) * p.so_t + (int64_t)y * p.group * p.so_h, p.so_t,
+                 p.so_h, s.queries - p.max_q, p.group, first, step);
 }
 
 // A vector's position among its request's queries: vec / group, exactly (vec + 1/2 is no multiple of the group, and below

@@ -353,11 +353,13 @@ extern "C" int karpo_cache_attend(const KarpoCacheAttendArgs* a, void* stream) {
   p.so_t = a->o_stride_tok;
   p.so_h = a->o_stride_head;
   p.heads = a->heads;
+  p.no_scale = isnan(a->scale);  // (the packed attention takes a NaN for the least scale)
   p.k = reinterpret_cast<uint16_t*>(ws + u.k_offset);
   p.v = reinterpret_cast<uint16_t*>(ws + u.v_offset);
   p.rows = u.rows;
   p.k_cu = reinterpret_cast<int32_t*>(ws);
   if (launch_cache_read(p, static_cast<hipStream_t>(stream)) != hipSuccess) return KARPO_ATTN_ERR_LAUNCH;
+  if (p.no_scale) return KARPO_ATTN_OK;
   u.fwd.k = p.k;
   u.fwd.v = p.v;
   u.fwd.k_cu = p.k_cu;

@@ -24,14 +24,16 @@ __device__ __forceinline__ u32x4 bf16_of_8(unsigned a, unsigned b, float scale) 
                bf16_pair(b, scale, true)};
 }
 
-// NaN into `count` rows of `heads` heads from o on, by threads `first`, `first` + `step`, ...
+constexpr unsigned kNanPair = 0x7fc07fc0u;  // two bf16
+
+// Pairs `x` into `count` rows of `heads` heads from o on, by threads `first`, `first` + `step`, ...
 template <int D>
-__device__ __forceinline__ void fill_nan(uint16_t* o, int64_t s_row, int64_t s_head, int64_t count, int heads, int64_t first,
-                                         int64_t step) {
+__device__ __forceinline__ void fill_rows(unsigned x, uint16_t* o, int64_t s_row, int64_t s_head, int64_t count, int heads,
+                                          int64_t first, int64_t step) {
   for (int64_t e = first; e < count * heads * (D / 8); e += step) {
     const int64_t vec = e / (D / 8), row = vec / heads;
     *reinterpret_cast<u32x4*>(o + row * s_row + (vec - row * heads) * s_head + e % (D / 8) * 8) =
-        u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+        u32x4{x, x, x, x};
   }
 }
 

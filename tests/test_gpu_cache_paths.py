@@ -219,3 +219,22 @@ def test_more_tokens_than_total_keys_are_no_matter_where_nothing_is_unpacked(gpu
 def test_queries_without_a_bound_are_nan(gpu):
     cache, table, query, q_cu = make(gpu, 64, 4, 2, 32, [40], [2])
     assert torch.isnan(attend(gpu, cache, table, query, q_cu, [40], 0, 0.1)).all()
+
+
+# ---- a scale that is no number
+
+@pytest.mark.parametrize("head_dim,heads,kv_heads,lengths,counts,path", [
+    (64, 4, 2, [130, 0, 20], [2, 1, 30], WHOLE), (128, 4, 2, [900, 0, 20], [2, 1, 30], SPLIT),
+    (64, 16, 2, [3000, 0, 20, 2900], [2000, 5, 30, 1900], UNPACKED)])
+def test_a_scale_that_is_no_number_on_each_path(gpu, head_dim, heads, kv_heads, lengths, counts, path):
+    """NaN for every request that holds tokens, zeros for the one that holds none, nothing behind the last."""
+    cache, table, query, q_cu = make(gpu, head_dim, heads, kv_heads, 64, lengths, counts)
+    query = torch.cat((query, query[:3]))
+    total = sum(lengths)
+    assert path_of(cache, heads, counts, query.shape[0], len(lengths), len(table[0]), total_keys=total) == path
+    out = attend_into(gpu, torch.full(query.shape, 7.0, dtype=torch.bfloat16, device=gpu), cache, table, query, q_cu, lengths,
+                      max(counts), math.nan, total)
+    for i, n in enumerate(lengths):
+        rows = out[q_cu[i]:q_cu[i + 1]]
+        assert torch.isnan(rows).all() if n else (rows == 0).all()
+    assert (out[q_cu[-1]:] == 7).all()
