@@ -24,6 +24,7 @@ from typing import NamedTuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib
 from .ops import _current_stream, _on_device
@@ -162,6 +163,10 @@ def _on_gpu(what: str, index: int) -> None:
 def _no_grad(what: str, *tensors: Tensor) -> None:
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise RuntimeError(f"kv_cache.{what} has no backward: call it under torch.inference_mode() or torch.no_grad()")
+    # (without a dual level, nearly always, no tensor has a tangent: 0.07 us in place of 0.3 a tensor)
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"kv_cache.{what} has no forward-mode derivative: call it under torch.inference_mode(), or with "
+                           "tensors without tangents")
 
 
 def reserve(table: Tensor, lengths: Tensor, counts: Tensor, free: Tensor, free_count: Tensor, rows: int,

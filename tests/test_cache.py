@@ -274,3 +274,41 @@ def test_c_abi_calls_without_rows_launch_nothing():
     assert lib.karpo_cache_attend(ctypes.byref(b), None) == 0
     b.total_q, b.max_q = 3, 0
     assert lib.karpo_cache_attend(ctypes.byref(b), None) == 0
+
+
+def _calls_with(rows):
+    """``append`` of keys, of values, and ``attend`` of queries."""
+    plain, writes = torch.zeros((3, 2, 64), dtype=torch.bfloat16), torch.zeros((1, 4), dtype=torch.int32)
+    return (lambda: kv_cache.append(_cache(), rows, plain, writes), lambda: kv_cache.append(_cache(), plain, rows, writes),
+            lambda: kv_cache.attend(rows, _cache(), torch.zeros((1, 2), dtype=torch.int32), _ints(0, 3), _ints(3), 3, 0.125))
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_append_and_attend_refuse_inputs_with_a_tangent(grad):
+    """A tangent would be lost without a word: refused, also where no backward is recorded; not under inference_mode, which
+    carries none."""
+    rows = torch.zeros((3, 2, 64), dtype=torch.bfloat16)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(rows, torch.ones_like(rows))
+        with torch.set_grad_enabled(grad):
+            for call in _calls_with(dual):
+                with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                    call()
+            for call in _calls_with(rows):
+                with pytest.raises(ValueError, match="MI355X"):
+                    call()
+        with torch.inference_mode():
+            for call in _calls_with(dual):
+                with pytest.raises(ValueError, match="MI355X"):
+                    call()
+
+
+def test_attend_refuses_a_function_transform():
+    def f(rows):
+        return _calls_with(rows)[2]()
+
+    rows = torch.zeros((3, 2, 64), dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+        torch.func.jvp(f, (rows,), (rows,))
+    with pytest.raises(RuntimeError, match="no backward"):
+        torch.func.grad(lambda x: f(x).sum())(rows)
