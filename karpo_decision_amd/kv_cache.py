@@ -12,7 +12,8 @@ head share, so a cached element is a bf16 value exactly, and ``read`` and ``atte
 Blocks that several requests' tables share are read only: a request appends to blocks of its own.
 
 Lengths, bounds, tables and free lists are read on the device when the kernels run: nothing syncs, calls go on the
-current stream of the tensors' device and capture into graphs. All of it is forward only.
+current stream of the tensors' device and capture into graphs. All of it is forward only. The calls are no torch operators:
+torch.compile breaks its graph around them, and what has to record them whole (fullgraph, export) cannot.
 """
 
 from __future__ import annotations
@@ -24,6 +25,7 @@ from typing import NamedTuple
 
 import torch
 from torch import Tensor
+from torch._subclasses import FakeTensor
 from torch.autograd import forward_ad
 
 from . import _lib
@@ -160,6 +162,11 @@ def _on_gpu(what: str, index: int) -> None:
         raise ValueError(f"{what} runs on an MI355X GPU, not on the CPU")
 
 
+def _real(what: str, t: Tensor) -> None:
+    if type(t) is not Tensor and isinstance(t, FakeTensor):  # (has no memory, and these are no operators to record)
+        raise RuntimeError(f"kv_cache.{what} runs on real tensors: a tracer cannot record it")
+
+
 def _no_grad(what: str, *tensors: Tensor) -> None:
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise RuntimeError(f"kv_cache.{what} has no backward: call it under torch.inference_mode() or torch.no_grad()")
@@ -176,6 +183,7 @@ def reserve(table: Tensor, lengths: Tensor, counts: Tensor, free: Tensor, free_c
     end of the first ``free_count[0]`` entries of ``free``, and what the step's layers need (``Step``). ``rows`` bounds
     the counts' sum and is the packed new tokens' row count. The inputs but the table are left as they are: the free
     list goes on with ``free_left``, the requests with ``Step.lengths``."""
+    _real("reserve", table)
     index = table.get_device()
     fields = _table_fields(table, lengths, index)
     n, rows = fields[3], int(rows)
@@ -212,6 +220,7 @@ def append(cache: Cache, key: Tensor, value: Tensor, writes: Tensor) -> None:
     twice). A block's scale is the least power of two that holds what it got; where new tokens need a larger one, the
     block's earlier tokens are rounded again to it. What lies past e4m3's range at the largest scale, infinities too, is
     stored at the range's end, NaN as NaN. Rows and slots that no write names are left as they were."""
+    _real("append", key)
     _no_grad("append", key, value)
     index, bf16 = key.get_device(), torch.bfloat16
     fields = _cache_fields(cache, index)
@@ -238,6 +247,7 @@ def read(cache: Cache, table: Tensor, lengths: Tensor, rows: int) -> tuple[Tenso
     """(key, value, k_cu): the first ``lengths[i]`` cached tokens of each request as packed bf16 keys and values
     (``rows``, kv heads, D), request i's at k_cu[i]:k_cu[i + 1] (int32 on the device), what ``hip_attention.attend``
     takes. ``rows`` bounds the lengths' sum; rows behind the last request are not written."""
+    _real("read", table)
     index = table.get_device()
     fields = _cache_fields(cache, index)
     rows_fields = _table_fields(table, lengths, index)
@@ -265,6 +275,7 @@ def attend(query: Tensor, cache: Cache, table: Tensor, q_cu: Tensor, lengths: Te
     request's query count, ``total_keys`` the lengths' sum (default: all that the table can hold; it sizes the workspace
     of long query runs). Where one of them does not hold, rows that were not computed are NaN: those of a request past
     its first ``max_q``, or, in long chunks, those of all requests. Rows behind the last request are not written."""
+    _real("attend", query)
     _no_grad("attend", query)
     index = query.get_device()
     fields = _cache_fields(cache, index)

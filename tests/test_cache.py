@@ -312,3 +312,17 @@ def test_attend_refuses_a_function_transform():
         torch.func.jvp(f, (rows,), (rows,))
     with pytest.raises(RuntimeError, match="no backward"):
         torch.func.grad(lambda x: f(x).sum())(rows)
+
+
+def test_fake_tensors_are_refused():
+    """They have no memory to give to a kernel."""
+    with torch._subclasses.FakeTensorMode():
+        cache = kv_cache.create(4, 2, 64, 32, device="cuda")
+        rows = torch.empty((3, 2, 64), dtype=torch.bfloat16, device="cuda")
+        table, one, two = (torch.empty(n, dtype=torch.int32, device="cuda") for n in ((1, 2), (1,), (2,)))
+        for call in (lambda: kv_cache.reserve(table, one, one, two, one, 3, 32),
+                     lambda: kv_cache.append(cache, rows, rows, torch.empty((1, 4), dtype=torch.int32, device="cuda")),
+                     lambda: kv_cache.read(cache, table, one, 3),
+                     lambda: kv_cache.attend(rows, cache, table, two, one, 3, 0.125)):
+            with pytest.raises(RuntimeError, match="real tensors"):
+                call()
