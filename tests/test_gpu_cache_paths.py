@@ -38,13 +38,14 @@ def path_of(cache, heads, counts, rows, n, width, window=-1, total_keys=None, ma
     _lib.check(_lib.load().karpo_cache_attend_workspace_bytes(ctypes.byref(a), ctypes.byref(need)), "bytes")
     if need.value == 0:
         return WHOLE
-    # the unpacked rows, two bytes an element, keys and values; the split path's partials are vectors of fp32: its size is
-    # the same for any number of keys past the bound of the first path
-    a.total_keys, more = total + 4096, ctypes.c_size_t()
-    _lib.check(_lib.load().karpo_cache_attend_workspace_bytes(ctypes.byref(a), ctypes.byref(more)), "bytes")
-    if window >= 0:
-        return UNPACKED if need.value > 4 * min(total, n * (max_q + window)) * cache.kv_heads * cache.head_dim else SPLIT
-    return SPLIT if more.value == need.value else UNPACKED
+    # the split path's: the units before each request, and for every share two partials of a tile's vectors in fp32
+    d, vectors = cache.head_dim, max_q * heads // cache.kv_heads
+    most = 4 if d <= 128 else 2 if d == 256 else 1
+    nt = next(t for t in (1, 2, 4) if t == most or vectors <= 16 * t)
+    waves = 4 if nt == 1 and d <= 128 else 3 if (d, nt) == (64, 2) else 2 if d <= 128 or (d, nt) == (256, 1) else 1
+    y = cache.kv_heads * -(-vectors // (16 * nt))
+    split = -(-4 * (n + 1) // 256) * 256 + y * max(1, 256 * waves // y) * 2 * 16 * nt * (d + 2) * 4
+    return SPLIT if need.value == split else UNPACKED
 
 
 def make(device, head_dim, heads, kv_heads, block, lengths, counts, seed=0, width=None):
@@ -238,3 +239,195 @@ def test_a_scale_that_is_no_number_on_each_path(gpu, head_dim, heads, kv_heads, 
         rows = out[q_cu[i]:q_cu[i + 1]]
         assert torch.isnan(rows).all() if n else (rows == 0).all()
     assert (out[q_cu[-1]:] == 7).all()
+
+
+# ---- the split path (shares of the keys, joined)
+
+def attend_and_compare(device, path, head_dim, heads, kv_heads, block, lengths, counts, window=-1, causal=True, seed=0, width=None):
+    cache, table, query, q_cu = make(device, head_dim, heads, kv_heads, block, lengths, counts, seed, width)
+    n, scale = len(lengths), 1 / math.sqrt(head_dim)
+    assert path_of(cache, heads, counts, sum(counts), n, len(table[0]), window) == path
+    out = attend(device, cache, table, query, q_cu, lengths, max(counts), scale, causal=causal, window=window)
+    want = oracle.Cache(cache.keys, cache.values, cache.scales, block)
+    for i, tokens in enumerate(lengths):
+        if counts[i]:
+            close(out[q_cu[i]:q_cu[i + 1]], query[q_cu[i]:q_cu[i + 1]], *want.rows(table[i], 0, tokens), scale, causal, window,
+                  2.0 ** -8 if path == UNPACKED else 0.0)
+    return out
+
+
+@pytest.mark.parametrize("head_dim,heads,kv_heads,counts", [
+    (64, 4, 2, [1, 1, 1, 1, 1]), (64, 24, 2, [1, 2, 1, 0, 1]), (64, 24, 2, [5, 2, 1, 1, 4]), (128, 8, 4, [3, 1, 1, 7, 2]),
+    (128, 40, 2, [1, 1, 1, 1, 0]), (128, 16, 2, [7, 1, 2, 5, 1]), (256, 6, 2, [4, 1, 1, 1, 5]), (256, 24, 2, [2, 1, 2, 1, 2]),
+    (512, 8, 1, [1, 1, 2, 1, 1]), (512, 40, 2, [2, 1, 0, 1, 1]), (64, 80, 1, [2, 1, 1, 1, 1])])
+def test_split(gpu, head_dim, heads, kv_heads, counts):
+    """Every size of a workgroup's tile of query vectors, full and not: requests of one group and of many, one empty."""
+    attend_and_compare(gpu, SPLIT, head_dim, heads, kv_heads, 32, [1300, 0, 33, 7, 800], counts)
+
+
+@pytest.mark.parametrize("head_dim,heads,kv_heads,window", [(64, 4, 2, 700), (128, 4, 2, 651), (256, 4, 2, 1000), (512, 2, 1, 170),
+                                                            (512, 4, 2, 200)])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("counts", [[1, 1, 1, 1, 1], [5, 1, 32, 0, 9]])
+def test_split_with_a_window(gpu, head_dim, heads, kv_heads, window, causal, counts):
+    """Requests whose first groups no query sees, others within the window."""
+    attend_and_compare(gpu, SPLIT, head_dim, heads, kv_heads, 64, [1500, 64, 1201, 0, 900], counts, window=window,
+                       causal=causal)
+
+
+def test_split_of_many_requests(gpu):
+    """More than a workgroup's 256 threads take at once, twice: empty requests and requests without queries at those borders."""
+    lengths, counts = [(37 * i) % 200 for i in range(700)], [1 + (i % 3 == 0) for i in range(700)]
+    for i in (0, 254, 255, 256, 511, 512, 699):
+        lengths[i] = 0
+    for i in (1, 253, 255, 257, 510, 512, 513, 698, 699):
+        counts[i] = 0
+    lengths[300], lengths[514] = 900, 777
+    attend_and_compare(gpu, SPLIT, 64, 4, 2, 32, lengths, counts)
+
+
+@pytest.mark.parametrize("first,last", [(0, 256), (256, 512), (100, 101), (300, 300)])
+def test_split_where_few_of_many_requests_have_queries(gpu, first, last):
+    """Whole chunks of 256 requests without any, and a call without any at all."""
+    lengths = [40] * 600
+    lengths[0] = 700
+    counts = [1 if first <= i < last else 0 for i in range(600)]
+    cache, table, query, q_cu = make(gpu, 128, 4, 2, 32, lengths, counts or [0])
+    query = torch.cat((query, torch.ones((2, 4, 128)).bfloat16()))
+    assert path_of(cache, 4, [1], query.shape[0], 600, len(table[0])) == SPLIT
+    out = attend_into(gpu, torch.full(query.shape, 7.0, dtype=torch.bfloat16, device=gpu), cache, table, query, q_cu, lengths, 1,
+                      0.1, 600 * len(table[0]) * 32)
+    want = oracle.Cache(cache.keys, cache.values, cache.scales, 32)
+    for i in range(first, last, 7):
+        close(out[q_cu[i]:q_cu[i + 1]], query[q_cu[i]:q_cu[i + 1]], *want.rows(table[i], 0, lengths[i]), 0.1)
+    assert torch.isfinite(out).all() and (out[q_cu[-1]:] == 7).all()
+
+
+def test_split_without_tokens(gpu):
+    """Queries of requests that hold nothing, in a table that could: zeros."""
+    out = attend_and_compare(gpu, SPLIT, 128, 4, 2, 32, [0, 0, 0], [2, 1, 5], width=40)
+    assert (out == 0).all()
+
+
+def test_split_with_more_queries_than_tokens(gpu):
+    out = attend_and_compare(gpu, SPLIT, 64, 4, 2, 32, [4, 900], [9, 2])
+    assert (out[:5] == 0).all()
+
+
+def test_split_bounds_out_of_range_write_nothing(gpu):
+    """Query bounds past the query, decreasing or negative: their requests have no queries, the others theirs."""
+    lengths = [900, 20, 800, 60]
+    cache, table, query, _ = make(gpu, 64, 4, 2, 32, lengths, [2, 2, 2, 2])
+    assert path_of(cache, 4, [2], 8, 4, len(table[0])) == SPLIT
+    want = oracle.Cache(cache.keys, cache.values, cache.scales, 32)
+    for bounds, good in (([0, 2, 4, 6, 9], (0, 1, 2)), ([-3, 2, 4, 6, 8], (1, 2, 3)), ([0, 2, 4, 3, 5], (0, 1, 3)),
+                         ([9, 2, 4, 4, 2**31 - 1], (1,))):
+        out = attend_into(gpu, torch.full_like(query, 7.0, device=gpu), cache, table, query, bounds, lengths, 2, 0.1, 4000)
+        written = torch.zeros(8, dtype=torch.bool)
+        for i in good:
+            rows = slice(bounds[i], bounds[i + 1])
+            written[rows] = True
+            overlaps = bounds == [0, 2, 4, 3, 5] and i in (1, 3)  # (row 3 is two requests')
+            if not overlaps:
+                close(out[rows], query[rows], *want.rows(table[i], 0, lengths[i]), 0.1)
+        assert (out[~written.to(gpu)] == 7).all()
+
+
+def test_split_of_strided_queries_and_tables(gpu):
+    lengths = [900, 40]
+    cache, table, query, q_cu = make(gpu, 128, 4, 2, 32, lengths, [2, 1])
+    wide = torch.zeros((3, 6, 160), dtype=torch.bfloat16, device=gpu)
+    wide[:, 1:5, 16:144] = query.to(gpu)
+    tables = torch.full((2, 50), 10 ** 6, dtype=torch.int32, device=gpu)
+    tables[:, :len(table[0])] = ints(table, gpu)
+    with torch.inference_mode():
+        out = kv_cache.attend(wide[:, 1:5, 16:144], cache, tables[:, :len(table[0])], ints(q_cu, gpu), ints(lengths, gpu), 2, 0.1)
+    want = oracle.Cache(cache.keys, cache.values, cache.scales, 32)
+    for i, n in enumerate(lengths):
+        close(out[q_cu[i]:q_cu[i + 1]], query[q_cu[i]:q_cu[i + 1]], *want.rows(table[i], 0, n), 0.1)
+
+
+@pytest.mark.parametrize("head_dim,heads,kv_heads,counts,window", [(64, 4, 2, [6, 1], -1), (128, 8, 2, [9, 2], 700),
+                                                                   (512, 8, 1, [2, 1], -1), (256, 16, 8, [16, 3], 650)])
+def test_split_nan_reaches_the_queries_that_see_it_and_no_others(gpu, head_dim, heads, kv_heads, counts, window):
+    """NaN in one element of a last token's value, and in another's key; with a window also in tokens that no query sees."""
+    lengths, block = [1100, 833], 32
+    cache, table, query, q_cu = make(gpu, head_dim, heads, kv_heads, block, lengths, counts)
+    assert path_of(cache, heads, counts, sum(counts), 2, len(table[0]), window) == SPLIT
+    want = oracle.Cache(cache.keys, cache.values, cache.scales, block)
+    raw_k, raw_v = cache.keys.view(torch.uint8), cache.values.view(torch.uint8)
+    at = lengths[0] - 1
+    raw_v[table[0][at // block], 0, oracle.value_offset(at % block, 5, head_dim)] = 0x7f
+    at = lengths[1] - 1
+    raw_k[table[1][at // block], 0, oracle.key_offset(at % block, 7, head_dim)] = 0xff
+    if window >= 0:
+        for i in range(2):  # the last token before every query's window
+            at = lengths[i] - counts[i] - window - 1
+            raw_v[table[i][at // block], :, oracle.value_offset(at % block, 3, head_dim)] = 0xff
+            raw_k[table[i][at // block], :, oracle.key_offset(at % block, 9, head_dim)] = 0x7f
+    out = attend(gpu, cache, table, query, q_cu, lengths, max(counts), 0.1, window=window)
+    group = heads // kv_heads
+    expected = torch.zeros(out.shape, dtype=torch.bool)
+    expected[q_cu[1] - 1, :group, 5] = True
+    expected[q_cu[2] - 1, :group] = True
+    assert torch.equal(torch.isnan(out.cpu()), expected)
+    for i, n in enumerate(lengths):
+        rows = slice(q_cu[i], q_cu[i + 1] - 1)  # the queries before the last, which see neither
+        if rows.start < rows.stop:
+            key, value = want.rows(table[i], 0, n)
+            close(out[rows], query[rows], key[:n - 1], value[:n - 1], 0.1, window=window)
+
+
+def test_split_on_another_stream_and_beside_another_call(gpu):
+    lengths, counts = [2000, 5, 900], [1, 2, 1]
+    cache, table, query, q_cu = make(gpu, 128, 8, 2, 64, lengths, counts)
+    assert path_of(cache, 8, counts, 4, 3, len(table[0])) == SPLIT
+    args = (query.to(gpu), cache, ints(table, gpu), ints(q_cu, gpu), ints(lengths, gpu), 2, 0.1)
+    with torch.inference_mode():
+        want = kv_cache.attend(*args)
+        streams = [torch.cuda.Stream(gpu) for _ in range(2)]
+        got = []
+        for i in range(8):
+            with torch.cuda.stream(streams[i % 2]):
+                if i < 2:
+                    streams[i].wait_stream(torch.cuda.default_stream(gpu))
+                got.append(kv_cache.attend(*args))
+        torch.cuda.synchronize()
+    for out in got:
+        assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("head_dim,heads,kv_heads,window", [(128, 8, 2, -1), (256, 4, 2, 700)])
+def test_captured_split_calls_replay(gpu, head_dim, heads, kv_heads, window):
+    """Two graphs of one call after another: each replay reads the lengths, bounds and queries of then."""
+    most, counts = [2000, 1500, 900], [2, 1, 1]
+    cache, table, query, q_cu = make(gpu, head_dim, heads, kv_heads, 64, most, counts)
+    assert path_of(cache, heads, counts, 4, 3, len(table[0]), window) == SPLIT
+    query, table, q_cu, lengths = query.to(gpu), ints(table, gpu), ints(q_cu, gpu), ints(most, gpu)
+
+    def call():
+        return kv_cache.attend(query, cache, table, q_cu, lengths, 2, 0.1, window=window)
+
+    with torch.inference_mode():
+        call()
+        torch.cuda.synchronize()
+        graphs = []
+        for _ in range(2):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                out = call()
+            graphs.append((graph, out))
+        seen = []
+        for i, (change, bounds) in enumerate(((most, [0, 2, 3, 4]), ([1999, 0, 33], [0, 1, 3, 4]), ([32, 1500, 1], [0, 2, 2, 3]),
+                                              ([0, 0, 5], [0, 0, 2, 4]), (most, [0, 2, 3, 4]))):
+            lengths.copy_(ints(change, gpu))
+            q_cu.copy_(ints(bounds, gpu))
+            query.mul_(-0.75)
+            graph, out = graphs[i % 2]
+            out.zero_()
+            graph.replay()
+            want = call()
+            torch.cuda.synchronize()
+            assert torch.equal(out[:bounds[-1]], want[:bounds[-1]]) and (out[bounds[-1]:] == 0).all()
+            seen.append(out.clone())
+    assert not torch.equal(seen[0], seen[1]) and not torch.equal(seen[1], seen[2]) and not torch.equal(seen[0], seen[4])
