@@ -326,3 +326,21 @@ def test_fake_tensors_are_refused():
                      lambda: kv_cache.attend(rows, cache, table, two, one, 3, 0.125)):
             with pytest.raises(RuntimeError, match="real tensors"):
                 call()
+
+
+@pytest.mark.parametrize("tokens", [40, 90, 1000])
+def test_the_tolerance_of_attentions_weights_tells_one_bf16_term_from_two(tokens):
+    """The GPU test's two tokens of nearly one score whose values cancel: with the weights planted here as one bf16 term the
+    difference is outside the output's rounding plus 2^-14 of the weighted |value|, with two terms inside."""
+    inside = {1: True, 2: True}
+    for i in range(16):
+        x = (0.5 + torch.tensor(i / 32)).bfloat16().double()
+        score, value = torch.zeros(tokens, dtype=torch.float64), torch.zeros(tokens, dtype=torch.float64)
+        score[0], score[1], value[0], value[1] = x, 0.875 * x, 1.0, -1.0
+        w = torch.exp(score - score.max())
+        want, size = (w * value).sum() / w.sum(), (w * value.abs()).sum() / w.sum()
+        high = w.bfloat16().double()
+        for terms, p in ((1, high), (2, high + (w - high).bfloat16().double())):
+            out = ((p * value).sum() / w.sum()).bfloat16().double()
+            inside[terms] &= bool((out - want).abs() <= want.abs() * 2.0 ** -8 + size * 2.0 ** -14)
+    assert inside == {1: False, 2: True}

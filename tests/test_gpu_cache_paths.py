@@ -431,3 +431,85 @@ def test_captured_split_calls_replay(gpu, head_dim, heads, kv_heads, window):
             assert torch.equal(out[:bounds[-1]], want[:bounds[-1]]) and (out[bounds[-1]:] == 0).all()
             seen.append(out.clone())
     assert not torch.equal(seen[0], seen[1]) and not torch.equal(seen[1], seen[2]) and not torch.equal(seen[0], seen[4])
+
+
+# ---- sums that cannot hide a mistake
+
+def one_code(exponent):
+    """The e4m3 code of 2^-exponent (tensor), -8 .. 6."""
+    return ((7 - exponent) << 3).to(torch.uint8)
+
+
+@pytest.mark.parametrize("head_dim,heads,kv_heads,block,lengths,counts", [
+    (64, 1024, 1024, 64, [9000, 8300], [1, 1]), (512, 64, 64, 32, [9000, 8225], [64, 1]), (256, 512, 256, 128, [9000], [16]),
+    (128, 512, 512, 32, [17000, 16600], [1, 1]), (128, 8, 2, 64, [20011, 700, 9001], [2, 1, 3]),
+    (512, 4, 4, 128, [16001], [1])])
+def test_each_group_of_tokens_counts(gpu, head_dim, heads, kv_heads, block, lengths, counts):
+    """Equal scores, and values that are one in an element of their group's own: a group of 32 tokens left out, or read under
+    another block's scale (they differ from block to block and head to head), shows in its element. In all but the last two
+    cases a workgroup's share of one request is over 256 groups, 64 a wave, after which it looks up the table again."""
+    assert max(counts) * heads // kv_heads <= 64 and max(lengths) > 640  # the split path
+    gen = torch.Generator(device=gpu).manual_seed(1)
+    used = [-(-x // block) for x in lengths]
+    cache = kv_cache.create(sum(used), kv_heads, head_dim, block, device=gpu)
+    exps = torch.randint(-8, 7, (sum(used), kv_heads, 2), generator=gen, device=gpu)
+    cache.scales.copy_(torch.exp2(exps.float()))
+    order = torch.randperm(sum(used), generator=gen, device=gpu).tolist()
+    table = [[order.pop() for _ in range(u)] for u in used]
+    keys, values = cache.keys.view(torch.uint8), cache.values.view(torch.uint8)
+    tokens = range(block)
+    keys[:, :, offsets_of(oracle.key_offset, tokens, [0] * block, head_dim, gpu)] = one_code(exps[..., :1])
+    for row in table:
+        for j, ident in enumerate(row):
+            own = [(j * block + t) // 32 % head_dim for t in tokens]
+            values[ident][:, offsets_of(oracle.value_offset, tokens, own, head_dim, gpu)] = one_code(exps[ident, :, 1:])
+    query = torch.randn((sum(counts), heads, head_dim), generator=gen, device=gpu).bfloat16()
+    query[..., 0] = 4.0
+    width = max(used)
+    table = [r + [-1] * (width - len(r)) for r in table]
+    q_cu = [0]
+    for c in counts:
+        q_cu.append(q_cu[-1] + c)
+    assert path_of(cache, heads, counts, sum(counts), len(lengths), width) == SPLIT
+    out = attend(gpu, cache, table, query, q_cu, lengths, max(counts), 1.0).double()
+    for i, n in enumerate(lengths):
+        for r in range(counts[i]):
+            sees = n - counts[i] + r + 1
+            element = torch.arange(sees, device=gpu) // 32 % head_dim
+            want = torch.bincount(element, minlength=head_dim).double() / sees
+            off = (out[q_cu[i] + r] - want).abs()
+            assert (off <= want * (2.0 ** -8 + 2.0 ** -14)).all(), (i, r, off.max())
+
+
+def offsets_of(at, tokens, elements, head_dim, device):
+    return torch.tensor([at(t, d, head_dim) for t, d in zip(tokens, elements)], device=device)
+
+
+@pytest.mark.parametrize("head_dim,heads,kv_heads,lengths,path", [
+    (64, 4, 2, [40, 90], WHOLE), (128, 8, 2, [40, 90], WHOLE), (256, 4, 4, [40, 90], WHOLE), (512, 4, 4, [40, 90], WHOLE),
+    (64, 4, 2, [1000, 90], SPLIT), (128, 8, 2, [40, 1000], SPLIT), (256, 4, 2, [700, 90], SPLIT), (512, 4, 4, [40, 300], SPLIT),
+    (64, 64, 2, [1000, 90], SPLIT), (128, 120, 2, [40, 1000], SPLIT), (256, 64, 2, [700, 90], SPLIT)])
+def test_weights_are_as_fine_as_the_output(gpu, head_dim, heads, kv_heads, lengths, path):
+    """Two tokens of nearly one score whose values cancel, in one group: a weight rounded to one bf16 term (2^-9 off) shows in
+    the difference (tests/test_cache.py plants it), two terms (2^-17) do not."""
+    block = 32
+    cache, table, _, _ = make(gpu, head_dim, heads, kv_heads, block, lengths, [1, 1])
+    keys, values = cache.keys.view(torch.uint8), cache.values.view(torch.uint8)
+    keys.zero_(), values.zero_()
+    cache.scales.fill_(1.0)
+    for i in range(2):
+        at = lengths[i] // 2 // 2 * 2
+        ident, t = table[i][at // block], at % block
+        keys[ident, :, oracle.key_offset(t, 0, head_dim)] = 0x38       # 1
+        keys[ident, :, oracle.key_offset(t + 1, 0, head_dim)] = 0x36   # 7 / 8
+        for d in range(head_dim):
+            values[ident, :, oracle.value_offset(t, d, head_dim)] = 0x38
+            values[ident, :, oracle.value_offset(t + 1, d, head_dim)] = 0xb8
+    want = oracle.Cache(cache.keys, cache.values, cache.scales, block)
+    assert path_of(cache, heads, [1, 1], 2, 2, len(table[0])) == path
+    query = torch.zeros((2, heads, head_dim), dtype=torch.bfloat16)
+    for start in (0.5, 1.7):
+        query[..., 0] = start + torch.arange(2 * heads).view(2, heads) / 32
+        out = attend(gpu, cache, table, query, [0, 1, 2], lengths, 1, 1.0)
+        for i, n in enumerate(lengths):
+            close(out[i:i + 1], query[i:i + 1], *want.rows(table[i], 0, n), 1.0)
