@@ -513,3 +513,53 @@ def test_weights_are_as_fine_as_the_output(gpu, head_dim, heads, kv_heads, lengt
         out = attend(gpu, cache, table, query, [0, 1, 2], lengths, 1, 1.0)
         for i, n in enumerate(lengths):
             close(out[i:i + 1], query[i:i + 1], *want.rows(table[i], 0, n), 1.0)
+
+
+# ---- the uses that the cache is for
+
+@pytest.mark.parametrize("head_dim,heads,kv_heads,counts,path", [
+    (128, 8, 2, [1] * 16, SPLIT), (128, 8, 2, [1] * 15 + [5], SPLIT), (64, 32, 2, [900] + [1] * 15, UNPACKED),
+    (512, 8, 1, [2] * 16, SPLIT)])
+def test_branches_over_one_prompt(gpu, head_dim, heads, kv_heads, counts, path):
+    """Requests that share the whole blocks of one prompt, and each go on in blocks of their own."""
+    block, prompt = 32, 31 * 32
+    own = [max(counts[i], 1) + 3 * i for i in range(16)]
+    lengths = [prompt + x for x in own]
+    cache, table, query, q_cu = make(gpu, head_dim, heads, kv_heads, block, lengths, counts)
+    for row in table[1:]:
+        row[:31] = table[0][:31]
+    total = sum(lengths)
+    assert path_of(cache, heads, counts, sum(counts), 16, len(table[0]), total_keys=total) == path
+    out = attend(gpu, cache, table, query, q_cu, lengths, max(counts), 0.1, total_keys=total)
+    want = oracle.Cache(cache.keys, cache.values, cache.scales, block)
+    for i, n in enumerate(lengths):
+        close(out[q_cu[i]:q_cu[i + 1]], query[q_cu[i]:q_cu[i + 1]], *want.rows(table[i], 0, n), 0.1,
+              weights=2.0 ** -8 if path == UNPACKED else 0.0)
+
+
+@pytest.mark.parametrize("head_dim,heads,kv_heads,chunk,window", [(64, 4, 2, 200, -1), (64, 32, 2, 1000, -1), (256, 16, 8, 300, 511),
+                                                                  (128, 8, 2, 40, 700)])
+def test_a_chunk_among_single_tokens(gpu, head_dim, heads, kv_heads, chunk, window):
+    lengths, counts = [1300, 40, 1, 900, 333], [chunk, 1, 1, 1, 0]
+    cache, table, *_ = make(gpu, head_dim, heads, kv_heads, 64, lengths, counts)
+    path = path_of(cache, heads, counts, sum(counts), 5, len(table[0]), window)
+    attend_and_compare(gpu, path, head_dim, heads, kv_heads, 64, lengths, counts, window=window)
+
+
+def test_append_converts_every_bf16_value(gpu):
+    """All 65,536 bf16 values, in their order of magnitude, into blocks that hold one of nine scales already: codes and scales
+    are those of the definition."""
+    bits = torch.arange(65536, dtype=torch.int32)
+    order = (bits & 0x7fff) * 2 + (bits >> 15)  # by magnitude, signs side by side
+    x = bits[order.argsort()].to(torch.int16).view(torch.bfloat16).view(-1, 1, 64)  # 1,024 rows of 64
+    writes = [[w, 1, 31 * w, min(31, 1024 - 31 * w)] for w in range(-(-1024 // 31))]
+    for old in (-100, -61, -30, -9, -8, 0, 7, 60, 119):
+        cache = kv_cache.create(len(writes), 1, 64, 32, device=gpu)
+        cache.scales.fill_(2.0 ** old)
+        want = oracle.Cache(cache.keys, cache.values, cache.scales, 32)
+        want.append(x, -x, writes)
+        kv_cache.append(cache, x.to(gpu), (-x).to(gpu), ints(writes, gpu))
+        got = oracle.Cache(cache.keys, cache.values, cache.scales, 32)
+        assert torch.equal(got.exps, want.exps), old
+        for a, b in zip(got.codes, want.codes):
+            assert torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(a.nan_to_num(9e9), b.nan_to_num(9e9)), old
