@@ -23,7 +23,7 @@ struct Request {
 // One launch: every workgroup adds up all requests by itself (a few hundred loads that L2 holds) and then writes the rows
 // of its own range, so nothing waits on another workgroup. A new block's first token, and a request's first new token, write
 // the block's entries; which block a token's is follows from the sums alone. Bound by the launch and three rounds of dependent
-// loads (lengths, list or table, stores): 4.8 us for 48 requests of one token, 6.1 us for 65,536 tokens of 64.
+// loads (lengths, list or table, stores): 4.9 us for 48 requests of one token, 6.2 us for 65,536 tokens of 64.
 __global__ __launch_bounds__(kReserveThreads) void reserve_kernel(const ReserveParams p) {
   __shared__ int s_first[kReserveThreads + 1], s_need[kReserveThreads], s_write[kReserveThreads],
       s_tokens[kReserveThreads];
@@ -543,7 +543,8 @@ hipError_t launch_cache_append(const AppendParams& p, int64_t n_writes, hipStrea
 
 hipError_t launch_cache_read(const ReadParams& p, hipStream_t stream) {
   // A unit each wave, at most 32 workgroups per CU: 32,768 rows of 16 heads at 128 96.9 us with 1,024 workgroups, 85.5 with
-  // 2,048, 82.0 with 4,096, 77.6 with 8,192 (5.2 TB/s: how evenly the rows being written lie over the memory's channels).
+  // 2,048, 82.0 with 4,096, 77.6 with 8,192 (how evenly the rows being written lie over the memory's channels; measured before
+  // such rows were stored through the caches, 72 us since).
   const int64_t units = (p.rows / kCacheGroup + p.r.n_seq) * 2 * p.c.kv_heads * (p.c.head_dim == 64 ? 1 : p.c.head_dim / 128);
   const dim3 grid((unsigned)ka_min64((units + kReadWaves - 1) / kReadWaves + 1, 8192)), threads(64 * kReadWaves);
   auto launch = [&](auto d) {

@@ -130,14 +130,15 @@ __device__ __forceinline__ unsigned nan_codes(unsigned w) { return ((w & 0x7f7f7
 // flight a wave (8 KiB at head size 128, four waves a SIMD; 32 KiB at 512, one). Registers for them instead of LDS spilled at
 // head size 512: 240 us for one token over 131,072, 119 with LDS. Nothing but a request's end joins the waves.
 //
-// Measured (codes read / time of this kernel): 48 requests, 60,000 tokens in all, 16 heads of 128: 43.6 us, 5.6 TB/s; one of
-// 131,072 tokens, 4 heads of 512: 87.6 us, 6.1 TB/s; 32 requests, 4 tokens each, 1,024 seen, 8 heads of 256: 28.9 us, 3.9 TB/s
+// Measured (codes read / time of this kernel): 48 requests, 60,000 tokens in all, 16 heads of 128: 43.8 us, 5.6 TB/s; one of
+// 131,072 tokens, 4 heads of 512: 87.3 us, 6.1 TB/s; 32 requests, 4 tokens each, 1,024 seen, 8 heads of 256: 27.5 us, 4.0 TB/s
 // (8 us of it start and end: 2.3 us to the first table entry, then every wave's first group at once, 33 MB). A large copy
 // moves 4.9 TB/s.
 //
 // ONCE: one workgroup reads a request's codes of a head, once; they are streamed through the caches (48 requests at head size
 // 128 58.8 -> 52.8 us, 131,072 tokens at 512 105.0 -> 93.6; where several workgroups read them, 128 vectors over 32,768
-// tokens, 80 -> 88).
+// tokens, 80 -> 88). The rule goes by one request's query vectors alone: it does not see that requests whose tables share
+// blocks read the same codes, for which streaming is the wrong hint too (its cost there is not measured).
 template <int D, int NT, bool ONCE>
 __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_kernel(
     const AttendParams p) {
@@ -518,7 +519,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
 // Joins a request's shares: O = sum of 2^(m_w - M) O_w over sum of 2^(m_w - M) l_w, in an order that the sizes alone set.
 // Requests that one workgroup took whole are done already. Up to kFew shares: a thread walks them for four elements of a
 // vector. More: 64 elements of a vector by 16 threads of four and 16 rows, each row with every sixteenth share (so that
-// up to 16 cost one round of loads), and the rows joined through LDS. 4.2 to 5.9 us, launch and four rounds of loads; 33 us with
+// up to 16 cost one round of loads), and the rows joined through LDS. 4.4 to 6.6 us, launch and four rounds of loads; 33 us with
 // one walk over 64 shares of one request.
 template <int D>
 __global__ __launch_bounds__(256) void join_kernel(const AttendParams p, int vectors_per) {

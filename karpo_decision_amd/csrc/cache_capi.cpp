@@ -184,6 +184,9 @@ int64_t seen_keys(const KarpoCacheAttendArgs* a) {
 }
 
 // The rows that the queries can see, as packed bf16 keys and values, with the packed attention's own workspace behind them.
+// That kernel's weights enter its second product as one bf16 term, 2^-8 off, where the split path's are two: its matrix cores
+// are what bounds it, and a second term would be half as much work again. 2-norm error against 64 bits over a chunk of 2,048 over
+// 30,000 tokens 2.3e-3, of sums in fp32 (the output's rounding) 1.7e-3.
 struct Unpacked {
   int64_t rows, k_offset, v_offset, ws_offset;
   size_t bytes;

@@ -4,7 +4,7 @@ A serving step over requests that hold cached tokens (a prompt that more rounds 
 
     step = reserve(table, lengths, counts, free, free_count, rows, cache.block_size)  # once per step, for all layers
     append(cache, key, value, step.writes)                                            # each layer's own cache
-    out = attend(query, cache, table, step.q_cu, step.lengths, max_q, scale)
+    out = attend(query, cache, table, step.q_cu, step.lengths, max_q, scale, total_keys=total)  # total: of step.lengths
 
 ``hip_attention.attend`` reads keys that live for one call; here they live in a pool of blocks of 32, 64 or 128 tokens
 (``Cache``), found through a block table. An element is stored as an e4m3 code times a power of two that its block and
@@ -271,10 +271,14 @@ def attend(query: Tensor, cache: Cache, table: Tensor, q_cu: Tensor, lengths: Te
     at the last token. Query head h reads key/value head h // (heads / kv heads). Visible tokens: all of the request's,
     or with ``causal`` those up to the query's own, narrowed by ``window`` (how many earlier tokens stay visible; -1 for
     all); a query that sees none gets zeros. A NaN reaches the queries that see its token, and in long chunks (whose keys
-    are unpacked for the packed attention first) it can reach others of its tile, as there. ``max_q`` bounds every
-    request's query count, ``total_keys`` the lengths' sum (default: all that the table can hold; it sizes the workspace
-    of long query runs). Where one of them does not hold, rows that were not computed are NaN: those of a request past
-    its first ``max_q``, or, in long chunks, those of all requests. Rows behind the last request are not written."""
+    are unpacked for the packed attention first) it can reach others of its tile, as there. The softmax weights enter the
+    second product as two bf16 terms, in long chunks as one, as there: 2.3e-3 of the 2-norm off against 1.7e-3, the
+    output's own rounding. ``max_q`` bounds every request's query count, ``total_keys`` the lengths' sum. Long chunks
+    unpack up to ``total_keys`` tokens into a workspace (4 * kv heads * D bytes each), so give it where the table is wide:
+    the default is all that the table can hold, 51.6 GB for 48 requests in a table for 131,072 tokens, 16 heads of 128.
+    Where one of the two does not hold, rows that were not computed are NaN: those of a request past its first ``max_q``,
+    or, in long chunks, those of all requests. A NaN ``scale`` makes the rows of requests with tokens NaN. Rows behind the
+    last request are not written."""
     _real("attend", query)
     _no_grad("attend", query)
     index = query.get_device()
