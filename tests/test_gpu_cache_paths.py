@@ -490,7 +490,7 @@ def offsets_of(at, tokens, elements, head_dim, device):
     (64, 4, 2, [1000, 90], SPLIT), (128, 8, 2, [40, 1000], SPLIT), (256, 4, 2, [700, 90], SPLIT), (512, 4, 4, [40, 300], SPLIT),
     (64, 64, 2, [1000, 90], SPLIT), (128, 120, 2, [40, 1000], SPLIT), (256, 64, 2, [700, 90], SPLIT)])
 def test_weights_are_as_fine_as_the_output(gpu, head_dim, heads, kv_heads, lengths, path):
-    """Two tokens of nearly one score whose values cancel, in one group: a weight rounded to one bf16 term (2^-9 off) shows in
+    """Two tokens of nearly one score whose values cancel, in one group: a weight rounded to one bf16 term (2^-8 off) shows in
     the difference (tests/test_cache.py plants it), two terms (2^-17) do not."""
     block = 32
     cache, table, _, _ = make(gpu, head_dim, heads, kv_heads, block, lengths, [1, 1])
@@ -537,6 +537,37 @@ def test_branches_over_one_prompt(gpu, head_dim, heads, kv_heads, counts, path):
               weights=2.0 ** -8 if path == UNPACKED else 0.0)
 
 
+def test_a_branch_that_copies_the_block_it_shares_in_part(gpu):
+    """A second request over 80 tokens of a first, in blocks of 32: two blocks shared, the third, half full, copied; then both go
+    on by tokens of their own, larger than the block's, so that its scale grows in one and not in the other."""
+    block, heads, kv_heads, d = 32, 4, 2, 64
+    cache = kv_cache.create(8, kv_heads, d, block, device=gpu)
+    gen = torch.Generator().manual_seed(2)
+    key, value = (torch.randn((80 + 2, kv_heads, d), generator=gen).bfloat16() for _ in range(2))
+    key[81] *= 40
+    value[81] *= 40
+    table = torch.full((2, 4), -1, dtype=torch.int32, device=gpu)
+    free, left = ints([0, 1, 2, 3, 4, 5, 6, 7], gpu), ints([8], gpu)
+    with torch.inference_mode():
+        first = kv_cache.reserve(table, ints([0, 0], gpu), ints([80, 0], gpu), free, left, 80, block)
+        kv_cache.append(cache, key[:80].to(gpu), value[:80].to(gpu), first.writes)
+        a, b = int(table[0, 2]), 0  # (block 0 is free: blocks are taken from the list's end)
+        table[1, :2], table[1, 2] = table[0, :2], b
+        for t in (cache.keys.view(torch.uint8), cache.values.view(torch.uint8), cache.scales):
+            t[b] = t[a]
+        second = kv_cache.reserve(table, ints([80, 80], gpu), ints([1, 1], gpu), free[1:].contiguous(), first.free_left - 1, 2, block)
+        second.check()
+        kv_cache.append(cache, key[80:].to(gpu), value[80:].to(gpu), second.writes)
+        query = torch.randn((2, heads, d), generator=gen).bfloat16()
+        out = kv_cache.attend(query.to(gpu), cache, table, second.q_cu, second.lengths, 1, 0.1)
+    fed = kv_cache.create(8, kv_heads, d, block, device="cpu")
+    want = oracle.Cache(fed.keys, fed.values, fed.scales, block)
+    want.append(key[:80], value[:80], [[7, 0, 0, 32], [6, 0, 32, 32], [5, 0, 64, 16], [4, 0, 64, 16]])
+    want.append(key[80:], value[80:], [[5, 16, 0, 1], [4, 16, 1, 1]])
+    for i, blocks in enumerate(([7, 6, 5], [7, 6, 4])):
+        close(out[i:i + 1], query[i:i + 1], *want.rows(blocks, 0, 81), 0.1)
+
+
 @pytest.mark.parametrize("head_dim,heads,kv_heads,chunk,window", [(64, 4, 2, 200, -1), (64, 32, 2, 1000, -1), (256, 16, 8, 300, 511),
                                                                   (128, 8, 2, 40, 700)])
 def test_a_chunk_among_single_tokens(gpu, head_dim, heads, kv_heads, chunk, window):
@@ -563,3 +594,26 @@ def test_append_converts_every_bf16_value(gpu):
         assert torch.equal(got.exps, want.exps), old
         for a, b in zip(got.codes, want.codes):
             assert torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(a.nan_to_num(9e9), b.nan_to_num(9e9)), old
+
+
+def test_a_compiled_step_gives_what_the_calls_give(gpu):
+    """torch.compile breaks its graph around the calls: each sees the tensors of its own step, not those of the traced one."""
+    def step(cache, table, lengths, counts, free, left, key, value, query):
+        got = kv_cache.reserve(table, lengths, counts, free, left, 47, 32)
+        kv_cache.append(cache, key * 2, value, got.writes)
+        k, v, _ = kv_cache.read(cache, table, got.lengths, 47)
+        return kv_cache.attend(query + 1, cache, table, got.q_cu, got.lengths, 40, 0.1) * 2, k + 1, v
+
+    def inputs(seed):
+        gen = torch.Generator(device=gpu).manual_seed(seed)
+        rows = [torch.randn((47, h, 64), generator=gen, device=gpu).bfloat16() for h in (2, 2, 4)]
+        return (kv_cache.create(20, 2, 64, 32, device=gpu), torch.full((2, 6), -1, dtype=torch.int32, device=gpu),
+                ints([0, 0], gpu), ints([40, 7], gpu), torch.arange(20, dtype=torch.int32, device=gpu), ints([20], gpu), *rows)
+
+    torch._dynamo.reset()
+    compiled, kept = torch.compile(step, backend="eager"), []
+    with torch.inference_mode():
+        for seed in range(3):
+            kept.append(inputs(seed))  # (kept, so that the next step's tensors lie elsewhere)
+            for a, b in zip(compiled(*kept[-1]), step(*inputs(seed))):
+                assert torch.equal(a, b)
