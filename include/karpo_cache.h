@@ -1,9 +1,10 @@
 /*
- * karpo_cache.h - C ABI of the MI355X (gfx950) block cache: keys and values kept between calls in 8 bits, and the four
- * operators of a serving step over them.
+ * karpo_cache.h - C ABI of the MI355X (gfx950) block cache: keys and values kept between calls in 8 bits, and the
+ * operators of a serving step over them (in 4 bits: karpo_cache4.h).
  *
  *   karpo_cache_reserve  request lengths -> block table, slot map, positions and the list of block writes
  *   karpo_cache_append   new keys and values into their blocks
+ *   karpo_cache_append_rope  the same out of the projections: norms and position rotation on the way
  *   karpo_cache_read     cached rows of a batch back as packed bf16 keys and values
  *   karpo_cache_attend   packed attention of new queries over cached keys
  *
@@ -93,6 +94,29 @@ typedef struct KarpoCacheAppendArgs {
   int64_t n_writes;
 } KarpoCacheAppendArgs;
 
+/* What append does to the rows on the way, in fp32: key and value norms over head_dim, then the keys' rotation by halves over
+ * their first rope_dim elements. Nothing is rounded before the codes are. All zeros: nothing. */
+typedef struct KarpoCachePrologue {
+  int32_t k_norm; /* KARPO_NORM_* */
+  float k_norm_eps;
+  const void* k_norm_weight; /* device, [head_dim] bf16, 16-byte aligned, for KARPO_NORM_WEIGHT and _ONE_PLUS */
+  int32_t v_norm;
+  float v_norm_eps;
+  const void* v_norm_weight;
+  const void* rope_cos; /* device, [rope_rows][rope_dim] bf16, 16-byte aligned, or NULL (both): no rotation */
+  const void* rope_sin;
+  int64_t rope_stride; /* elements between the tables' rows, a multiple of 8 */
+  int64_t rope_rows;
+  int32_t rope_dim;         /* a multiple of 32, at most head_dim */
+  const int32_t* positions; /* device, [rows]: each row's row of the tables, or NULL: its own (rope_rows >= rows). A row
+                               whose position is outside the tables gets NaN for its rotated elements. */
+} KarpoCachePrologue;
+
+typedef struct KarpoCacheAppendRopeArgs {
+  KarpoCacheAppendArgs append;
+  KarpoCachePrologue prologue;
+} KarpoCacheAppendRopeArgs;
+
 typedef struct KarpoCacheReadArgs {
   KarpoCache cache;
   const int32_t* table; /* device, [n_seq] rows of `width` block ids */
@@ -137,6 +161,7 @@ int64_t karpo_cache_writes_capacity(int64_t rows, int32_t n_seq, int32_t block_s
 
 int karpo_cache_reserve(const KarpoCacheReserveArgs* args, void* stream);
 int karpo_cache_append(const KarpoCacheAppendArgs* args, void* stream);
+int karpo_cache_append_rope(const KarpoCacheAppendRopeArgs* args, void* stream);
 int karpo_cache_read(const KarpoCacheReadArgs* args, void* stream);
 
 /* Bytes of workspace karpo_cache_attend needs for these sizes (16-byte aligned; calls that overlap need their own). */

@@ -1,4 +1,5 @@
-"""ctypes binding of ``libkarpo_attn.so`` (``include/karpo_attn.h``, version 4, and ``include/karpo_cache.h``). The library is the only compute path: if it is
+"""ctypes binding of ``libkarpo_attn.so`` (``include/karpo_attn.h``, version 4, ``include/karpo_cache.h`` and
+``include/karpo_cache4.h``). The library is the only compute path: if it is
 missing this module raises, it never falls back to another implementation."""
 
 from __future__ import annotations
@@ -17,8 +18,10 @@ EXPORTS = ("karpo_attn_fwd", "karpo_attn_plan", "karpo_attn_plan_capacity", "kar
            "karpo_attn_device_status", "karpo_attn_fwd_noalloc")
 
 #: Every symbol ``include/karpo_cache.h`` declares.
-CACHE_EXPORTS = ("karpo_cache_writes_capacity", "karpo_cache_reserve", "karpo_cache_append", "karpo_cache_read",
-                 "karpo_cache_attend_workspace_bytes", "karpo_cache_attend")
+CACHE_EXPORTS = ("karpo_cache_writes_capacity", "karpo_cache_reserve", "karpo_cache_append", "karpo_cache_append_rope",
+                 "karpo_cache_read", "karpo_cache_attend_workspace_bytes", "karpo_cache_attend")
+#: Every symbol ``include/karpo_cache4.h`` declares.
+CACHE4_EXPORTS = ("karpo_cache4_append", "karpo_cache4_read", "karpo_cache4_attend_workspace_bytes", "karpo_cache4_attend")
 #: karpo_cache_reserve's status word.
 CACHE_NO_BLOCKS, CACHE_BAD_LENGTHS = 10, 11
 
@@ -130,6 +133,37 @@ class KarpoCacheAttendArgs(ctypes.Structure):
     ]
 
 
+class KarpoCachePrologue(ctypes.Structure):
+    _fields_ = [
+        ("k_norm", ctypes.c_int32), ("k_norm_eps", ctypes.c_float), ("k_norm_weight", ctypes.c_void_p),
+        ("v_norm", ctypes.c_int32), ("v_norm_eps", ctypes.c_float), ("v_norm_weight", ctypes.c_void_p),
+        ("rope_cos", ctypes.c_void_p), ("rope_sin", ctypes.c_void_p), ("rope_stride", ctypes.c_int64),
+        ("rope_rows", ctypes.c_int64), ("rope_dim", ctypes.c_int32), ("positions", ctypes.c_void_p),
+    ]
+
+
+class KarpoCacheAppendRopeArgs(ctypes.Structure):
+    _fields_ = [("append", KarpoCacheAppendArgs), ("prologue", KarpoCachePrologue)]
+
+
+# karpo_cache4.h's structures: the same fields over a KarpoCache4 (whose scales are bytes)
+
+class KarpoCache4(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p if name == "scales" else kind) for name, kind in KarpoCache._fields_]
+
+
+class KarpoCache4AppendArgs(ctypes.Structure):
+    _fields_ = [("cache", KarpoCache4), *KarpoCacheAppendArgs._fields_[1:], ("prologue", KarpoCachePrologue)]
+
+
+class KarpoCache4ReadArgs(ctypes.Structure):
+    _fields_ = [("cache", KarpoCache4), *KarpoCacheReadArgs._fields_[1:]]
+
+
+class KarpoCache4AttendArgs(ctypes.Structure):
+    _fields_ = [("cache", KarpoCache4), *KarpoCacheAttendArgs._fields_[1:]]
+
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 
@@ -176,11 +210,13 @@ def load() -> ctypes.CDLL:
         lib.karpo_attn_fwd_noalloc.restype = ctypes.c_int
         lib.karpo_cache_writes_capacity.argtypes = [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32]
         lib.karpo_cache_writes_capacity.restype = ctypes.c_int64
-        for name in ("reserve", "append", "read", "attend"):  # by the structures, or by their bytes (kv_cache)
-            fn = getattr(lib, "karpo_cache_" + name)
+        # by the structures, or by their bytes (kv_cache)
+        for name in ("cache_reserve", "cache_append", "cache_append_rope", "cache_read", "cache_attend", "cache4_append",
+                     "cache4_read", "cache4_attend"):
+            fn = getattr(lib, "karpo_" + name)
             fn.argtypes, fn.restype = [ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int
-        lib.karpo_cache_attend_workspace_bytes.argtypes = [ctypes.c_void_p, P(ctypes.c_size_t)]
-        lib.karpo_cache_attend_workspace_bytes.restype = ctypes.c_int
+        for fn in (lib.karpo_cache_attend_workspace_bytes, lib.karpo_cache4_attend_workspace_bytes):
+            fn.argtypes, fn.restype = [ctypes.c_void_p, P(ctypes.c_size_t)], ctypes.c_int
         _lib = lib
         return lib
 

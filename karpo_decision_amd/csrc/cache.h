@@ -1,5 +1,4 @@
-// The block cache's kernels' arguments (cache.hip, cache_attn.hip) and the layout of a block, shared with the C ABI
-// (cache_capi.cpp).
+// The block cache's kernels' arguments (cache.hip, cache_append.hip, cache_attn.hip), shared with the C ABI (cache_capi.cpp).
 #pragma once
 #include <hip/hip_runtime_api.h>
 #include <stdint.h>
@@ -11,7 +10,8 @@ constexpr int kCacheGroup = 32;  // tokens that a wave takes at once: two key ti
 struct CacheRef {
   uint8_t* keys;
   uint8_t* values;
-  float* scales;
+  float* scales;     // of a cache in 8 bits, null otherwise
+  uint8_t* scales4;  // of a cache in 4 bits, null otherwise
   int64_t blocks;
   int32_t kv_heads, head_dim, block_log2;
 };
@@ -54,6 +54,25 @@ struct AppendParams {
   int64_t rows;
 };
 hipError_t launch_cache_append(const AppendParams& p, int64_t n_writes, hipStream_t stream);
+
+// `append` with norms and rotation, and every `append` of a cache in 4 bits.
+struct NormRef {
+  int32_t mode;  // KARPO_NORM_*
+  float eps;
+  const uint16_t* weight;  // or null
+};
+struct AppendRowsParams {
+  AppendParams a;
+  NormRef k_norm, v_norm;
+  const uint16_t* cos;  // or null: no rotation
+  const uint16_t* sin;
+  int64_t rope_stride, rope_rows;
+  int32_t rope_dim;
+  const int32_t* positions;  // each row's row of the tables, or null: its own
+  int64_t n_writes;
+  int32_t by_die;  // all workgroups of a write on one die (the launch's)
+};
+hipError_t launch_cache_append_rows(AppendRowsParams p, hipStream_t stream);
 
 struct ReadParams {
   CacheRef c;

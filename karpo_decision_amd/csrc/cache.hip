@@ -348,20 +348,73 @@ __global__ __launch_bounds__(64 * WAVES) void append_kernel(const AppendParams p
 
 constexpr int kReadWaves = 4;
 
+// Rows of 32 tokens of one head's keys in 4 bits, t0 .. + N of the D / 64 parts that their tokens make (2,048 / D tokens each): a
+// lane takes 4 bytes, 8 elements of a token, D / 8 lanes side by side a whole row.
+template <int D, int N, class Store>
+__device__ __forceinline__ void read_keys4(const uint8_t* codes, const uint8_t* scales, bool known, int t0, int tokens_left,
+                                           uint16_t* to, int64_t step, int lane, Store store) {
+  constexpr int kLanes = D / 8, kRows = 64 / kLanes;  // a load: kRows tokens
+  constexpr int kLoads = N * 4;
+  const int sub = lane / kLanes, d0 = (lane - sub * kLanes) * 8, group = d0 >> 5;
+  unsigned w[kLoads], sc[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int token = (t0 * 4 + i) * kRows + sub, t2 = token >> 4, t16 = token & 15;
+    const int byte = D == 64 ? (t2 * 2 + group) * 16 + t16 : ((group & 3) * 16 + t16) * (D / 64) + (group >> 2) * 2 + t2;
+    w[i] = known ? *reinterpret_cast<const unsigned*>(codes + (t2 * (D / 32) + group) * 256 + t16 * 16 + ((d0 & 31) >> 1)) : 0;
+    sc[i] = known ? scales[byte] : 0;
+  }
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int token = (t0 * 4 + i) * kRows + sub;
+    const float scale = __uint_as_float(sc[i] << 23);
+    if (token < tokens_left) store(to + token * step + d0, bf16_of_8_codes4(w[i], scale));
+  }
+}
+// The same of values, t0 .. + N of their tiles of 64 elements: a lane takes the bytes of 4 tokens x 8 elements, four words, and stores 16 bytes of each token's row; eight
+// lanes side by side make 128 of a row.
+template <int D, int N, class Store>
+__device__ __forceinline__ void read_values4(const uint8_t* codes, const uint8_t* scales, bool known, int t0, int tokens_left,
+                                             uint16_t* to, int64_t step, int lane, Store store) {
+  const int j = lane & 3, g = (lane >> 2) & 1, q = (lane >> 3) & 3, t2 = lane >> 5;
+  unsigned w[N][4], sc[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const uint8_t* const from = codes + (t0 + n) * 1024 + (q * 16 + 4 * j) * 16 + g * 8 + t2 * 4;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[n][k] = known ? *reinterpret_cast<const unsigned*>(from + k * 16) : 0;
+    sc[n] = known ? *reinterpret_cast<const unsigned*>(scales + (2 * (t0 + n) + g) * 32 + q * 8 + t2 * 4) : 0;
+  }
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    unsigned row[4];
+    transposed(w[n], row);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int token = 16 * t2 + 4 * q + i;
+      const float scale = __uint_as_float(sc[n] >> (8 * i) << 23);  // (the conversion goes by the exponent alone)
+      if (token < tokens_left)
+        store(to + token * step + (t0 + n) * 64 + g * 32 + j * 8, bf16_of_8_codes4(row[i], scale));
+    }
+  }
+}
+
 // A wave takes 32 tokens of one head's keys or values at a time, the heads of a group one after the other, so that the rows
 // that a workgroup writes lie side by side. Keys: 8 codes a lane make 16 bytes of a row, 8 lanes the 128 of a tile's row.
 // Values: the tokens lie innermost, so the codes go through LDS (one tile after the other, 64 bytes between their halves
 // against bank conflicts), out of which a lane takes 4 tokens x 8 elements: 16 bytes of four rows. Each workgroup adds up all
 // lengths by itself and takes an equal share of all groups. Bound by HBM: 32,768 rows of 16 heads at 128 72 us, 5.6 TB/s; 9,244
 // rows of 4 heads at 512 19.8 us, 5.7 TB/s (112 and 36.6 us with 8-byte stores of the values and a head a workgroup).
-template <int D, bool STREAM>
+//
+// In 4 bits (read_rows4) a unit is 2 KiB of codes, out of which go 8 KiB of rows.
+template <int D, bool STREAM, int BITS>
 __global__ __launch_bounds__(64 * kReadWaves) void read_kernel(const ReadParams p) {
-  constexpr int kThreads = 64 * kReadWaves, kTiles = D / 32;
-  constexpr int kAtOnce = kTiles < 4 ? kTiles : 4;  // KiB of codes that a lane's loads have in flight
+  constexpr int kThreads = 64 * kReadWaves, kTiles = D * BITS / 256;
+  constexpr int kAtOnce = BITS == 4 ? (kTiles < 2 ? kTiles : 2) : kTiles < 4 ? kTiles : 4;  // KiB of codes in a unit
   constexpr int kTileBytes = 2 * (512 + 64);
   __shared__ int s_part[kReadWaves][2];
   __shared__ int s_group[kThreads + 1], s_row[kThreads], s_start[kThreads], s_tokens[kThreads];
-  __shared__ __align__(16) char s_codes[kReadWaves][kAtOnce * kTileBytes];
+  __shared__ __align__(16) char s_codes[BITS == 8 ? kReadWaves : 1][BITS == 8 ? kAtOnce * kTileBytes : 16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int heads = p.c.kv_heads, b = p.c.block_log2;
 
@@ -456,6 +509,16 @@ __global__ __launch_bounds__(64 * kReadWaves) void read_kernel(const ReadParams 
       const bool known = id >= 0 && id < p.c.blocks;
       const int64_t head = (int64_t)(known ? id : 0) * heads + h;
       const int inside = token0 & ((1 << b) - 1);
+      if constexpr (BITS == 4) {
+        const uint8_t* const codes = (value ? p.c.values : p.c.keys) + ((head << b) + inside) * (D / 2);
+        const uint8_t* const scales = p.c.scales4 + ((head << b) + inside) * (D / 16) + (value ? D : 0);
+        uint16_t* const to = (value ? p.v : p.k) + (out_row * heads + h) * D;
+        if (value)
+          read_values4<D, kAtOnce>(codes, scales, known, t0, tokens_left, to, (int64_t)heads * D, lane, store);
+        else
+          read_keys4<D, kAtOnce>(codes, scales, known, t0, tokens_left, to, (int64_t)heads * D, lane, store);
+        continue;
+      }
       const uint8_t* const src = (value ? p.c.values : p.c.keys) + (head << b) * D + inside * D;
       const float scale = known ? p.c.scales[2 * head + (value ? 1 : 0)] : 1.f;  // (zeros under any other block's could be NaN)
       uint16_t* const dst = (value ? p.v : p.k) + (out_row * heads + h) * D;
@@ -545,11 +608,15 @@ hipError_t launch_cache_read(const ReadParams& p, hipStream_t stream) {
   // A unit each wave, at most 32 workgroups per CU: 32,768 rows of 16 heads at 128 96.9 us with 1,024 workgroups, 85.5 with
   // 2,048, 82.0 with 4,096, 77.6 with 8,192 (how evenly the rows being written lie over the memory's channels; measured before
   // such rows were stored through the caches, 72 us since).
+  const bool four = p.c.scales4 != nullptr;
   const int64_t units = (p.rows / kCacheGroup + p.r.n_seq) * 2 * p.c.kv_heads * (p.c.head_dim == 64 ? 1 : p.c.head_dim / 128);
   const dim3 grid((unsigned)ka_min64((units + kReadWaves - 1) / kReadWaves + 1, 8192)), threads(64 * kReadWaves);
   auto launch = [&](auto d) {
     constexpr int D = decltype(d)::value;
-    if (p.stream) read_kernel<D, true><<<grid, threads, 0, stream>>>(p); else read_kernel<D, false><<<grid, threads, 0, stream>>>(p);
+    if (four)
+      p.stream ? read_kernel<D, true, 4><<<grid, threads, 0, stream>>>(p) : read_kernel<D, false, 4><<<grid, threads, 0, stream>>>(p);
+    else
+      p.stream ? read_kernel<D, true, 8><<<grid, threads, 0, stream>>>(p) : read_kernel<D, false, 8><<<grid, threads, 0, stream>>>(p);
   };
   switch (p.c.head_dim) {
     case 64: launch(std::integral_constant<int, 64>()); break;

@@ -1,0 +1,390 @@
+// The block cache's append with the norms and the position rotation on the way (karpo_cache_append_rope), and every append of
+// the cache in 4 bits (karpo_cache4_append).
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "cache.h"
+#include "cache_common.h"
+#include "karpo_cache.h"
+#include "karpo_cache4.h"
+
+namespace karpo {
+
+namespace {
+
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+
+// x's sum / maximum over N neighbouring lanes (N = 4, 8, .. 64; in every one of them).
+template <int N, class F>
+__device__ __forceinline__ unsigned over_lanes(unsigned x, F join) {
+  x = join(x, (unsigned)__builtin_amdgcn_update_dpp(0, x, 0xb1, 0xf, 0xf, true));  // quad_perm 1 0 3 2
+  x = join(x, (unsigned)__builtin_amdgcn_update_dpp(0, x, 0x4e, 0xf, 0xf, true));  // quad_perm 2 3 0 1
+  if constexpr (N >= 8) x = join(x, (unsigned)__builtin_amdgcn_update_dpp(0, x, 0x141, 0xf, 0xf, true));   // mirrored within 8
+  if constexpr (N >= 16) x = join(x, (unsigned)__builtin_amdgcn_update_dpp(0, x, 0x140, 0xf, 0xf, true));  // within 16
+  if constexpr (N >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = join(r[0], r[1]);
+  }
+  if constexpr (N >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    x = join(r[0], r[1]);
+  }
+  return x;
+}
+template <int N>
+__device__ __forceinline__ float sum_over(float x) {
+  return __uint_as_float(over_lanes<N>(__float_as_uint(x), [](unsigned a, unsigned b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
+}
+template <int N>
+__device__ __forceinline__ unsigned max_over(unsigned x) {
+  return over_lanes<N>(x, [](unsigned a, unsigned b) { return max(a, b); });
+}
+
+// The least e with m <= 448 * 2^e (448 = 1.75 * 2^8), with BITS 4 m <= 6 * 2^e (6 = 1.5 * 2^2), for the fp32 magnitude with
+// these bits.
+template <int BITS>
+__device__ __forceinline__ int exponent_of(unsigned bits) {
+  const int e = (int)(bits >> 23) - 127;
+  if constexpr (BITS == 8)
+    return min(max(e - 8 + ((bits & 0x7fffff) > 0x600000 ? 1 : 0), KARPO_CACHE_MIN_EXP), KARPO_CACHE_MAX_EXP);
+  else
+    return min(max(e - 2 + ((bits & 0x7fffff) > 0x400000 ? 1 : 0), KARPO_CACHE4_MIN_EXP), KARPO_CACHE4_MAX_EXP);
+}
+
+// Four fp32 over `scale` as e4m3 codes, eight as e2m1 codes (nearest, ties to even).
+__device__ __forceinline__ unsigned codes8(float a, float b, float c, float d, float scale) {
+  const s16x2 low = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(s16x2{0, 0}, a, b, scale, false);
+  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(low, c, d, scale, true));
+}
+__device__ __forceinline__ unsigned codes4(const float (&y)[8], float scale) {
+  unsigned w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0, y[0], y[1], scale, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[2], y[3], scale, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[4], y[5], scale, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[6], y[7], scale, 3);
+}
+// Four e4m3 codes under the scale `old` as codes under `scale`: rounded again.
+__device__ __forceinline__ unsigned codes_again(unsigned w, float old, float scale) {
+  auto at = [](unsigned pair, bool up) { return __uint_as_float(up ? pair & 0xffff0000u : pair << 16); };
+  const unsigned a = bf16_pair(w, old, false), b = bf16_pair(w, old, true);
+  return codes8(at(a, false), at(a, true), at(b, false), at(b, true), scale);
+}
+
+// A write: `count` tokens from slot `first` of a block on, out of the rows from `row` on.
+struct Write {
+  int first, row, count;
+  int64_t head;  // block * heads + head
+};
+
+// One write's keys, or values, of one head: WAVES waves, D / 8 lanes a token of 8 elements each (16 bytes a lane and load), the
+// tokens in PASSES passes. y = x * rsqrt(mean x^2 + eps) * w, its first rope_dim elements turned by halves, in fp32; the one
+// rounding is that to the codes. A token's sum of squares and, in 4 bits, the largest of 32 elements (four lanes) go across
+// lanes in registers; the element half a rotation away comes from its lane as the raw bf16 pair, normed again here. In 8 bits all
+// rows stay in registers until the block's maximum is known. Keys are stored from there (a token's 64 elements lie together);
+// of values the tokens lie innermost, so their codes go through LDS, a token's side by side, out of which a lane takes 4 tokens x
+// 4 bytes four times: four 16-byte pieces of the cache. Lanes past the write take its last token again and store nothing, so
+// that loads need no branches and all passes' are in flight at once.
+template <int D, int BLOCK, int PASSES, int WAVES, int BITS, bool VALUE, bool TURNED>
+__device__ __forceinline__ void append_rows(const AppendRowsParams& p, const Write& wr, int h, char* s_codes) {
+  constexpr int kLanes = D / 8, kRows = 64 / kLanes, kStep = kRows * WAVES;
+  constexpr int kBytes = BITS == 8 ? D : D / 2;  // of a token's codes
+  constexpr int kPitch = kBytes + 16;
+  const CacheRef& c = p.a.c;
+  const int first = wr.first, count = wr.count;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int sub = lane / kLanes, l = lane - sub * kLanes, d0 = l * 8;
+  uint8_t* const out = (VALUE ? c.values : c.keys) + wr.head * BLOCK * kBytes;
+  const int64_t stride = VALUE ? p.a.sv_t : p.a.sk_t;
+  const uint16_t* const in = (VALUE ? p.a.v + h * p.a.sv_h : p.a.k + h * p.a.sk_h) + wr.row * stride + d0;
+  float* const scale_of = BITS == 8 ? c.scales + 2 * wr.head + (VALUE ? 1 : 0) : nullptr;
+  const unsigned old_bits = BITS == 8 && first > 0 ? __float_as_uint(*scale_of) : 0;
+  auto token_of = [&](int t) { return t * kStep + wave * kRows + sub; };
+
+  int64_t at[PASSES];  // the tokens' rows of the tables
+  if constexpr (TURNED) {
+#pragma unroll
+    for (int t = 0; t < PASSES; ++t) {
+      at[t] = (int64_t)wr.row + min(token_of(t), count - 1);
+      if (p.positions != nullptr) at[t] = p.positions[at[t]];
+    }
+  }
+  u32x4 x[PASSES];
+#pragma unroll
+  for (int t = 0; t < PASSES; ++t) x[t] = *reinterpret_cast<const u32x4*>(in + min(token_of(t), count - 1) * stride);
+
+  // norm: (x * w) * r, w the weight, 1 + weight or 1; rotation of the first rope_dim elements, partner rh away. A product of two
+  // bf16 numbers, and of three, is exact in fp32, so a weighted key takes two roundings, (xw * cos - xw' * sin) and the
+  // product with r (normed first and then turned it is five).
+  const NormRef& norm = VALUE ? p.v_norm : p.k_norm;
+  const bool normed = norm.mode != KARPO_NORM_NONE;
+  const float wm = norm.mode == KARPO_NORM_WEIGHT || norm.mode == KARPO_NORM_ONE_PLUS ? 1.f : 0.f;
+  const float wa = norm.mode == KARPO_NORM_WEIGHT ? 0.f : 1.f;
+  const int rd = TURNED ? p.rope_dim : 0, rh = rd >> 1;
+  const bool inside = d0 < rd;
+  const int dp = inside ? (d0 < rh ? d0 + rh : d0 - rh) : d0;
+  const float sign = d0 < rh ? -1.f : 1.f;
+  u32x4 wv = {0, 0, 0, 0}, wp = {0, 0, 0, 0};
+  if (wm != 0.f) {
+    wv = *reinterpret_cast<const u32x4*>(norm.weight + d0);
+    if constexpr (TURNED) wp = *reinterpret_cast<const u32x4*>(norm.weight + dp);
+  }
+  const int partner = (sub * kLanes + (dp >> 3)) * 4;  // its lane's byte address
+  auto row_of = [&](int t, float (&y)[8]) {
+    float r = 1.f;
+    if (normed) {
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(bf16_at(x[t], e), bf16_at(x[t], e), ss);
+      r = 1.f / __builtin_sqrtf(sum_over<kLanes>(ss) * (1.f / D) + norm.eps);
+    }
+    auto weighted = [&](const u32x4& v, const u32x4& w, int e) { return bf16_at(v, e) * (wm * bf16_at(w, e) + wa); };
+    if constexpr (TURNED) {
+      u32x4 px;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) px[k] = (unsigned)__builtin_amdgcn_ds_bpermute(partner, (int)x[t][k]);
+      const bool known = at[t] >= 0 && at[t] < p.rope_rows;
+      const int64_t from = (known ? at[t] : 0) * p.rope_stride + (inside ? d0 : 0);
+      u32x4 cv = *reinterpret_cast<const u32x4*>(p.cos + from), sv = *reinterpret_cast<const u32x4*>(p.sin + from);
+      if (!known) cv = u32x4{kNanPair, kNanPair, kNanPair, kNanPair};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float n = weighted(x[t], wv, e);
+        const float turn = __builtin_fmaf(n, bf16_at(cv, e), sign * weighted(px, wp, e) * bf16_at(sv, e));
+        y[e] = (inside ? turn : n) * r;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = weighted(x[t], wv, e) * r;
+    }
+  };
+
+  bool grown = false;
+  float scale = 1.f, old_scale = 1.f;
+  if constexpr (BITS == 8) {
+    float y[PASSES][8];
+    unsigned best = 0;
+#pragma unroll
+    for (int t = 0; t < PASSES; ++t) {
+      row_of(t, y[t]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) best = max(best, __float_as_uint(y[t][e]) & 0x7fffffffu);
+    }
+    auto joined = [&](unsigned mine) {  // over the workgroup
+      mine = max_over<64>(mine);
+      if constexpr (WAVES > 1) {
+        unsigned* const s_best = reinterpret_cast<unsigned*>(s_codes);
+        __syncthreads();
+        if (lane == 0) s_best[wave] = mine;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) mine = max(mine, s_best[w]);
+        __syncthreads();  // (the codes take the array)
+      }
+      return mine;
+    };
+    best = joined(best);
+    const bool odd = best >= 0x7f800000u;  // infinities or NaN: the largest of the others
+    if (__builtin_expect(odd, 0)) {
+      best = 0;
+#pragma unroll
+      for (int t = 0; t < PASSES; ++t)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const unsigned m = __float_as_uint(y[t][e]) & 0x7fffffffu;
+          best = max(best, m < 0x7f800000u ? m : 0u);
+        }
+      best = joined(best);
+    }
+    int e = exponent_of<8>(best), old = e;
+    if (first > 0) {
+      old = min(max((int)((old_bits >> 23) & 0xff) - 127, KARPO_CACHE_MIN_EXP), KARPO_CACHE_MAX_EXP);
+      e = max(e, old);
+    }
+    grown = old < e;  // the earlier tokens' codes are rounded again
+    scale = power_of_two(e);
+    old_scale = power_of_two(old);
+    if (tid == 0) *scale_of = scale;
+    if (__builtin_expect(odd || e == KARPO_CACHE_MAX_EXP, 0)) {
+      const float most = 448.f * scale;
+#pragma unroll
+      for (int t = 0; t < PASSES; ++t)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y[t][k] = __builtin_fabsf(y[t][k]) > most ? __builtin_copysignf(most, y[t][k]) : y[t][k];
+    }
+#pragma unroll
+    for (int t = 0; t < PASSES; ++t) {
+      const int slot = first + token_of(t);
+      const u32x2 w = {codes8(y[t][0], y[t][1], y[t][2], y[t][3], scale), codes8(y[t][4], y[t][5], y[t][6], y[t][7], scale)};
+      if (token_of(t) < count) {
+        if constexpr (VALUE)
+          *reinterpret_cast<u32x2*>(s_codes + slot * kPitch + d0) = w;
+        else
+          *reinterpret_cast<u32x2*>(out + ((slot >> 4) * (D / 64) + (d0 >> 6)) * 1024 + (slot & 15) * 64 + (d0 & 63)) = w;
+      }
+    }
+    if (!VALUE && grown) {
+      for (int u = tid; u < first * (D / 16); u += 64 * WAVES) {
+        const int slot = u / (D / 16), piece = u % (D / 16);
+        u32x4* const dst =
+            reinterpret_cast<u32x4*>(out + ((slot >> 4) * (D / 64) + (piece >> 2)) * 1024 + (slot & 15) * 64 + (piece & 3) * 16);
+        u32x4 w = *dst;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = codes_again(w[k], old_scale, scale);
+        *dst = w;
+      }
+    }
+  } else {
+    uint8_t* const scales = c.scales4 + wr.head * (BLOCK / 32) * 2 * D + (VALUE ? D : 0);
+#pragma unroll
+    for (int t = 0; t < PASSES; ++t) {
+      const int slot = first + token_of(t);
+      float y[8];
+      row_of(t, y);
+      unsigned best = 0, all = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const unsigned m = __float_as_uint(y[e]) & 0x7fffffffu;
+        best = max(best, m < 0x7f800000u ? m : 0u);
+        all = max(all, m);
+      }
+      best = max_over<4>(best);
+      all = max_over<4>(all);
+      const int e = exponent_of<4>(best);
+      const unsigned w = codes4(y, power_of_two(e));
+      if (token_of(t) < count) {
+        const int group = d0 >> 5, t2 = (slot >> 4) & 1, t16 = slot & 15;
+        if constexpr (VALUE)
+          *reinterpret_cast<unsigned*>(s_codes + slot * kPitch + (d0 >> 1)) = w;
+        else
+          *reinterpret_cast<unsigned*>(out + (slot >> 5) * 16 * D + (t2 * (D / 32) + group) * 256 + t16 * 16 +
+                                       ((d0 & 31) >> 1)) = w;
+        if ((l & 3) == 0) {
+          const int byte = VALUE     ? group * 32 + (t16 >> 2) * 8 + t2 * 4 + (t16 & 3)
+                           : D == 64 ? (t2 * 2 + group) * 16 + t16
+                                     : ((group & 3) * 16 + t16) * (D / 64) + (group >> 2) * 2 + t2;
+          scales[(slot >> 5) * 2 * D + byte] = all > 0x7f800000u ? 255 : (uint8_t)(e + 127);
+        }
+      }
+    }
+  }
+  if constexpr (VALUE) {
+    __syncthreads();
+    const int h0 = grown ? 0 : first >> 5, h1 = (first + count - 1) >> 5;
+    constexpr int kTiles = kBytes / 32;  // KiB of codes of 32 tokens
+    for (int u = tid; u < (h1 - h0 + 1) * kTiles * 16; u += 64 * WAVES) {
+      const int j = u & 3, q = (u >> 2) & 3, tile = (u >> 4) % kTiles, half = h0 + (u >> 4) / kTiles;
+      // bytes of the tokens 16 t + 4 q + 0 .. 3 that are new, and that are rounded again
+      unsigned is_new[2] = {0, 0}, is_old[2] = {0, 0};
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int slot = half * 32 + t * 16 + q * 4 + i;
+          if (slot >= first && slot < first + count) is_new[t] |= 0xffu << (8 * i);
+          if (grown && slot < first) is_old[t] |= 0xffu << (8 * i);
+        }
+      if ((is_new[0] | is_new[1] | is_old[0] | is_old[1]) == 0) continue;
+      const bool whole = (is_new[0] & is_new[1]) == 0xffffffffu;
+      u32x4 w[4];
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          unsigned r[4], o[4];
+          const char* const from = s_codes + (half * 32 + t * 16 + q * 4) * kPitch + tile * 32 + g * 16 + j * 4;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) r[i] = *reinterpret_cast<const unsigned*>(from + i * kPitch);
+          transposed(r, o);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k][2 * g + t] = o[k];
+        }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int dl = 4 * j + k;
+        u32x4* const dst = reinterpret_cast<u32x4*>(out + (half * kTiles + tile) * 1024 +
+                                                    (BITS == 8 ? dl * 64 + q * 16 : (q * 16 + dl) * 16));
+        if (!whole) {
+          const u32x4 was = *dst;
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            unsigned kept = was[m];
+            if constexpr (BITS == 8)
+              if (grown) kept = (codes_again(kept, old_scale, scale) & is_old[m & 1]) | (kept & ~is_old[m & 1]);
+            w[k][m] = (w[k][m] & is_new[m & 1]) | (kept & ~is_new[m & 1]);
+          }
+        }
+        *dst = w[k];
+      }
+    }
+  }
+}
+
+template <int D, int BLOCK, int PASSES, int WAVES, int BITS>
+__global__ __launch_bounds__(64 * WAVES) void append_rows_kernel(const AppendRowsParams p) {
+  constexpr int kStep = 512 / D * WAVES;  // tokens of a pass
+  __shared__ __align__(16) char s_codes[BLOCK * ((BITS == 8 ? D : D / 2) + 16)];
+  const int heads = p.a.c.kv_heads;
+  int64_t unit;
+  int which;
+  if (p.by_die) {  // workgroups go round the eight dies: write 8 k + i on die i
+    const int64_t turn = blockIdx.x >> 3, k = turn / (2 * heads);
+    which = (int)(turn - k * 2 * heads);
+    unit = 8 * k + (blockIdx.x & 7);
+    if (unit >= p.n_writes) return;
+  } else {
+    unit = blockIdx.x / (2 * heads);
+    which = (int)(blockIdx.x - unit * 2 * heads);
+  }
+  const int4 w = *reinterpret_cast<const int4*>(p.a.writes + 4 * unit);
+  const int id = w.x, first = w.y, row = w.z, count = w.w, h = which >> 1;
+  if (count < 1 || id < 0 || id >= p.a.c.blocks || first < 0 || count > BLOCK - first || row < 0 || row > p.a.rows - count)
+    return;
+  const Write wr = {first, row, count, (int64_t)id * heads + h};
+  auto run = [&](auto passes) {
+    constexpr int N = decltype(passes)::value;
+    if (which & 1)
+      append_rows<D, BLOCK, N, WAVES, BITS, true, false>(p, wr, h, s_codes);
+    else if (p.cos != nullptr)
+      append_rows<D, BLOCK, N, WAVES, BITS, false, true>(p, wr, h, s_codes);
+    else
+      append_rows<D, BLOCK, N, WAVES, BITS, false, false>(p, wr, h, s_codes);
+  };
+  if (count <= kStep) run(std::integral_constant<int, 1>()); else run(std::integral_constant<int, PASSES>());
+}
+
+template <int D, int BITS>
+hipError_t launch(const AppendRowsParams& p, hipStream_t stream) {
+  const int64_t units = p.by_die ? (p.n_writes + 7) / 8 * 8 : p.n_writes;
+  const dim3 grid((unsigned)(units * 2 * p.a.c.kv_heads));
+  auto run = [&](auto blocks) {
+    constexpr int kPieces = D * decltype(blocks)::value / 512;  // of 64 lanes x 8 elements
+    constexpr int kWaves = kPieces <= 8 ? 1 : kPieces <= 64 ? kPieces / 8 : 8, kPasses = kPieces / kWaves;
+    append_rows_kernel<D, decltype(blocks)::value, kPasses, kWaves, BITS><<<grid, dim3(64 * kWaves), 0, stream>>>(p);
+  };
+  switch (p.a.c.block_log2) {
+    case 5: run(std::integral_constant<int, 32>()); break;
+    case 6: run(std::integral_constant<int, 64>()); break;
+    case 7: run(std::integral_constant<int, 128>()); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_cache_append_rows(AppendRowsParams p, hipStream_t stream) {
+  p.by_die = p.n_writes >= 8;  // (the rotary tables' rows are read by each head: out of one die's L2)
+  const bool four = p.a.c.scales4 != nullptr;
+  switch (p.a.c.head_dim) {
+    case 64: return four ? launch<64, 4>(p, stream) : launch<64, 8>(p, stream);
+    case 128: return four ? launch<128, 4>(p, stream) : launch<128, 8>(p, stream);
+    case 256: return four ? launch<256, 4>(p, stream) : launch<256, 8>(p, stream);
+    case 512: return four ? launch<512, 4>(p, stream) : launch<512, 8>(p, stream);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+}  // namespace karpo

@@ -1,4 +1,4 @@
-// The block cache's C ABI (karpo_cache.h): argument checks, workspace sizes and launches. Everything that the kernels
+// The block cache's C ABI (karpo_cache.h, karpo_cache4.h: the same functions over either cache): argument checks, workspace sizes and launches. Everything that the kernels
 // index with is checked here or in the kernel itself, before a launch or a load.
 #include <math.h>
 #include <stdint.h>
@@ -6,6 +6,7 @@
 
 #include "cache.h"
 #include "karpo_cache.h"
+#include "karpo_cache4.h"
 
 using namespace karpo;
 
@@ -23,16 +24,22 @@ bool overlaps(const void* a, int64_t na, const void* b, int64_t nb) {
 // Tokens of a table's row; all rows of a table in groups of 32 tokens (and 64 more each, which the shares add) fit 32 bits.
 constexpr int64_t kMostTokens = (int64_t)1 << 26;
 
-int check_cache(const KarpoCache& c, CacheRef* ref) {
+void scales_of(const KarpoCache& c, CacheRef* ref) { ref->scales = c.scales; }
+void scales_of(const KarpoCache4& c, CacheRef* ref) { ref->scales4 = static_cast<uint8_t*>(c.scales); }
+uintptr_t scale_alignment(const KarpoCache&) { return 8; }
+uintptr_t scale_alignment(const KarpoCache4&) { return 16; }
+
+template <class Cache>
+int check_cache(const Cache& c, CacheRef* ref) {
   const int b = block_log2(c.block_size);
   if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256 && c.head_dim != 512) return KARPO_ATTN_ERR_HEAD_DIM;
   if (c.kv_heads < 1 || c.kv_heads > 8192) return KARPO_ATTN_ERR_HEADS;
   if (b < 0 || c.blocks < 1 || c.blocks > INT32_MAX) return KARPO_ATTN_ERR_ARG;
   if (!c.keys || !c.values || !c.scales) return KARPO_ATTN_ERR_NULL;
-  if (!aligned(c.keys, 16) || !aligned(c.values, 16) || !aligned(c.scales, 8)) return KARPO_ATTN_ERR_LAYOUT;
+  if (!aligned(c.keys, 16) || !aligned(c.values, 16) || !aligned(c.scales, scale_alignment(c))) return KARPO_ATTN_ERR_LAYOUT;
   ref->keys = static_cast<uint8_t*>(c.keys);
   ref->values = static_cast<uint8_t*>(c.values);
-  ref->scales = c.scales;
+  scales_of(c, ref);
   ref->blocks = c.blocks;
   ref->kv_heads = c.kv_heads;
   ref->head_dim = c.head_dim;
@@ -124,35 +131,108 @@ extern "C" int karpo_cache_reserve(const KarpoCacheReserveArgs* a, void* stream)
   return KARPO_ATTN_OK;
 }
 
-extern "C" int karpo_cache_append(const KarpoCacheAppendArgs* a, void* stream) {
-  if (a == nullptr) return KARPO_ATTN_ERR_NULL;
-  AppendParams p;
-  memset(&p, 0, sizeof(p));
-  const int st = check_cache(a->cache, &p.c);
+namespace {
+
+// The checks that every append makes; *none: there is nothing to write.
+template <class Args>
+int append_params(const Args* a, AppendParams* p, bool* none) {
+  memset(p, 0, sizeof(*p));
+  *none = false;
+  const int st = check_cache(a->cache, &p->c);
   if (st != KARPO_ATTN_OK) return st;
   if (a->rows < 0 || a->rows > INT32_MAX || a->n_writes < 0 || a->n_writes > INT32_MAX / (2 * a->cache.kv_heads))
     return KARPO_ATTN_ERR_ARG;
-  const int64_t bytes = p.c.blocks * ((int64_t)p.c.kv_heads * p.c.head_dim << p.c.block_log2);
-  if (overlaps(p.c.keys, bytes, p.c.values, bytes)) return KARPO_ATTN_ERR_ARG;  // (either's writes would be the other's)
-  if (a->rows == 0 || a->n_writes == 0) return KARPO_ATTN_OK;
+  const int64_t elements = p->c.blocks * ((int64_t)p->c.kv_heads * p->c.head_dim << p->c.block_log2);
+  const int64_t bytes = p->c.scales4 != nullptr ? elements / 2 : elements;
+  if (overlaps(p->c.keys, bytes, p->c.values, bytes)) return KARPO_ATTN_ERR_ARG;  // (either's writes would be the other's)
+  *none = a->rows == 0 || a->n_writes == 0;
+  if (*none) return KARPO_ATTN_OK;
   if (!a->k || !a->v || !a->writes) return KARPO_ATTN_ERR_NULL;
   if (!row_strides(a->k, a->k_stride_tok, a->k_stride_head) || !row_strides(a->v, a->v_stride_tok, a->v_stride_head) ||
       !aligned(a->writes, 16))
     return KARPO_ATTN_ERR_LAYOUT;
-  p.k = static_cast<const uint16_t*>(a->k);
-  p.v = static_cast<const uint16_t*>(a->v);
-  p.sk_t = a->k_stride_tok;
-  p.sk_h = a->k_stride_head;
-  p.sv_t = a->v_stride_tok;
-  p.sv_h = a->v_stride_head;
-  p.writes = a->writes;
-  p.rows = a->rows;
+  p->k = static_cast<const uint16_t*>(a->k);
+  p->v = static_cast<const uint16_t*>(a->v);
+  p->sk_t = a->k_stride_tok;
+  p->sk_h = a->k_stride_head;
+  p->sv_t = a->v_stride_tok;
+  p->sv_h = a->v_stride_head;
+  p->writes = a->writes;
+  p->rows = a->rows;
+  return KARPO_ATTN_OK;
+}
+
+int norm_of(int32_t mode, float eps, const void* weight, NormRef* n) {
+  if (mode < KARPO_NORM_NONE || mode > KARPO_NORM_PLAIN) return KARPO_ATTN_ERR_PROLOGUE;
+  if ((mode == KARPO_NORM_WEIGHT || mode == KARPO_NORM_ONE_PLUS) && (weight == nullptr || !aligned(weight, 16)))
+    return KARPO_ATTN_ERR_PROLOGUE;
+  n->mode = mode;
+  n->eps = eps;
+  n->weight = static_cast<const uint16_t*>(weight);
+  return KARPO_ATTN_OK;
+}
+
+// Norms and rotation of rows with head_dim elements; p.a is set.
+int prologue_params(const KarpoCachePrologue& f, int32_t head_dim, AppendRowsParams* p) {
+  int st = norm_of(f.k_norm, f.k_norm_eps, f.k_norm_weight, &p->k_norm);
+  if (st == KARPO_ATTN_OK) st = norm_of(f.v_norm, f.v_norm_eps, f.v_norm_weight, &p->v_norm);
+  if (st != KARPO_ATTN_OK) return st;
+  if ((f.rope_cos == nullptr) != (f.rope_sin == nullptr)) return KARPO_ATTN_ERR_PROLOGUE;
+  if (f.rope_cos == nullptr) return KARPO_ATTN_OK;
+  if (f.rope_dim <= 0 || f.rope_dim % 32 != 0 || f.rope_dim > head_dim || f.rope_stride < f.rope_dim || f.rope_stride % 8 != 0 ||
+      !aligned(f.rope_cos, 16) || !aligned(f.rope_sin, 16) || f.rope_rows < 1 || !aligned(f.positions, 4))
+    return KARPO_ATTN_ERR_PROLOGUE;
+  if (f.positions == nullptr && f.rope_rows < p->a.rows) return KARPO_ATTN_ERR_PROLOGUE;
+  p->cos = static_cast<const uint16_t*>(f.rope_cos);
+  p->sin = static_cast<const uint16_t*>(f.rope_sin);
+  p->rope_stride = f.rope_stride;
+  p->rope_rows = f.rope_rows;
+  p->rope_dim = f.rope_dim;
+  p->positions = f.positions;
+  return KARPO_ATTN_OK;
+}
+
+template <class Args>
+int append_rows(const Args* a, const KarpoCachePrologue& f, void* stream) {
+  AppendRowsParams p;
+  memset(&p, 0, sizeof(p));
+  bool none;
+  int st = append_params(a, &p.a, &none);
+  if (st != KARPO_ATTN_OK) return st;
+  if (a->n_writes > INT32_MAX / (2 * a->cache.kv_heads) - 8) return KARPO_ATTN_ERR_ARG;  // (rounded up to the eight dies)
+  p.a.rows = a->rows;
+  st = prologue_params(f, a->cache.head_dim, &p);
+  if (st != KARPO_ATTN_OK || none) return st;
+  p.n_writes = a->n_writes;
+  if (launch_cache_append_rows(p, static_cast<hipStream_t>(stream)) != hipSuccess) return KARPO_ATTN_ERR_LAUNCH;
+  return KARPO_ATTN_OK;
+}
+
+}  // namespace
+
+extern "C" int karpo_cache_append(const KarpoCacheAppendArgs* a, void* stream) {
+  if (a == nullptr) return KARPO_ATTN_ERR_NULL;
+  AppendParams p;
+  bool none;
+  const int st = append_params(a, &p, &none);
+  if (st != KARPO_ATTN_OK || none) return st;
   if (launch_cache_append(p, a->n_writes, static_cast<hipStream_t>(stream)) != hipSuccess)
     return KARPO_ATTN_ERR_LAUNCH;
   return KARPO_ATTN_OK;
 }
 
-extern "C" int karpo_cache_read(const KarpoCacheReadArgs* a, void* stream) {
+extern "C" int karpo_cache_append_rope(const KarpoCacheAppendRopeArgs* a, void* stream) {
+  return a == nullptr ? KARPO_ATTN_ERR_NULL : append_rows(&a->append, a->prologue, stream);
+}
+
+extern "C" int karpo_cache4_append(const KarpoCache4AppendArgs* a, void* stream) {
+  return a == nullptr ? KARPO_ATTN_ERR_NULL : append_rows(a, a->prologue, stream);
+}
+
+namespace {
+
+template <class Args>
+int read_rows(const Args* a, void* stream) {
   if (a == nullptr) return KARPO_ATTN_ERR_NULL;
   ReadParams p;
   memset(&p, 0, sizeof(p));
@@ -173,12 +253,11 @@ extern "C" int karpo_cache_read(const KarpoCacheReadArgs* a, void* stream) {
   return KARPO_ATTN_OK;
 }
 
-namespace {
-
 int64_t round_up(int64_t x, int64_t n) { return (x + n - 1) / n * n; }
 
 // A bound of the tokens that the queries of all requests see.
-int64_t seen_keys(const KarpoCacheAttendArgs* a) {
+template <class Args>
+int64_t seen_keys(const Args* a) {
   const int64_t each = (int64_t)a->max_q + a->window_left;
   return a->window_left >= 0 && each < a->total_keys && each * a->n_seq < a->total_keys ? each * a->n_seq : a->total_keys;
 }
@@ -193,7 +272,8 @@ struct Unpacked {
   KarpoAttnArgs fwd;
 };
 
-int unpacked_of(const KarpoCacheAttendArgs* a, Unpacked* u) {
+template <class Args>
+int unpacked_of(const Args* a, Unpacked* u) {
   // (with a window, each request's rows begin at a multiple of 32)
   int64_t rows = seen_keys(a);
   if (rows < a->total_keys) {
@@ -235,7 +315,8 @@ int unpacked_of(const KarpoCacheAttendArgs* a, Unpacked* u) {
 }
 
 // Sizes and head counts (everything the workspace's size depends on).
-int check_attend(const KarpoCacheAttendArgs* a, CacheRef* c, CacheRows* r) {
+template <class Args>
+int check_attend(const Args* a, CacheRef* c, CacheRows* r) {
   if (a == nullptr) return KARPO_ATTN_ERR_NULL;
   int st = check_cache(a->cache, c);
   if (st != KARPO_ATTN_OK) return st;
@@ -258,7 +339,8 @@ int check_attend(const KarpoCacheAttendArgs* a, CacheRef* c, CacheRows* r) {
 //   8 heads of 256: one request, 256 vectors 210, 134; 1,024 vectors 443, 474; 16 requests, 128 vectors 119, 88; 256 143, 149
 //   4 heads of 512: one request, 512 vectors 284, 282; 1,024 vectors 436, 542; 16 requests, 512 vectors 251, 280
 //   one request of 2,000 tokens: 16 heads of 128, 1,024 vectors 62, 52; 8 of 256, 71, 54; 4 of 512, 78, 56
-bool split(const KarpoCacheAttendArgs* a) {
+template <class Args>
+bool split(const Args* a) {
   const int d = a->cache.head_dim;
   const double vectors = (double)a->max_q * (a->heads / a->cache.kv_heads);
   if (vectors <= 64) return true;
@@ -274,15 +356,15 @@ bool split(const KarpoCacheAttendArgs* a) {
   return by_split <= unpacked;
 }
 
-AttendShape shape_of(const KarpoCacheAttendArgs* a, const CacheRef& c, const CacheRows& r) {
+template <class Args>
+AttendShape shape_of(const Args* a, const CacheRef& c, const CacheRows& r) {
   int64_t seen = a->total_keys < r.most ? a->total_keys : r.most;
   if (a->window_left >= 0 && (int64_t)a->max_q + a->window_left < seen) seen = (int64_t)a->max_q + a->window_left;
   return attend_shape(c, a->n_seq, a->heads / a->cache.kv_heads, a->max_q, seen);
 }
 
-}  // namespace
-
-extern "C" int karpo_cache_attend_workspace_bytes(const KarpoCacheAttendArgs* a, size_t* bytes) {
+template <class Args>
+int workspace_bytes(const Args* a, size_t* bytes) {
   CacheRef c;
   CacheRows r;
   const int st = check_attend(a, &c, &r);
@@ -299,7 +381,8 @@ extern "C" int karpo_cache_attend_workspace_bytes(const KarpoCacheAttendArgs* a,
   return KARPO_ATTN_OK;
 }
 
-extern "C" int karpo_cache_attend(const KarpoCacheAttendArgs* a, void* stream) {
+template <class Args>
+int attend(const Args* a, void* stream) {
   ReadParams p;
   memset(&p, 0, sizeof(p));
   int st = check_attend(a, &p.c, &p.r);
@@ -370,3 +453,18 @@ extern "C" int karpo_cache_attend(const KarpoCacheAttendArgs* a, void* stream) {
   u.fwd.workspace_bytes = a->workspace_bytes - (size_t)u.ws_offset;
   return karpo_attn_fwd(&u.fwd, stream);
 }
+
+}  // namespace
+
+extern "C" int karpo_cache_read(const KarpoCacheReadArgs* a, void* stream) { return read_rows(a, stream); }
+extern "C" int karpo_cache4_read(const KarpoCache4ReadArgs* a, void* stream) { return read_rows(a, stream); }
+
+extern "C" int karpo_cache_attend_workspace_bytes(const KarpoCacheAttendArgs* a, size_t* bytes) {
+  return workspace_bytes(a, bytes);
+}
+extern "C" int karpo_cache4_attend_workspace_bytes(const KarpoCache4AttendArgs* a, size_t* bytes) {
+  return workspace_bytes(a, bytes);
+}
+
+extern "C" int karpo_cache_attend(const KarpoCacheAttendArgs* a, void* stream) { return attend(a, stream); }
+extern "C" int karpo_cache4_attend(const KarpoCache4AttendArgs* a, void* stream) { return attend(a, stream); }

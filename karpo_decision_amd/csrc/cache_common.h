@@ -24,6 +24,25 @@ __device__ __forceinline__ u32x4 bf16_of_8(unsigned a, unsigned b, float scale) 
                bf16_pair(b, scale, true)};
 }
 
+// Eight e2m1 codes times `scale`, a power of two, as packed bf16, exactly (the conversion goes by the scale's exponent alone;
+// exponent 255 gives NaN).
+__device__ __forceinline__ u32x4 bf16_of_8_codes4(unsigned w, float scale) {
+  return u32x4{__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0)),
+               __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1)),
+               __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2)),
+               __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3))};
+}
+
+// Four words of four bytes side by side each as four bytes side by side of each of the four words.
+__device__ __forceinline__ void transposed(const unsigned (&r)[4], unsigned (&out)[4]) {
+  const unsigned l01 = __builtin_amdgcn_perm(r[1], r[0], 0x05010400u), h01 = __builtin_amdgcn_perm(r[1], r[0], 0x07030602u);
+  const unsigned l23 = __builtin_amdgcn_perm(r[3], r[2], 0x05010400u), h23 = __builtin_amdgcn_perm(r[3], r[2], 0x07030602u);
+  out[0] = __builtin_amdgcn_perm(l23, l01, 0x05040100u);
+  out[1] = __builtin_amdgcn_perm(l23, l01, 0x07060302u);
+  out[2] = __builtin_amdgcn_perm(h23, h01, 0x05040100u);
+  out[3] = __builtin_amdgcn_perm(h23, h01, 0x07060302u);
+}
+
 constexpr unsigned kNanPair = 0x7fc07fc0u;  // two bf16
 
 // Pairs `x` into `count` rows of `heads` heads from o on, by threads `first`, `first` + `step`, ...

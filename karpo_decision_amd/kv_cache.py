@@ -1,14 +1,17 @@
-"""A block cache on MI355X: keys and values kept between calls in 8 bits, and the packed attention that reads them.
+"""A block cache on MI355X: keys and values kept between calls in 8 or 4 bits, and the packed attention that reads them.
 
 A serving step over requests that hold cached tokens (a prompt that more rounds or branches follow, an answer that grows):
 
     step = reserve(table, lengths, counts, free, free_count, rows, cache.block_size)  # once per step, for all layers
     append(cache, key, value, step.writes)                                            # each layer's own cache
+    # or out of the projections: append(..., k_norm=ops.gemma_norm(attn.k_norm), rope=(cos, sin), positions=step.positions)
     out = attend(query, cache, table, step.q_cu, step.lengths, max_q, scale, total_keys=total)  # total: of step.lengths
 
 ``hip_attention.attend`` reads keys that live for one call; here they live in a pool of blocks of 32, 64 or 128 tokens
 (``Cache``), found through a block table. An element is stored as an e4m3 code times a power of two that its block and
-head share, so a cached element is a bf16 value exactly, and ``read`` and ``attend`` work on the same numbers.
+head share (8 bits), or as an e2m1 code times a power of two of its own for each 32 elements of a token's head (4.25 bits;
+``create(bits=4)``), so a cached element is a bf16 value exactly, and ``read`` and ``attend`` work on the same numbers. All
+calls take either cache.
 Blocks that several requests' tables share are read only: a request appends to blocks of its own.
 
 Lengths, bounds, tables and free lists are read on the device when the kernels run: nothing syncs, calls go on the
@@ -29,7 +32,7 @@ from torch._subclasses import FakeTensor
 from torch.autograd import forward_ad
 
 from . import _lib
-from .ops import _current_stream, _on_device
+from .ops import NORM_NONE, NORM_ONE_PLUS, NORM_WEIGHT, Norm, _bf16_table, _current_stream, _on_device
 
 BLOCK_SIZES = (32, 64, 128)
 HEAD_DIMS = (64, 128, 256, 512)
@@ -37,17 +40,23 @@ _MOST = (1 << 31) - 1
 _MOST_ROWS = _MOST - (1 << 16)
 
 # The argument structures of karpo_cache.h, field by field (_lib has them by name): packing them costs a third of what
-# building them by name does, and a small call's time is its host path.
+# building them by name does, and a small call's time is its host path. Those of karpo_cache4.h have the same layout.
 _CACHE = "PPPqiii4x"
 _RESERVE = struct.Struct("@PqiiPPPPiiqPPPPPqPP")
 _APPEND = struct.Struct("@" + _CACHE + "PPqqqqqPq")
+_APPEND_ROWS = struct.Struct("@" + _CACHE + "PPqqqqqPq" + "ifPifPPPqqi4xP")  # KarpoCacheAppendRopeArgs, KarpoCache4AppendArgs
 _READ = struct.Struct("@" + _CACHE + "PqiiPPPqP")
 _ATTEND = struct.Struct("@" + _CACHE + "PPqqqqPPPqiiiiqqfii4xPN")
 
 
+_FP8, _FP4, _E8M0 = torch.float8_e4m3fn, torch.float4_e2m1fn_x2, torch.float8_e8m0fnu
+
+
 class Cache(NamedTuple):
-    """One layer's keys and values: ``keys`` and ``values`` (blocks, kv heads, block_size * D) float8_e4m3fn, laid out as
-    ``karpo_cache.h`` says, and ``scales`` (blocks, kv heads, 2) fp32, the powers of two of a block's keys and values."""
+    """One layer's keys and values. In 8 bits: ``keys`` and ``values`` (blocks, kv heads, block_size * D) float8_e4m3fn, laid
+    out as ``karpo_cache.h`` says, and ``scales`` (blocks, kv heads, 2) fp32, the powers of two of a block's keys and values. In
+    4 bits: ``keys`` and ``values`` (blocks, kv heads, block_size * D / 2) float4_e2m1fn_x2 and ``scales`` (blocks, kv heads,
+    block_size / 32, 2, D) float8_e8m0fnu, laid out as ``karpo_cache4.h`` says."""
 
     keys: Tensor
     values: Tensor
@@ -64,7 +73,11 @@ class Cache(NamedTuple):
 
     @property
     def head_dim(self) -> int:
-        return self.keys.shape[2] // self.block_size
+        return self.keys.shape[2] * (8 // self.bits) // self.block_size
+
+    @property
+    def bits(self) -> int:
+        return 4 if self.keys.dtype is _FP4 else 8
 
 
 class Step(NamedTuple):
@@ -94,14 +107,22 @@ class Step(NamedTuple):
 
 
 def create(blocks: int, kv_heads: int, head_dim: int, block_size: int = 64,
-           device: torch.device | str = "cuda") -> Cache:
-    """An empty cache of ``blocks`` blocks."""
+           device: torch.device | str = "cuda", bits: int = 8) -> Cache:
+    """An empty cache of ``blocks`` blocks, in 8 or 4 bits (an element is up to 2^-4 of its magnitude off in 8 bits; in 4, up to
+    a quarter, or a 24th of the largest of its 32 elements: 12% of the 2-norm for normally distributed ones)."""
     if block_size not in BLOCK_SIZES:
         raise ValueError(f"block_size must be 32, 64 or 128, not {block_size}")
     if head_dim not in HEAD_DIMS:
         raise ValueError(f"head_dim must be 64, 128, 256 or 512, not {head_dim}")
     if blocks < 1 or kv_heads < 1:
         raise ValueError(f"a cache has at least one block and one head, not {blocks} and {kv_heads}")
+    if bits not in (4, 8):
+        raise ValueError(f"bits must be 8 or 4, not {bits}")
+    if bits == 4:
+        keys, values = (torch.zeros((blocks, kv_heads, block_size * head_dim // 2), dtype=torch.uint8, device=device).view(_FP4)
+                        for _ in range(2))
+        scales = torch.zeros((blocks, kv_heads, block_size // 32, 2, head_dim), dtype=torch.uint8, device=device)
+        return Cache(keys, values, scales.view(_E8M0), block_size)
     keys, values = (torch.zeros((blocks, kv_heads, block_size * head_dim), dtype=torch.uint8, device=device)
                     .view(torch.float8_e4m3fn) for _ in range(2))
     return Cache(keys, values, torch.zeros((blocks, kv_heads, 2), dtype=torch.float32, device=device), block_size)
@@ -110,7 +131,9 @@ def create(blocks: int, kv_heads: int, head_dim: int, block_size: int = 64,
 def _cache_fields(cache: Cache, index: int) -> tuple[int, ...]:
     """The cache's fields of an argument structure; ``index``: the other tensors' device."""
     keys, values, scales, block = cache
-    shape, fp8 = keys.shape, torch.float8_e4m3fn
+    shape, fp8 = keys.shape, _FP8
+    if keys.dtype is _FP4:
+        return _cache4_fields(cache, index)
     if len(shape) == 3 and block in BLOCK_SIZES:  # all is well: one pass
         blocks, heads, size = shape
         head_dim = size // block
@@ -128,6 +151,27 @@ def _cache_fields(cache: Cache, index: int) -> tuple[int, ...]:
     raise ValueError(f"a cache has contiguous keys and values (blocks, kv heads, block_size * head_dim) and scales (blocks, "
                      f"kv heads, 2), block_size 32, 64 or 128 and head_dim 64, 128, 256 or 512, not {tuple(shape)}, "
                      f"{tuple(values.shape)}, {tuple(scales.shape)} and {block}")
+
+
+def _cache4_fields(cache: Cache, index: int) -> tuple[int, ...]:
+    keys, values, scales, block = cache
+    shape = keys.shape
+    if len(shape) == 3 and block in BLOCK_SIZES:
+        blocks, heads, size = shape
+        head_dim = 2 * size // block
+        if (head_dim in HEAD_DIMS and 2 * size == head_dim * block and values.shape == shape and blocks > 0 and heads > 0
+                and scales.shape == (blocks, heads, block // 32, 2, head_dim) and values.dtype is _FP4
+                and scales.dtype is _E8M0 and keys.is_contiguous() and values.is_contiguous() and scales.is_contiguous()
+                and keys.get_device() == values.get_device() == scales.get_device() == index):
+            return keys.data_ptr(), values.data_ptr(), scales.data_ptr(), blocks, heads, head_dim, block
+    if values.dtype != _FP4 or scales.dtype != _E8M0:
+        raise ValueError(f"a cache in 4 bits has float4_e2m1fn_x2 keys and values and float8_e8m0fnu scales, not {keys.dtype}, "
+                         f"{values.dtype} and {scales.dtype}")
+    if not keys.get_device() == values.get_device() == scales.get_device() == index:
+        raise ValueError(f"the cache is on {keys.device}, {values.device} and {scales.device}, the other tensors elsewhere")
+    raise ValueError(f"a cache in 4 bits has contiguous keys and values (blocks, kv heads, block_size * head_dim / 2) and scales "
+                     f"(blocks, kv heads, block_size / 32, 2, head_dim), block_size 32, 64 or 128 and head_dim 64, 128, 256 or "
+                     f"512, not {tuple(shape)}, {tuple(values.shape)}, {tuple(scales.shape)} and {block}")
 
 
 def _check_ints(index: int, **tensors: Tensor) -> None:
@@ -215,11 +259,61 @@ def reserve(table: Tensor, lengths: Tensor, counts: Tensor, free: Tensor, free_c
     return Step(q_cu, new, slots.view(torch.int64), positions, writes.view(jobs, 4), left, status)
 
 
-def append(cache: Cache, key: Tensor, value: Tensor, writes: Tensor) -> None:
+def _norm_fields(name: str, norm: Norm | None, key: Tensor, keep: list) -> tuple[int, float, int]:
+    """(mode, eps, weight's pointer) of one of ``append``'s norms."""
+    if norm is None or norm.mode == NORM_NONE:
+        return 0, 0.0, 0
+    weight = norm.weight if norm.mode in (NORM_WEIGHT, NORM_ONE_PLUS) else None
+    if weight is None:
+        if norm.mode in (NORM_WEIGHT, NORM_ONE_PLUS):
+            raise ValueError(f"{name}: this norm has a weight of shape ({key.shape[2]},), not None")
+        return norm.mode, norm.eps, 0
+    if weight.shape != key.shape[2:]:
+        raise ValueError(f"{name}'s weight must have shape ({key.shape[2]},), not {tuple(weight.shape)}")
+    weight = _bf16_table(weight, key.device)
+    keep.append(weight)
+    return norm.mode, norm.eps, weight.data_ptr()
+
+
+def _rope_fields(rope: tuple[Tensor, Tensor] | None, positions: Tensor | None, key: Tensor, keep: list) -> tuple[int, ...]:
+    """(cos, sin, stride, rows, rotated elements, positions) of ``append``'s rotation."""
+    if rope is None:
+        if positions is not None:
+            raise ValueError("positions are rows of the rope tables: pass rope=(cos, sin) with them")
+        return 0, 0, 0, 0, 0, 0
+    cos, sin = (_bf16_table(t, key.device) for t in rope)
+    rows, index = key.shape[0], key.get_device()
+    if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[0] < 1 or cos.shape[1] % 32 or not 0 < cos.shape[1] <= key.shape[2]:
+        raise ValueError(f"rope tables must be two (positions, rotated) tables of one shape, rotated a multiple of 32 up to "
+                         f"{key.shape[2]}, not {tuple(cos.shape)} and {tuple(sin.shape)}")
+    if cos.stride(0) != sin.stride(0) or cos.stride(0) < cos.shape[1]:
+        cos, sin = cos.contiguous(), sin.contiguous()
+    keep += (cos, sin)
+    at = 0
+    if positions is None:
+        if cos.shape[0] < rows:
+            raise ValueError(f"without positions the rope tables need a row for each of {rows} rows, not {cos.shape[0]}")
+    else:
+        if not _ints(positions, index):
+            _check_ints(index, positions=positions)
+        if positions.shape[0] != rows:
+            raise ValueError(f"positions must hold a number for each of {rows} rows, not {positions.shape[0]}")
+        at = positions.data_ptr()
+    return cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0], cos.shape[1], at
+
+
+def append(cache: Cache, key: Tensor, value: Tensor, writes: Tensor, *, k_norm: Norm | None = None, v_norm: Norm | None = None,
+           rope: tuple[Tensor, Tensor] | None = None, positions: Tensor | None = None) -> None:
     """New keys and values (rows, kv heads, D) bf16 into the blocks that ``writes`` lists (``Step.writes``; no block
-    twice). A block's scale is the least power of two that holds what it got; where new tokens need a larger one, the
-    block's earlier tokens are rounded again to it. What lies past e4m3's range at the largest scale, infinities too, is
-    stored at the range's end, NaN as NaN. Rows and slots that no write names are left as they were."""
+    twice). In 8 bits a block's scale is the least power of two that holds what it got; where new tokens need a larger one, the
+    block's earlier tokens are rounded again to it. In 4 bits each 32 elements have their own, and a NaN among them makes all of
+    them NaN. What lies past the format's range at the largest scale, infinities too, is stored at the range's end, NaN as NaN.
+    Rows and slots that no write names are left as they were.
+
+    ``k_norm`` and ``v_norm`` (``ops.gemma_norm``, ``ops.qwen_norm``) norm the rows on the way, ``rope`` then turns the keys by
+    halves over their first R elements: bf16 tables (cos, sin) of shape (positions, R), of which row i's is row ``positions[i]``
+    (int32, ``Step.positions``), or row i without. All in fp32, rounded once, to the cache's codes (``ops.norm_rope`` before a
+    plain append rounds to bf16 twice more). A key whose position is outside the tables gets NaN for what is turned."""
     _real("append", key)
     _no_grad("append", key, value)
     index, bf16 = key.get_device(), torch.bfloat16
@@ -236,11 +330,23 @@ def append(cache: Cache, key: Tensor, value: Tensor, writes: Tensor) -> None:
     if (writes.dim() != 2 or writes.shape[1] != 4 or writes.dtype is not torch.int32 or writes.get_device() != index
             or not writes.is_contiguous()):
         raise ValueError("writes must be a contiguous (n, 4) int32 tensor on the other tensors' device")
+    call = (*fields, key.data_ptr(), value.data_ptr(), sk[0], sk[1], sv[0], sv[1], shape[0], writes.data_ptr(), writes.shape[0])
+    four = cache.keys.dtype is _FP4
+    if not four and k_norm is None and v_norm is None and rope is None and positions is None:
+        _on_gpu("append", index)
+        with _on_device(index):
+            _lib.check(_lib.load().karpo_cache_append(_APPEND.pack(*call), _current_stream(index)), "append")
+        return
+    extra = [n.weight for n in (k_norm, v_norm) if n is not None and n.weight is not None] + list(rope or ())
+    _no_grad("append", *extra)
+    keep: list[Tensor] = []  # (converted tables go back to the stream-ordered allocator after the launch)
+    args = (*call, *_norm_fields("k_norm", k_norm, key, keep), *_norm_fields("v_norm", v_norm, key, keep),
+            *_rope_fields(rope, positions, key, keep))
     _on_gpu("append", index)
-    args = _APPEND.pack(*fields, key.data_ptr(), value.data_ptr(), sk[0], sk[1], sv[0], sv[1], shape[0],
-                        writes.data_ptr(), writes.shape[0])
+    lib = _lib.load()
     with _on_device(index):
-        _lib.check(_lib.load().karpo_cache_append(args, _current_stream(index)), "append")
+        run = lib.karpo_cache4_append if four else lib.karpo_cache_append_rope
+        _lib.check(run(_APPEND_ROWS.pack(*args), _current_stream(index)), "append")
 
 
 def read(cache: Cache, table: Tensor, lengths: Tensor, rows: int) -> tuple[Tensor, Tensor, Tensor]:
@@ -260,7 +366,9 @@ def read(cache: Cache, table: Tensor, lengths: Tensor, rows: int) -> tuple[Tenso
     k_cu = table.new_empty(rows_fields[3] + 1)
     args = _READ.pack(*fields, *rows_fields, lengths.data_ptr(), key.data_ptr(), value.data_ptr(), rows, k_cu.data_ptr())
     with _on_device(index):
-        _lib.check(_lib.load().karpo_cache_read(args, _current_stream(index)), "read")
+        lib = _lib.load()
+        run = lib.karpo_cache4_read if cache.keys.dtype is _FP4 else lib.karpo_cache_read
+        _lib.check(run(args, _current_stream(index)), "read")
     return key, value, k_cu
 
 
@@ -314,11 +422,13 @@ def attend(query: Tensor, cache: Cache, table: Tensor, q_cu: Tensor, lengths: Te
             lengths.data_ptr(), *rows_fields, shape[1], int(max_q), shape[0], int(total_keys), float(scale),
             int(window), 0 if causal else -1)
     need = ctypes.c_size_t()
-    _lib.check(lib.karpo_cache_attend_workspace_bytes(_ATTEND.pack(*call, 0, 0), need), "attend")
+    size_of, run = ((lib.karpo_cache4_attend_workspace_bytes, lib.karpo_cache4_attend) if cache.keys.dtype is _FP4 else
+                    (lib.karpo_cache_attend_workspace_bytes, lib.karpo_cache_attend))
+    _lib.check(size_of(_ATTEND.pack(*call, 0, 0), need), "attend")
     size, at = need.value, 0
     with _on_device(index):
         if size:  # from the caching allocator (stream-ordered reuse)
             workspace = table.new_empty(size, dtype=torch.uint8)
             at = workspace.data_ptr()
-        _lib.check(lib.karpo_cache_attend(_ATTEND.pack(*call, at, size), _current_stream(index)), "attend")
+        _lib.check(run(_ATTEND.pack(*call, at, size), _current_stream(index)), "attend")
     return out
