@@ -1,4 +1,4 @@
-// The block cache's kernels' arguments (cache.hip, cache_append.hip, cache_attn.hip), shared with the C ABI (cache_capi.cpp).
+// The block cache's kernels' arguments (cache.hip, cache_append.hip, cache_attn.hip, cache4_attn.hip), shared with the C ABI (cache_capi.cpp).
 #pragma once
 #include <hip/hip_runtime_api.h>
 #include <stdint.h>
@@ -70,9 +70,10 @@ struct AppendRowsParams {
   int32_t rope_dim;
   const int32_t* positions;  // each row's row of the tables, or null: its own
   int64_t n_writes;
-  int32_t by_die;  // all workgroups of a write on one die (the launch's)
+  int32_t many;        // the rows are more than the L2 caches hold
+  int32_t heads_each;  // then: heads that a workgroup takes, one after the other (the launch's)
 };
-hipError_t launch_cache_append_rows(AppendRowsParams p, hipStream_t stream);
+hipError_t launch_cache_append_rows(const AppendRowsParams& p, hipStream_t stream);
 
 struct ReadParams {
   CacheRef c;
@@ -112,7 +113,8 @@ struct AttendParams {
   uint32_t sign;       // 0x80008000 where the scale is negative: the queries are
   int32_t parts;       // workgroups for each of the grid's y
   float* partial;      // [y][parts][2] of (O [vectors][D], m [vectors], l [vectors])
-  int32_t* units;      // [n_seq + 1] groups of 32 tokens before each request
+  int32_t* units;      // [n_seq + 1] groups of 32 tokens before each request (in 4 bits [n_seq + 2]: where each begins on the
+                       // line that the workgroups cut, and the pieces)
 };
 
 // The split path's launch for these sizes: `vectors` query vectors (position x head of the group) per workgroup, `tiles`
@@ -125,5 +127,8 @@ struct AttendShape {
 // `seen`: a bound of the tokens that a request's queries see.
 AttendShape attend_shape(const CacheRef& c, int32_t n_seq, int32_t group, int32_t max_q, int64_t seen);
 hipError_t launch_cache_attend(const AttendParams& p, const AttendShape& s, hipStream_t stream);
+// The same for a cache in 4 bits.
+AttendShape attend4_shape(const CacheRef& c, int32_t n_seq, int32_t group, int32_t max_q, int64_t seen);
+hipError_t launch_cache4_attend(const AttendParams& p, const AttendShape& s, hipStream_t stream);
 
 }  // namespace karpo

@@ -44,6 +44,16 @@ __device__ __forceinline__ unsigned max_over(unsigned x) {
   return over_lanes<N>(x, [](unsigned a, unsigned b) { return max(a, b); });
 }
 
+// 1 / sqrt(x), less than a step off: the instruction's estimate and one Newton step. (The instruction takes no subnormal numbers:
+// they are scaled first; 0 gives infinity, infinity 0.)
+__device__ __forceinline__ float reciprocal_root(float x) {
+  const bool small = x < 0x1p-96f;
+  x = small ? x * 0x1p64f : x;
+  const float v = __builtin_amdgcn_rsqf(x), e = __builtin_fmaf(-x * v, v, 1.f);
+  const float r = e == e ? __builtin_fmaf(0.5f * v, e, v) : v;
+  return small ? r * 0x1p32f : r;
+}
+
 // The least e with m <= 448 * 2^e (448 = 1.75 * 2^8), with BITS 4 m <= 6 * 2^e (6 = 1.5 * 2^2), for the fp32 magnitude with
 // these bits.
 template <int BITS>
@@ -75,8 +85,7 @@ __device__ __forceinline__ unsigned codes_again(unsigned w, float old, float sca
 
 // A write: `count` tokens from slot `first` of a block on, out of the rows from `row` on.
 struct Write {
-  int first, row, count;
-  int64_t head;  // block * heads + head
+  int block, first, row, count;
 };
 
 // One write's keys, or values, of one head: WAVES waves, D / 8 lanes a token of 8 elements each (16 bytes a lane and load), the
@@ -87,8 +96,8 @@ struct Write {
 // of values the tokens lie innermost, so their codes go through LDS, a token's side by side, out of which a lane takes 4 tokens x
 // 4 bytes four times: four 16-byte pieces of the cache. Lanes past the write take its last token again and store nothing, so
 // that loads need no branches and all passes' are in flight at once.
-template <int D, int BLOCK, int PASSES, int WAVES, int BITS, bool VALUE, bool TURNED>
-__device__ __forceinline__ void append_rows(const AppendRowsParams& p, const Write& wr, int h, char* s_codes) {
+template <int D, int BLOCK, int PASSES, int WAVES, int BITS, bool MANY, bool VALUE, bool TURNED>
+__device__ __forceinline__ void append_rows(const AppendRowsParams& p, const Write& wr, int h0, int h1, char* s_codes) {
   constexpr int kLanes = D / 8, kRows = 64 / kLanes, kStep = kRows * WAVES;
   constexpr int kBytes = BITS == 8 ? D : D / 2;  // of a token's codes
   constexpr int kPitch = kBytes + 16;
@@ -96,24 +105,9 @@ __device__ __forceinline__ void append_rows(const AppendRowsParams& p, const Wri
   const int first = wr.first, count = wr.count;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int sub = lane / kLanes, l = lane - sub * kLanes, d0 = l * 8;
-  uint8_t* const out = (VALUE ? c.values : c.keys) + wr.head * BLOCK * kBytes;
   const int64_t stride = VALUE ? p.a.sv_t : p.a.sk_t;
-  const uint16_t* const in = (VALUE ? p.a.v + h * p.a.sv_h : p.a.k + h * p.a.sk_h) + wr.row * stride + d0;
-  float* const scale_of = BITS == 8 ? c.scales + 2 * wr.head + (VALUE ? 1 : 0) : nullptr;
-  const unsigned old_bits = BITS == 8 && first > 0 ? __float_as_uint(*scale_of) : 0;
+  const uint16_t* const in = (VALUE ? p.a.v : p.a.k) + wr.row * stride + d0;
   auto token_of = [&](int t) { return t * kStep + wave * kRows + sub; };
-
-  int64_t at[PASSES];  // the tokens' rows of the tables
-  if constexpr (TURNED) {
-#pragma unroll
-    for (int t = 0; t < PASSES; ++t) {
-      at[t] = (int64_t)wr.row + min(token_of(t), count - 1);
-      if (p.positions != nullptr) at[t] = p.positions[at[t]];
-    }
-  }
-  u32x4 x[PASSES];
-#pragma unroll
-  for (int t = 0; t < PASSES; ++t) x[t] = *reinterpret_cast<const u32x4*>(in + min(token_of(t), count - 1) * stride);
 
   // norm: (x * w) * r, w the weight, 1 + weight or 1; rotation of the first rope_dim elements, partner rh away. A product of two
   // bf16 numbers, and of three, is exact in fp32, so a weighted key takes two roundings, (xw * cos - xw' * sin) and the
@@ -125,53 +119,99 @@ __device__ __forceinline__ void append_rows(const AppendRowsParams& p, const Wri
   const int rd = TURNED ? p.rope_dim : 0, rh = rd >> 1;
   const bool inside = d0 < rd;
   const int dp = inside ? (d0 < rh ? d0 + rh : d0 - rh) : d0;
-  const float sign = d0 < rh ? -1.f : 1.f;
+
+  // the tokens' rows of the tables, for all heads; the first head's rows; the norm's weight (a next head's rows are loaded when the
+  // last one's are through)
+  int64_t at[PASSES];
+  if constexpr (TURNED) {
+#pragma unroll
+    for (int t = 0; t < PASSES; ++t) {
+      at[t] = (int64_t)wr.row + min(token_of(t), count - 1);
+      if (p.positions != nullptr) at[t] = p.positions[at[t]];
+    }
+  }
+  u32x4 x[PASSES], cv[PASSES], sv[PASSES];
+  auto load = [&](int h) {  // head h's rows
+#pragma unroll
+    for (int t = 0; t < PASSES; ++t) {
+      const u32x4* const from = reinterpret_cast<const u32x4*>(in + min(token_of(t), count - 1) * stride +
+                                                               h * (VALUE ? p.a.sv_h : p.a.sk_h));
+      if constexpr (MANY) x[t] = __builtin_nontemporal_load(from); else x[t] = *from;
+    }
+  };
+  load(h0);
   u32x4 wv = {0, 0, 0, 0}, wp = {0, 0, 0, 0};
   if (wm != 0.f) {
     wv = *reinterpret_cast<const u32x4*>(norm.weight + d0);
     if constexpr (TURNED) wp = *reinterpret_cast<const u32x4*>(norm.weight + dp);
   }
-  const int partner = (sub * kLanes + (dp >> 3)) * 4;  // its lane's byte address
-  auto row_of = [&](int t, float (&y)[8]) {
-    float r = 1.f;
-    if (normed) {
-      float ss = 0.f;
+  if constexpr (TURNED) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(bf16_at(x[t], e), bf16_at(x[t], e), ss);
-      r = 1.f / __builtin_sqrtf(sum_over<kLanes>(ss) * (1.f / D) + norm.eps);
+    for (int t = 0; t < PASSES; ++t) {
+      const bool known = at[t] >= 0 && at[t] < p.rope_rows;
+      const int64_t from = (known ? at[t] : 0) * p.rope_stride + (inside ? d0 : 0);
+      cv[t] = *reinterpret_cast<const u32x4*>(p.cos + from);
+      sv[t] = *reinterpret_cast<const u32x4*>(p.sin + from);
+      if (!known) cv[t] = u32x4{kNanPair, kNanPair, kNanPair, kNanPair};
     }
-    auto weighted = [&](const u32x4& v, const u32x4& w, int e) { return bf16_at(v, e) * (wm * bf16_at(w, e) + wa); };
+  }
+  float w_mine[8], w_other[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    w_mine[e] = wm * bf16_at(wv, e) + wa;
+    w_other[e] = (wm * bf16_at(wp, e) + wa) * (d0 < rh ? -1.f : 1.f);
+  }
+  const int partner = (sub * kLanes + (dp >> 3)) * 4;  // its lane's byte address
+
+  int h = h0;
+  do {
+    if constexpr (MANY && TURNED) {  // (kept as they are: their 64 elements in fp32 would be registers over all heads)
+#pragma unroll
+      for (int t = 0; t < PASSES; ++t)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) asm volatile("" : "+v"(cv[t][k]), "+v"(sv[t][k]));
+    }
+  const int64_t head = (int64_t)wr.block * c.kv_heads + h;
+  uint8_t* const out = (VALUE ? c.values : c.keys) + head * BLOCK * kBytes;
+  float* const scale_of = BITS == 8 ? c.scales + 2 * head + (VALUE ? 1 : 0) : nullptr;
+  const unsigned old_bits = BITS == 8 && first > 0 ? __float_as_uint(*scale_of) : 0;
+  auto row_of = [&](int t, float (&y)[8]) {
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(bf16_at(x[t], e), bf16_at(x[t], e), ss);
+    const float root = reciprocal_root(sum_over<kLanes>(ss) * (1.f / D) + norm.eps), r = normed ? root : 1.f;
     if constexpr (TURNED) {
       u32x4 px;
 #pragma unroll
       for (int k = 0; k < 4; ++k) px[k] = (unsigned)__builtin_amdgcn_ds_bpermute(partner, (int)x[t][k]);
-      const bool known = at[t] >= 0 && at[t] < p.rope_rows;
-      const int64_t from = (known ? at[t] : 0) * p.rope_stride + (inside ? d0 : 0);
-      u32x4 cv = *reinterpret_cast<const u32x4*>(p.cos + from), sv = *reinterpret_cast<const u32x4*>(p.sin + from);
-      if (!known) cv = u32x4{kNanPair, kNanPair, kNanPair, kNanPair};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float n = weighted(x[t], wv, e);
-        const float turn = __builtin_fmaf(n, bf16_at(cv, e), sign * weighted(px, wp, e) * bf16_at(sv, e));
+        const float n = bf16_at(x[t], e) * w_mine[e];
+        const float turn = __builtin_fmaf(n, bf16_at(cv[t], e), bf16_at(px, e) * w_other[e] * bf16_at(sv[t], e));
         y[e] = (inside ? turn : n) * r;
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = weighted(x[t], wv, e) * r;
+      for (int e = 0; e < 8; ++e) y[e] = bf16_at(x[t], e) * w_mine[e] * r;
     }
+  };
+  // the largest magnitude of y and `best`, NaN as nothing
+  auto larger = [&](const float (&y)[8], float best) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) best = __builtin_fmaxf(__builtin_fmaxf(best, __builtin_fabsf(y[e])), __builtin_fabsf(y[e + 1]));
+    return best;
   };
 
   bool grown = false;
   float scale = 1.f, old_scale = 1.f;
   if constexpr (BITS == 8) {
-    float y[PASSES][8];
-    unsigned best = 0;
+    float y[PASSES][8], most_of = 0.f;
 #pragma unroll
     for (int t = 0; t < PASSES; ++t) {
       row_of(t, y[t]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) best = max(best, __float_as_uint(y[t][e]) & 0x7fffffffu);
+      most_of = larger(y[t], most_of);
     }
+    if (MANY && h + 1 < h1) load(h + 1);
     auto joined = [&](unsigned mine) {  // over the workgroup
       mine = max_over<64>(mine);
       if constexpr (WAVES > 1) {
@@ -181,12 +221,12 @@ __device__ __forceinline__ void append_rows(const AppendRowsParams& p, const Wri
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) mine = max(mine, s_best[w]);
-        __syncthreads();  // (the codes take the array)
+        __syncthreads();  // (the codes, or the next head's maxima, take the array)
       }
       return mine;
     };
-    best = joined(best);
-    const bool odd = best >= 0x7f800000u;  // infinities or NaN: the largest of the others
+    unsigned best = joined(__float_as_uint(most_of));
+    const bool odd = best >= 0x7f800000u;  // infinities: the largest of the others
     if (__builtin_expect(odd, 0)) {
       best = 0;
 #pragma unroll
@@ -237,21 +277,27 @@ __device__ __forceinline__ void append_rows(const AppendRowsParams& p, const Wri
       }
     }
   } else {
-    uint8_t* const scales = c.scales4 + wr.head * (BLOCK / 32) * 2 * D + (VALUE ? D : 0);
+    uint8_t* const scales = c.scales4 + head * (BLOCK / 32) * 2 * D + (VALUE ? D : 0);
 #pragma unroll
     for (int t = 0; t < PASSES; ++t) {
       const int slot = first + token_of(t);
       float y[8];
       row_of(t, y);
-      unsigned best = 0, all = 0;
+      // (a sum is NaN where an element is, or where infinities of both signs are)
+      unsigned best = max_over<4>(__float_as_uint(larger(y, 0.f)));
+      const float sum = ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+      bool nan = false;
+      if (__any(!(__builtin_fabsf(sum) < INFINITY) || best >= 0x7f800000u)) {  // seldom: the largest of the others, and is one NaN
+        unsigned fine = 0, all = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const unsigned m = __float_as_uint(y[e]) & 0x7fffffffu;
-        best = max(best, m < 0x7f800000u ? m : 0u);
-        all = max(all, m);
+        for (int e = 0; e < 8; ++e) {
+          const unsigned m = __float_as_uint(y[e]) & 0x7fffffffu;
+          fine = max(fine, m < 0x7f800000u ? m : 0u);
+          all = max(all, m);
+        }
+        best = max_over<4>(fine);
+        nan = max_over<4>(all) > 0x7f800000u;
       }
-      best = max_over<4>(best);
-      all = max_over<4>(all);
       const int e = exponent_of<4>(best);
       const unsigned w = codes4(y, power_of_two(e));
       if (token_of(t) < count) {
@@ -265,17 +311,18 @@ __device__ __forceinline__ void append_rows(const AppendRowsParams& p, const Wri
           const int byte = VALUE     ? group * 32 + (t16 >> 2) * 8 + t2 * 4 + (t16 & 3)
                            : D == 64 ? (t2 * 2 + group) * 16 + t16
                                      : ((group & 3) * 16 + t16) * (D / 64) + (group >> 2) * 2 + t2;
-          scales[(slot >> 5) * 2 * D + byte] = all > 0x7f800000u ? 255 : (uint8_t)(e + 127);
+          scales[(slot >> 5) * 2 * D + byte] = nan ? 255 : (uint8_t)(e + 127);
         }
       }
     }
+    if (MANY && h + 1 < h1) load(h + 1);
   }
   if constexpr (VALUE) {
     __syncthreads();
-    const int h0 = grown ? 0 : first >> 5, h1 = (first + count - 1) >> 5;
+    const int half0 = grown ? 0 : first >> 5, half1 = (first + count - 1) >> 5;
     constexpr int kTiles = kBytes / 32;  // KiB of codes of 32 tokens
-    for (int u = tid; u < (h1 - h0 + 1) * kTiles * 16; u += 64 * WAVES) {
-      const int j = u & 3, q = (u >> 2) & 3, tile = (u >> 4) % kTiles, half = h0 + (u >> 4) / kTiles;
+    for (int u = tid; u < (half1 - half0 + 1) * kTiles * 16; u += 64 * WAVES) {
+      const int j = u & 3, q = (u >> 2) & 3, tile = (u >> 4) % kTiles, half = half0 + (u >> 4) / kTiles;
       // bytes of the tokens 16 t + 4 q + 0 .. 3 that are new, and that are rounded again
       unsigned is_new[2] = {0, 0}, is_old[2] = {0, 0};
 #pragma unroll
@@ -319,50 +366,55 @@ __device__ __forceinline__ void append_rows(const AppendRowsParams& p, const Wri
         *dst = w[k];
       }
     }
+    if (MANY && h + 1 < h1) __syncthreads();  // (the next head's codes take the array)
   }
+  } while (MANY && ++h < h1);
 }
 
-template <int D, int BLOCK, int PASSES, int WAVES, int BITS>
+template <int D, int BLOCK, int PASSES, int WAVES, int BITS, bool MANY>
 __global__ __launch_bounds__(64 * WAVES) void append_rows_kernel(const AppendRowsParams p) {
   constexpr int kStep = 512 / D * WAVES;  // tokens of a pass
   __shared__ __align__(16) char s_codes[BLOCK * ((BITS == 8 ? D : D / 2) + 16)];
-  const int heads = p.a.c.kv_heads;
-  int64_t unit;
-  int which;
-  if (p.by_die) {  // workgroups go round the eight dies: write 8 k + i on die i
-    const int64_t turn = blockIdx.x >> 3, k = turn / (2 * heads);
-    which = (int)(turn - k * 2 * heads);
-    unit = 8 * k + (blockIdx.x & 7);
-    if (unit >= p.n_writes) return;
-  } else {
-    unit = blockIdx.x / (2 * heads);
-    which = (int)(blockIdx.x - unit * 2 * heads);
-  }
+  const int heads = p.a.c.kv_heads, groups = (heads + p.heads_each - 1) / p.heads_each;  // (of heads)
+  const int64_t unit = blockIdx.x / (2 * groups);
+  const int which = (int)(blockIdx.x - unit * 2 * groups), h0 = (which >> 1) * p.heads_each, h1 = min(h0 + p.heads_each, heads);
   const int4 w = *reinterpret_cast<const int4*>(p.a.writes + 4 * unit);
-  const int id = w.x, first = w.y, row = w.z, count = w.w, h = which >> 1;
-  if (count < 1 || id < 0 || id >= p.a.c.blocks || first < 0 || count > BLOCK - first || row < 0 || row > p.a.rows - count)
+  const Write wr = {w.x, w.y, w.z, w.w};
+  if (wr.count < 1 || wr.block < 0 || wr.block >= p.a.c.blocks || wr.first < 0 || wr.count > BLOCK - wr.first || wr.row < 0 ||
+      wr.row > p.a.rows - wr.count)
     return;
-  const Write wr = {first, row, count, (int64_t)id * heads + h};
   auto run = [&](auto passes) {
     constexpr int N = decltype(passes)::value;
     if (which & 1)
-      append_rows<D, BLOCK, N, WAVES, BITS, true, false>(p, wr, h, s_codes);
+      append_rows<D, BLOCK, N, WAVES, BITS, MANY, true, false>(p, wr, h0, h1, s_codes);
     else if (p.cos != nullptr)
-      append_rows<D, BLOCK, N, WAVES, BITS, false, true>(p, wr, h, s_codes);
+      append_rows<D, BLOCK, N, WAVES, BITS, MANY, false, true>(p, wr, h0, h1, s_codes);
     else
-      append_rows<D, BLOCK, N, WAVES, BITS, false, false>(p, wr, h, s_codes);
+      append_rows<D, BLOCK, N, WAVES, BITS, MANY, false, false>(p, wr, h0, h1, s_codes);
   };
-  if (count <= kStep) run(std::integral_constant<int, 1>()); else run(std::integral_constant<int, PASSES>());
+  if (wr.count <= kStep) run(std::integral_constant<int, 1>()); else run(std::integral_constant<int, PASSES>());
 }
+
+constexpr int kMostPasses = 4;
 
 template <int D, int BITS>
 hipError_t launch(const AppendRowsParams& p, hipStream_t stream) {
-  const int64_t units = p.by_die ? (p.n_writes + 7) / 8 * 8 : p.n_writes;
-  const dim3 grid((unsigned)(units * 2 * p.a.c.kv_heads));
   auto run = [&](auto blocks) {
-    constexpr int kPieces = D * decltype(blocks)::value / 512;  // of 64 lanes x 8 elements
-    constexpr int kWaves = kPieces <= 8 ? 1 : kPieces <= 64 ? kPieces / 8 : 8, kPasses = kPieces / kWaves;
-    append_rows_kernel<D, decltype(blocks)::value, kPasses, kWaves, BITS><<<grid, dim3(64 * kWaves), 0, stream>>>(p);
+    constexpr int kBlock = decltype(blocks)::value, kPieces = D * kBlock / 512;  // of 64 lanes x 8 elements
+    constexpr int kWaves = kPieces <= 16 * kMostPasses ? kPieces / kMostPasses : 16, kPasses = kPieces / kWaves;
+    // many rows: up to eight heads a workgroup while there are four workgroups a CU (blocks of 64 Ki elements would spill)
+    AppendRowsParams q = p;
+    q.heads_each = 1;
+    const bool many = p.many && kPasses <= kMostPasses;
+    while (many && q.heads_each < 8 && p.n_writes * p.a.c.kv_heads >= 1024 * q.heads_each) q.heads_each *= 2;
+    const dim3 grid((unsigned)(p.n_writes * 2 * ((p.a.c.kv_heads + q.heads_each - 1) / q.heads_each)));
+    if constexpr (kPasses <= kMostPasses) {
+      if (many) {
+        append_rows_kernel<D, kBlock, kPasses, kWaves, BITS, true><<<grid, dim3(64 * kWaves), 0, stream>>>(q);
+        return;
+      }
+    }
+    append_rows_kernel<D, kBlock, kPasses, kWaves, BITS, false><<<grid, dim3(64 * kWaves), 0, stream>>>(q);
   };
   switch (p.a.c.block_log2) {
     case 5: run(std::integral_constant<int, 32>()); break;
@@ -375,8 +427,7 @@ hipError_t launch(const AppendRowsParams& p, hipStream_t stream) {
 
 }  // namespace
 
-hipError_t launch_cache_append_rows(AppendRowsParams p, hipStream_t stream) {
-  p.by_die = p.n_writes >= 8;  // (the rotary tables' rows are read by each head: out of one die's L2)
+hipError_t launch_cache_append_rows(const AppendRowsParams& p, hipStream_t stream) {
   const bool four = p.a.c.scales4 != nullptr;
   switch (p.a.c.head_dim) {
     case 64: return four ? launch<64, 4>(p, stream) : launch<64, 8>(p, stream);

@@ -3,33 +3,19 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-#include <type_traits>
-
 #include "cache.h"
-#include "cache_common.h"
+#include "cache_attn_common.h"
 
 namespace karpo {
 
 namespace {
 
-constexpr int kAttendWaves = 4;
-constexpr int kAttendThreads = 64 * kAttendWaves;
 // Waves per SIMD (and workgroups per CU).
 __host__ __device__ constexpr int attend_waves(int d, int nt) {
   return nt == 1 && d <= 128 ? 4 : d == 64 && nt == 2 ? 3 : d <= 128 || (d == 256 && nt == 1) ? 2 : 1;
 }
-// Tokens that a wave takes at once: as many bytes of either format, but no more than 32 where a workgroup has several tiles of
-// query vectors (the scores of 64 do not fit the registers then).
-__host__ __device__ constexpr int group_of(int bits, int nt) { return bits == 4 && nt == 1 ? 64 : kCacheGroup; }
-// Bytes of LDS for the waves' copies of a group's keys (as many for the values), and of their scales in 4 bits.
-__host__ __device__ constexpr int ring_bytes(int d, int nt, int bits) {
-  return kAttendWaves * group_of(bits, nt) * d * bits / 8;
-}
-__host__ __device__ constexpr int scale_bytes(int d, int nt) { return kAttendWaves * group_of(4, nt) * d / 32; }
-// Elements of the output that the waves join at once, and their sums' bytes (in the keys' array, when the groups are done).
-constexpr int slab_of(int d, int nt) { return nt == 1 && d > 64 ? d / 2 : d / 4 > 32 ? d / 4 : 32; }
-constexpr int sums_bytes(int d, int nt) { return kAttendWaves * 16 * nt * (slab_of(d, nt) + 4) * 4; }
-
+// Bytes of LDS for the waves' copies of a group's keys (as many for the values).
+constexpr int ring_bytes(int d) { return kAttendWaves * kCacheGroup * d; }
 // Requests of which at most this many tokens are seen are not split (a quarter of it at head size 512): one workgroup walks
 // their groups, five a wave, and there is nothing to join. Split against whole, 8 requests: head size 64, 512 tokens 16.9,
 // 12.8 us, 2,048 tokens 16.7, 21.6; 128, 768 tokens 16.7, 13.9, 1,024 tokens 16.6, 16.7; 256, 512 tokens 16.7, 14.5, 768
@@ -37,39 +23,6 @@ constexpr int sums_bytes(int d, int nt) { return kAttendWaves * 16 * nt * (slab_
 // 44.0; at 512 61.4, 60.7.
 constexpr int64_t kWholeTokens = 640;
 constexpr int kLeastUnits = kAttendWaves;  // groups of 32 tokens that a workgroup takes at least
-
-struct Seen {
-  int tokens, row, queries;  // cached tokens; first query row; query rows
-  int first, groups;         // first group of tokens that a query sees, and how many up to the last token
-  int units;                 // groups, or 1 where there are queries and no tokens (their rows are zeros)
-};
-
-template <int GROUP>
-__device__ __forceinline__ Seen seen_of(const AttendParams& p, int i) {
-  Seen s;
-  s.tokens = min(max(p.r.lengths[i], 0), p.r.most);
-  const int a = p.q_cu[i], b = p.q_cu[i + 1];
-  s.row = a;
-  s.queries = a >= 0 && b > a && b <= p.total_q ? b - a : 0;
-  const int64_t before = (int64_t)s.tokens - s.queries - p.left;
-  s.first = p.left >= 0 && before > 0 ? (int)(before < s.tokens ? before : s.tokens) / GROUP : 0;
-  s.groups = (s.tokens + GROUP - 1) / GROUP - s.first;
-  s.units = s.queries > 0 ? max(s.groups, 1) : 0;
-  return s;
-}
-
-// NaN into a request's rows past max_q, which nothing computes, of the key/value head's query heads (by the workgroups of its
-// first vectors; here, at the attention kernel's end or in the join, it costs that kernel's loop no registers).
-template <int D>
-__device__ __forceinline__ void fill_past(const AttendParams& p, const Seen& s, int y, int first, int step) {
-  if (s.queries > p.max_q && y < p.c.kv_heads)
-    fill_rows<D>(kNanPair, p.o + (s.row + (int64_t)p.max_q) * p.so_t + (int64_t)y * p.group * p.so_h, p.so_t,
-                 p.so_h, s.queries - p.max_q, p.group, first, step);
-}
-
-// A vector's position among its request's queries: vec / group, exactly (vec + 1/2 is no multiple of the group, and below
-// 2^16 further from one than the product's rounding).
-__device__ __forceinline__ int position_of(int vec, const AttendParams& p) { return (int)((vec + 0.5f) * p.per_group); }
 
 // What a request takes of the sums: a workgroup that goes on to a next request spends about as long on the change (joining its
 // waves, the new queries and tables, the first copies) as on kStart groups. Shares by groups alone left the last workgroups of
@@ -93,88 +46,12 @@ struct Shares {
   }
 };
 
-// x's maximum / sum over the four lanes of a column (16 apart).
-__device__ __forceinline__ float column_max(float x) {
-  x = half_swap_max(x);
-  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __builtin_elementwise_maximum(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float column_sum(float x) {
-  x = half_swap_sum(x);
-  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
 __device__ __forceinline__ bf16x8 operand(unsigned a, unsigned b, float scale) {
   return __builtin_bit_cast(bf16x8, bf16_of_8(a, b, scale));
 }
 
-// Two fp32 as packed bf16, in one instruction.
-__device__ __forceinline__ unsigned pair_of(float a, float b) {
-  return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{a, b}), bf16x2));
-}
-
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
-}
-
-// A barrier for what goes through LDS: copies and stores stay in flight.
-__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-
-// Two e2m1 codes, byte BYTE of `w`, under the scale with these exponent bits, as packed bf16.
-template <int BYTE>
-__device__ __forceinline__ unsigned pair_at(unsigned w, unsigned scale) {
-  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, __uint_as_float(scale), BYTE));
-}
-
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-
-// Which of a word's four e4m3 codes are NaN, as 0x80 in their bytes.
+// Which of a word's four codes are NaN, as 0x80 in their bytes.
 __device__ __forceinline__ unsigned nan_codes(unsigned w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
-
-// The waits that count a group's copies: CODES of 16 bytes a lane and, in 4 bits, one for each 32 tokens' scales.
-template <int D, int NT, int BITS>
-constexpr int copies_of() {
-  return group_of(BITS, NT) * D * BITS / 8 / 1024 + (BITS == 4 ? group_of(BITS, NT) / 32 : 0);
-}
-
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-
-// acc + (16 keys x 128 elements of e2m1 codes, with byte KB of the lane's word of scales) x (e4m3 terms of 16 query vectors,
-// with byte QB of theirs).
-template <int KB, int QB>
-__device__ __forceinline__ f32x4 mfma_codes4(const u32x4& k, unsigned k_scale, const u32x4& q0, const u32x4& q1, unsigned q_scale,
-                                             f32x4 acc) {
-  const i32x8 a = {(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
-  const i32x8 b = {(int)q0[0], (int)q0[1], (int)q0[2], (int)q0[3], (int)q1[0], (int)q1[1], (int)q1[2], (int)q1[3]};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 0, KB, (int)k_scale, QB, (int)q_scale);
-}
-
-typedef short s16x2 __attribute__((ext_vector_type(2)));
-
-// 16 bf16 over 2^e as 16 e4m3 codes, and what they leave over (exact in fp32) over 2^(e - 4).
-__device__ __forceinline__ void two_terms(const u32x4 (&x)[2], int e, u32x4* high, u32x4* low) {
-  const float scale = power_of_two(e), fine = power_of_two(e - 4);
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    float v[4], h[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = bf16_at(x[w >> 1], (w & 1) * 4 + k);
-    s16x2 c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(s16x2{0, 0}, v[0], v[1], scale, false);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, v[2], v[3], scale, true);
-    (*high)[w] = __builtin_bit_cast(unsigned, c);
-#pragma unroll
-    for (int k = 0; k < 4; k += 2) {
-      const unsigned back = bf16_pair((*high)[w], scale, k != 0);
-      h[k] = __uint_as_float(back << 16);
-      h[k + 1] = __uint_as_float(back & 0xffff0000u);
-    }
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(s16x2{0, 0}, v[0] - h[0], v[1] - h[1], fine, false);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, v[2] - h[2], v[3] - h[3], fine, true);
-    (*low)[w] = __builtin_bit_cast(unsigned, c);
-  }
-}
 
 // One lane's view of a group of 32 tokens with 16x16x32 matrix instructions: S^T = K Q^T has the keys as rows (two tiles),
 // the query vectors as columns: column lane % 16, keys 16 t + 4 (lane / 16) + i. Those are this lane's eight weights, and as
@@ -199,20 +76,10 @@ __device__ __forceinline__ void two_terms(const u32x4 (&x)[2], int e, u32x4* hig
 // tokens, 80 -> 88). The rule goes by one request's query vectors alone: it does not see that requests whose tables share
 // blocks read the same codes (one token each of 16 branches over a prompt of 8,192 tokens, 16 heads of 128, takes 59 us, of 16
 // requests with blocks of their own 90; without the streaming not measured).
-//
-// In 4 bits the keys' codes are the first operand of S^T = K Q^T as they come out of the cache (16x16x128 scaled matrix
-// instructions: 16 tokens x 128 elements, a lane's 32 elements under their own scale), the queries the second, as two e4m3 terms
-// (8 significant bits, a bf16's, for elements within 2^-14 of the largest of their 32; 2^-22 of that largest otherwise). A
-// value's scale is its token's, and tokens are what the second product sums over, so values become bf16 in registers: two
-// elements of a token a conversion, two tokens' of an element a permutation. Of head size 64 a lane's operand holds two tiles of
-// 16 tokens, and the queries fill its one half or the other.
-template <int D, int NT, bool ONCE, int BITS>
+template <int D, int NT, bool ONCE>
 __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_kernel(
     const AttendParams p) {
-  constexpr int kGroup = group_of(BITS, NT), kHalves = kGroup / 32, kScores = kGroup / 4;  // kScores: a lane's, of a vector
-  constexpr int kHalfBytes = 32 * D * BITS / 8;    // of 32 tokens' keys
-  constexpr int kLoads = kHalfBytes / 1024;        // KiB of keys, and of values, in 32 tokens
-  constexpr int kCopies = copies_of<D, NT, BITS>();  // a group's copies of keys, and of values
+  constexpr int kLoads = D / 32;       // KiB of keys, and of values, in a group
   constexpr int kChunks = D / 64;      // 64-element chunks of a key tile
   constexpr int kSlab = slab_of(D, NT);
   constexpr int kVectors = 16 * NT;
@@ -221,21 +88,14 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
   __shared__ int s_at[2];
   __shared__ float s_m[kAttendWaves][kVectors], s_l[kAttendWaves][kVectors];
   // (arrays of their own: a read then waits for the copies into its own array and no others)
-  constexpr int kRing = ring_bytes(D, NT, BITS);
-  __shared__ __align__(16) char s_keys[kRing > sums_bytes(D, NT) ? kRing : sums_bytes(D, NT)];
-  __shared__ __align__(16) char s_values[kRing];
+  __shared__ __align__(16) char s_keys[ring_bytes(D) > sums_bytes(D, NT) ? ring_bytes(D) : sums_bytes(D, NT)];
+  __shared__ __align__(16) char s_values[ring_bytes(D)];
   __shared__ u32x4 s_q[kVectors * D / 8];
-  constexpr int kSpans = D < 128 ? 1 : D / 128;  // of 128 elements
-  __shared__ __align__(16) char s_key_scales[BITS == 4 ? scale_bytes(D, NT) : 16];
-  __shared__ __align__(16) char s_value_scales[BITS == 4 ? scale_bytes(D, NT) : 16];
-  __shared__ unsigned s_q_scales[BITS == 4 ? kSpans * NT * 64 : 1];
   float(*const s_o)[kVectors][kSlab + 4] = reinterpret_cast<float(*)[kVectors][kSlab + 4]>(s_keys);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
-  KA_LDS char* const key_ring = (KA_LDS char*)s_keys + wave * (kRing / kAttendWaves);
-  KA_LDS char* const value_ring = (KA_LDS char*)s_values + wave * (kRing / kAttendWaves);
-  KA_LDS char* const key_scales = (KA_LDS char*)s_key_scales + wave * (BITS == 4 ? kHalves * D : 0);
-  KA_LDS char* const value_scales = (KA_LDS char*)s_value_scales + wave * (BITS == 4 ? kHalves * D : 0);
+  KA_LDS char* const key_ring = (KA_LDS char*)s_keys + wave * (kCacheGroup * D);
+  KA_LDS char* const value_ring = (KA_LDS char*)s_values + wave * (kCacheGroup * D);
   const int heads = p.c.kv_heads, b = p.c.block_log2;
   const int h = blockIdx.y % heads, vector0 = (blockIdx.y / heads) * kVectors;
 
@@ -244,7 +104,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
   int v[1], all[1];
   auto scan = [&](int c0) {
     own = Seen{0, 0, 0, 0, 0, 0};
-    if (c0 + tid < p.r.n_seq) own = seen_of<kGroup>(p, c0 + tid);
+    if (c0 + tid < p.r.n_seq) own = seen_of(p, c0 + tid);
     v[0] = weight_of(own.units);
     block_scan<kAttendThreads, 1>(v, all, s_part);
   };
@@ -252,7 +112,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
   if (p.whole) {  // workgroup i takes request i
     c0 = blockIdx.x;
     c_end = c0 + 1;
-    own = seen_of<kGroup>(p, c0);
+    own = seen_of(p, c0);
     all[0] = total = own.units;
     v[0] = 0;
     if (tid != 0) own.units = 0;  // (thread 0's)
@@ -309,9 +169,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
       // the query vectors' operands (entry (2 c + k) * NT + n, one lane's 16 bytes after the other), and the keys that each
       // vector sees: lo .. hi
       constexpr int kMine = (2 * kChunks + kAttendWaves - 1) / kAttendWaves;  // of the entries of a tile, this wave's
-      // (in 4 bits: of the spans of 128 elements of all tiles, a lane's elements 16 quad .. + 16 and 64 further on)
-      constexpr int kParts = D < 128 ? 1 : 2, kSpansMine = (kSpans * NT + kAttendWaves - 1) / kAttendWaves;
-      u32x4 q_mine[NT][kMine], q_span[kSpansMine][2 * kParts];
+      u32x4 q_mine[NT][kMine];
       int lo[NT], hi[NT];
       const int shift = s.tokens - s.queries;
 #pragma unroll
@@ -321,23 +179,11 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
         const int pos = valid ? position_of(vec, p) : 0;
         const uint16_t* const src =
             p.q + (s.row + (int64_t)pos) * p.sq_t + (int64_t)(h * p.group + (valid ? vec - pos * p.group : 0)) * p.sq_h;
-        if constexpr (BITS == 8) {
 #pragma unroll
-          for (int c = 0; c < kMine; ++c) {
-            const int e = wave + c * kAttendWaves;
-            if (2 * kChunks >= kAttendWaves || e < 2 * kChunks)
-              q_mine[n][c] = *reinterpret_cast<const u32x4*>(src + (e >> 1) * 64 + quad * 16 + (e & 1) * 8);
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < kSpansMine; ++c) {
-            const int e = wave + c * kAttendWaves;  // span e / NT of tile e % NT
-            if (e < kSpans * NT && e % NT == n) {
-#pragma unroll
-              for (int k = 0; k < 2 * kParts; ++k)
-                q_span[c][k] = *reinterpret_cast<const u32x4*>(src + (e / NT) * 128 + (k >> 1) * 64 + quad * 16 + (k & 1) * 8);
-            }
-          }
+        for (int c = 0; c < kMine; ++c) {
+          const int e = wave + c * kAttendWaves;
+          if (2 * kChunks >= kAttendWaves || e < 2 * kChunks)
+            q_mine[n][c] = *reinterpret_cast<const u32x4*>(src + (e >> 1) * 64 + quad * 16 + (e & 1) * 8);
         }
         lo[n] = p.left < 0 ? 0 : pos + shift - p.left;
         hi[n] = p.right < 0 ? s.tokens - 1 : (int)min<int64_t>((int64_t)pos + shift + p.right, s.tokens - 1);
@@ -359,21 +205,12 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
       }
 
       const int32_t* const table = p.r.table + (int64_t)i * p.r.table_stride;
-      const int lane_offset = BITS == 8 ? col * 64 + quad * 16 : lane * 16;
-      int ids = 0, next_ids = 0;  // (next_ids: of a group's second 32 tokens)
+      const int lane_offset = col * 64 + quad * 16;
+      int ids = 0;
       float k_scales = 1.f, v_scales = 1.f;
       // lane k looks up the wave's groups g + 4 k
       auto look_up = [&](int g) {
         const int mine = min(g + lane * kAttendWaves, g1 - 1);
-        if constexpr (BITS == 4) {
-          auto of = [&](int half) {
-            const int id = table[min(half, (s.tokens - 1) >> 5) >> (b - 5)];
-            return id < 0 || id >= p.c.blocks ? -1 : id;
-          };
-          ids = of(mine * kHalves);
-          if constexpr (kHalves == 2) next_ids = of(mine * kHalves + 1);
-          return;
-        }
         ids = table[mine >> (b - 5)];
         if (ids < 0 || ids >= p.c.blocks) ids = -1;
         const float2 sc = *reinterpret_cast<const float2*>(p.c.scales + 2 * ((int64_t)max(ids, 0) * heads + h));
@@ -382,31 +219,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
       };
       // One group's codes into the wave's ring, 16 bytes a lane and KiB; zeros for a block that is not of the pool, and where
       // there is no group (so that every turn of the loop issues the same copies, and a wait can count them).
-      auto copy4 = [&](bool value, KA_LDS char* to, KA_LDS char* scales_to, int g, int k, bool any) {
-#pragma unroll
-        for (int e = 0; e < kHalves; ++e) {
-          const int half = g * kHalves + e, id = __builtin_amdgcn_readlane(e == 0 ? ids : next_ids, k & 63);
-          const bool some = any && id >= 0 && half * 32 < s.tokens;
-          const int64_t head = (int64_t)max(id, 0) * heads + h;
-          const int64_t token = (head << b) + (half & ((1 << (b - 5)) - 1)) * 32;
-          const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-              (void*)((value ? p.c.values : p.c.keys) + token * (D / 2)), (short)0, some ? kHalfBytes : 0, kBufferFlags);
-#pragma unroll
-          for (int t = 0; t < kLoads; ++t)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (KA_LDS void*)(to + e * kHalfBytes + t * 1024), 16, lane_offset, t * 1024,
-                                                     0, ONCE ? kCopyStream : 0);
-          const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-              (void*)(p.c.scales4 + token * (D / 16) + (value ? D : 0)), (short)0, some ? D : 0, kBufferFlags);
-          if (lane < D / 16)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (KA_LDS void*)(scales_to + e * D), 16, lane * 16, 0, 0, 0);
-        }
-      };
       auto copy = [&](const uint8_t* from, KA_LDS char* to, int g, int k, bool any) {
-        if constexpr (BITS == 4) {
-          const bool value = from == p.c.values;
-          copy4(value, to, value ? value_scales : key_scales, g, k, any);
-          return;
-        }
         const int id = __builtin_amdgcn_readlane(ids, k & 63);
         const int64_t head = (int64_t)max(id, 0) * heads + h;
         const uint8_t* const src = from + ((head << b) + (int64_t)(g & ((1 << (b - 5)) - 1)) * kCacheGroup) * D;
@@ -422,7 +235,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
       };
       // all but the last issued group's keys, or values, have arrived / the reads of the ring are done
       auto arrived = [&]() {
-        wait_vmcnt<kCopies>();
+        wait_vmcnt<kLoads>();
         asm volatile("" ::: "memory");
       };
       auto read_out = [&]() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
@@ -430,48 +243,13 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
       int k = 0;
       const bool some = g0 + wave < g1;
       if (some) look_up(g0 + wave);
-      if constexpr (BITS == 8) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int c = 0; c < kMine; ++c) {
-            const int e = wave + c * kAttendWaves;
-            if (2 * kChunks >= kAttendWaves || e < 2 * kChunks) s_q[(e * NT + n) * 64 + lane] = q_mine[n][c] ^ p.sign;
-          }
-      } else {
-#pragma unroll
-        for (int c = 0; c < kSpansMine; ++c) {
+        for (int c = 0; c < kMine; ++c) {
           const int e = wave + c * kAttendWaves;
-          if (e < kSpans * NT) {
-            // the largest of each 32 elements: of a lane's 16 and those of the lane 16 away; 448 * 2^e holds it
-            int part_e[2] = {0, 0};
-#pragma unroll
-            for (int k = 0; k < kParts; ++k) {
-              unsigned m = 0;
-#pragma unroll
-              for (int w = 0; w < 8; ++w) {
-                const unsigned x = q_span[c][2 * k + (w >> 2)][w & 3];
-                m = max(m, max(x & 0x7fff, x >> 16 & 0x7fff));
-              }
-              m = max(m, (unsigned)__shfl_xor((int)m, 16));
-              part_e[k] = min(max((int)(m >> 7) - 127 - 8 + ((m & 0x7f) > 0x60 ? 1 : 0), -100), 120);
-            }
-            // the scales go by 32 elements in order, which these lanes have
-            const int from = col + 16 * ((2 * quad) & 3);
-            const int first = __shfl(part_e[0], from), second = kParts == 2 ? __shfl(part_e[1], from) : first;
-            const int mine_e = kParts == 1 || quad < 2 ? first : second;
-            s_q_scales[e * 64 + lane] = (unsigned)(mine_e + 127) | (unsigned)(mine_e - 4 + 127) << 8;
-#pragma unroll
-            for (int k = 0; k < kParts; ++k) {
-              const u32x4 x[2] = {q_span[c][2 * k] ^ p.sign, q_span[c][2 * k + 1] ^ p.sign};
-              u32x4 high, low;
-              two_terms(x, part_e[k], &high, &low);
-              s_q[((e * 2 + 0) * kParts + k) * 64 + lane] = high;
-              s_q[((e * 2 + 1) * kParts + k) * 64 + lane] = low;
-            }
-          }
+          if (2 * kChunks >= kAttendWaves || e < 2 * kChunks) s_q[(e * NT + n) * 64 + lane] = q_mine[n][c] ^ p.sign;
         }
-      }
       if (some) {
         copy(p.c.keys, key_ring, g0 + wave, 0, true);
         copy(p.c.values, value_ring, g0 + wave, 0, true);
@@ -482,60 +260,9 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
         const float v_scale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v_scales), k));
         const int next = g + kAttendWaves;
         arrived();
-        f32x4 st[NT][kScores / 4];
+        f32x4 st[NT][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int t = 0; t < kScores / 4; ++t) st[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if constexpr (BITS == 4) {
-          constexpr int kWords = D < 256 ? 1 : D / 256;  // of a lane's scales of 32 tokens
-          unsigned ks[kHalves][kWords];
-#pragma unroll
-          for (int e = 0; e < kHalves; ++e) {
-            const KA_LDS char* const from = key_scales + e * D + lane * (D / 64);
-            if constexpr (D == 64) ks[e][0] = *reinterpret_cast<const KA_LDS uint8_t*>(from);
-            if constexpr (D == 128) ks[e][0] = *reinterpret_cast<const KA_LDS uint16_t*>(from);
-            if constexpr (D == 256) ks[e][0] = *reinterpret_cast<const KA_LDS unsigned*>(from);
-            if constexpr (D == 512) {
-              const u32x2 w = *reinterpret_cast<const KA_LDS u32x2*>(from);
-              ks[e][0] = w[0];
-              ks[e][kWords - 1] = w[1];
-            }
-          }
-          const u32x4 none = {0, 0, 0, 0};
-#pragma unroll
-          for (int dt = 0; dt < kSpans; ++dt)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              const int entry = dt * NT + n;
-              const unsigned qs = s_q_scales[entry * 64 + lane];
-              u32x4 q[2][2];  // [term][part]
-#pragma unroll
-              for (int term = 0; term < 2; ++term)
-#pragma unroll
-                for (int k = 0; k < kParts; ++k) q[term][k] = s_q[((entry * 2 + term) * kParts + k) * 64 + lane];
-#pragma unroll
-              for (int e = 0; e < kHalves; ++e)
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                  const u32x4 a = tile(key_ring + e * kHalfBytes, D == 64 ? 0 : t * kSpans + dt);
-                  f32x4& acc = st[n][2 * e + t];
-                  auto add = [&](auto byte) {
-                    constexpr int KB = decltype(byte)::value;
-                    // (of head size 64 the other tile's tokens meet zeros, which a NaN scale of theirs would make NaN)
-                    const unsigned k_scale = D == 64 && quad >> 1 != t ? 0u : ks[e][dt >> 1];
-                    const u32x4 h0 = D == 64 && t == 1 ? none : q[0][0], h1 = D == 64 ? (t == 1 ? q[0][0] : none) : q[0][1];
-                    const u32x4 l0 = D == 64 && t == 1 ? none : q[1][0], l1 = D == 64 ? (t == 1 ? q[1][0] : none) : q[1][1];
-                    acc = mfma_codes4<KB, 0>(a, k_scale, h0, h1, qs, acc);
-                    acc = mfma_codes4<KB, 1>(a, k_scale, l0, l1, qs, acc);
-                  };
-                  if (D == 64 || (2 * dt + t) % 4 == 0) add(std::integral_constant<int, 0>());
-                  else if ((2 * dt + t) % 4 == 1) add(std::integral_constant<int, 1>());
-                  else if ((2 * dt + t) % 4 == 2) add(std::integral_constant<int, 2>());
-                  else add(std::integral_constant<int, 3>());
-                }
-            }
-        } else
+        for (int n = 0; n < NT; ++n) st[n][0] = st[n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < 2 * kChunks; ++c) {
           bf16x8 q[NT];
@@ -556,19 +283,19 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
         }
         copy(p.c.keys, key_ring, next, k, next < g1);
 
-        const int key0 = g * kGroup;
-        const bool masked = key0 < full_lo || key0 + kGroup - 1 > full_hi;
-        bf16x8 weight[NT][2 * kHalves];  // [2 (32 tokens) + term]
-        unsigned is_seen[NT];  // one bit of each of the lane's keys
+        const int key0 = g * kCacheGroup;
+        const bool masked = key0 < full_lo || key0 + kCacheGroup - 1 > full_hi;
+        bf16x8 weight[NT][2];
+        unsigned is_seen[NT];  // one bit of each of the lane's eight keys
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          float x[kScores];
+          float x[8];
 #pragma unroll
-          for (int e = 0; e < kScores; ++e) x[e] = st[n][e >> 2][e & 3];
+          for (int e = 0; e < 8; ++e) x[e] = st[n][e >> 2][e & 3];
           is_seen[n] = 0;
           if (masked) {
 #pragma unroll
-            for (int e = 0; e < kScores; ++e) {
+            for (int e = 0; e < 8; ++e) {
               const int key = key0 + (e >> 2) * 16 + quad * 4 + (e & 3);
               const bool sees = key >= lo[n] && key <= hi[n];
               x[e] = sees ? x[e] : -INFINITY;
@@ -576,8 +303,6 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
             }
           }
           float best = max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max3(x[6], x[7], x[7]));
-          if constexpr (kScores == 16)
-            best = max3(best, max3(max3(x[8], x[9], x[10]), x[11], x[12]), max3(x[13], x[14], x[15]));
           best = column_max(best) * p.scale;
           // the running maximum is raised (and O rescaled) only where it grows by more than 2^8: weights are then at most 2^8
           if (__any(!(best <= top[n] + 8.f) && best != -INFINITY)) {
@@ -589,108 +314,23 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
             for (int t = 0; t < D / 16; ++t) o[n][t] *= f;
           }
           const float base = top[n] == -INFINITY ? 0.f : top[n];
+          float w[8];
 #pragma unroll
-          for (int half = 0; half < kHalves; ++half) {
-            float w[8];
+          for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], p.scale, -base));
+          u32x4 high, low;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * half + e], p.scale, -base));
-            u32x4 high, low;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              high[e] = pair_of(w[2 * e], w[2 * e + 1]);
-              low[e] = pair_of(w[2 * e] - __uint_as_float(high[e] << 16),
-                               w[2 * e + 1] - __uint_as_float(high[e] & 0xffff0000u));
-            }
-            weight[n][2 * half] = __builtin_bit_cast(bf16x8, high);
-            weight[n][2 * half + 1] = __builtin_bit_cast(bf16x8, low);
-            const float add = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-            sum[n] += add;
+          for (int e = 0; e < 4; ++e) {
+            high[e] = pair_of(w[2 * e], w[2 * e + 1]);
+            low[e] = pair_of(w[2 * e] - __uint_as_float(high[e] << 16),
+                             w[2 * e + 1] - __uint_as_float(high[e] & 0xffff0000u));
           }
+          weight[n][0] = __builtin_bit_cast(bf16x8, high);
+          weight[n][1] = __builtin_bit_cast(bf16x8, low);
+          const float add = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+          sum[n] += add;
         }
 
         arrived();
-        if constexpr (BITS == 4) {
-          constexpr int kGroups = D / 32;
-          // this lane's tokens' scales, of 32 elements of 32 tokens: bytes 4 t + i
-          auto scales_at = [&](int half, int group) {
-            return reinterpret_cast<KA_LDS u32x2*>(value_scales + half * D + group * 32 + quad * 8);
-          };
-          bool nan = false;
-          if (masked) {
-            unsigned any = 0;  // 0x80 where a byte is 255
-#pragma unroll
-            for (int half = 0; half < kHalves; ++half)
-#pragma unroll
-              for (int group = 0; group < kGroups; ++group) {
-                const u32x2 w = *scales_at(half, group);
-#pragma unroll
-                for (int t = 0; t < 2; ++t) any |= ((w[t] & 0x7f7f7f7fu) + 0x01010101u) & w[t] & 0x80808080u;
-              }
-            nan = __any(any != 0);
-          }
-          if (nan) {  // a NaN reaches the vectors that see its token, and no others (zero times NaN would be NaN)
-#pragma unroll 1
-            for (int half = 0; half < kHalves; ++half)
-#pragma unroll
-              for (int group = 0; group < kGroups; ++group) {
-                u32x2 w = *scales_at(half, group);
-                unsigned marks = 0;
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                  for (int i = 0; i < 4; ++i)
-                    if ((w[t] >> (8 * i) & 255) == 255) {
-                      marks |= 1u << (4 * t + i);
-                      w[t] &= ~(255u << (8 * i));
-                    }
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                  const float hit = column_sum((is_seen[n] >> (8 * half) & marks) != 0 ? 1.f : 0.f);
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) {
-                    o[n][2 * group][e] += hit > 0.f ? NAN : 0.f;
-                    o[n][2 * group + 1][e] += hit > 0.f ? NAN : 0.f;
-                  }
-                }
-                *scales_at(half, group) = w;  // (every lane of the quad the same: what a lane read before, it may not keep)
-              }
-          }
-#pragma unroll
-          for (int half = 0; half < kHalves; ++half)
-#pragma unroll
-            for (int t64 = 0; t64 < kLoads; ++t64) {
-              const u32x4 w = tile(value_ring + half * kHalfBytes, t64);
-#pragma unroll
-              for (int d = 0; d < 2; ++d) {
-                const int group = 2 * t64 + d;
-                const u32x2 sc = *scales_at(half, group);
-                u32x4 even, odd;
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                  // (the conversion goes by its scale's exponent bits alone, 30 .. 23)
-                  const unsigned c = w[2 * d + t];
-                  const unsigned r0 = pair_at<0>(c, sc[t] << 23), r1 = pair_at<1>(c, sc[t] << 15);
-                  const unsigned r2 = pair_at<2>(c, sc[t] << 7), r3 = pair_at<3>(c, sc[t] >> 1);
-                  even[2 * t] = __builtin_amdgcn_perm(r1, r0, 0x05040100u);
-                  even[2 * t + 1] = __builtin_amdgcn_perm(r3, r2, 0x05040100u);
-                  odd[2 * t] = __builtin_amdgcn_perm(r1, r0, 0x07060302u);
-                  odd[2 * t + 1] = __builtin_amdgcn_perm(r3, r2, 0x07060302u);
-                }
-                const bf16x8 a = __builtin_bit_cast(bf16x8, even), c = __builtin_bit_cast(bf16x8, odd);
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                  for (int term = 0; term < 2; ++term) {
-                    const bf16x8 wt = weight[n][2 * half + term];
-                    o[n][2 * group] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, wt, o[n][2 * group], 0, 0, 0);
-                    o[n][2 * group + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(c, wt, o[n][2 * group + 1], 0, 0, 0);
-                  }
-              }
-            }
-          read_out();
-          copy(p.c.values, value_ring, next, k, next < g1);
-          continue;
-        }
         bool nan = false;
         if (masked) {
           unsigned any = 0;
@@ -786,16 +426,8 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
           const float f = top[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top[n] - top_of(16 * n + col));
 #pragma unroll
           for (int t = 0; t < D / 16; ++t)
-            if (t * 16 >= d0 && t * 16 < d0 + kSlab) {
-              if constexpr (BITS == 8)
-                *reinterpret_cast<f32x4*>(&s_o[wave][16 * n + col][t * 16 - d0 + quad * 4]) = o[n][t] * f;
-              else {  // (tiles of even and of odd elements)
-                const f32x4 a = o[n][t & ~1] * f, c = o[n][t | 1] * f;
-                const int k = t & 1;
-                *reinterpret_cast<f32x4*>(&s_o[wave][16 * n + col][(t & ~1) * 16 - d0 + quad * 8 + 4 * k]) =
-                    f32x4{a[2 * k], c[2 * k], a[2 * k + 1], c[2 * k + 1]};
-              }
-            }
+            if (t * 16 >= d0 && t * 16 < d0 + kSlab)
+              *reinterpret_cast<f32x4*>(&s_o[wave][16 * n + col][t * 16 - d0 + quad * 4]) = o[n][t] * f;
         }
         lds_barrier();
         for (int e = tid; e < vectors * (kSlab / 4); e += kAttendThreads) {
@@ -818,7 +450,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
     }
     carry += all[0];
   }
-  if (p.whole) fill_past<D>(p, seen_of<kGroup>(p, blockIdx.x), blockIdx.y, tid, kAttendThreads);
+  if (p.whole) fill_past<D>(p, seen_of(p, blockIdx.x), blockIdx.y, tid, kAttendThreads);
 }
 
 // Joins a request's shares: O = sum of 2^(m_w - M) O_w over sum of 2^(m_w - M) l_w, in an order that the sizes alone set.
@@ -826,14 +458,14 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
 // vector. More: 64 elements of a vector by 16 threads of four and 16 rows, each row with every sixteenth share (so that
 // up to 16 cost one round of loads), and the rows joined through LDS. 4.4 to 6.6 us, launch and four rounds of loads; 33 us with
 // one walk over 64 shares of one request.
-template <int D, int GROUP>
+template <int D>
 __global__ __launch_bounds__(256) void join_kernel(const AttendParams p, int vectors_per) {
   constexpr int kSlabs = D / 64, kFew = 4;
   __shared__ float s_m[16], s_l[16];
   __shared__ f32x4 s_x[16][16];
   const int i = blockIdx.x, heads = p.c.kv_heads;
   const int total = p.units[p.r.n_seq], begin = p.units[i];
-  const Seen s = seen_of<GROUP>(p, i);
+  const Seen s = seen_of(p, i);
   if (s.units == 0) return;
   fill_past<D>(p, s, blockIdx.y, blockIdx.z * 256 + threadIdx.x, gridDim.z * 256);
   const Shares shares(total, p.parts);
@@ -907,23 +539,18 @@ __global__ __launch_bounds__(256) void join_kernel(const AttendParams p, int vec
   }
 }
 
-template <int D, int NT, int BITS>
-void launch_format(const AttendParams& p, const AttendShape& s, hipStream_t stream) {
+template <int D, int NT>
+void launch(const AttendParams& p, const AttendShape& s, hipStream_t stream) {
   const unsigned y = (unsigned)(p.c.kv_heads * s.tiles), x = (unsigned)(p.whole ? p.r.n_seq : s.parts);
   if (s.tiles == 1)
-    attend_kernel<D, NT, true, BITS><<<dim3(x, y), dim3(kAttendThreads), 0, stream>>>(p);
+    attend_kernel<D, NT, true><<<dim3(x, y), dim3(kAttendThreads), 0, stream>>>(p);
   else
-    attend_kernel<D, NT, false, BITS><<<dim3(x, y), dim3(kAttendThreads), 0, stream>>>(p);
+    attend_kernel<D, NT, false><<<dim3(x, y), dim3(kAttendThreads), 0, stream>>>(p);
   if (p.whole) return;
   // a workgroup for 64 elements of each vector, or as many as fill the GPU several times over
   const int64_t pairs = (int64_t)p.r.n_seq * y, most = (2048 + pairs - 1) / pairs, items = (int64_t)s.used * (D / 64);
   const unsigned z = (unsigned)(items < most ? items : most);
-  join_kernel<D, group_of(BITS, NT)><<<dim3((unsigned)p.r.n_seq, y, z), dim3(256), 0, stream>>>(p, 16 * NT);
-}
-
-template <int D, int NT>
-void launch(const AttendParams& p, const AttendShape& s, hipStream_t stream) {
-  if (p.c.scales4 != nullptr) launch_format<D, NT, 4>(p, s, stream); else launch_format<D, NT, 8>(p, s, stream);
+  join_kernel<D><<<dim3((unsigned)p.r.n_seq, y, z), dim3(256), 0, stream>>>(p, 16 * NT);
 }
 
 }  // namespace

@@ -199,11 +199,11 @@ int append_rows(const Args* a, const KarpoCachePrologue& f, void* stream) {
   bool none;
   int st = append_params(a, &p.a, &none);
   if (st != KARPO_ATTN_OK) return st;
-  if (a->n_writes > INT32_MAX / (2 * a->cache.kv_heads) - 8) return KARPO_ATTN_ERR_ARG;  // (rounded up to the eight dies)
   p.a.rows = a->rows;
   st = prologue_params(f, a->cache.head_dim, &p);
   if (st != KARPO_ATTN_OK || none) return st;
   p.n_writes = a->n_writes;
+  p.many = 4 * a->rows * a->cache.kv_heads * a->cache.head_dim > kL2Bytes;
   if (launch_cache_append_rows(p, static_cast<hipStream_t>(stream)) != hipSuccess) return KARPO_ATTN_ERR_LAUNCH;
   return KARPO_ATTN_OK;
 }
@@ -360,7 +360,9 @@ template <class Args>
 AttendShape shape_of(const Args* a, const CacheRef& c, const CacheRows& r) {
   int64_t seen = a->total_keys < r.most ? a->total_keys : r.most;
   if (a->window_left >= 0 && (int64_t)a->max_q + a->window_left < seen) seen = (int64_t)a->max_q + a->window_left;
-  return attend_shape(c, a->n_seq, a->heads / a->cache.kv_heads, a->max_q, seen);
+  const int32_t group = a->heads / a->cache.kv_heads;
+  return c.scales4 != nullptr ? attend4_shape(c, a->n_seq, group, a->max_q, seen)
+                              : attend_shape(c, a->n_seq, group, a->max_q, seen);
 }
 
 template <class Args>
@@ -422,7 +424,9 @@ int attend(const Args* a, void* stream) {
       t.units = static_cast<int32_t*>(a->workspace);
       t.partial = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + shape.units_bytes);
     }
-    if (launch_cache_attend(t, shape, static_cast<hipStream_t>(stream)) != hipSuccess) return KARPO_ATTN_ERR_LAUNCH;
+    const hipError_t done = t.c.scales4 != nullptr ? launch_cache4_attend(t, shape, static_cast<hipStream_t>(stream))
+                                                   : launch_cache_attend(t, shape, static_cast<hipStream_t>(stream));
+    if (done != hipSuccess) return KARPO_ATTN_ERR_LAUNCH;
     return KARPO_ATTN_OK;
   }
   Unpacked u;

@@ -79,9 +79,9 @@ def path_of(cache, heads, max_q, rows, n, width, window=-1, total_keys=None):
     d, vectors = cache.head_dim, max_q * heads // cache.kv_heads
     most = 4 if d <= 128 else 2 if d == 256 else 1
     nt = next(t for t in (1, 2, 4) if t == most or vectors <= 16 * t)
-    waves = 4 if nt == 1 and d <= 128 else 3 if (d, nt) == (64, 2) else 2 if d <= 128 or (d, nt) == (256, 1) else 1
+    waves = 4 if (d, nt) == (64, 1) else 3 if (d, nt) in ((64, 2), (128, 1)) else 2 if d <= 128 or (d, nt) == (256, 1) else 1
     y = cache.kv_heads * -(-vectors // (16 * nt))
-    split = -(-4 * (n + 1) // 256) * 256 + y * max(1, 256 * waves // y) * 2 * 16 * nt * (d + 2) * 4
+    split = -(-4 * (n + 2) // 256) * 256 + y * max(1, 256 * waves // y) * 2 * 16 * nt * (d + 2) * 4
     return SPLIT if need.value == split else UNPACKED
 
 

@@ -108,7 +108,6 @@ def test_append_skips_writes_out_of_range(gpu):
 
 @pytest.mark.parametrize("n", [1, 7, 8, 9, 17])
 def test_append_of_several_writes(gpu, n):
-    """Counts around the eight dies that writes are dealt over."""
     cache = random_cache(gpu, n, 2, 64, 32, seed=n)
     rows = torch.randn((3 * n, 2, 64), device=gpu).bfloat16()
     _append_and_compare(cache, rows, rows * 2, [[n - 1 - i, i % 30, 3 * i, 1 + i % 3] for i in range(n)])
