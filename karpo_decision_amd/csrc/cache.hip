@@ -348,47 +348,69 @@ __global__ __launch_bounds__(64 * WAVES) void append_kernel(const AppendParams p
 
 constexpr int kReadWaves = 4;
 
-// Rows of 32 tokens of one head's keys in 4 bits, t0 .. + N of the D / 64 parts that their tokens make (2,048 / D tokens each): a
-// lane takes 4 bytes, 8 elements of a token, D / 8 lanes side by side a whole row.
+// LDS of a wave for the unit of a cache in 4 bits: two KiB of codes, each 256 bytes (of keys 32 elements of 16 tokens, of values
+// the tokens of a quad) a few banks from the last, and the keys' scales as fp32.
+constexpr int kKeyPitch4 = 256 + 64, kValuePitch4 = 256 + 16, kUnit4Bytes = 2 * (4 * kKeyPitch4 + 256);
+
+// Of 32 tokens of one head's keys in 4 bits the tiles t0 .. + N of 1 KiB (16 tokens x 128 elements; of head size 64 32 x 64) as
+// rows: a lane takes 4 bytes out of LDS, 8 elements of a token, so that 16 lanes (8) store 256 bytes (128) of a row.
 template <int D, int N, class Store>
 __device__ __forceinline__ void read_keys4(const uint8_t* codes, const uint8_t* scales, bool known, int t0, int tokens_left,
-                                           uint16_t* to, int64_t step, int lane, Store store) {
-  constexpr int kLanes = D / 8, kRows = 64 / kLanes;  // a load: kRows tokens
-  constexpr int kLoads = N * 4;
-  const int sub = lane / kLanes, d0 = (lane - sub * kLanes) * 8, group = d0 >> 5;
-  unsigned w[kLoads], sc[kLoads];
-#pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int token = (t0 * 4 + i) * kRows + sub, t2 = token >> 4, t16 = token & 15;
-    const int byte = D == 64 ? (t2 * 2 + group) * 16 + t16 : ((group & 3) * 16 + t16) * (D / 64) + (group >> 2) * 2 + t2;
-    w[i] = known ? *reinterpret_cast<const unsigned*>(codes + (t2 * (D / 32) + group) * 256 + t16 * 16 + ((d0 & 31) >> 1)) : 0;
-    sc[i] = known ? scales[byte] : 0;
-  }
-#pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int token = (t0 * 4 + i) * kRows + sub;
-    const float scale = __uint_as_float(sc[i] << 23);
-    if (token < tokens_left) store(to + token * step + d0, bf16_of_8_codes4(w[i], scale));
-  }
-}
-// The same of values, t0 .. + N of their tiles of 64 elements: a lane takes the bytes of 4 tokens x 8 elements, four words, and stores 16 bytes of each token's row; eight
-// lanes side by side make 128 of a row.
-template <int D, int N, class Store>
-__device__ __forceinline__ void read_values4(const uint8_t* codes, const uint8_t* scales, bool known, int t0, int tokens_left,
-                                             uint16_t* to, int64_t step, int lane, Store store) {
-  const int j = lane & 3, g = (lane >> 2) & 1, q = (lane >> 3) & 3, t2 = lane >> 5;
-  unsigned w[N][4], sc[N];
+                                           uint16_t* to, int64_t step, int lane, char* lds, Store store) {
+  constexpr int kSpans = D < 128 ? 1 : D / 128, kLanes = D < 128 ? 8 : 16, kRows = 64 / kLanes;
+  const int l = lane % kLanes, sub = lane / kLanes;
+  u32x4 w[N];
+  unsigned sc[N];
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    const uint8_t* const from = codes + (t0 + n) * 1024 + (q * 16 + 4 * j) * 16 + g * 8 + t2 * 4;
+    const int t2 = (t0 + n) / kSpans, dt = (t0 + n) % kSpans;
+    w[n] = known ? *reinterpret_cast<const u32x4*>(codes + (t0 + n) * 1024 + lane * 16) : u32x4{0, 0, 0, 0};
+    sc[n] = known ? scales[D == 64 ? lane : lane * (D / 64) + dt * 2 + t2] : 0;
+  }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) w[n][k] = known ? *reinterpret_cast<const unsigned*>(from + k * 16) : 0;
+  for (int n = 0; n < N; ++n) {
+    char* const mine = lds + n * (4 * kKeyPitch4 + 256);
+    *reinterpret_cast<u32x4*>(mine + (lane >> 4) * kKeyPitch4 + (lane & 15) * 16) = w[n];
+    *reinterpret_cast<unsigned*>(mine + 4 * kKeyPitch4 + lane * 4) = sc[n] << 23;
+  }
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const char* const mine = lds + n * (4 * kKeyPitch4 + 256);
+    const int t2 = (t0 + n) / kSpans, dt = (t0 + n) % kSpans;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int token = i * kRows + sub;  // of the tile
+      const int piece = D == 64 ? (token >> 4) * 2 + (l >> 2) : l >> 2, t16 = token & 15;
+      const unsigned c = *reinterpret_cast<const unsigned*>(mine + piece * kKeyPitch4 + t16 * 16 + (l & 3) * 4);
+      const float scale = *reinterpret_cast<const float*>(mine + 4 * kKeyPitch4 + (piece * 16 + t16) * 4);
+      const int row = D == 64 ? token : t2 * 16 + token;
+      if (row < tokens_left) store(to + row * step + dt * 128 + l * 8, bf16_of_8_codes4(c, scale));
+    }
+  }
+}
+// The same of values, tiles of 32 tokens x 64 elements: a lane takes the bytes of 4 tokens x 8 elements, four words, and stores 16
+// bytes of each token's row; eight lanes side by side make 128 of a row.
+template <int D, int N, class Store>
+__device__ __forceinline__ void read_values4(const uint8_t* codes, const uint8_t* scales, bool known, int t0, int tokens_left,
+                                             uint16_t* to, int64_t step, int lane, char* lds, Store store) {
+  const int j = lane & 3, g = (lane >> 2) & 1, q = (lane >> 3) & 3, t2 = lane >> 5;
+  u32x4 w[N];
+  unsigned sc[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    w[n] = known ? *reinterpret_cast<const u32x4*>(codes + (t0 + n) * 1024 + lane * 16) : u32x4{0, 0, 0, 0};
     sc[n] = known ? *reinterpret_cast<const unsigned*>(scales + (2 * (t0 + n) + g) * 32 + q * 8 + t2 * 4) : 0;
   }
 #pragma unroll
+  for (int n = 0; n < N; ++n)
+    *reinterpret_cast<u32x4*>(lds + n * 4 * kValuePitch4 + (lane >> 4) * kValuePitch4 + (lane & 15) * 16) = w[n];
+#pragma unroll
   for (int n = 0; n < N; ++n) {
-    unsigned row[4];
-    transposed(w[n], row);
+    unsigned r[4], row[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      r[k] = *reinterpret_cast<const unsigned*>(lds + n * 4 * kValuePitch4 + q * kValuePitch4 + (4 * j + k) * 16 + g * 8 + t2 * 4);
+    transposed(r, row);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int token = 16 * t2 + 4 * q + i;
@@ -414,7 +436,7 @@ __global__ __launch_bounds__(64 * kReadWaves) void read_kernel(const ReadParams 
   constexpr int kTileBytes = 2 * (512 + 64);
   __shared__ int s_part[kReadWaves][2];
   __shared__ int s_group[kThreads + 1], s_row[kThreads], s_start[kThreads], s_tokens[kThreads];
-  __shared__ __align__(16) char s_codes[BITS == 8 ? kReadWaves : 1][BITS == 8 ? kAtOnce * kTileBytes : 16];
+  __shared__ __align__(16) char s_codes[kReadWaves][BITS == 8 ? kAtOnce * kTileBytes : kUnit4Bytes];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int heads = p.c.kv_heads, b = p.c.block_log2;
 
@@ -514,9 +536,9 @@ __global__ __launch_bounds__(64 * kReadWaves) void read_kernel(const ReadParams 
         const uint8_t* const scales = p.c.scales4 + ((head << b) + inside) * (D / 16) + (value ? D : 0);
         uint16_t* const to = (value ? p.v : p.k) + (out_row * heads + h) * D;
         if (value)
-          read_values4<D, kAtOnce>(codes, scales, known, t0, tokens_left, to, (int64_t)heads * D, lane, store);
+          read_values4<D, kAtOnce>(codes, scales, known, t0, tokens_left, to, (int64_t)heads * D, lane, s_codes[wave], store);
         else
-          read_keys4<D, kAtOnce>(codes, scales, known, t0, tokens_left, to, (int64_t)heads * D, lane, store);
+          read_keys4<D, kAtOnce>(codes, scales, known, t0, tokens_left, to, (int64_t)heads * D, lane, s_codes[wave], store);
         continue;
       }
       const uint8_t* const src = (value ? p.c.values : p.c.keys) + (head << b) * D + inside * D;
