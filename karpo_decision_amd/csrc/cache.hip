@@ -636,9 +636,11 @@ hipError_t launch_cache_read(const ReadParams& p, hipStream_t stream) {
   auto launch = [&](auto d) {
     constexpr int D = decltype(d)::value;
     if (four)
-      p.stream ? read_kernel<D, true, 4><<<grid, threads, 0, stream>>>(p) : read_kernel<D, false, 4><<<grid, threads, 0, stream>>>(p);
+      p.stream ? read_kernel<D, true, 4><<<grid, threads, 0, stream>>>(p)
+               : read_kernel<D, false, 4><<<grid, threads, 0, stream>>>(p);
     else
-      p.stream ? read_kernel<D, true, 8><<<grid, threads, 0, stream>>>(p) : read_kernel<D, false, 8><<<grid, threads, 0, stream>>>(p);
+      p.stream ? read_kernel<D, true, 8><<<grid, threads, 0, stream>>>(p)
+               : read_kernel<D, false, 8><<<grid, threads, 0, stream>>>(p);
   };
   switch (p.c.head_dim) {
     case 64: launch(std::integral_constant<int, 64>()); break;

@@ -19,7 +19,14 @@ __host__ __device__ constexpr int attend4_waves(int d, int nt) {
 // Bytes of LDS for the waves' copies of a group's keys (as many for the values).
 constexpr int ring4_bytes(int d) { return kAttendWaves * kCacheGroup * d / 2; }
 
-constexpr int64_t kWholeTokens4 = 640;  // (requests of which at most this many tokens are seen are not split)
+// Requests of which at most so many tokens are seen are not split: a workgroup's walk is then shorter than the partials' way
+// through memory and a second launch. us split, whole at heads of 128 with 16 key heads: 8 requests of 128 tokens 12.4, 7.3, of
+// 640 15.9, 11.4, of 1,500 18.9, 18.7; one of 1,024 13.7, 13.6; heads of 512, 2 requests of 256 15.8, 13.0, of 512 16.7, 17.6.
+constexpr int whole_tokens4(int d) { return d == 512 ? 256 : 640; }
+// Where more than half of the CUs have a workgroup, a longer walk is no loss (48 requests of 4 query tokens and 1,024 cached
+// ones: heads of 64 18.4, 13.0; 128 33.4, 27.4; 256 36.1, 29.9; 512 64.4, 60.5), up to what one long request among short ones
+// may take.
+constexpr int kWholeTokens4 = 1024;
 constexpr int kLeastUnits4 = 4;         // groups of 32 tokens that a workgroup takes at least, of a request that is split
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
@@ -716,7 +723,7 @@ AttendShape attend4_shape(const CacheRef& c, int32_t n_seq, int32_t group, int32
   const int64_t parts = 256 * attend4_waves(c.head_dim, tiles) / y;
   s.parts = parts < 1 ? 1 : (int)parts;
   s.used = (int)(vectors < s.vectors ? vectors : s.vectors);
-  s.whole = seen <= (c.head_dim == 512 ? kWholeTokens4 / 4 : kWholeTokens4);
+  s.whole = seen <= (n_seq * y > 128 ? kWholeTokens4 : whole_tokens4(c.head_dim));
   s.units_bytes = (4 * ((int64_t)n_seq + 2) + 255) / 256 * 256;
   s.bytes = s.whole ? 0 : s.units_bytes + y * s.parts * 2 * s.vectors * (c.head_dim + 2) * 4;
   return s;

@@ -171,203 +171,205 @@ __device__ __forceinline__ void append_rows(const AppendRowsParams& p, const Wri
 #pragma unroll
         for (int k = 0; k < 4; ++k) asm volatile("" : "+v"(cv[t][k]), "+v"(sv[t][k]));
     }
-  const int64_t head = (int64_t)wr.block * c.kv_heads + h;
-  uint8_t* const out = (VALUE ? c.values : c.keys) + head * BLOCK * kBytes;
-  float* const scale_of = BITS == 8 ? c.scales + 2 * head + (VALUE ? 1 : 0) : nullptr;
-  const unsigned old_bits = BITS == 8 && first > 0 ? __float_as_uint(*scale_of) : 0;
-  auto row_of = [&](int t, float (&y)[8]) {
-    float ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(bf16_at(x[t], e), bf16_at(x[t], e), ss);
-    const float root = reciprocal_root(sum_over<kLanes>(ss) * (1.f / D) + norm.eps), r = normed ? root : 1.f;
-    if constexpr (TURNED) {
-      u32x4 px;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) px[k] = (unsigned)__builtin_amdgcn_ds_bpermute(partner, (int)x[t][k]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float n = bf16_at(x[t], e) * w_mine[e];
-        const float turn = __builtin_fmaf(n, bf16_at(cv[t], e), bf16_at(px, e) * w_other[e] * bf16_at(sv[t], e));
-        y[e] = (inside ? turn : n) * r;
+    const int64_t head = (int64_t)wr.block * c.kv_heads + h;
+    uint8_t* const out = (VALUE ? c.values : c.keys) + head * BLOCK * kBytes;
+    float* const scale_of = BITS == 8 ? c.scales + 2 * head + (VALUE ? 1 : 0) : nullptr;
+    const unsigned old_bits = BITS == 8 && first > 0 ? __float_as_uint(*scale_of) : 0;
+    auto row_of = [&](int t, float (&y)[8]) {
+      float ss = 0.f;
+  #pragma unroll
+      for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(bf16_at(x[t], e), bf16_at(x[t], e), ss);
+      const float root = reciprocal_root(sum_over<kLanes>(ss) * (1.f / D) + norm.eps), r = normed ? root : 1.f;
+      if constexpr (TURNED) {
+        u32x4 px;
+  #pragma unroll
+        for (int k = 0; k < 4; ++k) px[k] = (unsigned)__builtin_amdgcn_ds_bpermute(partner, (int)x[t][k]);
+  #pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float n = bf16_at(x[t], e) * w_mine[e];
+          const float turn = __builtin_fmaf(n, bf16_at(cv[t], e), bf16_at(px, e) * w_other[e] * bf16_at(sv[t], e));
+          y[e] = (inside ? turn : n) * r;
+        }
+      } else {
+  #pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = bf16_at(x[t], e) * w_mine[e] * r;
+      }
+    };
+    // the largest magnitude of y and `best`, NaN as nothing
+    auto larger = [&](const float (&y)[8], float best) {
+  #pragma unroll
+      for (int e = 0; e < 8; e += 2)
+        best = __builtin_fmaxf(__builtin_fmaxf(best, __builtin_fabsf(y[e])), __builtin_fabsf(y[e + 1]));
+      return best;
+    };
+
+    bool grown = false;
+    float scale = 1.f, old_scale = 1.f;
+    if constexpr (BITS == 8) {
+      float y[PASSES][8], most_of = 0.f;
+  #pragma unroll
+      for (int t = 0; t < PASSES; ++t) {
+        row_of(t, y[t]);
+        most_of = larger(y[t], most_of);
+      }
+      if (MANY && h + 1 < h1) load(h + 1);
+      auto joined = [&](unsigned mine) {  // over the workgroup
+        mine = max_over<64>(mine);
+        if constexpr (WAVES > 1) {
+          unsigned* const s_best = reinterpret_cast<unsigned*>(s_codes);
+          __syncthreads();
+          if (lane == 0) s_best[wave] = mine;
+          __syncthreads();
+  #pragma unroll
+          for (int w = 0; w < WAVES; ++w) mine = max(mine, s_best[w]);
+          __syncthreads();  // (the codes, or the next head's maxima, take the array)
+        }
+        return mine;
+      };
+      unsigned best = joined(__float_as_uint(most_of));
+      const bool odd = best >= 0x7f800000u;  // infinities: the largest of the others
+      if (__builtin_expect(odd, 0)) {
+        best = 0;
+  #pragma unroll
+        for (int t = 0; t < PASSES; ++t)
+  #pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const unsigned m = __float_as_uint(y[t][e]) & 0x7fffffffu;
+            best = max(best, m < 0x7f800000u ? m : 0u);
+          }
+        best = joined(best);
+      }
+      int e = exponent_of<8>(best), old = e;
+      if (first > 0) {
+        old = min(max((int)((old_bits >> 23) & 0xff) - 127, KARPO_CACHE_MIN_EXP), KARPO_CACHE_MAX_EXP);
+        e = max(e, old);
+      }
+      grown = old < e;  // the earlier tokens' codes are rounded again
+      scale = power_of_two(e);
+      old_scale = power_of_two(old);
+      if (tid == 0) *scale_of = scale;
+      if (__builtin_expect(odd || e == KARPO_CACHE_MAX_EXP, 0)) {
+        const float most = 448.f * scale;
+  #pragma unroll
+        for (int t = 0; t < PASSES; ++t)
+  #pragma unroll
+          for (int k = 0; k < 8; ++k) y[t][k] = __builtin_fabsf(y[t][k]) > most ? __builtin_copysignf(most, y[t][k]) : y[t][k];
+      }
+  #pragma unroll
+      for (int t = 0; t < PASSES; ++t) {
+        const int slot = first + token_of(t);
+        const u32x2 w = {codes8(y[t][0], y[t][1], y[t][2], y[t][3], scale), codes8(y[t][4], y[t][5], y[t][6], y[t][7], scale)};
+        if (token_of(t) < count) {
+          if constexpr (VALUE)
+            *reinterpret_cast<u32x2*>(s_codes + slot * kPitch + d0) = w;
+          else
+            *reinterpret_cast<u32x2*>(out + ((slot >> 4) * (D / 64) + (d0 >> 6)) * 1024 + (slot & 15) * 64 + (d0 & 63)) = w;
+        }
+      }
+      if (!VALUE && grown) {
+        for (int u = tid; u < first * (D / 16); u += 64 * WAVES) {
+          const int slot = u / (D / 16), piece = u % (D / 16);
+          u32x4* const dst =
+              reinterpret_cast<u32x4*>(out + ((slot >> 4) * (D / 64) + (piece >> 2)) * 1024 + (slot & 15) * 64 + (piece & 3) * 16);
+          u32x4 w = *dst;
+  #pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = codes_again(w[k], old_scale, scale);
+          *dst = w;
+        }
       }
     } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = bf16_at(x[t], e) * w_mine[e] * r;
-    }
-  };
-  // the largest magnitude of y and `best`, NaN as nothing
-  auto larger = [&](const float (&y)[8], float best) {
-#pragma unroll
-    for (int e = 0; e < 8; e += 2) best = __builtin_fmaxf(__builtin_fmaxf(best, __builtin_fabsf(y[e])), __builtin_fabsf(y[e + 1]));
-    return best;
-  };
-
-  bool grown = false;
-  float scale = 1.f, old_scale = 1.f;
-  if constexpr (BITS == 8) {
-    float y[PASSES][8], most_of = 0.f;
-#pragma unroll
-    for (int t = 0; t < PASSES; ++t) {
-      row_of(t, y[t]);
-      most_of = larger(y[t], most_of);
-    }
-    if (MANY && h + 1 < h1) load(h + 1);
-    auto joined = [&](unsigned mine) {  // over the workgroup
-      mine = max_over<64>(mine);
-      if constexpr (WAVES > 1) {
-        unsigned* const s_best = reinterpret_cast<unsigned*>(s_codes);
-        __syncthreads();
-        if (lane == 0) s_best[wave] = mine;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) mine = max(mine, s_best[w]);
-        __syncthreads();  // (the codes, or the next head's maxima, take the array)
-      }
-      return mine;
-    };
-    unsigned best = joined(__float_as_uint(most_of));
-    const bool odd = best >= 0x7f800000u;  // infinities: the largest of the others
-    if (__builtin_expect(odd, 0)) {
-      best = 0;
-#pragma unroll
-      for (int t = 0; t < PASSES; ++t)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const unsigned m = __float_as_uint(y[t][e]) & 0x7fffffffu;
-          best = max(best, m < 0x7f800000u ? m : 0u);
+      uint8_t* const scales = c.scales4 + head * (BLOCK / 32) * 2 * D + (VALUE ? D : 0);
+  #pragma unroll
+      for (int t = 0; t < PASSES; ++t) {
+        const int slot = first + token_of(t);
+        float y[8];
+        row_of(t, y);
+        // (a sum is NaN where an element is, or where infinities of both signs are)
+        unsigned best = max_over<4>(__float_as_uint(larger(y, 0.f)));
+        const float sum = ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+        bool nan = false;
+        // seldom: the largest of the others, and is one NaN
+        if (__any(!(__builtin_fabsf(sum) < INFINITY) || best >= 0x7f800000u)) {
+          unsigned fine = 0, all = 0;
+  #pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const unsigned m = __float_as_uint(y[e]) & 0x7fffffffu;
+            fine = max(fine, m < 0x7f800000u ? m : 0u);
+            all = max(all, m);
+          }
+          best = max_over<4>(fine);
+          nan = max_over<4>(all) > 0x7f800000u;
         }
-      best = joined(best);
-    }
-    int e = exponent_of<8>(best), old = e;
-    if (first > 0) {
-      old = min(max((int)((old_bits >> 23) & 0xff) - 127, KARPO_CACHE_MIN_EXP), KARPO_CACHE_MAX_EXP);
-      e = max(e, old);
-    }
-    grown = old < e;  // the earlier tokens' codes are rounded again
-    scale = power_of_two(e);
-    old_scale = power_of_two(old);
-    if (tid == 0) *scale_of = scale;
-    if (__builtin_expect(odd || e == KARPO_CACHE_MAX_EXP, 0)) {
-      const float most = 448.f * scale;
-#pragma unroll
-      for (int t = 0; t < PASSES; ++t)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) y[t][k] = __builtin_fabsf(y[t][k]) > most ? __builtin_copysignf(most, y[t][k]) : y[t][k];
-    }
-#pragma unroll
-    for (int t = 0; t < PASSES; ++t) {
-      const int slot = first + token_of(t);
-      const u32x2 w = {codes8(y[t][0], y[t][1], y[t][2], y[t][3], scale), codes8(y[t][4], y[t][5], y[t][6], y[t][7], scale)};
-      if (token_of(t) < count) {
-        if constexpr (VALUE)
-          *reinterpret_cast<u32x2*>(s_codes + slot * kPitch + d0) = w;
-        else
-          *reinterpret_cast<u32x2*>(out + ((slot >> 4) * (D / 64) + (d0 >> 6)) * 1024 + (slot & 15) * 64 + (d0 & 63)) = w;
-      }
-    }
-    if (!VALUE && grown) {
-      for (int u = tid; u < first * (D / 16); u += 64 * WAVES) {
-        const int slot = u / (D / 16), piece = u % (D / 16);
-        u32x4* const dst =
-            reinterpret_cast<u32x4*>(out + ((slot >> 4) * (D / 64) + (piece >> 2)) * 1024 + (slot & 15) * 64 + (piece & 3) * 16);
-        u32x4 w = *dst;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = codes_again(w[k], old_scale, scale);
-        *dst = w;
-      }
-    }
-  } else {
-    uint8_t* const scales = c.scales4 + head * (BLOCK / 32) * 2 * D + (VALUE ? D : 0);
-#pragma unroll
-    for (int t = 0; t < PASSES; ++t) {
-      const int slot = first + token_of(t);
-      float y[8];
-      row_of(t, y);
-      // (a sum is NaN where an element is, or where infinities of both signs are)
-      unsigned best = max_over<4>(__float_as_uint(larger(y, 0.f)));
-      const float sum = ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
-      bool nan = false;
-      if (__any(!(__builtin_fabsf(sum) < INFINITY) || best >= 0x7f800000u)) {  // seldom: the largest of the others, and is one NaN
-        unsigned fine = 0, all = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const unsigned m = __float_as_uint(y[e]) & 0x7fffffffu;
-          fine = max(fine, m < 0x7f800000u ? m : 0u);
-          all = max(all, m);
-        }
-        best = max_over<4>(fine);
-        nan = max_over<4>(all) > 0x7f800000u;
-      }
-      const int e = exponent_of<4>(best);
-      const unsigned w = codes4(y, power_of_two(e));
-      if (token_of(t) < count) {
-        const int group = d0 >> 5, t2 = (slot >> 4) & 1, t16 = slot & 15;
-        if constexpr (VALUE)
-          *reinterpret_cast<unsigned*>(s_codes + slot * kPitch + (d0 >> 1)) = w;
-        else
-          *reinterpret_cast<unsigned*>(out + (slot >> 5) * 16 * D + (t2 * (D / 32) + group) * 256 + t16 * 16 +
-                                       ((d0 & 31) >> 1)) = w;
-        if ((l & 3) == 0) {
-          const int byte = VALUE     ? group * 32 + (t16 >> 2) * 8 + t2 * 4 + (t16 & 3)
-                           : D == 64 ? (t2 * 2 + group) * 16 + t16
-                                     : ((group & 3) * 16 + t16) * (D / 64) + (group >> 2) * 2 + t2;
-          scales[(slot >> 5) * 2 * D + byte] = nan ? 255 : (uint8_t)(e + 127);
-        }
-      }
-    }
-    if (MANY && h + 1 < h1) load(h + 1);
-  }
-  if constexpr (VALUE) {
-    __syncthreads();
-    const int half0 = grown ? 0 : first >> 5, half1 = (first + count - 1) >> 5;
-    constexpr int kTiles = kBytes / 32;  // KiB of codes of 32 tokens
-    for (int u = tid; u < (half1 - half0 + 1) * kTiles * 16; u += 64 * WAVES) {
-      const int j = u & 3, q = (u >> 2) & 3, tile = (u >> 4) % kTiles, half = half0 + (u >> 4) / kTiles;
-      // bytes of the tokens 16 t + 4 q + 0 .. 3 that are new, and that are rounded again
-      unsigned is_new[2] = {0, 0}, is_old[2] = {0, 0};
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int slot = half * 32 + t * 16 + q * 4 + i;
-          if (slot >= first && slot < first + count) is_new[t] |= 0xffu << (8 * i);
-          if (grown && slot < first) is_old[t] |= 0xffu << (8 * i);
-        }
-      if ((is_new[0] | is_new[1] | is_old[0] | is_old[1]) == 0) continue;
-      const bool whole = (is_new[0] & is_new[1]) == 0xffffffffu;
-      u32x4 w[4];
-#pragma unroll
-      for (int g = 0; g < 2; ++g)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          unsigned r[4], o[4];
-          const char* const from = s_codes + (half * 32 + t * 16 + q * 4) * kPitch + tile * 32 + g * 16 + j * 4;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) r[i] = *reinterpret_cast<const unsigned*>(from + i * kPitch);
-          transposed(r, o);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) w[k][2 * g + t] = o[k];
-        }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int dl = 4 * j + k;
-        u32x4* const dst = reinterpret_cast<u32x4*>(out + (half * kTiles + tile) * 1024 +
-                                                    (BITS == 8 ? dl * 64 + q * 16 : (q * 16 + dl) * 16));
-        if (!whole) {
-          const u32x4 was = *dst;
-#pragma unroll
-          for (int m = 0; m < 4; ++m) {
-            unsigned kept = was[m];
-            if constexpr (BITS == 8)
-              if (grown) kept = (codes_again(kept, old_scale, scale) & is_old[m & 1]) | (kept & ~is_old[m & 1]);
-            w[k][m] = (w[k][m] & is_new[m & 1]) | (kept & ~is_new[m & 1]);
+        const int e = exponent_of<4>(best);
+        const unsigned w = codes4(y, power_of_two(e));
+        if (token_of(t) < count) {
+          const int group = d0 >> 5, t2 = (slot >> 4) & 1, t16 = slot & 15;
+          if constexpr (VALUE)
+            *reinterpret_cast<unsigned*>(s_codes + slot * kPitch + (d0 >> 1)) = w;
+          else
+            *reinterpret_cast<unsigned*>(out + (slot >> 5) * 16 * D + (t2 * (D / 32) + group) * 256 + t16 * 16 +
+                                         ((d0 & 31) >> 1)) = w;
+          if ((l & 3) == 0) {
+            const int byte = VALUE     ? group * 32 + (t16 >> 2) * 8 + t2 * 4 + (t16 & 3)
+                             : D == 64 ? (t2 * 2 + group) * 16 + t16
+                                       : ((group & 3) * 16 + t16) * (D / 64) + (group >> 2) * 2 + t2;
+            scales[(slot >> 5) * 2 * D + byte] = nan ? 255 : (uint8_t)(e + 127);
           }
         }
-        *dst = w[k];
       }
+      if (MANY && h + 1 < h1) load(h + 1);
     }
-    if (MANY && h + 1 < h1) __syncthreads();  // (the next head's codes take the array)
-  }
+    if constexpr (VALUE) {
+      __syncthreads();
+      const int half0 = grown ? 0 : first >> 5, half1 = (first + count - 1) >> 5;
+      constexpr int kTiles = kBytes / 32;  // KiB of codes of 32 tokens
+      for (int u = tid; u < (half1 - half0 + 1) * kTiles * 16; u += 64 * WAVES) {
+        const int j = u & 3, q = (u >> 2) & 3, tile = (u >> 4) % kTiles, half = half0 + (u >> 4) / kTiles;
+        // bytes of the tokens 16 t + 4 q + 0 .. 3 that are new, and that are rounded again
+        unsigned is_new[2] = {0, 0}, is_old[2] = {0, 0};
+  #pragma unroll
+        for (int t = 0; t < 2; ++t)
+  #pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int slot = half * 32 + t * 16 + q * 4 + i;
+            if (slot >= first && slot < first + count) is_new[t] |= 0xffu << (8 * i);
+            if (grown && slot < first) is_old[t] |= 0xffu << (8 * i);
+          }
+        if ((is_new[0] | is_new[1] | is_old[0] | is_old[1]) == 0) continue;
+        const bool whole = (is_new[0] & is_new[1]) == 0xffffffffu;
+        u32x4 w[4];
+  #pragma unroll
+        for (int g = 0; g < 2; ++g)
+  #pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            unsigned r[4], o[4];
+            const char* const from = s_codes + (half * 32 + t * 16 + q * 4) * kPitch + tile * 32 + g * 16 + j * 4;
+  #pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = *reinterpret_cast<const unsigned*>(from + i * kPitch);
+            transposed(r, o);
+  #pragma unroll
+            for (int k = 0; k < 4; ++k) w[k][2 * g + t] = o[k];
+          }
+  #pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int dl = 4 * j + k;
+          u32x4* const dst = reinterpret_cast<u32x4*>(out + (half * kTiles + tile) * 1024 +
+                                                      (BITS == 8 ? dl * 64 + q * 16 : (q * 16 + dl) * 16));
+          if (!whole) {
+            const u32x4 was = *dst;
+  #pragma unroll
+            for (int m = 0; m < 4; ++m) {
+              unsigned kept = was[m];
+              if constexpr (BITS == 8)
+                if (grown) kept = (codes_again(kept, old_scale, scale) & is_old[m & 1]) | (kept & ~is_old[m & 1]);
+              w[k][m] = (w[k][m] & is_new[m & 1]) | (kept & ~is_new[m & 1]);
+            }
+          }
+          *dst = w[k];
+        }
+      }
+      if (MANY && h + 1 < h1) __syncthreads();  // (the next head's codes take the array)
+    }
   } while (MANY && ++h < h1);
 }
 

@@ -28,6 +28,8 @@ void scales_of(const KarpoCache& c, CacheRef* ref) { ref->scales = c.scales; }
 void scales_of(const KarpoCache4& c, CacheRef* ref) { ref->scales4 = static_cast<uint8_t*>(c.scales); }
 uintptr_t scale_alignment(const KarpoCache&) { return 8; }
 uintptr_t scale_alignment(const KarpoCache4&) { return 16; }
+bool in_4_bits(const KarpoCache&) { return false; }
+bool in_4_bits(const KarpoCache4&) { return true; }
 
 template <class Cache>
 int check_cache(const Cache& c, CacheRef* ref) {
@@ -339,6 +341,9 @@ int check_attend(const Args* a, CacheRef* c, CacheRows* r) {
 //   8 heads of 256: one request, 256 vectors 210, 134; 1,024 vectors 443, 474; 16 requests, 128 vectors 119, 88; 256 143, 149
 //   4 heads of 512: one request, 512 vectors 284, 282; 1,024 vectors 436, 542; 16 requests, 512 vectors 251, 280
 //   one request of 2,000 tokens: 16 heads of 128, 1,024 vectors 62, 52; 8 of 256, 71, 54; 4 of 512, 78, 56
+// In 4 bits a walk takes a tenth less and the unpacking a third (of 144 shapes the choice is nowhere over 10% slower):
+//   one request of 32,768 tokens: 16 heads of 128, 128 vectors 173, 76; 1,024 452, 410; 8 of 256, 256 vectors 202, 146; 1,024 420,
+//   498; 4 of 512, 512 vectors 283, 302; 16 requests of 2,048: 16 of 128, 512 vectors 272, 259; 8 of 256, 512 vectors 225, 354
 template <class Args>
 bool split(const Args* a) {
   const int d = a->cache.head_dim;
@@ -351,8 +356,10 @@ bool split(const Args* a) {
   const double query_tiles = a->n_seq * ceil(vectors / 128) * a->cache.kv_heads;
   const double most = d == 512 ? 0.8e9 : 1.3e9, few = 0.35e9 + 0.5e6 * vectors;  // operations a microsecond
   const double rate = a->n_seq <= 2 && query_tiles < 256 && few < most ? few : most;
-  const double by_split = 17 + keys * (walk * ceil(vectors / tile) + (a->n_seq > 1 ? 3e-5 : 0));
-  const double unpacked = 33 + keys * d * 0.9e-6 + 4 * vectors * keys * d / rate;
+  const bool four = in_4_bits(a->cache);
+  const double by_split = 17 + keys * (four ? 0.9 * walk * ceil(vectors / tile)
+                                            : walk * ceil(vectors / tile) + (a->n_seq > 1 ? 3e-5 : 0));
+  const double unpacked = 33 + keys * d * (four ? 0.6e-6 : 0.9e-6) + 4 * vectors * keys * d / rate;
   return by_split <= unpacked;
 }
 

@@ -109,7 +109,7 @@ class Step(NamedTuple):
 def create(blocks: int, kv_heads: int, head_dim: int, block_size: int = 64,
            device: torch.device | str = "cuda", bits: int = 8) -> Cache:
     """An empty cache of ``blocks`` blocks, in 8 or 4 bits (an element is up to 2^-4 of its magnitude off in 8 bits; in 4, up to
-    a quarter, or a 24th of the largest of its 32 elements: 12% of the 2-norm for normally distributed ones)."""
+    a quarter, or a twelfth of the largest of its 32 elements: 12% of the 2-norm for normally distributed ones)."""
     if block_size not in BLOCK_SIZES:
         raise ValueError(f"block_size must be 32, 64 or 128, not {block_size}")
     if head_dim not in HEAD_DIMS:
@@ -259,47 +259,61 @@ def reserve(table: Tensor, lengths: Tensor, counts: Tensor, free: Tensor, free_c
     return Step(q_cu, new, slots.view(torch.int64), positions, writes.view(jobs, 4), left, status)
 
 
-def _norm_fields(name: str, norm: Norm | None, key: Tensor, keep: list) -> tuple[int, float, int]:
+def _table_address(t: Tensor, index: int) -> int:
+    """The address of a weight or table that is as the kernel takes it, or 0."""
+    at = t.data_ptr()
+    return at if t.dtype is torch.bfloat16 and t.get_device() == index and t.is_contiguous() and not at & 15 else 0
+
+
+def _norm_fields(name: str, norm: Norm | None, key: Tensor, index: int, head_dim: int, keep: list) -> tuple[int, float, int]:
     """(mode, eps, weight's pointer) of one of ``append``'s norms."""
     if norm is None or norm.mode == NORM_NONE:
         return 0, 0.0, 0
-    weight = norm.weight if norm.mode in (NORM_WEIGHT, NORM_ONE_PLUS) else None
-    if weight is None:
-        if norm.mode in (NORM_WEIGHT, NORM_ONE_PLUS):
-            raise ValueError(f"{name}: this norm has a weight of shape ({key.shape[2]},), not None")
-        return norm.mode, norm.eps, 0
-    if weight.shape != key.shape[2:]:
-        raise ValueError(f"{name}'s weight must have shape ({key.shape[2]},), not {tuple(weight.shape)}")
-    weight = _bf16_table(weight, key.device)
-    keep.append(weight)
-    return norm.mode, norm.eps, weight.data_ptr()
+    mode, weight = norm.mode, norm.weight
+    if mode != NORM_WEIGHT and mode != NORM_ONE_PLUS:
+        return mode, norm.eps, 0
+    if weight is None or weight.shape != (head_dim,):
+        raise ValueError(f"{name}'s weight must have shape ({head_dim},), not {None if weight is None else tuple(weight.shape)}")
+    at = _table_address(weight, index)
+    if not at:
+        keep.append(_bf16_table(weight, key.device))
+        at = keep[-1].data_ptr()
+    return mode, norm.eps, at
 
 
-def _rope_fields(rope: tuple[Tensor, Tensor] | None, positions: Tensor | None, key: Tensor, keep: list) -> tuple[int, ...]:
+def _rope_fields(rope: tuple[Tensor, Tensor] | None, positions: Tensor | None, key: Tensor, index: int, head_dim: int,
+                 keep: list) -> tuple[int, ...]:
     """(cos, sin, stride, rows, rotated elements, positions) of ``append``'s rotation."""
     if rope is None:
         if positions is not None:
             raise ValueError("positions are rows of the rope tables: pass rope=(cos, sin) with them")
         return 0, 0, 0, 0, 0, 0
-    cos, sin = (_bf16_table(t, key.device) for t in rope)
-    rows, index = key.shape[0], key.get_device()
-    if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[0] < 1 or cos.shape[1] % 32 or not 0 < cos.shape[1] <= key.shape[2]:
+    cos, sin = rope
+    shape = cos.shape
+    if len(shape) == 2 and _table_address(cos, index) and _table_address(sin, index):
+        stride = shape[1]
+    else:
+        cos, sin = (_bf16_table(t, key.device) for t in rope)
+        shape = cos.shape
+        if len(shape) == 2:
+            stride = cos.stride(0)
+            if stride != sin.stride(0) or stride < shape[1] or shape[0] == 1:
+                cos, sin, stride = cos.contiguous(), sin.contiguous(), shape[1]
+        keep += (cos, sin)
+    if len(shape) != 2 or sin.shape != shape or shape[0] < 1 or shape[1] % 32 or not 0 < shape[1] <= head_dim:
         raise ValueError(f"rope tables must be two (positions, rotated) tables of one shape, rotated a multiple of 32 up to "
-                         f"{key.shape[2]}, not {tuple(cos.shape)} and {tuple(sin.shape)}")
-    if cos.stride(0) != sin.stride(0) or cos.stride(0) < cos.shape[1]:
-        cos, sin = cos.contiguous(), sin.contiguous()
-    keep += (cos, sin)
-    at = 0
+                         f"{head_dim}, not {tuple(shape)} and {tuple(sin.shape)}")
+    at, rows = 0, key.shape[0]
     if positions is None:
-        if cos.shape[0] < rows:
-            raise ValueError(f"without positions the rope tables need a row for each of {rows} rows, not {cos.shape[0]}")
+        if shape[0] < rows:
+            raise ValueError(f"without positions the rope tables need a row for each of {rows} rows, not {shape[0]}")
     else:
         if not _ints(positions, index):
             _check_ints(index, positions=positions)
-        if positions.shape[0] != rows:
-            raise ValueError(f"positions must hold a number for each of {rows} rows, not {positions.shape[0]}")
+        if positions.numel() != rows:
+            raise ValueError(f"positions must hold a number for each of {rows} rows, not {positions.numel()}")
         at = positions.data_ptr()
-    return cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0], cos.shape[1], at
+    return cos.data_ptr(), sin.data_ptr(), stride, shape[0], shape[1], at
 
 
 def append(cache: Cache, key: Tensor, value: Tensor, writes: Tensor, *, k_norm: Norm | None = None, v_norm: Norm | None = None,
@@ -337,11 +351,11 @@ def append(cache: Cache, key: Tensor, value: Tensor, writes: Tensor, *, k_norm: 
         with _on_device(index):
             _lib.check(_lib.load().karpo_cache_append(_APPEND.pack(*call), _current_stream(index)), "append")
         return
-    extra = [n.weight for n in (k_norm, v_norm) if n is not None and n.weight is not None] + list(rope or ())
-    _no_grad("append", *extra)
+    _no_grad("append", *(n.weight for n in (k_norm, v_norm) if n is not None and n.weight is not None), *(rope or ()))
     keep: list[Tensor] = []  # (converted tables go back to the stream-ordered allocator after the launch)
-    args = (*call, *_norm_fields("k_norm", k_norm, key, keep), *_norm_fields("v_norm", v_norm, key, keep),
-            *_rope_fields(rope, positions, key, keep))
+    args = (*call, *_norm_fields("k_norm", k_norm, key, index, head_dim, keep),
+            *_norm_fields("v_norm", v_norm, key, index, head_dim, keep),
+            *_rope_fields(rope, positions, key, index, head_dim, keep))
     _on_gpu("append", index)
     lib = _lib.load()
     with _on_device(index):

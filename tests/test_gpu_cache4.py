@@ -275,6 +275,14 @@ def test_many_requests(gpu):
     check_attend(gpu, 64, 4, 2, 32, lengths[:-1] + [1500], [1 + (i % 3 == 0) for i in range(600)], SPLIT, total_keys=False)
 
 
+@pytest.mark.parametrize("head_dim,kv_heads,requests,more", [(64, 2, 70, 1), (128, 3, 48, 4), (256, 1, 130, 1), (512, 4, 33, 3)])
+def test_long_walks_of_many_requests(gpu, head_dim, kv_heads, requests, more):
+    """Workgroups that take up to 1,024 tokens whole."""
+    lengths = [(337 * i) % 1025 for i in range(requests - 1)] + [1024]
+    counts = [i % (more + 1) for i in range(requests - 1)] + [more]
+    check_attend(gpu, head_dim, 2 * kv_heads, kv_heads, 64, lengths, counts, WHOLE, total_keys=False)
+
+
 @pytest.mark.parametrize("head_dim,kv_heads", [(64, 2), (128, 2), (256, 1), (512, 1)])
 def test_one_long_request(gpu, head_dim, kv_heads):
     check_attend(gpu, head_dim, 4, kv_heads, 64, [9001], [1], SPLIT)
