@@ -13,7 +13,7 @@ import math
 import pytest
 import torch
 
-from cache4_cases import copy_of, ints, random_cache, raw, values_of
+from cache4_cases import close, copy_of, ints, random_cache, raw, values_of
 from karpo_decision_amd import kv_cache, ops
 from oracle import cache as oracle8
 from oracle import cache4 as oracle
@@ -329,3 +329,100 @@ def test_near_norm_rope_and_a_plain_append(gpu, bits):
             most = torch.maximum(a.abs(), b.abs()).view(64, 2, 4, 32).amax(-1, keepdim=True).expand(-1, -1, -1, 32).reshape(a.shape)
             half = torch.maximum(torch.maximum(a.abs(), b.abs()) / 4, most / 6)
         assert ((a - b).abs() <= 2 * half + 2.0 ** -7 * size).all()
+
+
+# ---- as they are used together
+
+class _Server:
+    """Four requests over a cache, their table, lengths and free list; ``round`` is one step of one layer."""
+
+    def __init__(self, device, bits, heads, kv_heads, d, block, tables, norms):
+        self.cache = kv_cache.create(24, kv_heads, d, block, device=device, bits=bits)
+        self.heads, self.tables, self.norms = heads, tables, norms
+        self.table = torch.full((4, 8), -1, dtype=torch.int32, device=device)
+        self.lengths = torch.zeros(4, dtype=torch.int32, device=device)
+        self.free, self.left = torch.arange(24, dtype=torch.int32, device=device), ints([24], device)
+
+    def round(self, counts, rows, most, query, key, value):
+        """(step, out, the queries as the attention takes them)"""
+        step = kv_cache.reserve(self.table, self.lengths, counts, self.free, self.left, rows, self.cache.block_size)
+        kv_cache.append(self.cache, key, value, step.writes, k_norm=self.norms[1], v_norm=self.norms[2], rope=self.tables,
+                        positions=step.positions)
+        at = step.positions.long()
+        turned = ops.norm_rope(query, self.norms[0], tuple(t[at] for t in self.tables))
+        out = kv_cache.attend(turned, self.cache, self.table, step.q_cu, step.lengths, most, 0.1)
+        self.lengths.copy_(step.lengths)
+        self.left.copy_(step.free_left)
+        return step, out, turned
+
+
+def _server(device, bits, heads, kv_heads, d, block, rotated):
+    gen = torch.Generator().manual_seed(3)
+    norms = [_norm(kind, d, device, gen) for kind in ("one_plus", "one_plus", "plain")]
+    return _Server(device, bits, heads, kv_heads, d, block, _tables(200, rotated, gen, device), norms)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("heads,kv_heads,d,block,rotated", [(4, 2, 64, 32, 64), (16, 2, 128, 64, 64), (2, 1, 256, 128, 256)])
+def test_rounds_of_a_server(gpu, bits, heads, kv_heads, d, block, rotated):
+    """Prompts, then tokens one by one and a few at a time. Each round's new rows in the cache are, bit for bit, those of a second
+    cache that gets them with their own tables' rows, and its outputs those of the rows that ``read`` finds."""
+    rounds = [[40, 7, 0, 65], [1, 1, 1, 1], [1, 1, 30, 0], [3, 2, 3, 1], [1, 1, 1, 1]]
+    gen = torch.Generator(device=gpu).manual_seed(4)
+    server = _server(gpu, bits, heads, kv_heads, d, block, rotated)
+    twin = copy_of(server.cache)
+    had = [0] * 4
+    with torch.inference_mode():
+        for counts in rounds:
+            n = sum(counts)
+            query = torch.randn((n, heads, d), generator=gen, device=gpu).bfloat16()
+            key, value = (torch.randn((n, kv_heads, d), generator=gen, device=gpu).bfloat16() for _ in range(2))
+            step, out, turned = server.round(ints(counts, gpu), n, max(counts), query, key, value)
+            step.check()
+            at = [p for h, c in zip(had, counts) for p in range(h, h + c)]
+            had = [h + c for h, c in zip(had, counts)]
+            assert step.lengths.tolist() == had
+            kv_cache.append(twin, key, value, step.writes, k_norm=server.norms[1], v_norm=server.norms[2],
+                            rope=tuple(t[at] for t in server.tables))
+            for a, b in zip(server.cache[:3], twin[:3]):
+                assert torch.equal(raw(a), raw(b))
+            keys, values, k_cu = (t.tolist() if i == 2 else t.cpu().double() for i, t in enumerate(
+                kv_cache.read(server.cache, server.table, step.lengths, sum(had))))
+            q_cu = step.q_cu.tolist()
+            for i in range(4):
+                close(out[q_cu[i]:q_cu[i + 1]], turned[q_cu[i]:q_cu[i + 1]], keys[k_cu[i]:k_cu[i + 1]],
+                      values[k_cu[i]:k_cu[i + 1]], 0.1, weights=2.0 ** -8 if bits == 8 else 0.0)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_a_captured_round_goes_on_from_replay_to_replay(gpu, bits):
+    """A captured step of one token each, its lengths and free list carried on by itself, against eager steps."""
+    gen = torch.Generator(device=gpu).manual_seed(5)
+    heads, kv_heads, d, block = 8, 2, 128, 32
+    captured, eager = (_server(gpu, bits, heads, kv_heads, d, block, 128) for _ in range(2))
+
+    def rows(n):
+        return (torch.randn((n, heads, d), generator=gen, device=gpu).bfloat16(),
+                *(torch.randn((n, kv_heads, d), generator=gen, device=gpu).bfloat16() for _ in range(2)))
+
+    with torch.inference_mode():
+        prompt, ones = rows(90), ints([1] * 4, gpu)
+        for s in (captured, eager):
+            s.round(ints([31, 0, 32, 27], gpu), 90, 32, *prompt)
+        fixed = rows(4)
+        # (a first call outside the graph, over another server)
+        _server(gpu, bits, heads, kv_heads, d, block, 128).round(ones, 4, 1, *fixed)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step, out, _ = captured.round(ones, 4, 1, *fixed)
+        for i in range(5):
+            for a, b in zip(fixed, rows(4)):
+                a.copy_(b)
+            graph.replay()
+            want_step, want, _ = eager.round(ones, 4, 1, *fixed)
+            torch.cuda.synchronize()
+            want_step.check()
+            assert torch.equal(out, want) and torch.equal(step.lengths, want_step.lengths), i
+            for a, b in zip(captured.cache[:3], eager.cache[:3]):
+                assert torch.equal(raw(a), raw(b)), i
