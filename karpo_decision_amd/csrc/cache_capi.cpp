@@ -41,7 +41,9 @@ int check_cache(const Cache& c, CacheRef* ref) {
   if (!aligned(c.keys, 16) || !aligned(c.values, 16) || !aligned(c.scales, scale_alignment(c))) return KARPO_ATTN_ERR_LAYOUT;
   ref->keys = static_cast<uint8_t*>(c.keys);
   ref->values = static_cast<uint8_t*>(c.values);
-  scales_of(c, ref);
+  ref->scales = nullptr;
+  ref->scales4 = nullptr;
+  scales_of(c, ref);  // (one of them; which one there is, is what tells the formats apart)
   ref->blocks = c.blocks;
   ref->kv_heads = c.kv_heads;
   ref->head_dim = c.head_dim;

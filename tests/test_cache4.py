@@ -270,3 +270,19 @@ def test_c_abi_calls_without_rows_launch_nothing():
     assert lib.karpo_cache4_attend(ctypes.byref(b), None) == 0
     for fn in (lib.karpo_cache4_append, lib.karpo_cache4_read, lib.karpo_cache4_attend, lib.karpo_cache_append_rope):
         assert fn(None, None) == 1
+
+
+def test_workspaces_go_by_the_format_of_the_call_alone():
+    """80 requests of 1,000 tokens are split in 8 bits and taken whole in 4; what a call of the other format before it left on the
+    stack changes neither."""
+    lib, more = _lib.load(), (4096, 4096, 128, 64, 128, 64, 4096, 4096, 4096, 32, 32, 80, 4, 1, 80, 1000, 0.1, -1, 0)
+    eight = _lib.KarpoCacheAttendArgs(_lib.KarpoCache(0x100000, 0x200000, 0x300000, 4, 2, 64, 32), *more)
+    four = _lib.KarpoCache4AttendArgs(_c_cache(), *more)
+    got = []
+    for _ in range(4):
+        for fn, a in ((lib.karpo_cache_attend_workspace_bytes, eight), (lib.karpo_cache4_attend_workspace_bytes, four)):
+            need = ctypes.c_size_t()
+            assert fn(ctypes.byref(a), ctypes.byref(need)) == 0
+            a.workspace, a.workspace_bytes = 4096, need.value
+            got.append(need.value)
+    assert got == got[:2] * 4 and got[0] > 0 and got[1] == 0
