@@ -70,8 +70,7 @@ struct AppendRowsParams {
   int32_t rope_dim;
   const int32_t* positions;  // each row's row of the tables, or null: its own
   int64_t n_writes;
-  int32_t many;        // the rows are more than the L2 caches hold
-  int32_t heads_each;  // then: heads that a workgroup takes, one after the other (the launch's)
+  int32_t heads_each;  // heads that a workgroup takes, one after the other (the launch's)
 };
 hipError_t launch_cache_append_rows(const AppendRowsParams& p, hipStream_t stream);
 

@@ -397,6 +397,9 @@ __global__ __launch_bounds__(64 * WAVES) void append_rows_kernel(const AppendRow
   if (wr.count <= kStep) run(std::integral_constant<int, 1>()); else run(std::integral_constant<int, PASSES>());
 }
 
+// Passes of a workgroup, whose loads are all in flight at once. With 2 (twice the waves) one token of 48 requests, 16 heads of 128:
+// 8.7 against 6.6 us, 2,500 tokens of 24 requests, 8 heads of 256: 19.5 against 14.3, 32,768 tokens of 16 heads of 128: 89.7
+// against 93.2.
 constexpr int kMostPasses = 4;
 
 template <int D, int BITS>
@@ -404,13 +407,18 @@ hipError_t launch(const AppendRowsParams& p, hipStream_t stream) {
   auto run = [&](auto blocks) {
     constexpr int kBlock = decltype(blocks)::value, kPieces = D * kBlock / 512;  // of 64 lanes x 8 elements
     constexpr int kWaves = kPieces <= 16 * kMostPasses ? kPieces / kMostPasses : 16, kPasses = kPieces / kWaves;
-    // many rows: up to eight heads a workgroup while there are four workgroups a CU (blocks of 64 Ki elements would spill)
+    // Many rows (over 96 MiB of keys and values: as many as come from HBM): up to eight heads a workgroup, which then load their
+    // tokens' cos and sin once, while there are four workgroups a CU, and the rows past the caches. us with it, without, rotated, in
+    // 8 bits, 16 heads of 128: 64 MiB 29.8, 27.3; 128 MiB 50.6, 57.0; 256 MiB 96.5, 107; 8 of 256: 64 MiB 37.9, 31.5; 128 MiB 61.2,
+    // 66.8; 256 MiB 99.5, 123; in 4 bits (and read back) 16 of 128: 128 MiB 76.3, 87.2; 4 of 512: 64 MiB 57.5, 53.7; 128 MiB 94.0,
+    // 99.5. Not of head size 512 in 8 bits (4 heads: 128 MiB 112, 90.5; 256 MiB 176, 174), and blocks of 64 Ki elements would spill.
+    constexpr bool kMany = kPasses <= kMostPasses && !(BITS == 8 && D == 512);
     AppendRowsParams q = p;
     q.heads_each = 1;
-    const bool many = p.many && kPasses <= kMostPasses;
+    const bool many = kMany && 4 * p.a.rows * p.a.c.kv_heads * D > (int64_t)96 << 20;
     while (many && q.heads_each < 8 && p.n_writes * p.a.c.kv_heads >= 1024 * q.heads_each) q.heads_each *= 2;
     const dim3 grid((unsigned)(p.n_writes * 2 * ((p.a.c.kv_heads + q.heads_each - 1) / q.heads_each)));
-    if constexpr (kPasses <= kMostPasses) {
+    if constexpr (kMany) {
       if (many) {
         append_rows_kernel<D, kBlock, kPasses, kWaves, BITS, true><<<grid, dim3(64 * kWaves), 0, stream>>>(q);
         return;

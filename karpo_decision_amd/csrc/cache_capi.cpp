@@ -207,7 +207,6 @@ int append_rows(const Args* a, const KarpoCachePrologue& f, void* stream) {
   st = prologue_params(f, a->cache.head_dim, &p);
   if (st != KARPO_ATTN_OK || none) return st;
   p.n_writes = a->n_writes;
-  p.many = 4 * a->rows * a->cache.kv_heads * a->cache.head_dim > kL2Bytes;
   if (launch_cache_append_rows(p, static_cast<hipStream_t>(stream)) != hipSuccess) return KARPO_ATTN_ERR_LAUNCH;
   return KARPO_ATTN_OK;
 }

@@ -273,20 +273,20 @@ def test_a_captured_append_reads_its_inputs_at_each_replay(gpu, bits):
 @pytest.mark.parametrize("d,kv_heads,block,rope", [(64, 13, 64, True), (128, 6, 128, True), (256, 3, 32, False), (512, 9, 64, True),
                                                    (512, 4, 128, True)])
 def test_many_rows_at_once_and_in_pieces(gpu, bits, d, kv_heads, block, rope):
-    """More rows than the L2 caches hold, where a workgroup takes several heads: the same bits as in calls of few blocks each, which
+    """Over 96 MiB of rows, where a workgroup takes several heads: the same bits as in calls of few blocks each, which
     the other tests compare with the formulas. Ragged writes, some of one token."""
     gen = torch.Generator().manual_seed(11)
-    blocks = -(-(36 << 20) // (4 * kv_heads * d * block))
+    blocks = -(-(104 << 20) // (4 * kv_heads * d * block))
     counts = torch.randint(block - 3, block + 1, (blocks,), generator=gen)
     counts[::9] = 1
     firsts = torch.minimum(torch.randint(0, 4, (blocks,), generator=gen), block - counts)
     starts = torch.cumsum(counts, 0) - counts
     ids = torch.randperm(blocks, generator=gen)
     writes = torch.stack((ids, firsts, starts, counts), 1).int().to(gpu)
-    rows = -(-(33 << 20) // (4 * kv_heads * d))
+    rows = -(-(97 << 20) // (4 * kv_heads * d))
     rows = max(rows, int(counts.sum()))
     key, value = (torch.randn((rows, kv_heads, d), generator=gen).bfloat16().to(gpu) for _ in range(2))
-    assert 4 * rows * kv_heads * d > 32 << 20
+    assert 4 * rows * kv_heads * d > 96 << 20
     tables = _tables(500, d, gen, gpu) if rope else None
     positions = torch.randint(0, 500, (rows,), generator=gen, dtype=torch.int32).to(gpu) if rope else None
     norm = _norm("weight", d, gpu, gen)
@@ -297,7 +297,7 @@ def test_many_rows_at_once_and_in_pieces(gpu, bits, d, kv_heads, block, rope):
             part = writes[i:i + 8].clone()
             a, b = int(part[0, 2]), int(part[-1, 2] + part[-1, 3])
             part[:, 2] -= a
-            assert 4 * (b - a) * kv_heads * d <= 32 << 20
+            assert 4 * (b - a) * kv_heads * d <= 96 << 20
             kv_cache.append(two, key[a:b], value[a:b], part, k_norm=norm, v_norm=norm, rope=tables,
                             positions=None if positions is None else positions[a:b])
     for a, b in zip(one[:3], two[:3]):
