@@ -428,7 +428,9 @@ __device__ __forceinline__ void read_values4(const uint8_t* codes, const uint8_t
 // lengths by itself and takes an equal share of all groups. Bound by HBM: 32,768 rows of 16 heads at 128 72 us, 5.6 TB/s; 9,244
 // rows of 4 heads at 512 19.8 us, 5.7 TB/s (112 and 36.6 us with 8-byte stores of the values and a head a workgroup).
 //
-// In 4 bits (read_rows4) a unit is 2 KiB of codes, out of which go 8 KiB of rows.
+// In 4 bits (read_keys4, read_values4) a unit is 2 KiB of codes, out of which go 8 KiB of rows, keys through LDS too: a row's 128
+// bytes are of four lanes' operands. 32,768 rows of 16 heads at 128 51 us (339 MB, 6.7 TB/s; 56 with keys stored 16 bytes here and
+// there, straight from the operands), 6,762 of 4 at 512 14.5 us (70 MB).
 template <int D, bool STREAM, int BITS>
 __global__ __launch_bounds__(64 * kReadWaves) void read_kernel(const ReadParams p) {
   constexpr int kThreads = 64 * kReadWaves, kTiles = D * BITS / 256;

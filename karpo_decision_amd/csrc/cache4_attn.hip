@@ -86,6 +86,7 @@ struct Line {
     return unit < longer ? (int)((unsigned)unit / (unsigned)(each + 1)) : more + (int)((unsigned)(unit - longer) / (unsigned)each);
   }
 };
+// 48 requests, 16 heads of 128: kStart4 of 8, 12, 16, 24 groups 40.0, 37.6, 37.1, 38.2 us. kTries: lengths of pieces that are tried.
 constexpr int kStart4 = 16, kTries = 5;
 
 // As in the kernel over 8 bits: S^T = K Q^T with keys as rows, a lane's eight weights (keys 16 t + 4 (lane / 16) + i of column
@@ -99,6 +100,11 @@ constexpr int kStart4 = 16, kTries = 5;
 // and tokens are what the second product sums over, so values become bf16 in registers: two elements of a token a conversion,
 // two tokens' of an element a permutation. Of head size 64 a lane's operand holds two tiles of 16 tokens, and the queries fill
 // its one half or the other.
+//
+// Bound by HBM: one request of 131,073 tokens, 32 / 4 heads of 512, 55 us for 285 MB (5.2 TB/s; the walk itself at 6 to 7, its start
+// and end take 5 to 7 us together), 48 requests of 68,664 together, 32 / 16 of 128, 37 us for 150 MB, of which the start, the changes
+// from request to request (2 us each) and the unequal ends are 14. The matrix units are busy for 19 and 15% of that. Deeper rings,
+// groups of 64 tokens and four waves a SIMD at head size 128 (42.3 against 40.1 us) were no faster.
 //
 // ONCE: one workgroup reads a request's codes of a head, once; they are streamed through the caches.
 template <int D, int NT, bool ONCE>
@@ -608,7 +614,8 @@ __global__ __launch_bounds__(kAttendThreads, attend4_waves(D, NT)) void attend4_
 // Joins a request's shares: O = sum of 2^(m_w - M) O_w over sum of 2^(m_w - M) l_w, in an order that the sizes alone set.
 // Requests that one workgroup took whole are done already. Up to kFew shares: a thread walks them for four elements of a
 // vector. More: 64 elements of a vector by 16 threads of four and 16 rows, each row with every sixteenth share, and the rows
-// joined through LDS.
+// joined through LDS. A launch and three rounds of dependent loads bound it: 48 requests, 32 heads of 128, 4.1 us; one request
+// over 256 shares, 32 heads of 512, 4.7.
 template <int D>
 __global__ __launch_bounds__(256) void join4_kernel(const AttendParams p, int vectors_per) {
   constexpr int kSlabs = D / 64, kFew = 4;
