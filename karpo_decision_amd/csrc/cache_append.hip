@@ -97,7 +97,7 @@ struct Write {
 // 4 bytes four times: four 16-byte pieces of the cache. Lanes past the write take its last token again and store nothing, so
 // that loads need no branches and all passes' are in flight at once.
 //
-// Many rows are bound by HBM: 32,768 of 16 heads of 128, normed and rotated, 94 us in 8 bits (402 MB and 17 MB of tables, 4.5 TB/s;
+// Many rows are bound by HBM: 32,768 of 16 heads of 128, normed and rotated, 90 us in 8 bits (402 MB and 17 MB of tables, 4.7 TB/s;
 // 145 with loads pass by pass and one head a workgroup) and 78 us in 4 (356 MB); few by three rounds of dependent loads (the write,
 // its rows and positions, cos and sin) and the joins over the workgroup: one token of 48 requests 6.7 us, 2,500 tokens of 24
 // requests, 8 heads of 256, 14.4. Of that document's 134 million codes 62 are another than the 64-bit row's (133 where each step
@@ -379,8 +379,9 @@ __device__ __forceinline__ void append_rows(const AppendRowsParams& p, const Wri
   } while (MANY && ++h < h1);
 }
 
+// (three waves a SIMD where one walks heads over 8 bits: without the bound two, and a document of 16 heads of 128 93.8 us, not 89.6)
 template <int D, int BLOCK, int PASSES, int WAVES, int BITS, bool MANY>
-__global__ __launch_bounds__(64 * WAVES) void append_rows_kernel(const AppendRowsParams p) {
+__global__ __launch_bounds__(64 * WAVES, MANY && BITS == 8 ? 3 : 1) void append_rows_kernel(const AppendRowsParams p) {
   constexpr int kStep = 512 / D * WAVES;  // tokens of a pass
   __shared__ __align__(16) char s_codes[BLOCK * ((BITS == 8 ? D : D / 2) + 16)];
   const int heads = p.a.c.kv_heads, groups = (heads + p.heads_each - 1) / p.heads_each;  // (of heads)
@@ -415,10 +416,11 @@ hipError_t launch(const AppendRowsParams& p, hipStream_t stream) {
     constexpr int kWaves = kPieces <= 16 * kMostPasses ? kPieces / kMostPasses : 16, kPasses = kPieces / kWaves;
     // Many rows (over 96 MiB of keys and values: as many as come from HBM): up to eight heads a workgroup, which then load their
     // tokens' cos and sin once, while there are four workgroups a CU, and the rows past the caches. us with it, without, rotated, in
-    // 8 bits, 16 heads of 128: 64 MiB 29.8, 27.3; 128 MiB 50.6, 57.0; 256 MiB 96.5, 107; 8 of 256: 64 MiB 37.9, 31.5; 128 MiB 61.2,
-    // 66.8; 256 MiB 99.5, 123; in 4 bits (and read back) 16 of 128: 128 MiB 76.3, 87.2; 4 of 512: 64 MiB 57.5, 53.7; 128 MiB 94.0,
-    // 99.5. Not of head size 512 in 8 bits (4 heads: 128 MiB 112, 90.5; 256 MiB 176, 174), and blocks of 64 Ki elements would spill.
-    constexpr bool kMany = kPasses <= kMostPasses && !(BITS == 8 && D == 512);
+    // 8 bits, 16 heads of 128: 64 MiB 29.8, 27.3; 128 MiB 52.0, 58.9; 256 MiB 84.4, 106; 8 of 256: 64 MiB 37.9, 31.5; 128 MiB 64.5,
+    // 67.2; 256 MiB 104, 124; 4 of 512 in blocks of 32: 128 MiB 62.2, 94.9; in 4 bits (and read back) 16 of 128: 128 MiB 76.3, 87.2;
+    // 4 of 512: 64 MiB 57.5, 53.7; 128 MiB 94.0, 99.5. Not where sixteen waves leave too few registers for it: blocks of 32 Ki
+    // elements in 8 bits (8 heads of 256, blocks of 128: 128 MiB 110, 79.8; 4 of 512, blocks of 64: 112, 93.1), of 64 Ki in both.
+    constexpr bool kMany = kPasses <= kMostPasses && !(BITS == 8 && kWaves == 16);
     AppendRowsParams q = p;
     q.heads_each = 1;
     const bool many = kMany && 4 * p.a.rows * p.a.c.kv_heads * D > (int64_t)96 << 20;

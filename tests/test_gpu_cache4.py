@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import os
 
 import pytest
 import torch
@@ -281,6 +282,28 @@ def test_long_walks_of_many_requests(gpu, head_dim, kv_heads, requests, more):
     lengths = [(337 * i) % 1025 for i in range(requests - 1)] + [1024]
     counts = [i % (more + 1) for i in range(requests - 1)] + [more]
     check_attend(gpu, head_dim, 2 * kv_heads, kv_heads, 64, lengths, counts, WHOLE, total_keys=False)
+
+
+@pytest.mark.parametrize("seed", range(int(os.environ.get("KARPO_RANDOM_BATCHES", "16"))))
+def test_random_batches(gpu, seed):
+    """Requests of every kind together: empty ones, short and long ones, none, one or many queries, with and without a window."""
+    gen = torch.Generator().manual_seed(1000 + seed)
+
+    def one_of(*choices):
+        return choices[int(torch.randint(len(choices), (1,), generator=gen))]
+
+    def up_to(most):  # evenly over the logarithm
+        return int(2.0 ** (torch.rand(1, generator=gen).item() * math.log2(most + 1))) - 1
+
+    head_dim, kv_heads, group, block = one_of(64, 128, 256, 512), one_of(1, 2, 3), one_of(1, 2, 5, 8), one_of(32, 64, 128)
+    requests, longest, most = 1 + up_to(400), one_of(90, 1100, 5000), one_of(1, 1, 4, 40)
+    lengths, counts = [], []
+    while len(lengths) < requests and sum(lengths) < 40000:
+        lengths.append(up_to(longest))
+        counts.append(min(one_of(0, 1, 1, most), lengths[-1] + 1))
+    counts[0] = max(1, counts[0])
+    check_attend(gpu, head_dim, kv_heads * group, kv_heads, block, lengths, counts, window=one_of(-1, -1, 0, 100, 1000),
+                 causal=one_of(True, True, False), seed=seed, total_keys=one_of(True, False))
 
 
 @pytest.mark.parametrize("head_dim,kv_heads", [(64, 2), (128, 2), (256, 1), (512, 1)])

@@ -156,6 +156,29 @@ def test_append(gpu, bits, d, block, r, k_kind, v_kind):
 
 
 @pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("seed", range(6))
+def test_append_of_random_writes(gpu, bits, seed):
+    gen = torch.Generator().manual_seed(seed)
+
+    def one_of(*choices):
+        return choices[int(torch.randint(len(choices), (1,), generator=gen))]
+
+    d, block, heads, blocks = one_of(64, 128, 256, 512), one_of(32, 64, 128), one_of(1, 2, 3), 9
+    r = 32 * int(torch.randint(1, d // 32 + 1, (1,), generator=gen))
+    cache = _cache(bits, gpu, blocks, heads, d, block, seed=seed)
+    writes, rows = [], 0
+    for ident in torch.randperm(blocks, generator=gen)[:one_of(1, 4, blocks)].tolist():
+        first = one_of(0, 0, int(torch.randint(block, (1,), generator=gen)))
+        count = one_of(1, block - first, 1 + int(torch.randint(block - first, (1,), generator=gen)))
+        writes.append([ident, first, rows, count])
+        rows += count + one_of(0, 2)  # (rows that no write names)
+    key, value = (torch.randn((rows, heads, d), generator=gen).bfloat16().to(gpu) for _ in range(2))
+    positions = torch.randint(0, 77, (rows,), generator=gen, dtype=torch.int32).to(gpu)
+    kinds = [one_of(None, "weight", "one_plus", "plain") for _ in range(2)]
+    _append_and_compare(cache, key, value, writes, *(_norm(kind, d, gpu, gen) for kind in kinds), _tables(77, r, gen, gpu), positions)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("rope", [False, True])
 def test_rows_without_positions_or_rotation(gpu, bits, rope):
     """Row i takes the tables' row i; or nothing but the norms."""
@@ -271,7 +294,7 @@ def test_a_captured_append_reads_its_inputs_at_each_replay(gpu, bits):
 
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("d,kv_heads,block,rope", [(64, 13, 64, True), (128, 6, 128, True), (256, 3, 32, False), (512, 9, 64, True),
-                                                   (512, 4, 128, True)])
+                                                   (512, 4, 128, True), (512, 5, 32, True), (256, 5, 128, True)])
 def test_many_rows_at_once_and_in_pieces(gpu, bits, d, kv_heads, block, rope):
     """Over 96 MiB of rows, where a workgroup takes several heads: the same bits as in calls of few blocks each, which
     the other tests compare with the formulas. Ragged writes, some of one token."""
