@@ -25,8 +25,8 @@ constexpr int ring4_bytes(int d) { return kAttendWaves * kCacheGroup * d / 2; }
 constexpr int whole_tokens4(int d) { return d == 512 ? 256 : 640; }
 // Where more than half of the CUs have a workgroup, a longer walk is no loss (48 requests of 4 query tokens and 1,024 cached
 // ones: heads of 64 18.4, 13.0; 128 33.4, 27.4; 256 36.1, 29.9; 512 64.4, 60.5), up to what one long request among short ones
-// may take.
-constexpr int kWholeTokens4 = 1024;
+// may take: one of 1,280 seen tokens 12.5 to 20 us, of heads of 512 30, against 13.5 to 19 and 23 where its shares are split.
+constexpr int most_whole_tokens4(int d) { return d == 512 ? 1024 : 1280; }
 constexpr int kLeastUnits4 = 4;         // groups of 32 tokens that a workgroup takes at least, of a request that is split
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
@@ -730,7 +730,7 @@ AttendShape attend4_shape(const CacheRef& c, int32_t n_seq, int32_t group, int32
   const int64_t parts = 256 * attend4_waves(c.head_dim, tiles) / y;
   s.parts = parts < 1 ? 1 : (int)parts;
   s.used = (int)(vectors < s.vectors ? vectors : s.vectors);
-  s.whole = seen <= (n_seq * y > 128 ? kWholeTokens4 : whole_tokens4(c.head_dim));
+  s.whole = seen <= (n_seq * y > 128 ? most_whole_tokens4(c.head_dim) : whole_tokens4(c.head_dim));
   s.units_bytes = (4 * ((int64_t)n_seq + 2) + 255) / 256 * 256;
   s.bytes = s.whole ? 0 : s.units_bytes + y * s.parts * 2 * s.vectors * (c.head_dim + 2) * 4;
   return s;

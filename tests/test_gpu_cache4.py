@@ -278,8 +278,9 @@ def test_many_requests(gpu):
 
 @pytest.mark.parametrize("head_dim,kv_heads,requests,more", [(64, 2, 70, 1), (128, 3, 48, 4), (256, 1, 130, 1), (512, 4, 33, 3)])
 def test_long_walks_of_many_requests(gpu, head_dim, kv_heads, requests, more):
-    """Workgroups that take up to 1,024 tokens whole."""
-    lengths = [(337 * i) % 1025 for i in range(requests - 1)] + [1024]
+    """Workgroups that take up to 1,024 tokens whole, 1,280 of head sizes below 512."""
+    longest = 1024 if head_dim == 512 else 1280
+    lengths = [(337 * i) % (longest + 1) for i in range(requests - 1)] + [longest]
     counts = [i % (more + 1) for i in range(requests - 1)] + [more]
     check_attend(gpu, head_dim, 2 * kv_heads, kv_heads, 64, lengths, counts, WHOLE, total_keys=False)
 
