@@ -100,8 +100,9 @@ struct Write {
 // Many rows are bound by HBM: 32,768 of 16 heads of 128, normed and rotated, 90 us in 8 bits (402 MB and 17 MB of tables, 4.7 TB/s;
 // 145 with loads pass by pass and one head a workgroup) and 78 us in 4 (356 MB); few by three rounds of dependent loads (the write,
 // its rows and positions, cos and sin) and the joins over the workgroup: one token of 48 requests 6.7 us, 2,500 tokens of 24
-// requests, 8 heads of 256, 14.4. Of that document's 134 million codes 62 are another than the 64-bit row's (133 where each step
-// of the formulas is rounded to fp32 by itself): rows that close to the border between two codes.
+// requests, 8 heads of 256, 14.4. Of four such documents' 537 million codes 278 are another than the 64-bit rows' (566 where each
+// step of the formulas is rounded to fp32 by itself): elements that close to the border between two codes. With the root as a
+// sum of two terms 273, and 93.5 us.
 template <int D, int BLOCK, int PASSES, int WAVES, int BITS, bool MANY, bool VALUE, bool TURNED>
 __device__ __forceinline__ void append_rows(const AppendRowsParams& p, const Write& wr, int h0, int h1, char* s_codes) {
   constexpr int kLanes = D / 8, kRows = 64 / kLanes, kStep = kRows * WAVES;
@@ -183,27 +184,27 @@ __device__ __forceinline__ void append_rows(const AppendRowsParams& p, const Wri
     const unsigned old_bits = BITS == 8 && first > 0 ? __float_as_uint(*scale_of) : 0;
     auto row_of = [&](int t, float (&y)[8]) {
       float ss = 0.f;
-  #pragma unroll
+#pragma unroll
       for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(bf16_at(x[t], e), bf16_at(x[t], e), ss);
       const float root = reciprocal_root(sum_over<kLanes>(ss) * (1.f / D) + norm.eps), r = normed ? root : 1.f;
       if constexpr (TURNED) {
         u32x4 px;
-  #pragma unroll
+#pragma unroll
         for (int k = 0; k < 4; ++k) px[k] = (unsigned)__builtin_amdgcn_ds_bpermute(partner, (int)x[t][k]);
-  #pragma unroll
+#pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float n = bf16_at(x[t], e) * w_mine[e];
           const float turn = __builtin_fmaf(n, bf16_at(cv[t], e), bf16_at(px, e) * w_other[e] * bf16_at(sv[t], e));
           y[e] = (inside ? turn : n) * r;
         }
       } else {
-  #pragma unroll
+#pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = bf16_at(x[t], e) * w_mine[e] * r;
       }
     };
     // the largest magnitude of y and `best`, NaN as nothing
     auto larger = [&](const float (&y)[8], float best) {
-  #pragma unroll
+#pragma unroll
       for (int e = 0; e < 8; e += 2)
         best = __builtin_fmaxf(__builtin_fmaxf(best, __builtin_fabsf(y[e])), __builtin_fabsf(y[e + 1]));
       return best;
@@ -213,7 +214,7 @@ __device__ __forceinline__ void append_rows(const AppendRowsParams& p, const Wri
     float scale = 1.f, old_scale = 1.f;
     if constexpr (BITS == 8) {
       float y[PASSES][8], most_of = 0.f;
-  #pragma unroll
+#pragma unroll
       for (int t = 0; t < PASSES; ++t) {
         row_of(t, y[t]);
         most_of = larger(y[t], most_of);
@@ -226,7 +227,7 @@ __device__ __forceinline__ void append_rows(const AppendRowsParams& p, const Wri
           __syncthreads();
           if (lane == 0) s_best[wave] = mine;
           __syncthreads();
-  #pragma unroll
+#pragma unroll
           for (int w = 0; w < WAVES; ++w) mine = max(mine, s_best[w]);
           __syncthreads();  // (the codes, or the next head's maxima, take the array)
         }
@@ -236,9 +237,9 @@ __device__ __forceinline__ void append_rows(const AppendRowsParams& p, const Wri
       const bool odd = best >= 0x7f800000u;  // infinities: the largest of the others
       if (__builtin_expect(odd, 0)) {
         best = 0;
-  #pragma unroll
+#pragma unroll
         for (int t = 0; t < PASSES; ++t)
-  #pragma unroll
+#pragma unroll
           for (int e = 0; e < 8; ++e) {
             const unsigned m = __float_as_uint(y[t][e]) & 0x7fffffffu;
             best = max(best, m < 0x7f800000u ? m : 0u);
@@ -256,12 +257,12 @@ __device__ __forceinline__ void append_rows(const AppendRowsParams& p, const Wri
       if (tid == 0) *scale_of = scale;
       if (__builtin_expect(odd || e == KARPO_CACHE_MAX_EXP, 0)) {
         const float most = 448.f * scale;
-  #pragma unroll
+#pragma unroll
         for (int t = 0; t < PASSES; ++t)
-  #pragma unroll
+#pragma unroll
           for (int k = 0; k < 8; ++k) y[t][k] = __builtin_fabsf(y[t][k]) > most ? __builtin_copysignf(most, y[t][k]) : y[t][k];
       }
-  #pragma unroll
+#pragma unroll
       for (int t = 0; t < PASSES; ++t) {
         const int slot = first + token_of(t);
         const u32x2 w = {codes8(y[t][0], y[t][1], y[t][2], y[t][3], scale), codes8(y[t][4], y[t][5], y[t][6], y[t][7], scale)};
@@ -278,14 +279,14 @@ __device__ __forceinline__ void append_rows(const AppendRowsParams& p, const Wri
           u32x4* const dst =
               reinterpret_cast<u32x4*>(out + ((slot >> 4) * (D / 64) + (piece >> 2)) * 1024 + (slot & 15) * 64 + (piece & 3) * 16);
           u32x4 w = *dst;
-  #pragma unroll
+#pragma unroll
           for (int k = 0; k < 4; ++k) w[k] = codes_again(w[k], old_scale, scale);
           *dst = w;
         }
       }
     } else {
       uint8_t* const scales = c.scales4 + head * (BLOCK / 32) * 2 * D + (VALUE ? D : 0);
-  #pragma unroll
+#pragma unroll
       for (int t = 0; t < PASSES; ++t) {
         const int slot = first + token_of(t);
         float y[8];
@@ -297,7 +298,7 @@ __device__ __forceinline__ void append_rows(const AppendRowsParams& p, const Wri
         // seldom: the largest of the others, and is one NaN
         if (__any(!(__builtin_fabsf(sum) < INFINITY) || best >= 0x7f800000u)) {
           unsigned fine = 0, all = 0;
-  #pragma unroll
+#pragma unroll
           for (int e = 0; e < 8; ++e) {
             const unsigned m = __float_as_uint(y[e]) & 0x7fffffffu;
             fine = max(fine, m < 0x7f800000u ? m : 0u);
@@ -333,9 +334,9 @@ __device__ __forceinline__ void append_rows(const AppendRowsParams& p, const Wri
         const int j = u & 3, q = (u >> 2) & 3, tile = (u >> 4) % kTiles, half = half0 + (u >> 4) / kTiles;
         // bytes of the tokens 16 t + 4 q + 0 .. 3 that are new, and that are rounded again
         unsigned is_new[2] = {0, 0}, is_old[2] = {0, 0};
-  #pragma unroll
+#pragma unroll
         for (int t = 0; t < 2; ++t)
-  #pragma unroll
+#pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int slot = half * 32 + t * 16 + q * 4 + i;
             if (slot >= first && slot < first + count) is_new[t] |= 0xffu << (8 * i);
@@ -344,26 +345,26 @@ __device__ __forceinline__ void append_rows(const AppendRowsParams& p, const Wri
         if ((is_new[0] | is_new[1] | is_old[0] | is_old[1]) == 0) continue;
         const bool whole = (is_new[0] & is_new[1]) == 0xffffffffu;
         u32x4 w[4];
-  #pragma unroll
+#pragma unroll
         for (int g = 0; g < 2; ++g)
-  #pragma unroll
+#pragma unroll
           for (int t = 0; t < 2; ++t) {
             unsigned r[4], o[4];
             const char* const from = s_codes + (half * 32 + t * 16 + q * 4) * kPitch + tile * 32 + g * 16 + j * 4;
-  #pragma unroll
+#pragma unroll
             for (int i = 0; i < 4; ++i) r[i] = *reinterpret_cast<const unsigned*>(from + i * kPitch);
             transposed(r, o);
-  #pragma unroll
+#pragma unroll
             for (int k = 0; k < 4; ++k) w[k][2 * g + t] = o[k];
           }
-  #pragma unroll
+#pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int dl = 4 * j + k;
           u32x4* const dst = reinterpret_cast<u32x4*>(out + (half * kTiles + tile) * 1024 +
                                                       (BITS == 8 ? dl * 64 + q * 16 : (q * 16 + dl) * 16));
           if (!whole) {
             const u32x4 was = *dst;
-  #pragma unroll
+#pragma unroll
             for (int m = 0; m < 4; ++m) {
               unsigned kept = was[m];
               if constexpr (BITS == 8)
