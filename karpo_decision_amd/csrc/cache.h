@@ -122,6 +122,7 @@ struct AttendShape {
   int vectors, used, tiles, parts;  // used: the most of them that any workgroup has
   bool whole;
   int64_t units_bytes, bytes;  // of the workspace: the units, then the partials
+  bool wide = false;  // whole, in 4 bits: by eight waves a request
 };
 // `seen`: a bound of the tokens that a request's queries see.
 AttendShape attend_shape(const CacheRef& c, int32_t n_seq, int32_t group, int32_t max_q, int64_t seen);

@@ -17,11 +17,13 @@ __host__ __device__ constexpr int attend4_waves(int d, int nt) {
   return nt == 1 ? (d == 64 ? 4 : d == 128 ? 3 : d == 256 ? 2 : 1) : d == 64 && nt == 2 ? 3 : d <= 128 ? 2 : 1;
 }
 // Bytes of LDS for the waves' copies of a group's keys (as many for the values).
-constexpr int ring4_bytes(int d) { return kAttendWaves * kCacheGroup * d / 2; }
+constexpr int ring4_bytes(int d, int waves) { return waves * kCacheGroup * d / 2; }
+// And for their sums while they are joined.
+constexpr int sums4_bytes(int d, int nt, int waves) { return waves * 16 * nt * (slab_of(d, nt) + 4) * 4; }
 
 // Requests of which at most so many tokens are seen are not split: a workgroup's walk is then shorter than the partials' way
 // through memory and a second launch. us split, whole at heads of 128 with 16 key heads: 8 requests of 128 tokens 12.4, 7.3, of
-// 640 15.9, 11.4, of 1,500 18.9, 18.7; one of 1,024 13.7, 13.6; heads of 512, 2 requests of 256 15.8, 13.0, of 512 16.7, 17.6.
+// 640 15.9, 11.4 (10.3 by eight waves), of 1,500 18.9, 18.7; one of 1,024 13.7, 13.6; heads of 512, 2 requests of 256 15.8, 13.0, of 512 16.7, 17.6.
 constexpr int whole_tokens4(int d) { return d == 512 ? 256 : 640; }
 // Where more than half of the CUs have a workgroup, a longer walk is no loss (48 requests of 4 query tokens and 1,024 cached
 // ones: heads of 64 18.4, 13.0; 128 33.4, 27.4; 256 36.1, 29.9; 512 64.4, 60.5), up to what one long request among short ones
@@ -107,7 +109,7 @@ constexpr int kStart4 = 16, kTries = 5;
 // groups of 64 tokens and four waves a SIMD at head size 128 (42.3 against 40.1 us) were no faster.
 //
 // ONCE: one workgroup reads a request's codes of a head, once; they are streamed through the caches.
-template <int D, int NT, bool ONCE>
+template <int D, int NT, bool ONCE, int WAVES>
 __device__ __forceinline__ void attend4_share(const AttendParams& p, const Seen& s, int request, int g0, int g1, int h,
                                               int vector0, int vectors, bool whole, float* part) {
   constexpr int kGroupBytes = kCacheGroup * D / 2;
@@ -116,12 +118,12 @@ __device__ __forceinline__ void attend4_share(const AttendParams& p, const Seen&
   constexpr int kSpans = D < 128 ? 1 : D / 128, kParts = D < 128 ? 1 : 2;  // spans of 128 elements, two pieces of 64 each
   constexpr int kGroups = D / 32;                                          // of 32 elements under a scale
   constexpr int kSlab = slab_of(D, NT), kVectors = 16 * NT;
-  constexpr int kRing = ring4_bytes(D);
-  __shared__ float s_m[kAttendWaves][kVectors], s_l[kAttendWaves][kVectors];
+  constexpr int kRing = ring4_bytes(D, WAVES);
+  __shared__ float s_m[WAVES][kVectors], s_l[WAVES][kVectors];
   // (arrays of their own: a read then waits for the copies into its own array and no others)
-  __shared__ __align__(16) char s_keys[kRing > sums_bytes(D, NT) ? kRing : sums_bytes(D, NT)];
+  __shared__ __align__(16) char s_keys[kRing > sums4_bytes(D, NT, WAVES) ? kRing : sums4_bytes(D, NT, WAVES)];
   __shared__ __align__(16) char s_values[kRing];
-  __shared__ __align__(16) char s_key_scales[kAttendWaves * 1024], s_value_scales[kAttendWaves * 1024];  // (D bytes each in use)
+  __shared__ __align__(16) char s_key_scales[WAVES * 1024], s_value_scales[WAVES * 1024];  // (D bytes each in use)
   __shared__ u32x4 s_q[kVectors * D / 8];
   __shared__ unsigned s_q_scales[kSpans * NT * 64];
   float(*const s_o)[kVectors][kSlab + 4] = reinterpret_cast<float(*)[kVectors][kSlab + 4]>(s_keys);
@@ -138,7 +140,7 @@ __device__ __forceinline__ void attend4_share(const AttendParams& p, const Seen&
   const int heads = p.c.kv_heads, b = p.c.block_log2;
 
   // the query vectors' elements (a wave's spans of them: 16 quad .. + 16 of each 64), and the keys that each vector sees
-  constexpr int kMine = (kSpans * NT + kAttendWaves - 1) / kAttendWaves;
+  constexpr int kMine = (kSpans * NT + WAVES - 1) / WAVES;
   u32x4 q_mine[kMine][2 * kParts];
   int lo[NT], hi[NT];
   const int shift = s.tokens - s.queries;
@@ -151,7 +153,7 @@ __device__ __forceinline__ void attend4_share(const AttendParams& p, const Seen&
         p.q + (s.row + (int64_t)pos) * p.sq_t + (int64_t)(h * p.group + (valid ? vec - pos * p.group : 0)) * p.sq_h;
 #pragma unroll
     for (int c = 0; c < kMine; ++c) {
-      const int e = wave + c * kAttendWaves;  // span e / NT of tile e % NT
+      const int e = wave + c * WAVES;  // span e / NT of tile e % NT
       if (e < kSpans * NT && e % NT == n) {
 #pragma unroll
         for (int k = 0; k < 2 * kParts; ++k)
@@ -180,7 +182,7 @@ __device__ __forceinline__ void attend4_share(const AttendParams& p, const Seen&
   int ids = 0;
   // lane k looks up the wave's groups g + 4 k
   auto look_up = [&](int g) {
-    ids = table[min(g + lane * kAttendWaves, g1 - 1) >> (b - 5)];
+    ids = table[min(g + lane * WAVES, g1 - 1) >> (b - 5)];
     if (ids < 0 || ids >= p.c.blocks) ids = -1;
   };
   // One group's codes and scales into the wave's ring, 16 bytes a lane; zeros for a block that is not of the pool (and for the
@@ -222,7 +224,7 @@ __device__ __forceinline__ void attend4_share(const AttendParams& p, const Seen&
   }
 #pragma unroll
   for (int c = 0; c < kMine; ++c) {
-    const int e = wave + c * kAttendWaves;
+    const int e = wave + c * WAVES;
     if (e < kSpans * NT) {
       // the largest of each 32 elements: of a lane's 16 and those of the lane 16 away; 448 * 2^e holds it
       int part_e[2] = {0, 0};
@@ -253,8 +255,8 @@ __device__ __forceinline__ void attend4_share(const AttendParams& p, const Seen&
     }
   }
   lds_barrier();
-  for (int g = g0 + wave; g < g1; g += kAttendWaves) {
-    const int next = g + kAttendWaves;
+  for (int g = g0 + wave; g < g1; g += WAVES) {
+    const int next = g + WAVES;
     arrived();
     f32x4 st[NT][2];
 #pragma unroll
@@ -440,13 +442,13 @@ __device__ __forceinline__ void attend4_share(const AttendParams& p, const Seen&
   auto top_of = [&](int c) {
     float up = s_m[0][c];
 #pragma unroll
-    for (int w = 1; w < kAttendWaves; ++w) up = __builtin_elementwise_maximum(up, s_m[w][c]);
+    for (int w = 1; w < WAVES; ++w) up = __builtin_elementwise_maximum(up, s_m[w][c]);
     return up;
   };
   auto total_of = [&](int c, float up) {
     float l = 0.f;
 #pragma unroll
-    for (int w = 0; w < kAttendWaves; ++w)
+    for (int w = 0; w < WAVES; ++w)
       l += s_m[w][c] == -INFINITY ? 0.f : s_l[w][c] * __builtin_amdgcn_exp2f(s_m[w][c] - up);
     return l;
   };
@@ -469,11 +471,11 @@ __device__ __forceinline__ void attend4_share(const AttendParams& p, const Seen&
         }
     }
     lds_barrier();
-    for (int e = tid; e < vectors * (kSlab / 4); e += kAttendThreads) {
+    for (int e = tid; e < vectors * (kSlab / 4); e += 64 * WAVES) {
       const int c = e / (kSlab / 4), d = (e % (kSlab / 4)) * 4;
       f32x4 x = *reinterpret_cast<const f32x4*>(&s_o[0][c][d]);
 #pragma unroll
-      for (int w = 1; w < kAttendWaves; ++w) x += *reinterpret_cast<const f32x4*>(&s_o[w][c][d]);
+      for (int w = 1; w < WAVES; ++w) x += *reinterpret_cast<const f32x4*>(&s_o[w][c][d]);
       if (whole) {
         const float l = total_of(c, top_of(c));
         const int vec = vector0 + c, pos = position_of(vec, p), head = h * p.group + vec - pos * p.group;
@@ -592,7 +594,7 @@ __global__ __launch_bounds__(kAttendThreads, attend4_waves(D, NT)) void attend4_
         continue;
       }
 
-      attend4_share<D, NT, ONCE>(
+      attend4_share<D, NT, ONCE, kAttendWaves>(
           p, s, i, g0, g1, h, vector0, vectors, begin >= u0 && end <= u1,
           p.partial + (((int64_t)blockIdx.y * p.parts + blockIdx.x) * 2 + (begin <= u0 ? 0 : 1)) * (kVectors * (D + 2)));
     }
@@ -601,14 +603,15 @@ __global__ __launch_bounds__(kAttendThreads, attend4_waves(D, NT)) void attend4_
 }
 
 // One workgroup for each request, and nothing to join.
-template <int D, int NT, bool ONCE>
-__global__ __launch_bounds__(kAttendThreads, attend4_waves(D, NT)) void attend4_whole_kernel(const AttendParams p) {
+template <int D, int NT, bool ONCE, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES > kAttendWaves ? 2 : attend4_waves(D, NT))
+    void attend4_whole_kernel(const AttendParams p) {
   const int heads = p.c.kv_heads, h = blockIdx.y % heads, vector0 = (blockIdx.y / heads) * 16 * NT;
   const Seen s = seen_of(p, blockIdx.x);
   const int vectors = (int)min<int64_t>((int64_t)min(s.queries, p.max_q) * p.group - vector0, 16 * NT);
   if (vectors > 0)
-    attend4_share<D, NT, ONCE>(p, s, blockIdx.x, s.first, s.first + s.groups, h, vector0, vectors, true, nullptr);
-  fill_past<D>(p, s, blockIdx.y, threadIdx.x, kAttendThreads);
+    attend4_share<D, NT, ONCE, WAVES>(p, s, blockIdx.x, s.first, s.first + s.groups, h, vector0, vectors, true, nullptr);
+  fill_past<D>(p, s, blockIdx.y, threadIdx.x, 64 * WAVES);
 }
 
 // Joins a request's shares: O = sum of 2^(m_w - M) O_w over sum of 2^(m_w - M) l_w, in an order that the sizes alone set.
@@ -702,10 +705,16 @@ void launch(const AttendParams& p, const AttendShape& s, hipStream_t stream) {
   const unsigned y = (unsigned)(p.c.kv_heads * s.tiles), x = (unsigned)(p.whole ? p.r.n_seq : s.parts);
   const dim3 grid(x, y), threads(kAttendThreads);
   if (p.whole) {
+    if constexpr (NT == 1 && D <= 256) {
+      if (s.wide) {
+        attend4_whole_kernel<D, NT, true, 2 * kAttendWaves><<<grid, dim3(2 * kAttendThreads), 0, stream>>>(p);
+        return;
+      }
+    }
     if (s.tiles == 1)
-      attend4_whole_kernel<D, NT, true><<<grid, threads, 0, stream>>>(p);
+      attend4_whole_kernel<D, NT, true, kAttendWaves><<<grid, threads, 0, stream>>>(p);
     else
-      attend4_whole_kernel<D, NT, false><<<grid, threads, 0, stream>>>(p);
+      attend4_whole_kernel<D, NT, false, kAttendWaves><<<grid, threads, 0, stream>>>(p);
     return;
   }
   if (s.tiles == 1) attend4_kernel<D, NT, true><<<grid, threads, 0, stream>>>(p);
@@ -731,6 +740,10 @@ AttendShape attend4_shape(const CacheRef& c, int32_t n_seq, int32_t group, int32
   s.parts = parts < 1 ? 1 : (int)parts;
   s.used = (int)(vectors < s.vectors ? vectors : s.vectors);
   s.whole = seen <= (n_seq * y > 128 ? most_whole_tokens4(c.head_dim) : whole_tokens4(c.head_dim));
+  // Twice the waves where a CU has one workgroup at most and its four waves would have more than two groups each. us with four,
+  // with eight, at heads of 128 with 16 key heads: 8 requests of 60 tokens 7.3, 7.8, of 250 8.4, 8.7, of 640 11.5, 10.3; 16 of 1,000
+  // 15.7, 13.5; 32 (512 workgroups) of 250 10.4, 11.3, of 640 15.3, 15.1; 8 heads of 256, 32 requests of 1,000 21.5, 19.5.
+  s.wide = s.whole && tiles == 1 && s.tiles == 1 && c.head_dim <= 256 && n_seq * y <= 256 && seen > 256;
   s.units_bytes = (4 * ((int64_t)n_seq + 2) + 255) / 256 * 256;
   s.bytes = s.whole ? 0 : s.units_bytes + y * s.parts * 2 * s.vectors * (c.head_dim + 2) * 4;
   return s;

@@ -276,6 +276,15 @@ def test_many_requests(gpu):
     check_attend(gpu, 64, 4, 2, 32, lengths[:-1] + [1500], [1 + (i % 3 == 0) for i in range(600)], SPLIT, total_keys=False)
 
 
+@pytest.mark.parametrize("head_dim,heads,kv_heads,lengths", [(64, 8, 2, [257, 260, 640, 31, 0, 511]), (128, 3, 3, [640, 300, 1]),
+                                                             (256, 8, 1, [290, 640, 639])])
+@pytest.mark.parametrize("window", [-1, 0, 290])
+def test_whole_requests_by_twice_the_waves(gpu, head_dim, heads, kv_heads, lengths, window):
+    """One workgroup of eight waves a request, some without a group of 32 tokens; the window's begin inside a group."""
+    check_attend(gpu, head_dim, heads, kv_heads, 32, lengths, [1] * len(lengths), WHOLE, window=window, total_keys=False)
+    check_attend(gpu, head_dim, heads, kv_heads, 64, lengths, [2] * len(lengths), WHOLE, window=window, causal=False)
+
+
 @pytest.mark.parametrize("head_dim,kv_heads,requests,more", [(64, 2, 70, 1), (128, 3, 48, 4), (256, 1, 130, 1), (512, 4, 33, 3)])
 def test_long_walks_of_many_requests(gpu, head_dim, kv_heads, requests, more):
     """Workgroups that take up to 1,024 tokens whole, 1,280 of head sizes below 512."""
@@ -349,7 +358,8 @@ def test_strided_queries_and_tables(gpu):
 
 
 @pytest.mark.parametrize("head_dim,heads,lengths,counts,path", [
-    (64, 4, [130, 100], [1, 2], WHOLE), (64, 4, [900, 100], [1, 2], SPLIT), (128, 4, [900, 100], [1, 1], SPLIT),
+    (64, 4, [130, 100], [1, 2], WHOLE), (128, 4, [400, 300], [2, 1], WHOLE), (64, 4, [900, 100], [1, 2], SPLIT),
+    (128, 4, [900, 100], [1, 1], SPLIT),
     (256, 4, [900, 100], [2, 1], SPLIT), (512, 4, [300, 100], [1, 1], SPLIT), (64, 16, [3000, 2900], [2000, 1900], UNPACKED)])
 def test_unknown_blocks_read_as_zeros(gpu, head_dim, heads, lengths, counts, path):
     """Beside a block 0 all of whose scales are NaN."""
@@ -397,7 +407,7 @@ def test_bounds_out_of_range_write_nothing(gpu, bounds, good):
 
 
 @pytest.mark.parametrize("head_dim,heads,kv_heads,lengths,counts,max_q,path", [
-    (64, 4, 2, [130, 100], [5, 2], 2, WHOLE), (512, 4, 2, [100, 60], [9, 1], 1, WHOLE),
+    (64, 4, 2, [130, 100], [5, 2], 2, WHOLE), (256, 4, 2, [530, 400, 0], [5, 2, 3], 2, WHOLE), (512, 4, 2, [100, 60], [9, 1], 1, WHOLE),
     (64, 4, 2, [900, 100, 0], [5, 3, 3], 2, SPLIT), (64, 80, 2, [900, 700], [7, 2], 2, SPLIT),
     (256, 4, 2, [900, 100], [1, 40], 33, SPLIT), (512, 4, 2, [300, 100], [9, 9], 1, SPLIT)])
 def test_queries_past_max_q_are_nan(gpu, head_dim, heads, kv_heads, lengths, counts, max_q, path):
@@ -431,7 +441,7 @@ def test_a_long_chunk_with_bounds_that_do_not_hold_is_nan(gpu, change):
 
 @pytest.mark.parametrize("head_dim,heads,kv_heads,counts", [(64, 4, 2, [6, 1]), (128, 8, 2, [9, 2]), (128, 2, 2, [3, 1]),
                                                             (512, 8, 1, [2, 1]), (256, 16, 8, [16, 3])])
-@pytest.mark.parametrize("more", [0, 900])
+@pytest.mark.parametrize("more", [0, 350, 900])
 def test_nan_reaches_the_queries_that_see_it_and_no_others(gpu, head_dim, heads, kv_heads, counts, more):
     """A NaN scale of 32 elements of a new token's value, and of another's key: earlier queries of the call do not see them."""
     lengths, block = [70 + more, 33], 32
