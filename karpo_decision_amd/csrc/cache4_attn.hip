@@ -23,7 +23,8 @@ constexpr int sums4_bytes(int d, int nt, int waves) { return waves * 16 * nt * (
 
 // Requests of which at most so many tokens are seen are not split: a workgroup's walk is then shorter than the partials' way
 // through memory and a second launch. us split, whole at heads of 128 with 16 key heads: 8 requests of 128 tokens 12.4, 7.3, of
-// 640 15.9, 11.4 (10.3 by eight waves), of 1,500 18.9, 18.7; one of 1,024 13.7, 13.6; heads of 512, 2 requests of 256 15.8, 13.0, of 512 16.7, 17.6.
+// 640 15.9, 11.4 (10.3 by eight waves), of 1,500 18.9, 18.7; one of 1,024 13.7, 13.6; heads of 512, 2 requests of 256 15.8, 13.0,
+// of 512 16.7, 17.6.
 constexpr int whole_tokens4(int d) { return d == 512 ? 256 : 640; }
 // Where more than half of the CUs have a workgroup, a longer walk is no loss (48 requests of 4 query tokens and 1,024 cached
 // ones: heads of 64 18.4, 13.0; 128 33.4, 27.4; 256 36.1, 29.9; 512 64.4, 60.5), up to what one long request among short ones
