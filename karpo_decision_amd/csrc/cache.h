@@ -1,4 +1,5 @@
-// The block cache's kernels' arguments (cache.hip, cache_append.hip, cache_attn.hip, cache4_attn.hip), shared with the C ABI (cache_capi.cpp).
+// The block cache's kernels' arguments (cache.hip, cache_append.hip, cache_attn.hip, cache4_attn.hip), shared with the C ABI
+// (cache_capi.cpp).
 #pragma once
 #include <hip/hip_runtime_api.h>
 #include <stdint.h>

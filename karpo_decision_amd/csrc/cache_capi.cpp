@@ -1,5 +1,5 @@
-// The block cache's C ABI (karpo_cache.h, karpo_cache4.h: the same functions over either cache): argument checks, workspace sizes and launches. Everything that the kernels
-// index with is checked here or in the kernel itself, before a launch or a load.
+// The block cache's C ABI (karpo_cache.h, karpo_cache4.h: the same functions over either cache): argument checks, workspace
+// sizes and launches. Everything that the kernels index with is checked here or in the kernel itself, before a launch or a load.
 #include <math.h>
 #include <stdint.h>
 #include <string.h>
