@@ -118,7 +118,7 @@ __device__ __forceinline__ void append_rows(const AppendRowsParams& p, const Wri
 
   // norm: (x * w) * r, w the weight, 1 + weight or 1; rotation of the first rope_dim elements, partner rh away. A product of two
   // bf16 numbers, and of three, is exact in fp32, so a weighted key takes two roundings, (xw * cos - xw' * sin) and the
-  // product with r (normed first and then turned it is five).
+  // product with r (normed first and then turned it is five; where w is 1 + weight, that sum and its products round too).
   const NormRef& norm = VALUE ? p.v_norm : p.k_norm;
   const bool normed = norm.mode != KARPO_NORM_NONE;
   const float wm = norm.mode == KARPO_NORM_WEIGHT || norm.mode == KARPO_NORM_ONE_PLUS ? 1.f : 0.f;
