@@ -11,6 +11,8 @@
  * exponent with max|finite element| <= 6 * 2^e, within KARPO_CACHE4_MIN_EXP .. MAX_EXP; codes are the nearest, ties to even, an
  * element past the range is stored at its end, an infinity too; a NaN makes its 32 elements NaN (the byte is 255). A token's
  * scales are its own: appending leaves the block's other tokens as they are.
+ * The pool need not be initialised: what a slot holds that no append wrote (bytes of 253 and 254 too, which append never writes)
+ * reaches no query that does not see its token.
  *
  * Layout (token t and element d within a block of one head; h = t / 32, an even element in the lower half of its byte):
  *   keys    h * 16 D + ((t / 16 % 2) * (D / 32) + d / 32) * 256 + (t % 16) * 16 + d % 32 / 2

@@ -168,6 +168,9 @@ __device__ __forceinline__ void attend4_share(const AttendParams& p, const Seen&
   const int pos_first = position_of(vector0, p), pos_last = position_of(vector0 + vectors - 1, p);
   const int full_lo = p.left < 0 ? 0 : pos_last + shift - p.left;
   const int full_hi = p.right < 0 ? s.tokens - 1 : (int)min<int64_t>((int64_t)pos_first + shift + p.right, s.tokens - 1);
+  // tokens that any vector sees
+  const int any_lo = p.left < 0 ? 0 : pos_first + shift - p.left;
+  const int any_hi = p.right < 0 ? s.tokens - 1 : (int)min<int64_t>((int64_t)pos_last + shift + p.right, s.tokens - 1);
 
   f32x4 o[NT][D / 16];  // [2 (32 elements) + which of each pair of them]
   float top[NT], sum[NT];
@@ -360,18 +363,26 @@ __device__ __forceinline__ void attend4_share(const AttendParams& p, const Seen&
 
     if (next < g1) arrived(); else wait_vmcnt<0>();
     asm volatile("" ::: "memory");
-    bool nan = false;
+    bool odd = false;
     if (masked) {
-      unsigned any = 0;  // 0x80 where a byte is 255
+      unsigned any = 0;  // 0x80 where a byte is 253 (KARPO_CACHE4_MAX_EXP + 128) or more
 #pragma unroll
       for (int group = 0; group < kGroups; ++group) {
         const u32x2 w = *scales_at(group);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) any |= ((w[t] & 0x7f7f7f7fu) + 0x01010101u) & w[t] & 0x80808080u;
+        for (int t = 0; t < 2; ++t) any |= ((w[t] & 0x7f7f7f7fu) + 0x03030303u) & w[t] & 0x80808080u;
       }
-      nan = __any(any != 0);
+      odd = __any(any != 0);
     }
-    if (nan) {  // a NaN reaches the vectors that see its token, and no others (zero times NaN would be NaN)
+    // a NaN reaches the vectors that see its token, and no others, and what a slot holds that nothing wrote (253 and 254: codes
+    // under them pass bf16's range) reaches none (zero times NaN or infinity would be NaN)
+    if (odd) {
+      unsigned hidden = 0;  // one bit of each of the lane's eight keys that no vector sees
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int key = key0 + (e >> 2) * 16 + quad * 4 + (e & 3);
+        hidden |= key < any_lo || key > any_hi ? 1u << e : 0u;
+      }
 #pragma unroll
       for (int group = 0; group < kGroups; ++group) {
         u32x2 w = *scales_at(group);
@@ -379,11 +390,11 @@ __device__ __forceinline__ void attend4_share(const AttendParams& p, const Seen&
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if ((w[t] >> (8 * i) & 255) == 255) {
-              marks |= 1u << (4 * t + i);
-              w[t] &= ~(255u << (8 * i));
-            }
+          for (int i = 0; i < 4; ++i) {
+            const bool nan = (w[t] >> (8 * i) & 255) == 255;
+            marks |= nan ? 1u << (4 * t + i) : 0u;
+            if (nan || (hidden >> (4 * t + i) & 1) != 0) w[t] &= ~(255u << (8 * i));
+          }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           const float hit = column_sum((is_seen[n] & marks) != 0 ? 1.f : 0.f);

@@ -1,0 +1,74 @@
+"""The block caches on the GPU where few numbers of real use lie: slots that no append wrote. Tolerances are
+``cache4_cases.close``'s."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from cache4_cases import SPLIT, UNPACKED, WHOLE, attend, close, make, path_of, raw, values_of
+from oracle import cache4 as oracle
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- slots that no append wrote
+
+def _leave_garbage(cache, table, written, seed):
+    """Scales of 2^126, 2^127 and NaN and any codes wherever no token of ``written`` (first, end of each request) is."""
+    gen = torch.Generator().manual_seed(seed)
+    block, d = cache.block_size, cache.head_dim
+    scales = raw(cache.scales).cpu().view(cache.blocks, cache.kv_heads, -1)
+    kept = scales.clone()
+    scales.copy_(torch.randint(253, 256, scales.shape, generator=gen, dtype=torch.uint8))
+    for value in (False, True):
+        at = oracle.offsets(block, d, value)[1][:, ::32]
+        for row, (first, end) in zip(table, written):
+            for j, ident in enumerate(row):
+                tokens = range(max(0, first - j * block), max(0, min(block, end - j * block)))
+                if len(tokens):
+                    mine = at[list(tokens)].reshape(-1)
+                    scales[ident][:, mine] = kept[ident][:, mine]
+    raw(cache.scales).copy_(scales.view(cache.scales.shape))
+
+
+@pytest.mark.parametrize("head_dim,heads,kv_heads,lengths,counts,path", [
+    (64, 4, 2, [1, 33, 70, 0, 130], [1, 1, 1, 1, 1], WHOLE), (128, 4, 2, [1, 33, 70, 0, 130], [1, 2, 1, 1, 3], WHOLE),
+    (256, 2, 1, [1, 33, 70, 0, 130], [1, 2, 1, 1, 3], WHOLE), (512, 2, 2, [1, 33, 70, 0, 250], [1, 2, 1, 1, 3], WHOLE),
+    (64, 8, 2, [257, 500, 31, 0], [1, 2, 1, 1], WHOLE), (128, 3, 3, [257, 500, 31, 0], [1, 2, 1, 1], WHOLE),
+    (256, 4, 2, [257, 500, 31, 0], [1, 2, 1, 1], WHOLE), (64, 8, 2, [1300, 77, 1], [1, 1, 1], SPLIT),
+    (64, 8, 2, [1300, 77, 9], [7, 8, 9], SPLIT), (64, 16, 1, [1300, 77], [30, 7], SPLIT), (128, 4, 2, [1300, 77, 1], [1, 1, 1], SPLIT),
+    (128, 8, 2, [1300, 77, 9], [7, 8, 9], SPLIT), (128, 16, 1, [1300, 77], [30, 7], SPLIT), (256, 4, 2, [1300, 77, 1], [1, 1, 1], SPLIT),
+    (256, 8, 1, [1300, 77, 9], [7, 8, 9], SPLIT), (512, 4, 2, [1300, 77, 1], [1, 1, 1], SPLIT),
+    (512, 8, 1, [1300, 77, 9], [7, 8, 9], SPLIT), (64, 16, 2, [3001, 2901], [2000, 1900], UNPACKED)])
+@pytest.mark.parametrize("block", [32, 64])
+def test_slots_that_nothing_wrote_reach_no_query(gpu, head_dim, heads, kv_heads, lengths, counts, path, block):
+    """Scales that append never writes (2^126 and 2^127, under which codes pass bf16's range) behind the requests' tokens."""
+    cache, table, query, q_cu = make(gpu, head_dim, heads, kv_heads, block, lengths, counts)
+    _leave_garbage(cache, table, [(0, n) for n in lengths], seed=head_dim)
+    n, total = len(lengths), sum(lengths)
+    assert path_of(cache, heads, max(counts), sum(counts), n, len(table[0]), total_keys=total) == path
+    out = attend(gpu, cache, table, query, q_cu, lengths, max(counts), 0.1, total_keys=total)
+    want = values_of(cache)
+    for i, length in enumerate(lengths):
+        close(out[q_cu[i]:q_cu[i + 1]], query[q_cu[i]:q_cu[i + 1]], *want.rows(table[i], 0, length), 0.1,
+              weights=2.0 ** -8 if path == UNPACKED else 0.0)
+
+
+@pytest.mark.parametrize("head_dim,heads,kv_heads,lengths,counts,window,path", [
+    (64, 4, 2, [300, 120], [1, 1], 40, WHOLE), (128, 8, 2, [300, 120], [3, 2], 40, WHOLE), (256, 4, 2, [600, 120], [1, 1], 300, WHOLE),
+    (512, 4, 2, [300, 120], [3, 1], 40, WHOLE), (128, 8, 2, [2000, 120], [9, 1], 900, SPLIT), (64, 8, 2, [2000, 1900], [60, 9], 900, SPLIT),
+    (256, 8, 1, [2000, 120], [40, 1], 900, SPLIT), (512, 8, 2, [2000, 120], [40, 1], 900, SPLIT)])
+def test_blocks_behind_a_window_reach_no_query(gpu, head_dim, heads, kv_heads, lengths, counts, window, path):
+    """Tokens that every query's window has left, in blocks that nothing wrote (a table that still names blocks given back); more
+    than one tile of query vectors, of which the later ones meet groups that only the earlier ones see."""
+    cache, table, query, q_cu = make(gpu, head_dim, heads, kv_heads, 32, lengths, counts)
+    firsts = [max(0, n - c - window) for n, c in zip(lengths, counts)]  # the first token that a query sees
+    _leave_garbage(cache, table, list(zip(firsts, lengths)), seed=head_dim)
+    assert path_of(cache, heads, max(counts), sum(counts), 2, len(table[0]), window, sum(lengths)) == path
+    out = attend(gpu, cache, table, query, q_cu, lengths, max(counts), 0.1, window=window, total_keys=sum(lengths))
+    want = values_of(cache)
+    for i, (first, length) in enumerate(zip(firsts, lengths)):
+        key, value = want.rows(table[i], 0, length)
+        key[:first], value[:first] = 0.0, 0.0
+        close(out[q_cu[i]:q_cu[i + 1]], query[q_cu[i]:q_cu[i + 1]], key, value, 0.1, window=window)
