@@ -45,16 +45,31 @@ __device__ __forceinline__ f32x4 mfma_codes4(const u32x4& k, unsigned k_scale, c
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 0, KB, (int)k_scale, QB, (int)q_scale);
 }
 
-// 16 bf16 over 2^e as 16 e4m3 codes, and what they leave over (exact in fp32) over 2^(e - 4).
+constexpr int kMostQueryExp = 120;  // of the scale of 32 of a query's elements: that of those past 448 * 2^119
+
+// 16 bf16 over 2^e as 16 e4m3 codes, and what they leave over (exact in fp32) over 2^(e - 4). Finite elements from 248 * 2^120 on
+// would round to 256 * 2^120, which neither bf16 nor a sum of fp32 holds: their first term is 240 * 2^120, and the second the rest
+// (8 to 15, 128 to 240 of its own scale's, which have steps of 16: exact).
 __device__ __forceinline__ void two_terms(const u32x4 (&x)[2], int e, u32x4* high, u32x4* low) {
   const float scale = power_of_two(e), fine = power_of_two(e - 4);
+  const bool largest = __any(e == kMostQueryExp);
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
     float v[4], h[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] = bf16_at(x[w >> 1], (w & 1) * 4 + k);
-    s16x2 c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(s16x2{0, 0}, v[0], v[1], scale, false);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, v[2], v[3], scale, true);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) h[k] = v[k];
+    if (__builtin_expect(largest, 0)) {
+      constexpr float kMost = 240.f * 0x1p120f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float m = __builtin_fabsf(v[k]);
+        h[k] = m > kMost && m < INFINITY ? __builtin_copysignf(kMost, v[k]) : v[k];
+      }
+    }
+    s16x2 c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(s16x2{0, 0}, h[0], h[1], scale, false);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, h[2], h[3], scale, true);
     (*high)[w] = __builtin_bit_cast(unsigned, c);
 #pragma unroll
     for (int k = 0; k < 4; k += 2) {
@@ -241,7 +256,7 @@ __device__ __forceinline__ void attend4_share(const AttendParams& p, const Seen&
           m = max(m, max(x & 0x7fff, x >> 16 & 0x7fff));
         }
         m = max(m, (unsigned)__shfl_xor((int)m, 16));
-        part_e[j] = min(max((int)(m >> 7) - 127 - 8 + ((m & 0x7f) > 0x60 ? 1 : 0), -100), 120);
+        part_e[j] = min(max((int)(m >> 7) - 127 - 8 + ((m & 0x7f) > 0x60 ? 1 : 0), -100), kMostQueryExp);
       }
       // the scales go by 32 elements in order, which these lanes have
       const int from = col + 16 * ((2 * quad) & 3);

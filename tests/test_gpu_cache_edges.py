@@ -1,7 +1,9 @@
-"""The block caches on the GPU where few numbers of real use lie: slots that no append wrote. Tolerances are
-``cache4_cases.close``'s."""
+"""The block caches on the GPU where few numbers of real use lie: slots that no append wrote, queries at the end of bf16's
+range. Tolerances are ``cache4_cases.close``'s."""
 
 from __future__ import annotations
+
+import math
 
 import pytest
 import torch
@@ -72,3 +74,44 @@ def test_blocks_behind_a_window_reach_no_query(gpu, head_dim, heads, kv_heads, l
         key, value = want.rows(table[i], 0, length)
         key[:first], value[:first] = 0.0, 0.0
         close(out[q_cu[i]:q_cu[i + 1]], query[q_cu[i]:q_cu[i + 1]], key, value, 0.1, window=window)
+
+
+# ---- queries at the end of bf16's range
+
+PATHS = [(64, 4, 2, [200, 33], [1, 2]), (64, 4, 2, [1500, 33], [1, 2]), (128, 16, 2, [200, 33], [5, 2]), (128, 16, 2, [1500, 33], [5, 2]),
+         (256, 4, 2, [500, 33], [1, 1]), (256, 8, 1, [1500, 33], [3, 2]), (512, 4, 1, [200, 33], [1, 2]), (512, 4, 1, [1500, 33], [1, 2])]
+
+
+@pytest.mark.parametrize("head_dim,heads,kv_heads,lengths,counts", PATHS)
+def test_the_largest_queries(gpu, head_dim, heads, kv_heads, lengths, counts):
+    """Finite elements up to (2 - 2^-7) * 2^127, each of the last sixteen numbers of bf16 and of the binade before among them, over
+    keys under the least scale, so that the scores (some 2^28) are as far from the ends as any."""
+    cache, table, query, q_cu = make(gpu, head_dim, heads, kv_heads, 32, lengths, counts)
+    at = oracle.offsets(32, head_dim, False)[1].reshape(-1).unique()
+    scales = raw(cache.scales).view(cache.blocks, kv_heads, -1)
+    scales[:, :, at.to(gpu)] = 27  # 2^-100
+    gen = torch.Generator().manual_seed(3)
+    bits = torch.randint(0x7ef0, 0x7f80, query.shape, generator=gen)  # from 1.875 * 2^126 to the last
+    bits = torch.where(torch.rand(query.shape, generator=gen) < 0.3, torch.randint(0x7f70, 0x7f80, query.shape, generator=gen), bits)
+    bits |= torch.randint(0, 2, query.shape, generator=gen) << 15
+    query = (bits - (bits >> 15 << 16)).to(torch.int16).view(torch.bfloat16)
+    assert torch.isfinite(query.float()).all() and query.float().abs().max() == 255 * 2.0 ** 120
+    out = attend(gpu, cache, table, query, q_cu, lengths, max(counts), 2.0 ** -31, total_keys=sum(lengths))
+    want = values_of(cache)
+    for i, n in enumerate(lengths):
+        close(out[q_cu[i]:q_cu[i + 1]], query[q_cu[i]:q_cu[i + 1]], *want.rows(table[i], 0, n), 2.0 ** -31)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("head_dim,heads,kv_heads,lengths,counts", PATHS)
+def test_queries_that_are_no_numbers(gpu, head_dim, heads, kv_heads, lengths, counts, bad):
+    """One element of one head of one query: that head's row is NaN, and no other."""
+    cache, table, query, q_cu = make(gpu, head_dim, heads, kv_heads, 32, lengths, counts)
+    bad_query = query.clone()
+    bad_query[-1, 1, 5] = bad
+    out = attend(gpu, cache, table, bad_query, q_cu, lengths, max(counts), 0.1, total_keys=sum(lengths)).clone()
+    assert torch.isnan(out[-1, 1]).all()
+    want = values_of(cache)
+    out[-1, 1] = attend(gpu, cache, table, query, q_cu, lengths, max(counts), 0.1, total_keys=sum(lengths))[-1, 1]
+    for i, n in enumerate(lengths):
+        close(out[q_cu[i]:q_cu[i + 1]], query[q_cu[i]:q_cu[i + 1]], *want.rows(table[i], 0, n), 0.1)
