@@ -382,7 +382,8 @@ __device__ __forceinline__ void read_keys4(const uint8_t* codes, const uint8_t* 
       const int token = i * kRows + sub;  // of the tile
       const int piece = D == 64 ? (token >> 4) * 2 + (l >> 2) : l >> 2, t16 = token & 15;
       const unsigned c = *reinterpret_cast<const unsigned*>(mine + piece * kKeyPitch4 + t16 * 16 + (l & 3) * 4);
-      const float scale = *reinterpret_cast<const float*>(mine + 4 * kKeyPitch4 + (piece * 16 + t16) * 4);
+      const float scale =  // (read as what was written: as a float the load could move before the store)
+          __uint_as_float(*reinterpret_cast<const unsigned*>(mine + 4 * kKeyPitch4 + (piece * 16 + t16) * 4));
       const int row = D == 64 ? token : t2 * 16 + token;
       if (row < tokens_left) store(to + row * step + dt * 128 + l * 8, bf16_of_8_codes4(c, scale));
     }

@@ -6,12 +6,13 @@ from __future__ import annotations
 import ctypes
 import math
 import re
+import subprocess
 from pathlib import Path
 
 import pytest
 import torch
 
-from karpo_decision_amd import _lib, kv_cache, ops
+from karpo_decision_amd import _lib, build, kv_cache, ops
 from oracle import cache4 as oracle
 
 HEADER = Path(__file__).resolve().parents[1] / "include" / "karpo_cache4.h"
@@ -286,3 +287,19 @@ def test_workspaces_go_by_the_format_of_the_call_alone():
             a.workspace, a.workspace_bytes = 4096, need.value
             got.append(need.value)
     assert got == got[:2] * 4 and got[0] > 0 and got[1] == 0
+
+
+def test_read_takes_lds_as_the_type_that_was_written(tmp_path):
+    """The reading kernels' byte arrays in LDS hold integers (and vectors, which may alias anything). A scalar access of another
+    type is one that the compiler may move across theirs, by its type tag in the compiled kernels' IR."""
+    ir = tmp_path / "kernels.ll"
+    subprocess.run([build.hipcc(), *build.HIP_FLAGS, "--cuda-device-only", "-S", "-emit-llvm", str(build.CSRC / "cache.hip"),
+                    "-o", str(ir)], check=True, capture_output=True)
+    text = ir.read_text()
+    nodes = dict(re.findall(r"^(!\d+) = (.*)$", text, re.M))
+    kinds = set()
+    for line in text.splitlines():
+        tag = re.search(r"\b(?:load|store) \w+\b.*addrspace\(3\).*!tbaa (!\d+)", line)
+        if tag:
+            kinds.add(nodes[re.match(r"!\{(!\d+)", nodes[tag[1]])[1]].split('"')[1])
+    assert kinds == {"int"}
