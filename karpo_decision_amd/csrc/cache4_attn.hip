@@ -352,9 +352,10 @@ __device__ __forceinline__ void attend4_share(const AttendParams& p, const Seen&
       }
       float best = max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max3(x[6], x[7], x[7]));
       best = column_max(best) * p.scale;
-      // the running maximum is raised (and O rescaled) only where it grows by more than 2^8: weights are then at most 2^8
-      if (__any(!(best <= top[n] + 8.f) && best != -INFINITY)) {
-        const float up = __builtin_elementwise_maximum(top[n], best);
+      // what the weights are taken against is raised (and O rescaled) only where a score passes it, and then to 2^8 above the
+      // largest: weights are at most 1, and sums of the largest values within fp32's range, as in the formula
+      if (__any(!(best <= top[n]) && best != -INFINITY)) {
+        const float up = __builtin_elementwise_maximum(top[n], best + 8.f);
         const float f = top[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top[n] - up);
         top[n] = up;
         sum[n] *= f;

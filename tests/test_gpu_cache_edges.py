@@ -1,5 +1,5 @@
-"""The block caches on the GPU where few numbers of real use lie: slots that no append wrote, queries at the end of bf16's
-range. Tolerances are ``cache4_cases.close``'s."""
+"""The block caches on the GPU where few numbers of real use lie: slots that no append wrote, queries and values at the end of
+bf16's range. Tolerances are ``cache4_cases.close``'s."""
 
 from __future__ import annotations
 
@@ -8,7 +8,8 @@ import math
 import pytest
 import torch
 
-from cache4_cases import SPLIT, UNPACKED, WHOLE, attend, close, make, path_of, raw, values_of
+from cache4_cases import SPLIT, UNPACKED, WHOLE, attend, close, ints, make, path_of, raw, values_of
+from karpo_decision_amd import kv_cache
 from oracle import cache4 as oracle
 
 pytestmark = pytest.mark.gpu
@@ -76,7 +77,7 @@ def test_blocks_behind_a_window_reach_no_query(gpu, head_dim, heads, kv_heads, l
         close(out[q_cu[i]:q_cu[i + 1]], query[q_cu[i]:q_cu[i + 1]], key, value, 0.1, window=window)
 
 
-# ---- queries at the end of bf16's range
+# ---- queries and values at the end of bf16's range
 
 PATHS = [(64, 4, 2, [200, 33], [1, 2]), (64, 4, 2, [1500, 33], [1, 2]), (128, 16, 2, [200, 33], [5, 2]), (128, 16, 2, [1500, 33], [5, 2]),
          (256, 4, 2, [500, 33], [1, 1]), (256, 8, 1, [1500, 33], [3, 2]), (512, 4, 1, [200, 33], [1, 2]), (512, 4, 1, [1500, 33], [1, 2])]
@@ -115,3 +116,26 @@ def test_queries_that_are_no_numbers(gpu, head_dim, heads, kv_heads, lengths, co
     out[-1, 1] = attend(gpu, cache, table, query, q_cu, lengths, max(counts), 0.1, total_keys=sum(lengths))[-1, 1]
     for i, n in enumerate(lengths):
         close(out[q_cu[i]:q_cu[i + 1]], query[q_cu[i]:q_cu[i + 1]], *want.rows(table[i], 0, n), 0.1)
+
+
+@pytest.mark.parametrize("bits", [4])
+@pytest.mark.parametrize("head_dim,kv_heads,tokens", [(64, 2, 140), (128, 2, 140), (256, 1, 140), (512, 1, 140), (64, 2, 400), (128, 2, 400),
+                                                      (256, 1, 400), (64, 16, 20000), (128, 16, 20000), (256, 8, 20000), (512, 4, 20000)])
+@pytest.mark.parametrize("count", [1, 9])
+def test_large_values_under_growing_scores(gpu, bits, head_dim, kv_heads, tokens, count):
+    """Values of 1.5 * 2^121 everywhere, scores that grow by 2^7 from one token to a later one: weights above 1 would take the sums
+    past fp32's range. The scores are 0 at every 512th token, 7 (in powers of two) 256 tokens (128 where there are no more) behind
+    it, and -42 elsewhere, so that 39 weights of 1 are the most that is summed up: below 2^127."""
+    hot = 128 if tokens < 256 else 256
+    cache = kv_cache.create(-(-tokens // 64), kv_heads, head_dim, 64, device=gpu, bits=bits)
+    key = torch.zeros((tokens, kv_heads, head_dim), device=gpu)
+    key[:, :, 0] = -6.0
+    key[::512, :, 0], key[hot::512, :, 0] = 0.0, 1.0
+    value = torch.full_like(key, 1.5 * 2.0 ** 121)
+    writes = [[j, 0, 64 * j, min(64, tokens - 64 * j)] for j in range(cache.blocks)]
+    kv_cache.append(cache, key.bfloat16(), value.bfloat16(), ints(writes, gpu))
+    query = torch.zeros((count, 2 * kv_heads, head_dim))
+    query[:, :, 0] = 1.0
+    out = attend(gpu, cache, [list(range(cache.blocks))], query.bfloat16(), [0, count], [tokens], count, 7 * math.log(2.0),
+                 total_keys=tokens)
+    assert ((out.float() / 2.0 ** 121 - 1.5).abs() <= 1.5 * 2.0 ** -8).all()
