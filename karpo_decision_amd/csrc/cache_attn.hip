@@ -22,6 +22,10 @@ constexpr int ring_bytes(int d) { return kAttendWaves * kCacheGroup * d; }
 // tokens 16.6, 18.3; 512, 128 tokens 17.0, 13.3, 256 tokens 16.8, 18.0. 128 requests of 512 tokens at head size 128 49.6,
 // 44.0; at 512 61.4, 60.7.
 constexpr int64_t kWholeTokens = 640;
+// Weights are up to 2^8 against the running maximum (it is raised where it grows by more); values are taken 2^-8 of theirs for as
+// long as they are summed up (exact, and free: it goes into their scale), so that sums of the largest ones stay within fp32's
+// range as in the formula.
+constexpr float kValueFactor = 0x1p-8f;
 constexpr int kLeastUnits = kAttendWaves;  // groups of 32 tokens that a workgroup takes at least
 
 // What a request takes of the sums: a workgroup that goes on to a next request spends about as long on the change (joining its
@@ -215,7 +219,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
         if (ids < 0 || ids >= p.c.blocks) ids = -1;
         const float2 sc = *reinterpret_cast<const float2*>(p.c.scales + 2 * ((int64_t)max(ids, 0) * heads + h));
         k_scales = ids < 0 ? 1.f : sc.x;  // (zeros under another block's scale, NaN where it was never written, could be NaN)
-        v_scales = ids < 0 ? 1.f : sc.y;
+        v_scales = ids < 0 ? 1.f : sc.y * kValueFactor;
       };
       // One group's codes into the wave's ring, 16 bytes a lane and KiB; zeros for a block that is not of the pool, and where
       // there is no group (so that every turn of the loop issues the same copies, and a wait can count them).
@@ -438,7 +442,7 @@ __global__ __launch_bounds__(kAttendThreads, attend_waves(D, NT)) void attend_ke
           if (whole) {
             const float l = total_of(c, top_of(c));
             const int vec = vector0 + c, pos = position_of(vec, p), head = h * p.group + vec - pos * p.group;
-            if (l == 0.f) x = f32x4{0.f, 0.f, 0.f, 0.f}; else x = x * (1.f / l);
+            if (l == 0.f) x = f32x4{0.f, 0.f, 0.f, 0.f}; else x = x * (1.f / l / kValueFactor);
             *reinterpret_cast<u32x2*>(p.o + (s.row + (int64_t)pos) * p.so_t + head * p.so_h + d0 + d) =
                 u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
           } else {
@@ -495,7 +499,7 @@ __global__ __launch_bounds__(256) void join_kernel(const AttendParams p, int vec
   };
   auto store = [&](const Sum& a, int c, int d) {
     const int vec = vector0 + c, pos = position_of(vec, p), head = h * p.group + vec - pos * p.group;
-    const f32x4 x = a.l == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : a.x * (1.f / a.l);
+    const f32x4 x = a.l == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : a.x * (1.f / a.l / kValueFactor);
     *reinterpret_cast<u32x2*>(p.o + (s.row + (int64_t)pos) * p.so_t + head * p.so_h + d) =
         u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
   };

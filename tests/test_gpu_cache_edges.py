@@ -118,7 +118,7 @@ def test_queries_that_are_no_numbers(gpu, head_dim, heads, kv_heads, lengths, co
         close(out[q_cu[i]:q_cu[i + 1]], query[q_cu[i]:q_cu[i + 1]], *want.rows(table[i], 0, n), 0.1)
 
 
-@pytest.mark.parametrize("bits", [4])
+@pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("head_dim,kv_heads,tokens", [(64, 2, 140), (128, 2, 140), (256, 1, 140), (512, 1, 140), (64, 2, 400), (128, 2, 400),
                                                       (256, 1, 400), (64, 16, 20000), (128, 16, 20000), (256, 8, 20000), (512, 4, 20000)])
 @pytest.mark.parametrize("count", [1, 9])
