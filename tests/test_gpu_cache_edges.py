@@ -1,5 +1,5 @@
 """The block caches on the GPU where few numbers of real use lie: slots that no append wrote, queries and values at the end of
-bf16's range. Tolerances are ``cache4_cases.close``'s."""
+bf16's range, sums in which each group of tokens shows. Tolerances are ``cache4_cases.close``'s."""
 
 from __future__ import annotations
 
@@ -11,6 +11,8 @@ import torch
 from cache4_cases import SPLIT, UNPACKED, WHOLE, attend, close, ints, make, path_of, raw, values_of
 from karpo_decision_amd import kv_cache
 from oracle import cache4 as oracle
+from test_gpu_cache4 import _append_and_compare
+from test_gpu_cache_rope import _server
 
 pytestmark = pytest.mark.gpu
 
@@ -139,3 +141,83 @@ def test_large_values_under_growing_scores(gpu, bits, head_dim, kv_heads, tokens
     out = attend(gpu, cache, [list(range(cache.blocks))], query.bfloat16(), [0, count], [tokens], count, 7 * math.log(2.0),
                  total_keys=tokens)
     assert ((out.float() / 2.0 ** 121 - 1.5).abs() <= 1.5 * 2.0 ** -8).all()
+
+
+# ---- each group of tokens shows
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("head_dim,heads,kv_heads,lengths,counts", [
+    (64, 4, 2, [4517, 90], [2, 1]), (128, 8, 2, [4517, 90], [2, 1]), (256, 4, 1, [4517, 90], [2, 1]), (512, 4, 1, [4517, 90], [2, 1]),
+    (128, 32, 16, [20001, 4000, 700], [1, 1, 1]), (64, 40, 1, [2100, 70], [9, 2]), (128, 4, 2, [640, 333], [1, 2]),
+    (256, 4, 2, [640, 333], [1, 2]), (512, 4, 2, [250, 100], [1, 2])])
+def test_no_group_is_left_out_or_taken_twice(gpu, bits, head_dim, heads, kv_heads, lengths, counts):
+    """Element d of a token's value is 1 where the token's group of 32 is d modulo the head size, and 0 elsewhere, under scores
+    so even that every token counts alike: an element holds its own groups' share, and one of them left out or taken twice
+    moves it by a tenth at least (of at most ten groups)."""
+    block = 64
+    gen = torch.Generator().manual_seed(head_dim)
+    blocks = [-(-n // block) for n in lengths]
+    ids = torch.randperm(sum(blocks), generator=gen).tolist()
+    cache = kv_cache.create(sum(blocks), kv_heads, head_dim, block, device=gpu, bits=bits)
+    table, q_cu = [], [0]
+    keys, values = [], []
+    for n, c, b in zip(lengths, counts, blocks):
+        table.append([ids.pop() for _ in range(b)])
+        q_cu.append(q_cu[-1] + c)
+        group = torch.arange(n) // 32
+        value = torch.zeros((n, kv_heads, head_dim))
+        value[torch.arange(n), :, group % head_dim] = 1.0
+        key = torch.randn((n, kv_heads, head_dim), generator=gen).bfloat16()
+        kv_cache.append(cache, key.to(gpu), value.bfloat16().to(gpu),
+                        ints([[ident, 0, block * j, min(block, n - block * j)] for j, ident in enumerate(table[-1])], gpu))
+        keys.append(oracle.quantised(key.double()) if bits == 4 else None)
+        values.append(value.double())
+    assert max(lengths) <= 10 * 32 * head_dim
+    query = torch.randn((q_cu[-1], heads, head_dim), generator=gen).bfloat16()
+    width = max(blocks)
+    padded = [row + [-1] * (width - len(row)) for row in table]
+    out = attend(gpu, cache, padded, query, q_cu, lengths, max(counts), 1e-4, total_keys=sum(lengths))
+    for i, n in enumerate(lengths):
+        if bits == 8:
+            keys[i] = kv_cache.read(cache, ints([padded[i]], gpu), ints([n], gpu), n)[0].cpu().double()
+        close(out[q_cu[i]:q_cu[i + 1]], query[q_cu[i]:q_cu[i + 1]], keys[i], values[i], 1e-4)
+
+
+# ---- append and rounds of a server
+
+@pytest.mark.parametrize("e", [0, -60, 100, -100, -104])
+def test_append_rounds_small_elements_beside_large_ones(gpu, e):
+    """Every finite bf16 value of at most 6 * 2^e, zeros, subnormal numbers and what rounds to nothing among them, 31 at a time
+    beside 6 * 2^e (below 2^-100 the scale is the least one)."""
+    every = torch.arange(1 << 16, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    top = torch.tensor(6.0 * 2.0 ** e).bfloat16()
+    part = every[every.float().abs() <= top.float()]
+    part = torch.cat((part, part.new_zeros(-part.numel() % 31))).view(-1, 31)
+    x = torch.cat((part, top.expand(part.shape[0], 1)), 1)
+    x = torch.cat((x, x.new_zeros((-x.shape[0] % 2, 32)))).view(-1, 1, 64)
+    cache = kv_cache.create(-(-x.shape[0] // 32), 1, 64, 32, device=gpu, bits=4)
+    writes = [[i, 0, 32 * i, min(32, x.shape[0] - 32 * i)] for i in range(cache.blocks)]
+    _append_and_compare(cache, x.to(gpu), -x.to(gpu), writes)
+
+
+@pytest.mark.parametrize("heads,kv_heads,d,block,rotated", [(4, 2, 64, 32, 64), (16, 2, 128, 64, 64), (2, 1, 256, 128, 256)])
+def test_rounds_of_a_server_in_8_bits_to_the_output_s_rounding(gpu, heads, kv_heads, d, block, rotated):
+    """Calls of at most 64 query vectors a key head are never unpacked: their weights are two bf16 terms, and the outputs lie within
+    the tolerance of the 4-bit cache's, without a term for weights of one."""
+    most = 64 * kv_heads // heads
+    rounds = [[min(c, most) for c in counts] for counts in ([40, 7, 0, 65], [1, 1, 1, 1], [1, 1, 30, 0], [3, 2, 3, 1], [1, 1, 1, 1])]
+    gen = torch.Generator(device=gpu).manual_seed(6)
+    server = _server(gpu, 8, heads, kv_heads, d, block, rotated)
+    with torch.inference_mode():
+        for counts in rounds:
+            n = sum(counts)
+            query = torch.randn((n, heads, d), generator=gen, device=gpu).bfloat16()
+            key, value = (torch.randn((n, kv_heads, d), generator=gen, device=gpu).bfloat16() for _ in range(2))
+            step, out, turned = server.round(ints(counts, gpu), n, max(counts), query, key, value)
+            step.check()
+            held = step.lengths.tolist()
+            keys, values, k_cu = kv_cache.read(server.cache, server.table, step.lengths, sum(held))
+            q_cu, k_cu = step.q_cu.tolist(), k_cu.tolist()
+            for i in range(4):
+                close(out[q_cu[i]:q_cu[i + 1]], turned[q_cu[i]:q_cu[i + 1]], keys[k_cu[i]:k_cu[i + 1]].double(),
+                      values[k_cu[i]:k_cu[i + 1]].double(), 0.1)
