@@ -25,7 +25,8 @@
  * Lengths below 0 count as 0, lengths past the table's row as the row's tokens.
  *
  * Softmax statistics and sums are fp32. The weights enter the second product as two bf16 terms (2^-17 off) for few queries, and
- * as one (2^-8) in long chunks, whose keys are unpacked for karpo_attn_fwd; which of the two goes by the sizes.
+ * as one (2^-8) in long chunks, whose keys are unpacked for karpo_attn_fwd; which of the two goes by the sizes. In long chunks, as
+ * there, weights go up to 2^8 before they are divided, and values from 2^119 on may become infinite.
  *
  * Conventions are those of karpo_attn.h: device pointers, sizes and strides in elements, launches on the given stream
  * only, no allocation, no synchronisation, failures as KARPO_ATTN_* status codes (karpo_attn_strerror). Lengths, bounds,

@@ -12,7 +12,8 @@ namespace karpo {
 
 namespace {
 
-// Waves per SIMD (and workgroups per CU): what the registers hold without spilling.
+// Waves per SIMD (and workgroups per CU): what the registers hold without spilling; attend4_kernel<128, 4> alone spills 7, four of
+// which each group loads again.
 __host__ __device__ constexpr int attend4_waves(int d, int nt) {
   return nt == 1 ? (d == 64 ? 4 : d == 128 ? 3 : d == 256 ? 2 : 1) : d == 64 && nt == 2 ? 3 : d <= 128 ? 2 : 1;
 }
@@ -21,10 +22,13 @@ constexpr int ring4_bytes(int d, int waves) { return waves * kCacheGroup * d / 2
 // And for their sums while they are joined.
 constexpr int sums4_bytes(int d, int nt, int waves) { return waves * 16 * nt * (slab_of(d, nt) + 4) * 4; }
 
-// Requests of which at most so many tokens are seen are not split: a workgroup's walk is then shorter than the partials' way
-// through memory and a second launch. us split, whole at heads of 128 with 16 key heads: 8 requests of 128 tokens 12.4, 7.3, of
-// 640 15.9, 11.4 (10.3 by eight waves), of 1,500 18.9, 18.7; one of 1,024 13.7, 13.6; heads of 512, 2 requests of 256 15.8, 13.0,
-// of 512 16.7, 17.6.
+// Requests of which at most so many tokens are seen (by the bounds that the call gives, the table's width among them) are not
+// split: a workgroup's walk is then shorter than the partials' way through memory and a second launch. us split, whole by four
+// waves at heads of 128 with 16 key heads: 8 requests of 128 tokens 12.4, 7.3, of 640 15.9, 11.4, of 1,500 18.9, 18.7; one of
+// 1,024 13.7, 13.6; heads of 512, 2 requests of 256 15.8, 13.0, of 512 16.7, 17.6. The bound is that of four waves. Where eight
+// would walk (AttendShape::wide) they are faster past it too: 8 requests of 1,000 tokens, 16 heads of 128 17.4, 12.6, 2 of 64
+// 13.4, 10.3, 8 of 256 18.0, 16.0; of 1,300 18.4, 14.1; 13.7, 11.6; 19.3, 18.1; one of 1,300, 16 heads of 128 13.9, 12.9, 8 of
+// 256 15.7, 17.2.
 constexpr int whole_tokens4(int d) { return d == 512 ? 256 : 640; }
 // Where more than half of the CUs have a workgroup, a longer walk is no loss (48 requests of 4 query tokens and 1,024 cached
 // ones: heads of 64 18.4, 13.0; 128 33.4, 27.4; 256 36.1, 29.9; 512 64.4, 60.5), up to what one long request among short ones

@@ -380,7 +380,10 @@ __device__ __forceinline__ void append_rows(const AppendRowsParams& p, const Wri
   } while (MANY && ++h < h1);
 }
 
-// (three waves a SIMD where one walks heads over 8 bits: without the bound two, and a document of 16 heads of 128 93.8 us, not 89.6)
+// (three waves a SIMD where one walks heads over 8 bits: without the bound two, and a document of 16 heads of 128 93.8 us, not
+// 89.6. Otherwise as the registers have it: 89 to 93 of them in 4 bits and 106 to 121 in 8, 133 and so three waves in blocks of 32
+// at heads of 64 and 512. Sixteen waves at heads of 512 have 128 each and spill: in blocks of 128 5 in 4 bits and 7 in 8, in
+// blocks of 64 1 in 8.)
 template <int D, int BLOCK, int PASSES, int WAVES, int BITS, bool MANY>
 __global__ __launch_bounds__(64 * WAVES, MANY && BITS == 8 ? 3 : 1) void append_rows_kernel(const AppendRowsParams p) {
   constexpr int kStep = 512 / D * WAVES;  // tokens of a pass

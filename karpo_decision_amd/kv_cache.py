@@ -395,12 +395,12 @@ def attend(query: Tensor, cache: Cache, table: Tensor, q_cu: Tensor, lengths: Te
     all); a query that sees none gets zeros. A NaN reaches the queries that see its token, and in long chunks (whose keys
     are unpacked for the packed attention first) it can reach others of its tile, as there. The softmax weights enter the
     second product as two bf16 terms, in long chunks as one, as there: 2.3e-3 of the 2-norm off against 1.7e-3, the
-    output's own rounding. ``max_q`` bounds every request's query count, ``total_keys`` the lengths' sum. Long chunks
-    unpack up to ``total_keys`` tokens into a workspace (4 * kv heads * D bytes each), so give it where the table is wide:
-    the default is all that the table can hold, 51.6 GB for 48 requests in a table for 131,072 tokens, 16 heads of 128.
-    Where one of the two does not hold, rows that were not computed are NaN: those of a request past its first ``max_q``,
-    or, in long chunks, those of all requests. A NaN ``scale`` makes the rows of requests with tokens NaN. Rows behind the
-    last request are not written."""
+    output's own rounding; values from 2^119 on may become infinite in long chunks. ``max_q`` bounds every request's
+    query count, ``total_keys`` the lengths' sum. Long chunks unpack up to ``total_keys`` tokens into a workspace (4 *
+    kv heads * D bytes each), so give it where the table is wide: the default is all that the table can hold, 51.6 GB
+    for 48 requests in a table for 131,072 tokens, 16 heads of 128. Where one of the two does not hold, rows that were
+    not computed are NaN: those of a request past its first ``max_q``, or, in long chunks, those of all requests. A NaN
+    ``scale`` makes the rows of requests with tokens NaN. Rows behind the last request are not written."""
     _real("attend", query)
     _no_grad("attend", query)
     index = query.get_device()
