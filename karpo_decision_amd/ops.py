@@ -54,8 +54,10 @@ def _bf16_table(t: Tensor, device: torch.device) -> Tensor:
         raise ValueError(f"a prologue table is on {t.device}, the tensors on {device}")
     if t.dtype != torch.bfloat16:
         t = t.to(torch.bfloat16)
-    if t.stride(-1) != 1 or (t.dim() == 2 and t.stride(0) % 8) or t.data_ptr() % 16:
+    if t.stride(-1) != 1 or (t.dim() == 2 and t.stride(0) % 8):
         t = t.contiguous()
+    if t.data_ptr() % 16:  # (a view into a larger tensor: contiguous() would leave a contiguous one where it is)
+        t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 

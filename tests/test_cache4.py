@@ -201,6 +201,16 @@ def test_fake_tensors_are_refused():
                 call()
 
 
+@pytest.mark.parametrize("first", [1, 3, 4, 8])
+def test_tables_at_any_address_are_taken(first):
+    """Weights and tables that begin anywhere in a larger tensor: the kernels load 16 bytes at once."""
+    whole = torch.arange(9 * 64 + 8, dtype=torch.float32).bfloat16()
+    for t in (whole[first:first + 64], whole[first:first + 9 * 64].view(9, 64)):
+        got = ops._bf16_table(t, t.device)
+        assert got.data_ptr() % 16 == 0 and got.is_contiguous() and torch.equal(got, t)
+        assert got.data_ptr() == t.data_ptr() or t.data_ptr() % 16
+
+
 # ---- refusals of the C ABI (the pointers are never followed)
 
 def _c_cache(**change):

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from cache4_cases import SPLIT, UNPACKED, WHOLE, attend, close, ints, make, path_of, raw, values_of
-from karpo_decision_amd import kv_cache
+from karpo_decision_amd import kv_cache, ops
 from oracle import cache4 as oracle
 from test_gpu_cache4 import _append_and_compare
 from test_gpu_cache_rope import _server
@@ -221,3 +221,21 @@ def test_rounds_of_a_server_in_8_bits_to_the_output_s_rounding(gpu, heads, kv_he
             for i in range(4):
                 close(out[q_cu[i]:q_cu[i + 1]], turned[q_cu[i]:q_cu[i + 1]], keys[k_cu[i]:k_cu[i + 1]].double(),
                       values[k_cu[i]:k_cu[i + 1]].double(), 0.1)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_weights_and_tables_at_any_address(gpu, bits):
+    """Out of the middle of larger tensors, not at a multiple of 16 bytes: as their copies, in ``append`` and ``norm_rope``."""
+    gen = torch.Generator(device=gpu).manual_seed(7)
+    key, value = (torch.randn((9, 2, 64), generator=gen, device=gpu).bfloat16() for _ in range(2))
+    weight, cos, sin = (torch.randn(n + 3, generator=gen, device=gpu).bfloat16()[3:] for n in (64, 9 * 64, 9 * 64))
+    assert all(t.data_ptr() % 16 for t in (weight, cos, sin))
+    got = []
+    with torch.inference_mode():
+        for w, c, s in ((weight, cos, sin), (weight.clone(), cos.clone(), sin.clone())):
+            cache = kv_cache.create(1, 2, 64, 32, device=gpu, bits=bits)
+            norm, rope = ops.Norm(ops.NORM_WEIGHT, w, 1e-6), (c.view(9, 64), s.view(9, 64))
+            kv_cache.append(cache, key, value, ints([[0, 0, 0, 9]], gpu), k_norm=norm, v_norm=norm, rope=rope)
+            got.append([*(raw(t) for t in cache[:3]), ops.norm_rope(key, norm, rope)])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
