@@ -239,3 +239,29 @@ def test_weights_and_tables_at_any_address(gpu, bits):
             got.append([*(raw(t) for t in cache[:3]), ops.norm_rope(key, norm, rope)])
     for a, b in zip(*got):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_a_compiled_step_with_norms_and_rotation(gpu, bits):
+    """torch.compile breaks its graph around the calls: each sees the tensors of its own step, not those of the traced one."""
+    def step(cache, table, lengths, counts, free, left, key, value, query, weight, cos, sin):
+        got = kv_cache.reserve(table, lengths, counts, free, left, 47, 32)
+        kv_cache.append(cache, key * 2, value, got.writes, k_norm=ops.Norm(ops.NORM_WEIGHT, weight, 1e-6), rope=(cos, sin),
+                        positions=got.positions)
+        k, v, _ = kv_cache.read(cache, table, got.lengths, 47)
+        return kv_cache.attend(query + 1, cache, table, got.q_cu, got.lengths, 40, 0.1) * 2, k + 1, v
+
+    def inputs(seed):
+        gen = torch.Generator(device=gpu).manual_seed(seed)
+        rows = [torch.randn(shape, generator=gen, device=gpu).bfloat16()
+                for shape in ((47, 2, 64), (47, 2, 64), (47, 4, 64), (64,), (50, 64), (50, 64))]
+        return (kv_cache.create(20, 2, 64, 32, device=gpu, bits=bits), torch.full((2, 6), -1, dtype=torch.int32, device=gpu),
+                ints([0, 0], gpu), ints([40, 7], gpu), torch.arange(20, dtype=torch.int32, device=gpu), ints([20], gpu), *rows)
+
+    torch._dynamo.reset()
+    compiled, kept = torch.compile(step, backend="eager"), []
+    with torch.inference_mode():
+        for seed in range(3):
+            kept.append(inputs(seed))  # (kept, so that the next step's tensors lie elsewhere)
+            for a, b in zip(compiled(*kept[-1]), step(*inputs(seed))):
+                assert torch.equal(a, b)
